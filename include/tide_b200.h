@@ -65,7 +65,8 @@ enum tide_status {
 enum tide_device_error {
   TIDE_DEVERR_POSITION = 1, /* exit position outside [0, n_total): row skipped */
   TIDE_DEVERR_TIMEOUT = 2,  /* a bounded spin wait expired; results invalid  */
-  TIDE_DEVERR_COUNT = 4     /* device row count above the row capacity       */
+  TIDE_DEVERR_COUNT = 4,    /* device row count above the row capacity       */
+  TIDE_DEVERR_PAGES = 8     /* no free page, or a block table too narrow     */
 };
 
 int tide_abi_version(void);
@@ -256,6 +257,117 @@ int tide_qk_norm_rope(int dtype, const void *q, const void *k, const void *v,
                       tide_stream_t stream);
 int tide_silu_mul(int dtype, const void *gate, const void *up, void *out, int64_t n_rows,
                   const int32_t *n_rows_dev, int64_t width, tide_stream_t stream);
+
+/* ---- ragged batches over a paged cache ---------------------------------- */
+/*
+ * Sequences of different lengths, packed: sequence i holds the token rows
+ * [cu_seqlens[i], cu_seqlens[i + 1]) (device int32, n_seqs + 1 entries,
+ * ascending).  Rows behind the last sequence are left as they were.
+ *
+ * A paged cache keeps a request's keys (and, in a second array, its values)
+ * in pages [n_pages, n_kv_heads, page_size, head_dim] of the rows' type:
+ * position p of request r lies in page block_tables[r * max_pages +
+ * p / page_size], at p % page_size.  A page with one KV head is one
+ * contiguous run, as a slot of the caches of tide_decode_attention is.  A
+ * page holds one request's positions; the entries of a block table past a
+ * request's last page are not read, nor is what lies in its last page past
+ * its length.  The reference has no such cache: its decode loop keeps the
+ * model's own (python/TIDE/runtime.py:223-313) and takes one length for the
+ * whole batch.
+ *
+ * tide_packed_attention: causal attention within each packed sequence,
+ *   out[i, h] = (sum_j e^(s_ij) v[j, h / G]) / (zero_keys[i] + sum_j e^(s_ij)),
+ *   s_ij = scale * q[i, h] . k[j, h / G],  j over the rows of i's sequence up
+ *   to i,  G = n_q_heads / n_kv_heads (any whole number).
+ * zero_keys (optional, int32 per row; negative counts as 0): so many further
+ * keys that are zero, as are their values.  With the survivors of a
+ * checkpoint as the rows and, for each, its position minus its rank among
+ * its sequence's survivors, this is attention over the whole sequence whose
+ * exited tokens are zero-padded (python/TIDE/runtime.py:194-221), without
+ * the zeros.
+ *
+ * tide_paged_attention: the new tokens of each request over its paged cache,
+ * which already holds their own keys and values:
+ *   new token t of sequence i (of n_i rows) sees the positions [0, L - n_i +
+ *   t], L = kv_lens[r], r = seq_ids[i] (i when NULL); a token that sees none
+ *   gets zeros.
+ * cu_seqlens NULL: one row per sequence (a decode step).  n_seqs_dev
+ * (optional): only the sequences below it run.  max_kv_len bounds the
+ * lengths, and sizes the workspace and the split of long contexts; a longer
+ * one counts as invalid.
+ *
+ * Both: bf16 or fp16, head_dim 64 or 128, scale > 0, up to 128 query heads
+ * per KV head; page_size a power of two of at least 16.  q, k, v: heads
+ * packed within a row, rows q_row_stride and kv_row_stride elements apart
+ * (0: packed; multiples of 8, so that column slices of one projection's
+ * output do).  A sequence with bad bounds, a request outside
+ * [0, n_requests), or a length outside [0, max_kv_len] is skipped, its rows
+ * left as they were, and sets TIDE_DEVERR_POSITION; a page outside
+ * [0, n_pages) reads as zeros and sets it too.  A NaN or infinity in a value
+ * row reaches the tokens that see that row, and no others. */
+int tide_packed_attention(int dtype, const void *q, const void *k, const void *v,
+                          int64_t q_row_stride, int64_t kv_row_stride, const int32_t *cu_seqlens,
+                          int64_t n_seqs, const int32_t *zero_keys, void *out, int64_t n_tokens,
+                          int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim, float scale,
+                          int32_t *error_word, tide_stream_t stream);
+size_t tide_paged_attention_workspace_size(int64_t n_tokens, int64_t n_seqs, int64_t n_q_heads,
+                                           int64_t n_kv_heads, int64_t head_dim,
+                                           int64_t max_kv_len);
+int tide_paged_attention(int dtype, const void *q, int64_t q_row_stride, const void *k_cache,
+                         const void *v_cache, int64_t n_pages, int64_t page_size,
+                         const int32_t *block_tables, int64_t max_pages, int64_t n_requests,
+                         const int32_t *kv_lens, const int32_t *cu_seqlens, const int32_t *seq_ids,
+                         int64_t n_seqs, const int32_t *n_seqs_dev, void *out, int64_t n_tokens,
+                         int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim,
+                         int64_t max_kv_len, float scale, void *workspace, size_t workspace_bytes,
+                         int32_t *error_word, tide_stream_t stream);
+
+/* Keys and values of new tokens into a paged cache: row i of k_new and v_new
+ * [n_rows, n_kv_heads, head_dim] (rows kv_row_stride elements apart; 0:
+ * packed) goes to slot s = slot_map[row_ids[i]] (slot_map[i] when row_ids is
+ * NULL), that is to page s / page_size at s % page_size, for i below
+ * *n_rows_dev (clamped to [0, n_rows]; n_rows when NULL).  k_new and v_new
+ * both NULL write zeros (the keys and values of exited tokens,
+ * python/TIDE/runtime.py:194-221).  A slot of -1 is skipped; any other slot
+ * outside the cache, or a row id outside [0, n_slot_map), skips its row and
+ * sets TIDE_DEVERR_POSITION.  No slot may be named twice in a call.  head_dim
+ * 64 or 128, bf16 or fp16, any page size; 16-byte aligned rows. */
+int tide_paged_append(int dtype, const void *k_new, const void *v_new, int64_t kv_row_stride,
+                      const int64_t *slot_map, int64_t n_slot_map, const int32_t *row_ids,
+                      const int32_t *n_rows_dev, int64_t n_rows, int64_t n_kv_heads,
+                      int64_t head_dim, void *k_cache, void *v_cache, int64_t n_pages,
+                      int64_t page_size, int32_t *error_word, tide_stream_t stream);
+
+/* The page bookkeeping of one step, from the requests' lengths:
+ *   1. a request with done[r] != 0 (optional) gives back the pages of its
+ *      context_lens[r] positions and starts over from length 0;
+ *   2. every request gets the pages that new_lens[r] more positions need,
+ *      written behind its present ones in block_tables [n_requests,
+ *      max_pages];
+ *   3. kv_lens[r] = its length with them; cu_seqlens [n_requests + 1]: the
+ *      packed offsets of the new tokens; and per new token, in packed order,
+ *      slot_map (its slot in the cache, page * page_size + offset) and
+ *      positions (its position in its request).  Entries past the last token
+ *      up to n_slots: slot -1, position 0.
+ * free_pages [n_pages] is a stack whose first *n_free entries are free pages:
+ * returned pages are pushed in order of request and position, new ones popped
+ * in order of request and position.  The new count goes to *n_free_out.
+ * kv_lens may be context_lens and n_free_out may be n_free (in place, as a
+ * captured step needs it).
+ * A request that needs more pages than are left, in order of requests, or
+ * more than max_pages, gets none: its kv_lens entry is its old length, its
+ * tokens' slots are -1, and TIDE_DEVERR_PAGES is set; once one did not find
+ * its pages, no later one gets new ones.  A negative length, or a new length
+ * above n_slots, counts as 0 and sets TIDE_DEVERR_COUNT, as does a free count
+ * outside [0, n_pages] (clamped) and a request whose tokens end past n_slots
+ * (it gets no pages).  A page returned to a full stack is dropped and sets
+ * TIDE_DEVERR_PAGES.  n_requests <= 8192. */
+int tide_page_tables(const int32_t *context_lens, const int32_t *new_lens, const int32_t *done,
+                     int64_t n_requests, int32_t *free_pages, const int32_t *n_free,
+                     int64_t n_pages, int32_t *block_tables, int64_t max_pages, int64_t page_size,
+                     int32_t *n_free_out, int32_t *kv_lens, int32_t *cu_seqlens, int64_t *slot_map,
+                     int64_t *positions, int64_t n_slots, int32_t *error_word,
+                     tide_stream_t stream);
 
 /* ---- router preparation (once per router) ------------------------------ */
 

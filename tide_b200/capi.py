@@ -12,7 +12,7 @@ PATH_AUTO, PATH_SIMT, PATH_TC, PATH_TC_SPLIT = 0, 1, 2, 3
 OK = 0
 ERR_INVALID, ERR_UNSUPPORTED, ERR_CUDA, ERR_WORKSPACE, ERR_ALIGNMENT = 1, 2, 3, 4, 5
 NOALLOC_MAX_ROWS = 1048576
-DEVERR_POSITION, DEVERR_TIMEOUT, DEVERR_COUNT = 1, 2, 4
+DEVERR_POSITION, DEVERR_TIMEOUT, DEVERR_COUNT, DEVERR_PAGES = 1, 2, 4, 8
 
 p = C.c_void_p
 i32, i64, f32, sz = C.c_int32, C.c_int64, C.c_float, C.c_size_t
@@ -57,6 +57,15 @@ PROTOTYPES = {
     "tide_qk_norm_rope": (C.c_int, [C.c_int, p, p, p, i64, i64, p, p, f32, p, f32, i64, p, p, p, p, i64,
                                     i64, i64, i64, p, p, p, i64, i64, p, p]),
     "tide_silu_mul": (C.c_int, [C.c_int, p, p, p, i64, p, i64, p]),
+    "tide_packed_attention": (C.c_int, [C.c_int, p, p, p, i64, i64, p, i64, p, p, i64, i64, i64,
+                                        i64, f32, p, p]),
+    "tide_paged_attention_workspace_size": (sz, [i64, i64, i64, i64, i64, i64]),
+    "tide_paged_attention": (C.c_int, [C.c_int, p, i64, p, p, i64, i64, p, i64, i64, p, p, p, i64,
+                                       p, p, i64, i64, i64, i64, i64, f32, p, sz, p, p]),
+    "tide_paged_append": (C.c_int, [C.c_int, p, p, i64, p, i64, p, p, i64, i64, i64, p, p, i64,
+                                    i64, p, p]),
+    "tide_page_tables": (C.c_int, [p, p, p, i64, p, p, i64, p, i64, i64, p, p, p, p, p, i64, p,
+                                   p]),
     "tide_router_fold": (C.c_int, [C.c_int, p, p, p, i64, i64, p, p, p, p, p]),
     "tide_checkpoint_workspace_size": (sz, [C.POINTER(CheckpointArgs)]),
     "tide_checkpoint": (C.c_int, [C.POINTER(CheckpointArgs), p]),

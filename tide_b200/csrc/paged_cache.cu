@@ -1,0 +1,357 @@
+// The paged cache's bookkeeping: block tables, slot maps and packed offsets
+// of a step from the requests' lengths, and the write of new keys and values.
+//
+// page_tables_kernel.  With the tokens held c_r (0 for a request that is
+// done), the new tokens n_r and the page size P,
+//   have_r = ceil(c_r / P),   need_r = ceil((c_r + n_r) / P) - have_r,
+//   upto_r = need_0 + ... + need_r,
+// and a request gets its pages iff upto_r <= free pages: page j of its new
+// ones is entry free - 1 - (upto_r - need_r + j) of the stack.  So three
+// prefix sums over the requests (tokens, pages needed, pages returned) give
+// every output in parallel, without an atomic: the result does not depend on
+// the order of threads.
+// All lengths are a few KB, so every CTA of the one cluster scans all of them
+// itself (no exchange), and the CTAs share the writing.  Two cluster barriers
+// order what may alias or overlap: the first lies between the last read of
+// the lengths, the free count and the old tables and the first write of their
+// successors; it also makes the pages returned by one CTA visible to the
+// others, which may hand them out again at once.
+//
+// paged_append_kernel copies 2 * kv_heads * head_dim elements per row: bound
+// by HBM, or by latency for a decode step's rows.
+#include <cooperative_groups.h>
+#include <stdio.h>
+
+#include "ragged.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace tide {
+namespace pages {
+
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxRequests = 8192;
+constexpr int kClusterCtas = 8;
+// New tokens from which a cluster shares the writing; below, one CTA.
+constexpr int64_t kClusterTokens = 4096;
+
+struct Params {
+  const int32_t *ctx, *add, *done;
+  int n_req;
+  int32_t *free_pages;
+  const int32_t *n_free;
+  int n_pages;
+  int32_t *tables;
+  int64_t max_pages;
+  int page;
+  int32_t *n_free_out, *kv, *cu;
+  int64_t *slots, *positions;
+  int64_t n_slots;
+  int32_t *err;
+};
+
+__device__ __forceinline__ int ceil_div(int a, int b) { return a / b + (a % b != 0); }
+
+template <typename V>
+__device__ __forceinline__ V warp_inclusive(V v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const V u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+
+// Inclusive prefix sums of three values over the block's threads, on top of
+// the running totals `carry` (updated to the new totals).
+__device__ __forceinline__ void block_scan(long long (&v)[3], long long (&carry)[3],
+                                           long long (*s_sum)[3], int tid) {
+  const int lane = tid & 31, warp = tid >> 5;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) v[k] = warp_inclusive(v[k], lane);
+  if (lane == 31)
+#pragma unroll
+    for (int k = 0; k < 3; ++k) s_sum[warp][k] = v[k];
+  __syncthreads();
+  long long before[3] = {0, 0, 0}, total[3] = {0, 0, 0};
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w)
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      if (w < warp) before[k] += s_sum[w][k];
+      total[k] += s_sum[w][k];
+    }
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    v[k] += before[k] + carry[k];
+    carry[k] += total[k];
+  }
+  __syncthreads();
+}
+
+__global__ void __launch_bounds__(kThreads) page_tables_kernel(Params p) {
+  extern __shared__ int32_t dyn[];
+  // per request: packed token offset, tokens held, first new page's rank (-1:
+  // no page was to be had), where its returned pages go
+  int32_t *s_cu = dyn;                    // [n_req + 1]
+  int32_t *s_ctx = s_cu + p.n_req + 1;    // [n_req]
+  int32_t *s_rank = s_ctx + p.n_req;      // [n_req]
+  int32_t *s_push = s_rank + p.n_req;     // [n_req]
+  __shared__ long long s_sum[kWarps][3];
+  __shared__ long long s_taken;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int cta = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
+  const int tid = threadIdx.x;
+  const bool first = cta == 0;  // the CTA that reports
+  const int64_t room = p.max_pages * p.page;
+
+  int n_free = __ldcg(p.n_free);
+  if (n_free < 0 || n_free > p.n_pages) {
+    if (first && tid == 0) raise_error(p.err, TIDE_DEVERR_COUNT);
+    n_free = min(max(n_free, 0), p.n_pages);
+  }
+  if (tid == 0) {
+    s_taken = 0;
+    s_cu[0] = 0;
+  }
+  __syncthreads();
+
+  // 1. prefix sums; the pages of the requests that are done, a share per CTA
+  long long carry[3] = {0, 0, 0};  // tokens, pages needed, pages returned
+  for (int base = 0; base < p.n_req; base += kThreads) {
+    const int r = base + tid;
+    const bool in = r < p.n_req;
+    int held = in ? __ldcg(p.ctx + r) : 0, add = in ? __ldcg(p.add + r) : 0;
+    const bool gone = in && p.done && __ldg(p.done + r) != 0;
+    if (held < 0 || add < 0 || add > p.n_slots) {
+      if (first) raise_error(p.err, TIDE_DEVERR_COUNT);
+      held = max(held, 0);
+      if (add < 0 || add > p.n_slots) add = 0;
+    }
+    const int back = gone ? (int)min((int64_t)ceil_div(held, p.page), p.max_pages) : 0;
+    const int ctx = gone ? 0 : held;
+    const bool wide = (int64_t)ctx + add > room;  // more than a row of the table holds
+    const int have = ceil_div(ctx, p.page);
+    const int need = wide || !add ? 0 : (int)(((int64_t)ctx + add + p.page - 1) / p.page) - have;
+    long long v[3] = {add, need, back};
+    block_scan(v, carry, s_sum, tid);
+    if (in) {
+      s_cu[r + 1] = (int32_t)min(v[0], (long long)INT32_MAX);
+      s_ctx[r] = ctx;
+      // the rank is checked against the free pages below, when they are
+      // known; a request whose tokens do not fit in n_slots gets none either
+      // (then no later one's do, so their ranks are not used)
+      const bool past = v[0] > p.n_slots;
+      s_rank[r] = wide || past ? -1 : (int32_t)(v[1] - need);
+      s_push[r] = (int32_t)min((long long)n_free + v[2] - back, (long long)p.n_pages);
+      if (first && wide) raise_error(p.err, TIDE_DEVERR_PAGES);
+      if (first && past) raise_error(p.err, TIDE_DEVERR_COUNT);
+    }
+  }
+  __syncthreads();
+  if (p.done)  // a warp per request that is done, shared by the CTAs
+    for (int r = cta * kWarps + (tid >> 5); r < p.n_req; r += ctas * kWarps) {
+      if (__ldg(p.done + r) == 0) continue;
+      const int back = (int)min((int64_t)ceil_div(max(__ldcg(p.ctx + r), 0), p.page), p.max_pages);
+      for (int j = tid & 31; j < back; j += 32) {
+        if ((long long)s_push[r] + j < p.n_pages)
+          p.free_pages[s_push[r] + j] = __ldcg(p.tables + (int64_t)r * p.max_pages + j);
+        else
+          raise_error(p.err, TIDE_DEVERR_PAGES);
+      }
+    }
+  const long long avail = min((long long)n_free + carry[2], (long long)p.n_pages);
+  // which requests got their pages; how many pages are taken
+  for (int r = tid; r < p.n_req; r += kThreads) {
+    const int ctx = s_ctx[r], add = s_cu[r + 1] - s_cu[r];
+    if (s_rank[r] < 0 || !add) continue;
+    const int need = ceil_div(ctx + add, p.page) - ceil_div(ctx, p.page);
+    const long long upto = (long long)s_rank[r] + need;
+    if (need && upto > avail) {
+      s_rank[r] = -1;
+      if (first) raise_error(p.err, TIDE_DEVERR_PAGES);
+    } else if (need) {
+      atomicMax((unsigned long long *)&s_taken, (unsigned long long)upto);  // order-free
+    }
+  }
+  cluster.sync();  // (also a block barrier) see the header
+
+  // 2. tables, lengths, offsets, free count
+  const int all = ctas * kThreads, me = cta * kThreads + tid;
+  for (int r = me; r < p.n_req; r += all) {
+    const int ctx = s_ctx[r], add = s_cu[r + 1] - s_cu[r], rank = s_rank[r];
+    p.kv[r] = rank < 0 ? ctx : ctx + add;
+    p.cu[r + 1] = s_cu[r + 1];
+  }
+  if (me == 0) {
+    p.cu[0] = 0;
+    *p.n_free_out = (int32_t)(avail - s_taken);
+  }
+  // 3. slots and positions, a token per thread; a token that opens a page
+  // writes its table entry
+  for (int64_t t = me; t < p.n_slots; t += all) {
+    int64_t slot = -1, pos = 0;
+    if (t < carry[0]) {
+      int lo = 0, hi = p.n_req;  // s_cu[lo] <= t < s_cu[hi]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s_cu[mid] <= t) lo = mid;
+        else hi = mid;
+      }
+      const int ctx = s_ctx[lo], rank = s_rank[lo];
+      pos = ctx + (t - s_cu[lo]);
+      if (rank >= 0) {
+        const int pg = (int)(pos / p.page), off = (int)(pos % p.page);
+        const int have = ceil_div(ctx, p.page);
+        int32_t *entry = p.tables + (int64_t)lo * p.max_pages + pg;
+        int page;
+        if (pg < have) {
+          page = __ldcg(entry);
+        } else {
+          page = __ldcg(p.free_pages + (avail - 1 - rank - (pg - have)));
+          if (off == 0) *entry = page;
+        }
+        slot = (int64_t)page * p.page + off;
+      }
+    }
+    p.slots[t] = slot;
+    p.positions[t] = pos;
+  }
+}
+
+// A warp per row: its 2 * hkv * d / 8 16-byte vectors, keys then values.
+template <int D>
+__global__ void __launch_bounds__(256)
+    paged_append_kernel(const uint4 *__restrict__ k_new, const uint4 *__restrict__ v_new,
+                        int64_t row_vecs, const int64_t *__restrict__ slot_map, int64_t n_map,
+                        const int32_t *__restrict__ row_ids, const int32_t *__restrict__ n_dev,
+                        int64_t n_rows, int hkv, uint4 *__restrict__ kc, uint4 *__restrict__ vc,
+                        int64_t n_pages, int page, int32_t *err) {
+  constexpr int kVecs = D / 8;  // 16-byte vectors of a head
+  const int lane = threadIdx.x & 31;
+  int64_t live = n_rows;
+  if (n_dev) live = min((int64_t)max(__ldg(n_dev), 0), n_rows);
+  const int64_t warps = (int64_t)gridDim.x * (blockDim.x / 32);
+  for (int64_t i = (int64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5); i < live;
+       i += warps) {
+    const int64_t m = row_ids ? (int64_t)__ldg(row_ids + i) : i;
+    if (m < 0 || m >= n_map) {
+      if (lane == 0) raise_error(err, TIDE_DEVERR_POSITION);
+      continue;
+    }
+    const int64_t slot = __ldg(slot_map + m);
+    if (slot == -1) continue;
+    const int64_t pg = slot / page;
+    if (slot < 0 || pg >= n_pages) {
+      if (lane == 0) raise_error(err, TIDE_DEVERR_POSITION);
+      continue;
+    }
+    const int64_t dst = (pg * hkv * page + slot % page) * kVecs;  // head 0
+    const int64_t head = (int64_t)page * kVecs;
+    const int n = hkv * kVecs;
+    for (int e = lane; e < n; e += 32) {
+      const int64_t to = dst + (e / kVecs) * head + e % kVecs;
+      const uint4 zero = make_uint4(0, 0, 0, 0);
+      const uint4 a = k_new ? k_new[i * row_vecs + e] : zero;
+      const uint4 b = v_new ? v_new[i * row_vecs + e] : zero;
+      kc[to] = a;
+      vc[to] = b;
+    }
+  }
+}
+
+}  // namespace pages
+}  // namespace tide
+
+namespace {
+
+int fail(int code, const char *msg) {
+  tide::set_last_error(msg);
+  return code;
+}
+
+int report(cudaError_t e, const char *what) {
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e == cudaSuccess) return TIDE_OK;
+  char buf[256];
+  snprintf(buf, sizeof(buf), "%s: %s", what, cudaGetErrorString(e));
+  return fail(TIDE_ERR_CUDA, buf);
+}
+
+}  // namespace
+
+extern "C" int tide_page_tables(const int32_t *context_lens, const int32_t *new_lens,
+                                const int32_t *done, int64_t n_requests, int32_t *free_pages,
+                                const int32_t *n_free, int64_t n_pages, int32_t *block_tables,
+                                int64_t max_pages, int64_t page_size, int32_t *n_free_out,
+                                int32_t *kv_lens, int32_t *cu_seqlens, int64_t *slot_map,
+                                int64_t *positions, int64_t n_slots, int32_t *error_word,
+                                tide_stream_t stream) {
+  using namespace tide::pages;
+  if (n_requests < 1 || n_requests > kMaxRequests)
+    return fail(TIDE_ERR_INVALID, "page_tables: n_requests must be 1..8192");
+  if (n_pages < 1 || n_pages > INT32_MAX || max_pages < 1 || page_size < 1 ||
+      max_pages > INT32_MAX / page_size || max_pages > INT32_MAX / n_requests || n_slots < 0 ||
+      n_slots > INT32_MAX)
+    return fail(TIDE_ERR_INVALID, "page_tables: bad sizes (pages, table width, slots)");
+  if (!context_lens || !new_lens || !free_pages || !n_free || !block_tables || !n_free_out ||
+      !kv_lens || !cu_seqlens || (n_slots && (!slot_map || !positions)))
+    return fail(TIDE_ERR_INVALID, "page_tables: NULL pointer");
+  Params p{context_lens, new_lens,  done,       (int)n_requests, free_pages, n_free,
+           (int)n_pages, block_tables, max_pages, (int)page_size,  n_free_out, kv_lens,
+           cu_seqlens,   slot_map,  positions,  n_slots,         error_word};
+  const size_t smem = (4 * (size_t)n_requests + 1) * sizeof(int32_t);
+  cudaError_t e = cudaFuncSetAttribute(page_tables_kernel,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)((4 * (size_t)kMaxRequests + 1) * sizeof(int32_t)));
+  if (e != cudaSuccess) return report(e, "page_tables");
+  const unsigned ctas = n_slots >= kClusterTokens ? kClusterCtas : 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas, 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = (cudaStream_t)stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return report(cudaLaunchKernelEx(&cfg, page_tables_kernel, p), "page_tables");
+}
+
+extern "C" int tide_paged_append(int dtype, const void *k_new, const void *v_new,
+                                 int64_t kv_row_stride, const int64_t *slot_map,
+                                 int64_t n_slot_map, const int32_t *row_ids,
+                                 const int32_t *n_rows_dev, int64_t n_rows, int64_t n_kv_heads,
+                                 int64_t head_dim, void *k_cache, void *v_cache, int64_t n_pages,
+                                 int64_t page_size, int32_t *error_word, tide_stream_t stream) {
+  using namespace tide::pages;
+  if (dtype != TIDE_DTYPE_BF16 && dtype != TIDE_DTYPE_F16)
+    return fail(TIDE_ERR_UNSUPPORTED, "paged_append: dtype must be bf16 or fp16");
+  if (head_dim != 64 && head_dim != 128)
+    return fail(TIDE_ERR_UNSUPPORTED, "paged_append: head_dim must be 64 or 128");
+  const int64_t width = n_kv_heads * head_dim;
+  if (kv_row_stride == 0) kv_row_stride = width;
+  if (n_rows < 0 || n_kv_heads < 1 || n_kv_heads > 65536 || kv_row_stride < width ||
+      kv_row_stride % 8 || n_pages < 1 || page_size < 1 || page_size > INT32_MAX ||
+      n_slot_map < 0 || (!row_ids && n_slot_map < n_rows))
+    return fail(TIDE_ERR_INVALID, "paged_append: bad sizes (rows, heads, stride, pages, slot map)");
+  if (n_rows == 0) return TIDE_OK;
+  if (!slot_map || !k_cache || !v_cache || (!k_new != !v_new))
+    return fail(TIDE_ERR_INVALID, "paged_append: NULL pointer");
+  if (((uintptr_t)k_new | (uintptr_t)v_new | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15)
+    return fail(TIDE_ERR_ALIGNMENT, "paged_append: rows and caches must be 16-byte aligned");
+  int64_t blocks = (n_rows + 7) / 8;
+  if (blocks > 148 * 32) blocks = 148 * 32;
+  cudaStream_t s = (cudaStream_t)stream;
+  auto kern = head_dim == 128 ? paged_append_kernel<128> : paged_append_kernel<64>;
+  kern<<<(unsigned)blocks, 256, 0, s>>>(
+      static_cast<const uint4 *>(k_new), static_cast<const uint4 *>(v_new), kv_row_stride / 8,
+      slot_map, n_slot_map, row_ids, n_rows_dev, n_rows, (int)n_kv_heads,
+      static_cast<uint4 *>(k_cache), static_cast<uint4 *>(v_cache), n_pages, (int)page_size,
+      error_word);
+  return report(cudaSuccess, "paged_append");
+}

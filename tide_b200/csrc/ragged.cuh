@@ -1,0 +1,91 @@
+// Ragged batches: which rows and keys each packed sequence has.  Shared by
+// the attention kernels over packed sequences and over a paged cache.
+#pragma once
+
+#include "common.cuh"
+
+namespace tide {
+
+struct RaggedBatch {
+  const int32_t *cu;       // [n_seqs + 1] packed offsets; NULL: one row per sequence
+  const int32_t *seq_ids;  // [n_seqs] request of each sequence; NULL: itself
+  const int32_t *kv_lens;  // [n_requests]; NULL: a sequence's keys are its own rows
+  const int32_t *n_dev;    // live sequence count, or NULL
+  int n_seqs;
+  int n_requests;
+  int n_tokens;
+  int max_kv;
+  int32_t *err;
+};
+
+struct Sequence {
+  int row0;  // first packed row
+  int n;     // rows (0: nothing to do)
+  int kv;    // keys that the last row sees
+  int req;   // request (row of the block table)
+};
+
+__device__ __forceinline__ int live_sequences(const RaggedBatch &b) {
+  if (!b.n_dev) return b.n_seqs;
+  const int n = __ldg(b.n_dev);
+  if (n > b.n_seqs) raise_error(b.err, TIDE_DEVERR_COUNT);
+  return min(max(n, 0), b.n_seqs);
+}
+
+// Sequence i of the batch; one with bad bounds, request or length is empty
+// and raises TIDE_DEVERR_POSITION.
+__device__ __forceinline__ Sequence sequence(const RaggedBatch &b, int i) {
+  Sequence s;
+  s.row0 = i;
+  s.n = 1;
+  if (b.cu) {
+    s.row0 = __ldg(b.cu + i);
+    const int end = __ldg(b.cu + i + 1);
+    s.n = end - s.row0;
+    if (s.row0 < 0 || end < s.row0 || end > b.n_tokens) {
+      raise_error(b.err, TIDE_DEVERR_POSITION);
+      s.n = 0;
+      s.row0 = 0;
+    }
+  }
+  s.req = i;
+  s.kv = s.n;
+  if (s.n && b.kv_lens) {
+    if (b.seq_ids) s.req = __ldg(b.seq_ids + i);
+    const bool known = s.req >= 0 && s.req < b.n_requests;
+    s.kv = known ? __ldg(b.kv_lens + s.req) : -1;
+    if (s.kv < 0 || s.kv > b.max_kv) {
+      raise_error(b.err, TIDE_DEVERR_POSITION);
+      s.n = s.kv = 0;
+    }
+  }
+  return s;
+}
+
+// The sequence that holds packed row `row`, or -1: the last one whose start
+// is at or before it (a scan, so that offsets out of order cannot hide one).
+__device__ __forceinline__ int sequence_of_row(const RaggedBatch &b, int live, int row) {
+  if (!b.cu) return row < live ? row : -1;
+  int lo = 0, hi = live;  // cu[lo] <= row < cu[hi], if sorted
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (__ldg(b.cu + mid) <= row) lo = mid;
+    else hi = mid;
+  }
+  if (lo >= live) return -1;
+  return __ldg(b.cu + lo) <= row && row < __ldg(b.cu + lo + 1) ? lo : -1;
+}
+
+// Where the keys are: rows of a packed tensor, or pages.
+struct KeySource {
+  const void *k, *v;
+  int64_t row_stride;      // packed: elements between rows
+  const int32_t *tables;   // paged: block tables [n_requests, max_pages]
+  int64_t max_pages;
+  int n_pages;
+  int page_shift;          // log2(page_size)
+};
+
+void set_last_error(const char *msg);
+
+}  // namespace tide

@@ -582,6 +582,162 @@ void silu_mul(const at::Tensor &gate, const at::Tensor &up, const at::Tensor &ou
                               cur_stream(gate)));
 }
 
+// ---- ragged batches over a paged cache ----------------------------------
+
+// An optional int32 device tensor of at least n elements.
+const int32_t *opt_i32(const std::optional<at::Tensor> &t, const char *name, int64_t n,
+                       const at::Device &dev) {
+  if (!t.has_value() || !t->defined()) return nullptr;
+  check_cuda_contig(*t, name);
+  TORCH_CHECK(t->device() == dev, name, " must be on the device of the rows");
+  TORCH_CHECK(t->scalar_type() == at::kInt && t->numel() >= n, name, " must be int32 with at least ", n,
+              " entries");
+  return t->data_ptr<int32_t>();
+}
+int32_t *i32(const at::Tensor &t, const char *name, int64_t n, const at::Device &dev) {
+  return const_cast<int32_t *>(opt_i32(t, name, n, dev));
+}
+
+// [n, heads, d] rows whose heads are packed; returns the row stride.
+int64_t packed_heads(const at::Tensor &t, const char *name) {
+  TORCH_CHECK(t.is_cuda() && t.dim() == 3, name, " must be a CUDA tensor [n, heads, d]");
+  TORCH_CHECK((t.size(2) <= 1 || t.stride(2) == 1) && (t.size(1) <= 1 || t.stride(1) == t.size(2)),
+              name, ": heads must be packed in each row");
+  return t.size(0) <= 1 ? t.size(1) * t.size(2) : t.stride(0);
+}
+
+void check_paged_caches(const at::Tensor &k_cache, const at::Tensor &v_cache, int64_t hkv, int64_t d,
+                        at::ScalarType dt, const at::Device &dev) {
+  check_cuda_contig(k_cache, "k_cache");
+  check_cuda_contig(v_cache, "v_cache");
+  TORCH_CHECK(k_cache.device() == dev && v_cache.device() == dev, "rows and caches must share a device");
+  TORCH_CHECK(k_cache.dim() == 4 && v_cache.sizes() == k_cache.sizes() && k_cache.size(3) == d &&
+              (hkv < 0 || k_cache.size(1) == hkv), "caches must be [n_pages, kv_heads, page_size, head_dim]");
+  TORCH_CHECK(k_cache.scalar_type() == dt && v_cache.scalar_type() == dt, "rows and caches must share a dtype");
+}
+
+void check_out(const at::Tensor &out, const at::Tensor &q) {
+  check_cuda_contig(out, "out");
+  TORCH_CHECK(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() &&
+              out.device() == q.device(), "out must be like q");
+}
+
+void packed_attention(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v,
+                      const at::Tensor &cu_seqlens, const std::optional<at::Tensor> &zero_keys,
+                      const at::Tensor &out, double scale,
+                      const std::optional<at::Tensor> &error_word) {
+  const int64_t qs = packed_heads(q, "q"), ks = packed_heads(k, "k"), vs = packed_heads(v, "v");
+  TORCH_CHECK(v.sizes() == k.sizes() && k.size(0) == q.size(0) && k.size(2) == q.size(2),
+              "q [n, hq, d], k and v [n, hkv, d]");
+  TORCH_CHECK(ks == vs, "k and v must share a row stride");
+  TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type() &&
+              k.device() == q.device() && v.device() == q.device(), "q, k and v must share dtype and device");
+  check_out(out, q);
+  TORCH_CHECK(cu_seqlens.numel() >= 1, "cu_seqlens must hold n_seqs + 1 offsets");
+  const int32_t *cu = i32(cu_seqlens, "cu_seqlens", 1, q.device());
+  const int32_t *z = opt_i32(zero_keys, "zero_keys", q.size(0), q.device());
+  const int32_t *err = opt_i32(error_word, "error_word", 1, q.device());
+  const c10::cuda::CUDAGuard guard(q.device());
+  TIDE_CHECK_OK(tide_packed_attention(to_dtype(q.scalar_type(), "packed_attention"), q.data_ptr(),
+                                      k.data_ptr(), v.data_ptr(), qs, ks, cu, cu_seqlens.numel() - 1,
+                                      z, out.data_ptr(), q.size(0), q.size(1), k.size(1), q.size(2),
+                                      (float)scale, const_cast<int32_t *>(err), cur_stream(q)));
+}
+
+void paged_attention(const at::Tensor &q, const at::Tensor &k_cache, const at::Tensor &v_cache,
+                     const at::Tensor &block_tables, const at::Tensor &kv_lens,
+                     const std::optional<at::Tensor> &cu_seqlens,
+                     const std::optional<at::Tensor> &seq_ids, const at::Tensor &out,
+                     int64_t max_kv_len, double scale, const std::optional<at::Tensor> &error_word,
+                     const std::optional<at::Tensor> &n_seqs_dev) {
+  const int64_t qs = packed_heads(q, "q");
+  const auto dev = q.device();
+  check_paged_caches(k_cache, v_cache, -1, q.size(2), q.scalar_type(), dev);
+  check_out(out, q);
+  TORCH_CHECK(block_tables.dim() == 2, "block_tables must be [n_requests, max_pages]");
+  const int32_t *bt = i32(block_tables, "block_tables", 0, dev);
+  const int64_t n_req = std::min(block_tables.size(0), kv_lens.numel());
+  const int32_t *lens = i32(kv_lens, "kv_lens", 0, dev);
+  const int32_t *cu = opt_i32(cu_seqlens, "cu_seqlens", 1, dev);
+  const int64_t n_seqs = cu ? cu_seqlens->numel() - 1 : q.size(0);
+  const int32_t *ids = opt_i32(seq_ids, "seq_ids", n_seqs, dev);
+  const int32_t *live = opt_i32(n_seqs_dev, "n_seqs_dev", 1, dev);
+  const int32_t *err = opt_i32(error_word, "error_word", 1, dev);
+  const c10::cuda::CUDAGuard guard(dev);
+  const int64_t need = (int64_t)tide_paged_attention_workspace_size(
+      q.size(0), n_seqs, q.size(1), k_cache.size(1), q.size(2), max_kv_len);
+  at::Tensor ws;  // of the current stream's allocator, so of this call alone
+  if (need) ws = at::empty({need}, q.options().dtype(at::kByte));
+  TIDE_CHECK_OK(tide_paged_attention(
+      to_dtype(q.scalar_type(), "paged_attention"), q.data_ptr(), qs, k_cache.data_ptr(),
+      v_cache.data_ptr(), k_cache.size(0), k_cache.size(2), bt, block_tables.size(1), n_req, lens, cu,
+      ids, n_seqs, live, out.data_ptr(), q.size(0), q.size(1), k_cache.size(1), q.size(2), max_kv_len,
+      (float)scale, need ? ws.data_ptr() : nullptr, (size_t)need, const_cast<int32_t *>(err),
+      cur_stream(q)));
+}
+
+void paged_append(const std::optional<at::Tensor> &k_new, const std::optional<at::Tensor> &v_new,
+                  const at::Tensor &slot_map, const std::optional<at::Tensor> &row_ids,
+                  const std::optional<at::Tensor> &n_rows_dev, const at::Tensor &k_cache,
+                  const at::Tensor &v_cache, const std::optional<at::Tensor> &error_word) {
+  const auto dev = k_cache.device();
+  check_paged_caches(k_cache, v_cache, -1, k_cache.dim() == 4 ? k_cache.size(3) : 0,
+                     k_cache.scalar_type(), dev);
+  check_cuda_contig(slot_map, "slot_map");
+  TORCH_CHECK(slot_map.scalar_type() == at::kLong && slot_map.device() == dev, "slot_map must be int64");
+  const bool rows = k_new.has_value() && k_new->defined();
+  TORCH_CHECK(rows == (v_new.has_value() && v_new->defined()), "k_new and v_new: both or neither");
+  int64_t n = row_ids.has_value() && row_ids->defined() ? row_ids->numel() : slot_map.numel(), stride = 0;
+  if (rows) {
+    stride = packed_heads(*k_new, "k_new");
+    TORCH_CHECK(packed_heads(*v_new, "v_new") == stride, "k_new and v_new must share a row stride");
+    TORCH_CHECK(v_new->sizes() == k_new->sizes() && k_new->size(1) == k_cache.size(1) &&
+                k_new->size(2) == k_cache.size(3), "k_new, v_new must be [n, kv_heads, d]");
+    TORCH_CHECK(k_new->scalar_type() == k_cache.scalar_type() && v_new->scalar_type() == k_cache.scalar_type() &&
+                k_new->device() == dev && v_new->device() == dev, "new rows and caches must share dtype and device");
+    n = k_new->size(0);
+  }
+  const int32_t *ids = opt_i32(row_ids, "row_ids", n, dev);
+  const int32_t *live = opt_i32(n_rows_dev, "n_rows_dev", 1, dev);
+  const int32_t *err = opt_i32(error_word, "error_word", 1, dev);
+  const c10::cuda::CUDAGuard guard(dev);
+  TIDE_CHECK_OK(tide_paged_append(
+      to_dtype(k_cache.scalar_type(), "paged_append"), opt_ptr(k_new), opt_ptr(v_new), stride,
+      slot_map.data_ptr<int64_t>(), slot_map.numel(), ids, live, n, k_cache.size(1), k_cache.size(3),
+      k_cache.data_ptr(), v_cache.data_ptr(), k_cache.size(0), k_cache.size(2),
+      const_cast<int32_t *>(err), cur_stream(k_cache)));
+}
+
+void page_tables(const at::Tensor &context_lens, const at::Tensor &new_lens,
+                 const std::optional<at::Tensor> &done, const at::Tensor &free_pages,
+                 const at::Tensor &n_free, const at::Tensor &block_tables, int64_t page_size,
+                 const at::Tensor &n_free_out, const at::Tensor &kv_lens, const at::Tensor &cu_seqlens,
+                 const at::Tensor &slot_map, const at::Tensor &positions,
+                 const std::optional<at::Tensor> &error_word) {
+  TORCH_CHECK(context_lens.is_cuda(), "context_lens must be a CUDA tensor");
+  const auto dev = context_lens.device();
+  const int64_t n = context_lens.numel();
+  TORCH_CHECK(block_tables.dim() == 2 && block_tables.size(0) >= n, "block_tables must be [n_requests, max_pages]");
+  for (const auto *t : {&slot_map, &positions}) {
+    check_cuda_contig(*t, "slot_map/positions");
+    TORCH_CHECK(t->scalar_type() == at::kLong && t->numel() == slot_map.numel() && t->device() == dev,
+                "slot_map and positions must be int64 of one length");
+  }
+  const int32_t *ctx = i32(context_lens, "context_lens", n, dev), *add = i32(new_lens, "new_lens", n, dev);
+  const int32_t *gone = opt_i32(done, "done", n, dev);
+  int32_t *pool = i32(free_pages, "free_pages", 1, dev);
+  const int32_t *count = i32(n_free, "n_free", 1, dev);
+  int32_t *bt = i32(block_tables, "block_tables", 0, dev);
+  int32_t *count_out = i32(n_free_out, "n_free_out", 1, dev);
+  int32_t *lens = i32(kv_lens, "kv_lens", n, dev), *cu = i32(cu_seqlens, "cu_seqlens", n + 1, dev);
+  const int32_t *err = opt_i32(error_word, "error_word", 1, dev);
+  const c10::cuda::CUDAGuard guard(dev);
+  TIDE_CHECK_OK(tide_page_tables(ctx, add, gone, n, pool, count, free_pages.numel(), bt,
+                                 block_tables.size(1), page_size, count_out, lens, cu,
+                                 slot_map.data_ptr<int64_t>(), positions.data_ptr<int64_t>(),
+                                 slot_map.numel(), const_cast<int32_t *>(err), cur_stream(context_lens)));
+}
+
 // ---- router fold and fused checkpoint ----------------------------------
 
 std::vector<at::Tensor> router_fold(const at::Tensor &down, const at::Tensor &norm_weight,
@@ -747,6 +903,17 @@ TORCH_LIBRARY(tide, m) {
   m.def("silu_mul(Tensor gate, Tensor up, Tensor(a!) out, Tensor? n_rows_dev=None) -> ()");
   m.def("kv_append(Tensor k_new, Tensor v_new, Tensor? slots, Tensor? n_rows_dev, Tensor(a!) k_cache, "
         "Tensor(b!) v_cache, int position, Tensor? position_dev, Tensor(c!)? error_word) -> ()");
+  m.def("packed_attention(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens, Tensor? zero_keys, "
+        "Tensor(a!) out, float scale, Tensor(b!)? error_word) -> ()");
+  m.def("paged_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, "
+        "Tensor kv_lens, Tensor? cu_seqlens, Tensor? seq_ids, Tensor(a!) out, int max_kv_len, "
+        "float scale, Tensor(b!)? error_word, Tensor? n_seqs_dev=None) -> ()");
+  m.def("paged_append(Tensor? k_new, Tensor? v_new, Tensor slot_map, Tensor? row_ids, "
+        "Tensor? n_rows_dev, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!)? error_word) -> ()");
+  m.def("page_tables(Tensor context_lens, Tensor new_lens, Tensor? done, Tensor(a!) free_pages, "
+        "Tensor n_free, Tensor(b!) block_tables, int page_size, Tensor(c!) n_free_out, "
+        "Tensor(d!) kv_lens, Tensor(e!) cu_seqlens, Tensor(f!) slot_map, Tensor(g!) positions, "
+        "Tensor(h!)? error_word) -> ()");
   m.def("router_fold(Tensor down, Tensor norm_weight, Tensor? norm_bias, ScalarType fold_dtype) "
         "-> Tensor[]");
   m.def("checkpoint_workspace_size(int n_rows, int hidden_dim) -> int", &checkpoint_workspace_size);
@@ -774,6 +941,10 @@ TORCH_LIBRARY_IMPL(tide, CUDA, m) {
   m.impl("rms_norm", &rms_norm);
   m.impl("qk_norm_rope", &qk_norm_rope);
   m.impl("silu_mul", &silu_mul);
+  m.impl("packed_attention", &packed_attention);
+  m.impl("paged_attention", &paged_attention);
+  m.impl("paged_append", &paged_append);
+  m.impl("page_tables", &page_tables);
   m.impl("router_fold", &router_fold);
   m.impl("checkpoint", &checkpoint);
 }
