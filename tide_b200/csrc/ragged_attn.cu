@@ -1,88 +1,794 @@
 // Attention over ragged batches: causal attention within packed sequences,
-// and of new tokens over a paged cache.
+// and of chunks of new tokens over a paged cache.
 //
 //   o[i, h] = sum_j e^(s_ij) v[j, h / G] / (z_i + sum_j e^(s_ij)),
 //   s_ij = scale * q[i, h] . k[j, h / G],
-// j over the keys that row i sees, z_i its zero keys.  One pass over the keys
-// with a running maximum m, sum l and unnormalised output, fp32 throughout.
+// j over the keys that row i sees, z_i its zero keys.
 //
-// A warp per (row, query head), its lanes over the head dimension.
+// A tile is 128 rows: floor(128 / G) consecutive tokens of a sequence times
+// the G query heads of one KV head, so that a key or value loaded serves all
+// heads that share it.  A unit of work is two such tiles, one behind the
+// other; a persistent CTA per SM walks over units.  Per block of 128 keys and
+// tile,
+//   S[128 x 128] = Q K^T      tcgen05.mma, operands in shared memory (TMA,
+//                             128-byte swizzle), S in tensor memory;
+//   P = 2^(S qs - m)          one thread per row: running maximum m and sum l,
+//                             P rounded to the rows' 16-bit type (half a step
+//                             of it relative per weight; the sum l is of the
+//                             unrounded ones) and written over S;
+//   O[128 x D] += P V         tcgen05.mma with P from tensor memory and V as
+//                             it lies in shared memory (its MN-major operand).
+// The tensor core and the two tiles' softmax warps alternate: while one
+// tile's scores go through the exponential, the other's products run.
+//
+// m is only raised, and O and l rescaled, when a row's maximum has grown by
+// more than 2^8 since: weights up to 256 cost nothing (fp32 sums; 16-bit
+// floats round relatively), and O stays where it is.  The rescale needs no
+// synchronisation of its own: the commit that publishes S_j comes after the
+// product that used P_j-1 in the same instruction stream, so O is complete
+// when S_j is.
+//
+// Roles of the 12 warps: 0-3 and 4-7 the softmax and the output of tile 0
+// and 1; 8 finds the units; 9 loads; 10 issues the products; 11 cleans the
+// value blocks that not every row sees: a masked weight is 0, but 0 * NaN is
+// not, so rows past the last visible key are zeroed, and a value that is not
+// finite at a position that only the later rows see is zeroed, noted, and
+// added to the outputs of the rows that do see it.
+//
+// Order of units: by the number of keys they read, most first (the level of a
+// unit: positions before its end, in units of its size), so that the last
+// ones to start are short.  A sequence's level range and the rank within a
+// level come from counting over the sequences, so no list of units is built.
+//
+// Long contexts with few rows are split over the keys (paged caches only):
+// the splits' unnormalised outputs, maxima and sums go to the workspace and
+// combine_kernel joins them, in a fixed order.
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <math.h>
 #include <stdio.h>
 
+#include <atomic>
+#include <type_traits>
+
 #include "ragged.cuh"
+#include "tc_ptx.cuh"
 
 namespace tide {
 namespace ragged {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kRows = 128;   // rows of a tile
+constexpr int kKeys = 128;   // keys of a block
+constexpr int kThreads = 384;
+constexpr int kCached = 4;   // sequences per lane that the unit search keeps in registers
+constexpr float kSlack = 8.f;  // log2 of how far a maximum may grow before a rescale
+
+template <int D>
+struct Shape {
+  static constexpr int kHalves = D / 64;               // 128-byte column groups
+  static constexpr uint32_t kTile = kRows * D * 2;     // bytes of a Q tile or a K or V block
+  static constexpr uint32_t kHalf = kRows * 128;       // bytes of one column group of it
+  static constexpr int kStages = D == 128 ? 5 : 10;    // K and V blocks in flight
+  static constexpr uint32_t kSmem = (2 + kStages) * kTile + 1024;  // + alignment
+};
 
 struct Params {
   RaggedBatch batch;
   KeySource src;
-  const void *q;
-  int64_t q_stride;
   const int32_t *zero_keys;
   void *out;
+  float *part_o;   // [splits, n_tokens, hq, D] (splits > 1)
+  float2 *part_ml; // [splits, n_tokens, hq]: maximum (scaled, base 2), sum
   int hq, hkv;
-  float qs;  // scale * log2(e)
+  int group;       // query heads per KV head
+  int tokens;      // of a tile: kRows / group
+  int splits;
+  int split_blocks;  // key blocks of a split
+  float qs;        // scale * log2(e)
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(256) row_attention_kernel(Params p) {
-  constexpr int kE = D / 32;  // elements per lane
-  const int row = blockIdx.x, lane = threadIdx.x & 31;
-  const int live = live_sequences(p.batch);
-  if (row == 0)  // a bad sequence is reported although no row finds it
-    for (int i = threadIdx.x; i < live; i += blockDim.x) sequence(p.batch, i);
-  const int i = sequence_of_row(p.batch, live, row);
-  if (i < 0) return;
+// One unit: up to 2 * tokens tokens of a sequence, one KV head, key blocks
+// [b0, b1).
+struct Unit {
+  int valid;
+  int row0;   // packed row of the first token
+  int n;      // tokens
+  int pos0;   // keys before the first token's own (it sees pos0 + 1)
+  int kvh;
+  int req;    // row of the block table
+  int key0;   // packed: row of the sequence's first key
+  int b0, b1;
+  int split;
+};
+
+// Tokens of tile t of the unit, and the end of its key blocks (b0 if none).
+__device__ __forceinline__ int tile_tokens(const Unit &u, int tokens, int t) {
+  return min(max(u.n - t * tokens, 0), tokens);
+}
+__device__ __forceinline__ int tile_sees(const Unit &u, int tokens, int t) {
+  return u.pos0 + t * tokens + tile_tokens(u, tokens, t);  // keys its last token sees
+}
+__device__ __forceinline__ int tile_end(const Unit &u, int tokens, int t) {
+  if (tile_tokens(u, tokens, t) == 0) return u.b0;
+  const int sees = max(tile_sees(u, tokens, t), 0);
+  return max(u.b0, min(u.b1, (sees + kKeys - 1) / kKeys));
+}
+
+// The rows [from, to) of value block j that the cleaner goes over: those past
+// the first token's own position, up to the last key that some token of the
+// unit sees, rounded up to the 16 keys that a product reads.
+__device__ __forceinline__ bool cleaned_rows(const Unit &u, int sees, int j, int *from, int *to) {
+  *from = max(0, u.pos0 + 1 - j * kKeys);
+  *to = (min(kKeys, sees - j * kKeys) + 15) / 16 * 16;
+  return *from < *to;
+}
+
+struct Shared {
+  uint64_t q_full[2], q_empty[2];
+  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t u_full[2], u_empty[2];
+  uint64_t drain;
+  uint64_t kv_full[10], kv_empty[10];
+  uint64_t raw_full[10];  // value blocks that have landed and are to be cleaned, in turn
+  Unit unit[2];
+  int odd[4];       // per unit (by its number mod 4): a value of the cleaned range is not finite
+  uint32_t tmem;
+  int abort;
+  // requested so far, for the wait after an abort
+  int loaded, raw_loaded, q_loaded[2];
+  int raw[10];      // whether a stage's last copy completes on raw_full
+};
+
+// Bounded wait of a whole warp; when it runs out the warp's role ends, and
+// with it, by sh.abort, every other.
+#define TIDE_WAIT(bar, parity)                                                         \
+  do {                                                                                 \
+    if (!__all_sync(0xffffffffu, ptx::mbar_wait((bar), (parity), &sh.abort))) {        \
+      sh.abort = 1;                                                                    \
+      raise_error(p.batch.err, TIDE_DEVERR_TIMEOUT);                                   \
+      return;                                                                          \
+    }                                                                                  \
+  } while (0)
+
+// ------------------------------------------------------------------ units
+__device__ __forceinline__ void seq_level(const Params &p, int i, int *count, int *level) {
   const Sequence s = sequence(p.batch, i);
-  if (!s.n) return;
-  const int sees = s.kv - s.n + (row - s.row0) + 1;
-  const int page = 1 << p.src.page_shift;
-  for (int h = threadIdx.x >> 5; h < p.hq; h += 8) {
-    const int kvh = h / (p.hq / p.hkv);
-    float qv[kE], acc[kE];
-    const T *q = static_cast<const T *>(p.q) + row * p.q_stride + (int64_t)h * D;
+  const int per = 2 * p.tokens;
+  *count = (s.n + per - 1) / per;
+  *level = max(s.kv - s.n, 0) / per;
+}
+
+__device__ void schedule_units(const Params &p, Shared &sh) {
+  constexpr unsigned kFull = 0xffffffffu;
+  const int lane = threadIdx.x & 31;
+  const int live = live_sequences(p.batch);
+  int cnt[kCached], lvl[kCached];
+  int top = 0;
 #pragma unroll
-    for (int e = 0; e < kE; ++e) {
-      qv[e] = Elem<T>::to_f(q[lane + 32 * e]) * p.qs;
-      acc[e] = 0.f;
-    }
-    const int z = p.zero_keys ? max(__ldg(p.zero_keys + row), 0) : 0;
-    float m = z ? 0.f : -INFINITY, l = (float)z;
-    for (int j = 0; j < sees; ++j) {
-      int64_t at;
-      bool real = true;
-      if (p.src.tables) {
-        const int pg = __ldg(p.src.tables + s.req * p.src.max_pages + (j >> p.src.page_shift));
-        real = pg >= 0 && pg < p.src.n_pages;
-        if (!real) {
-          if (lane == 0) raise_error(p.batch.err, TIDE_DEVERR_POSITION);
-        }
-        at = (((int64_t)pg * p.hkv + kvh) * page + (j & (page - 1))) * D;
-      } else {
-        at = (s.row0 + j) * p.src.row_stride + (int64_t)kvh * D;
-      }
-      const T *k = static_cast<const T *>(p.src.k) + at, *v = static_cast<const T *>(p.src.v) + at;
-      float dot = 0.f;
-#pragma unroll
-      for (int e = 0; e < kE; ++e)
-        if (real) dot = fmaf(qv[e], Elem<T>::to_f(k[lane + 32 * e]), dot);
-      dot = warp_sum(dot);
-      const float m1 = fmaxf(m, dot), a = exp2f(m - m1), w = exp2f(dot - m1);
-      l = l * a + w;
-#pragma unroll
-      for (int e = 0; e < kE; ++e)
-        acc[e] = fmaf(acc[e], a, real ? w * Elem<T>::to_f(v[lane + 32 * e]) : 0.f);
-      m = m1;
-    }
-    T *o = static_cast<T *>(p.out) + ((int64_t)row * p.hq + h) * D;
-    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // a NaN stays one
-#pragma unroll
-    for (int e = 0; e < kE; ++e) o[lane + 32 * e] = Elem<T>::from_f(acc[e] * inv);
+  for (int k = 0; k < kCached; ++k) {
+    cnt[k] = lvl[k] = 0;
+    if (lane + 32 * k < live) seq_level(p, lane + 32 * k, &cnt[k], &lvl[k]);
+    top = max(top, cnt[k] + lvl[k]);
   }
+  for (int i = lane + 32 * kCached; i < live; i += 32) {
+    int c, l;
+    seq_level(p, i, &c, &l);
+    top = max(top, c + l);
+  }
+  top = __reduce_max_sync(kFull, top);
+  auto units_from = [&](int x) {  // units of level x and above
+    int c = 0;
+#pragma unroll
+    for (int k = 0; k < kCached; ++k) c += min(max(cnt[k] + lvl[k] - x, 0), cnt[k]);
+    for (int i = lane + 32 * kCached; i < live; i += 32) {
+      int n, l;
+      seq_level(p, i, &n, &l);
+      c += min(max(n + l - x, 0), n);
+    }
+    return (int)__reduce_add_sync(kFull, (unsigned)c);
+  };
+  const int total = units_from(0);
+  const int per_rank = p.hkv * p.splits;
+  int x = top, above = 0, upto = 0;  // level, units above it, units of it and above
+  uint32_t n = 0;
+  for (int64_t u = blockIdx.x;; u += gridDim.x, ++n) {
+    const int slot = n & 1;
+    const int64_t rank = u / per_rank;
+    Unit w{};
+    if (rank < total) {
+      if (rank >= upto) {  // units_from(lo) > rank >= units_from(hi)
+        int lo = 0, hi = x;
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (units_from(mid) > rank) lo = mid;
+          else hi = mid;
+        }
+        x = lo;
+        upto = units_from(lo);
+        above = units_from(hi);
+      }
+      int r = (int)rank - above;  // the r-th sequence with a unit of level x
+      int seq = -1, level = 0;
+#pragma unroll
+      for (int k = 0; k < kCached; ++k) {
+        const bool has = lvl[k] <= x && x < lvl[k] + cnt[k];
+        const unsigned who = __ballot_sync(kFull, has);
+        if (seq < 0) {
+          if (r < __popc(who)) {
+            const bool me = has && __popc(who & ((1u << lane) - 1)) == r;
+            const int src = __ffs(__ballot_sync(kFull, me)) - 1;
+            seq = src + 32 * k;
+            level = __shfl_sync(kFull, lvl[k], src);
+          } else {
+            r -= __popc(who);
+          }
+        }
+      }
+      for (int b = 32 * kCached; seq < 0 && b < live; b += 32) {
+        int c = 0, l = 0;
+        if (b + lane < live) seq_level(p, b + lane, &c, &l);
+        const bool has = l <= x && x < l + c;
+        const unsigned who = __ballot_sync(kFull, has);
+        if (r < __popc(who)) {
+          const bool me = has && __popc(who & ((1u << lane) - 1)) == r;
+          const int src = __ffs(__ballot_sync(kFull, me)) - 1;
+          seq = src + b;
+          level = __shfl_sync(kFull, l, src);
+        } else {
+          r -= __popc(who);
+        }
+      }
+      const Sequence s = sequence(p.batch, seq);
+      const int at = (x - level) * 2 * p.tokens;
+      const int rest = (int)(u % per_rank);
+      w.valid = 1;
+      w.row0 = s.row0 + at;
+      w.n = min(2 * p.tokens, s.n - at);
+      w.pos0 = s.kv - s.n + at;
+      w.kvh = rest / p.splits;
+      w.split = rest % p.splits;
+      w.req = s.req;
+      w.key0 = s.row0;
+      w.b0 = w.split * p.split_blocks;
+      w.b1 = w.b0 + p.split_blocks;
+    }
+    if (n >= 2) TIDE_WAIT(&sh.u_empty[slot], ((n >> 1) + 1) & 1);
+    if (lane == 0) {
+      sh.unit[slot] = w;
+      ptx::mbar_arrive(&sh.u_full[slot]);
+    }
+    __syncwarp();
+    if (!w.valid) return;
+  }
+}
+
+// The next unit of a warp's role; its slot is free again once every warp has
+// read it.
+#define TIDE_NEXT_UNIT(u, n)                                          \
+  TIDE_WAIT(&sh.u_full[(n) & 1], ((n) >> 1) & 1);                     \
+  const Unit u = sh.unit[(n) & 1];                                    \
+  __syncwarp();                                                       \
+  if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&sh.u_empty[(n) & 1]); \
+  if (!u.valid) break
+
+// ---------------------------------------------------------------- loading
+template <int D, bool PAGED>
+__device__ void load_units(const Params &p, Shared &sh, unsigned char *q_smem,
+                           unsigned char *ring, const CUtensorMap *mq, const CUtensorMap *mk,
+                           const CUtensorMap *mv) {
+  using S = Shape<D>;
+  const int lane = threadIdx.x & 31;
+  uint32_t c = 0;         // K and V blocks requested so far
+  uint32_t raw = 0;       // of them to be cleaned
+  uint32_t nq[2] = {0, 0};
+  const int page = 1 << p.src.page_shift;
+  const int box = min(page, kKeys);           // rows of a copy
+  const int boxes = kKeys / box;              // copies a column group takes
+  const uint32_t q_bytes = (uint32_t)(p.tokens * p.group) * 128u * S::kHalves;
+  for (uint32_t n = 0;; ++n) {
+    TIDE_NEXT_UNIT(u, n);
+    const int e0 = tile_end(u, p.tokens, 0), e1 = tile_end(u, p.tokens, 1);
+    const int end = max(e0, e1);
+    if (end <= u.b0) continue;
+    const int sees = u.pos0 + u.n;
+    // the pages of a block, one per lane; the next block's are read ahead
+    auto page_of = [&](int j) {
+      int row = -1;
+      if (PAGED && lane < boxes && j < end && j * kKeys + lane * box < sees) {
+        const int at = j * kKeys + lane * box;
+        const int pg = __ldg(p.src.tables + u.req * p.src.max_pages + (at >> p.src.page_shift));
+        const bool real = pg >= 0 && pg < p.src.n_pages;
+        if (!real) raise_error(p.batch.err, TIDE_DEVERR_POSITION);
+        // a row past the cache's last reads as zeros
+        row = ((real ? pg : p.src.n_pages) * p.hkv + (real ? u.kvh : 0)) * page + (at & (page - 1));
+      }
+      return row;
+    };
+    auto load_q = [&](int t) {
+      if (nq[t] >= 1) TIDE_WAIT(&sh.q_empty[t], (nq[t] + 1) & 1);
+      if (lane == 0) {
+        ptx::mbar_expect_tx(&sh.q_full[t], q_bytes);
+#pragma unroll
+        for (int h = 0; h < S::kHalves; ++h)
+          ptx::tma_load_3d(q_smem + t * S::kTile + h * S::kHalf, mq, &sh.q_full[t], h * 64,
+                           u.kvh * p.group, u.row0 + t * p.tokens);
+      }
+      ++nq[t];
+      if (lane == 0) sh.q_loaded[t] = (int)nq[t];
+    };
+    int row = page_of(u.b0);
+    for (int j = u.b0; j < end; ++j) {
+      const int next = page_of(j + 1);
+      const int count = PAGED ? (min(kKeys, sees - j * kKeys) + box - 1) / box : 1;  // copies
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        const uint32_t stage = c % S::kStages, lap = c / S::kStages;
+        if (lap >= 1) TIDE_WAIT(&sh.kv_empty[stage], (lap + 1) & 1);
+        unsigned char *dst = ring + stage * S::kTile;
+        const CUtensorMap *m = kv ? mv : mk;
+        int from, to;
+        const bool dirty = kv && cleaned_rows(u, sees, j, &from, &to);
+        uint64_t *full = dirty ? &sh.raw_full[raw % S::kStages] : &sh.kv_full[stage];
+        raw += dirty;
+        if (lane == 0) {
+          ptx::mbar_expect_tx(full, PAGED ? (uint32_t)(count * box) * 128u * S::kHalves : S::kTile);
+          sh.raw[stage] = dirty;
+          sh.loaded = (int)c + 1;
+          sh.raw_loaded = (int)raw;
+        }
+        __syncwarp();
+        if (PAGED) {
+          const int r = lane / S::kHalves, h = lane % S::kHalves;
+          const int src = __shfl_sync(0xffffffffu, row, r);
+          if (r < count) ptx::tma_load_2d(dst + h * S::kHalf + r * box * 128, m, full, h * 64, src);
+        } else if (lane < S::kHalves) {
+          ptx::tma_load_3d(dst + lane * S::kHalf, m, full, lane * 64, u.kvh, u.key0 + j * kKeys);
+        }
+        ++c;
+        if (j == u.b0 && kv == 0) {
+          if (e0 > u.b0) load_q(0);
+          if (sh.abort) return;
+          if (e1 > u.b0) load_q(1);
+          if (sh.abort) return;
+        }
+      }
+      row = next;
+    }
+  }
+}
+
+// --------------------------------------------------------------- products
+template <typename T, int D>
+__device__ void issue_products(const Params &p, Shared &sh, uint32_t q_smem, uint32_t ring,
+                               uint32_t tmem) {
+  using S = Shape<D>;
+  const bool lead = (threadIdx.x & 31) == 0;
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  uint32_t c0 = 0;  // ring count of the unit's first K block
+  uint32_t nq[2] = {0, 0}, np[2] = {0, 0};
+  for (uint32_t n = 0;; ++n) {
+    TIDE_NEXT_UNIT(u, n);
+    const int end_of[2] = {tile_end(u, p.tokens, 0), tile_end(u, p.tokens, 1)};
+    const int end = max(end_of[0], end_of[1]);
+    if (end <= u.b0) continue;
+    const int sees_of[2] = {tile_sees(u, p.tokens, 0), tile_sees(u, p.tokens, 1)};
+    auto stage_of = [&](int j, int kv) { return (c0 + 2 * (j - u.b0) + kv) % S::kStages; };
+    auto lap_of = [&](int j, int kv) { return (c0 + 2 * (j - u.b0) + kv) / S::kStages; };
+    // S_t = Q_t K_j^T over the keys that tile t sees
+    auto scores = [&](int t, int j) {
+      const int cols = min(kKeys, (sees_of[t] - j * kKeys + 31) / 32 * 32);
+      const uint32_t idesc = ptx::f16_idesc(kBf16, kRows, cols);
+      const uint64_t a = ptx::sw128_kmajor_desc(q_smem + t * S::kTile);
+      const uint64_t b = ptx::sw128_kmajor_desc(ring + stage_of(j, 0) * S::kTile);
+      if (lead) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint64_t off = (k / 4) * (S::kHalf >> 4) + (k % 4) * 2;
+          ptx::mma_f16_ss(tmem + t * 256, a + off, b + off, idesc, k > 0);
+        }
+        ptx::mma_commit(&sh.s_full[t]);
+        if (j + 1 == end_of[t]) ptx::mma_commit(&sh.q_empty[t]);
+        // the last tile that reads K_j frees it
+        if (t == 1 || j >= end_of[1]) ptx::mma_commit(&sh.kv_empty[stage_of(j, 0)]);
+      }
+      __syncwarp();
+    };
+    TIDE_WAIT(&sh.kv_full[stage_of(u.b0, 0)], lap_of(u.b0, 0) & 1);
+    for (int t = 0; t < 2; ++t) {
+      if (u.b0 >= end_of[t]) continue;
+      TIDE_WAIT(&sh.q_full[t], nq[t] & 1);
+      ++nq[t];
+      ptx::tc_fence_after();
+      scores(t, u.b0);
+    }
+    for (int j = u.b0; j < end; ++j) {
+      TIDE_WAIT(&sh.kv_full[stage_of(j, 1)], lap_of(j, 1) & 1);
+      bool next_keys = false;
+      for (int t = 0; t < 2; ++t) {
+        if (j >= end_of[t]) continue;
+        TIDE_WAIT(&sh.p_full[t], np[t] & 1);
+        ++np[t];
+        ptx::tc_fence_after();
+        // O_t += P_t V_j over the keys that the tile sees, 16 at a time
+        const int steps = (min(kKeys, sees_of[t] - j * kKeys) + 15) / 16;
+        const uint32_t idesc = ptx::f16_idesc(kBf16, kRows, D) | ptx::kIdescMnMajorB;
+        const uint64_t b = ptx::sw128_mnmajor_desc(ring + stage_of(j, 1) * S::kTile, S::kHalf);
+        if (lead) {
+          for (int k = 0; k < steps; ++k)
+            ptx::mma_f16_ts(tmem + t * 256 + 128, tmem + t * 256 + k * 8, b + k * (2048 >> 4), idesc,
+                            j > u.b0 || k > 0);
+          if (t == 1 || j >= end_of[1]) ptx::mma_commit(&sh.kv_empty[stage_of(j, 1)]);
+          if (j + 1 >= end_of[t]) ptx::mma_commit(&sh.o_full[t]);
+        }
+        __syncwarp();
+        if (j + 1 < end_of[t]) {
+          if (!next_keys) TIDE_WAIT(&sh.kv_full[stage_of(j + 1, 0)], lap_of(j + 1, 0) & 1);
+          next_keys = true;
+          ptx::tc_fence_after();
+          scores(t, j + 1);
+        }
+      }
+    }
+    c0 += 2 * (end - u.b0);
+  }
+}
+
+// ---------------------------------------------------------------- cleaning
+template <typename T>
+__device__ __forceinline__ bool odd_value(uint32_t bits16) {
+  constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+  return (bits16 & kExp) == kExp;
+}
+
+template <typename T, int D>
+__device__ void clean_values(const Params &p, Shared &sh, unsigned char *ring) {
+  using S = Shape<D>;
+  const int lane = threadIdx.x & 31;
+  uint32_t c0 = 0, raw = 0;
+  for (uint32_t n = 0;; ++n) {
+    TIDE_NEXT_UNIT(u, n);
+    const int end = max(tile_end(u, p.tokens, 0), tile_end(u, p.tokens, 1));
+    if (lane == 0) sh.odd[n & 3] = 0;
+    __syncwarp();
+    if (end <= u.b0) continue;
+    const int sees = u.pos0 + u.n;
+    for (int j = u.b0; j < end; ++j) {
+      int from, to;
+      if (!cleaned_rows(u, sees, j, &from, &to)) continue;
+      const uint32_t stage = (c0 + 2 * (j - u.b0) + 1) % S::kStages;
+      TIDE_WAIT(&sh.raw_full[raw % S::kStages], (raw / S::kStages) & 1);
+      ++raw;
+      unsigned char *v = ring + stage * S::kTile;
+      const int seen = min(kKeys, sees - j * kKeys);  // rows that some token sees
+      bool odd = false;
+      // 8 16-byte vectors a row and column group; a swizzle moves them
+      // within their row only
+      for (int e = from * 8 + lane; e < to * 8; e += 32) {
+#pragma unroll
+        for (int h = 0; h < S::kHalves; ++h) {
+          uint4 *at = reinterpret_cast<uint4 *>(v + h * S::kHalf) + e;
+          uint4 x = *at;
+          uint32_t *w = reinterpret_cast<uint32_t *>(&x);
+          bool change = e >= seen * 8;
+          if (change) {
+            x = make_uint4(0, 0, 0, 0);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const bool lo = odd_value<T>(w[i]), hi = odd_value<T>(w[i] >> 16);
+              if (lo) w[i] &= 0xFFFF0000u;
+              if (hi) w[i] &= 0x0000FFFFu;
+              change |= lo | hi;
+            }
+            odd |= change;
+          }
+          if (change) *at = x;
+        }
+      }
+      if (__any_sync(0xffffffffu, odd) && lane == 0) sh.odd[n & 3] = 1;
+      ptx::fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&sh.kv_full[stage]);
+    }
+    c0 += 2 * (end - u.b0);
+  }
+}
+
+// ----------------------------------------------------------------- softmax
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __half>::value)
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// The values that the cleaner zeroed in the positions that this row sees, for
+// the columns [d0, d0 + 32): weight > 0 times a NaN or infinity is itself.
+template <typename T, int D, bool PAGED>
+__device__ __forceinline__ void add_odd_values(const Params &p, const Unit &u, int first, int last,
+                                               int d0, float *o) {
+  const T *v = static_cast<const T *>(p.src.v);
+  const int page = 1 << p.src.page_shift;
+  for (int pos = first; pos < last; ++pos) {
+    int64_t at;
+    if (PAGED) {
+      const int pg = __ldg(p.src.tables + u.req * p.src.max_pages + (pos >> p.src.page_shift));
+      if (pg < 0 || pg >= p.src.n_pages) continue;
+      at = (((int64_t)pg * p.hkv + u.kvh) * page + (pos & (page - 1))) * D;
+    } else {
+      at = (int64_t)(u.key0 + pos) * p.src.row_stride + (int64_t)u.kvh * D;
+    }
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+      const float x = Elem<T>::to_f(v[at + d0 + e]);
+      if (!isfinite(x)) o[e] += x;
+    }
+  }
+}
+
+template <typename T, int D, bool PAGED>
+__device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem) {
+  constexpr unsigned kFull = 0xffffffffu;
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) & 3;
+  const int r = warp * 32 + lane;                 // row of the tile
+  const int tok = r / p.group, head = r % p.group;
+  const uint32_t s_col = tmem + ((uint32_t)(warp * 32) << 16) + t * 256;
+  const uint32_t o_col = s_col + 128;
+  const float slack = kSlack / p.qs;
+  uint32_t ns = 0, no = 0;
+  for (uint32_t n = 0;; ++n) {
+    TIDE_NEXT_UNIT(u, n);
+    const int tokens = tile_tokens(u, p.tokens, t);
+    if (!tokens) continue;
+    const int end = tile_end(u, p.tokens, t);
+    const bool valid = tok < tokens;
+    const bool busy = __any_sync(kFull, valid);  // (the first token's warps always are)
+    const int sees = u.pos0 + t * p.tokens + tok + 1;  // keys this row sees
+    const int last = tile_sees(u, p.tokens, t);
+    const int64_t row = u.row0 + t * p.tokens + tok;
+    float m = -INFINITY, l = 0.f;
+    if (p.zero_keys && valid) {  // keys of score 0 whose values add nothing
+      const int z = max(__ldg(p.zero_keys + row), 0);
+      if (z) m = 0.f;
+      l = (float)z;
+    }
+    for (int j = u.b0; j < end; ++j) {
+      TIDE_WAIT(&sh.s_full[t], ns & 1);
+      ++ns;
+      if (busy) {
+        ptx::tc_fence_after();
+        const int cols = min(kKeys, last - j * kKeys);  // the rest has not been computed
+        uint32_t sr[kKeys];
+        float *s = reinterpret_cast<float *>(sr);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) ptx::tmem_ld32_async(s_col + q * 32, sr + q * 32);
+        ptx::tmem_wait_ld();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) ptx::tmem_landed(sr + q * 32);
+        const int lim = min(sees - j * kKeys, cols);
+        if (__any_sync(kFull, lim < kKeys)) {
+#pragma unroll
+          for (int i = 0; i < kKeys; ++i) s[i] = i < lim ? s[i] : -INFINITY;
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < kKeys; i += 8)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) mx[q] = fmaxf(fmaxf(mx[q], s[i + 2 * q]), s[i + 2 * q + 1]);
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        if (j == u.b0) {  // nothing in O yet
+          if (top > m) {
+            l *= ex2((m - top) * p.qs);
+            m = top;
+          }
+        } else {
+          const bool raise = top > m + slack;
+          if (__any_sync(kFull, raise)) {
+            const float a = raise ? ex2((m - top) * p.qs) : 1.f;
+            if (raise) m = top;
+            l *= a;
+            for (int q = 0; q < D; q += 32) {
+              uint32_t o[32];
+              ptx::tmem_ld32_async(o_col + q, o);
+              ptx::tmem_wait_ld();
+              ptx::tmem_landed(o);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
+              ptx::tmem_st32(o_col + q, o);
+            }
+          }
+        }
+        const float mq = m == -INFINITY ? 0.f : m * p.qs;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          uint32_t w[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float a = ex2(fmaf(s[q * 64 + 2 * i], p.qs, -mq));
+            const float b = ex2(fmaf(s[q * 64 + 2 * i + 1], p.qs, -mq));
+            sum[i & 1] += a;
+            sum[2 + (i & 1)] += b;
+            w[i] = pack2<T>(a, b);
+          }
+          ptx::tmem_st32(s_col + q * 32, w);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        ptx::tmem_wait_st();
+        ptx::tc_fence_before();
+      }
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&sh.p_full[t]);
+    }
+    const bool some = end > u.b0;
+    if (some) {
+      TIDE_WAIT(&sh.o_full[t], no & 1);
+      ++no;
+      ptx::tc_fence_after();
+    }
+    if (!busy) continue;
+    const bool odd = some && sh.odd[n & 3];
+    const int first = max(u.pos0 + 1, u.b0 * kKeys);
+    const int stop = min(sees, min(end * kKeys, last));
+    const int64_t at = row * p.hq + u.kvh * p.group + head;
+    const bool nothing = !some || (l == 0.f);
+    const float inv = nothing ? 0.f : 1.f / l;
+    if (p.splits > 1 && valid)
+      p.part_ml[(int64_t)u.split * p.batch.n_tokens * p.hq + at] = make_float2(m * p.qs, l);
+    if (p.splits > 1 && !some) continue;  // a sum of 0: its output is not read
+    for (int q = 0; q < D; q += 32) {
+      uint32_t o[32];
+      if (some) {
+        ptx::tmem_ld32_async(o_col + q, o);
+        ptx::tmem_wait_ld();
+        ptx::tmem_landed(o);
+      }
+      float *f = reinterpret_cast<float *>(o);
+      if (odd) add_odd_values<T, D, PAGED>(p, u, first, valid ? stop : first, q, f);
+      if (p.splits > 1) {
+        if (valid) {
+          float4 *dst = reinterpret_cast<float4 *>(
+              p.part_o + ((int64_t)u.split * p.batch.n_tokens * p.hq + at) * D + q);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) dst[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+        }
+        continue;
+      }
+      uint32_t w[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        w[i] = nothing ? 0u : pack2<T>(f[2 * i] * inv, f[2 * i + 1] * inv);
+      if (valid) {
+        uint4 *dst = reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + at * D + q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dst[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+      }
+    }
+    ptx::tc_fence_before();
+  }
+}
+
+template <typename T, int D, bool PAGED>
+__global__ void __launch_bounds__(kThreads, 1)
+    tile_attention_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap mq,
+                          const __grid_constant__ CUtensorMap mk,
+                          const __grid_constant__ CUtensorMap mv) {
+  using S = Shape<D>;
+  extern __shared__ unsigned char dyn[];
+  __shared__ Shared sh;
+  unsigned char *base = dyn + ((1024u - (ptx::smem_u32(dyn) & 1023u)) & 1023u);
+  unsigned char *q_smem = base, *ring = base + 2 * S::kTile;
+  const int warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < 2; ++t) {
+      ptx::mbar_init(&sh.q_full[t], 1);
+      ptx::mbar_init(&sh.q_empty[t], 1);
+      ptx::mbar_init(&sh.s_full[t], 1);
+      ptx::mbar_init(&sh.p_full[t], 4);
+      ptx::mbar_init(&sh.o_full[t], 1);
+      ptx::mbar_init(&sh.u_full[t], 1);
+      ptx::mbar_init(&sh.u_empty[t], 11);
+    }
+    ptx::mbar_init(&sh.drain, 1);
+    for (int i = 0; i < S::kStages; ++i) {
+      ptx::mbar_init(&sh.kv_full[i], 1);
+      ptx::mbar_init(&sh.kv_empty[i], 1);
+      ptx::mbar_init(&sh.raw_full[i], 1);
+      sh.raw[i] = 0;
+    }
+    ptx::fence_mbar_init();
+    sh.abort = 0;
+    sh.loaded = sh.raw_loaded = sh.q_loaded[0] = sh.q_loaded[1] = 0;
+  }
+  if (warp == 10) {
+    ptx::tmem_alloc(&sh.tmem, 512);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+
+  if (warp < 4) {
+    softmax_tile<T, D, PAGED>(p, sh, 0, tmem);
+  } else if (warp < 8) {
+    softmax_tile<T, D, PAGED>(p, sh, 1, tmem);
+  } else if (warp == 8) {
+    schedule_units(p, sh);
+  } else if (warp == 9) {
+    load_units<D, PAGED>(p, sh, q_smem, ring, &mq, &mk, &mv);
+  } else if (warp == 10) {
+    issue_products<T, D>(p, sh, ptx::smem_u32(q_smem), ptx::smem_u32(ring), tmem);
+    __syncwarp();
+    // every product done before its memory goes (after an abort too; bounded)
+    if ((threadIdx.x & 31) == 0) {
+      volatile int none = 0;
+      ptx::mma_commit(&sh.drain);
+      ptx::mbar_wait(&sh.drain, 0, &none);
+    }
+    __syncwarp();
+  } else {
+    clean_values<T, D>(p, sh, ring);
+  }
+  __syncthreads();
+  if (sh.abort && threadIdx.x == 0) {  // copies may still be landing: wait for them (bounded)
+    volatile int none = 0;
+    for (int c = max(0, sh.loaded - S::kStages); c < sh.loaded; ++c)
+      if (!sh.raw[c % S::kStages])
+        ptx::mbar_wait(&sh.kv_full[c % S::kStages], (c / S::kStages) & 1, &none);
+    for (int c = max(0, sh.raw_loaded - S::kStages); c < sh.raw_loaded; ++c)
+      ptx::mbar_wait(&sh.raw_full[c % S::kStages], (c / S::kStages) & 1, &none);
+    for (int t = 0; t < 2; ++t)
+      if (sh.q_loaded[t]) ptx::mbar_wait(&sh.q_full[t], (sh.q_loaded[t] - 1) & 1, &none);
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  if (warp == 10) ptx::tmem_dealloc(tmem, 512);
+}
+
+// Joins the splits of a row and head: with M = max_s m_s,
+//   o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s,  in the order of s.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Params p) {
+  constexpr int kE = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (w >= (int64_t)p.batch.n_tokens * p.hq) return;
+  const int row = (int)(w / p.hq);
+  const int seq = sequence_of_row(p.batch, live_sequences(p.batch), row);
+  if (seq < 0 || !sequence(p.batch, seq).n) return;
+  const int64_t step = (int64_t)p.batch.n_tokens * p.hq;
+  float top = -INFINITY;
+  for (int s = 0; s < p.splits; ++s) {
+    const float2 ml = p.part_ml[s * step + w];
+    if (ml.y != 0.f) top = fmaxf(top, ml.x);
+  }
+  float sum = 0.f, o[kE];
+#pragma unroll
+  for (int e = 0; e < kE; ++e) o[e] = 0.f;
+  for (int s = 0; s < p.splits; ++s) {
+    const float2 ml = p.part_ml[s * step + w];
+    if (ml.y == 0.f) continue;
+    const float a = exp2f(ml.x - top);
+    sum = fmaf(a, ml.y, sum);
+    const float *src = p.part_o + (s * step + w) * D + lane;
+#pragma unroll
+    for (int e = 0; e < kE; ++e) o[e] = fmaf(a, src[32 * e], o[e]);
+  }
+  T *out = static_cast<T *>(p.out) + w * D + lane;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int e = 0; e < kE; ++e) out[32 * e] = Elem<T>::from_f(o[e] * inv);
 }
 
 }  // namespace ragged
@@ -103,6 +809,37 @@ int report(cudaError_t e, const char *what) {
   return fail(TIDE_ERR_CUDA, buf);
 }
 
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> fn{nullptr};
+  auto f = fn.load(std::memory_order_acquire);
+  if (!f) {
+    void *sym = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &q) ==
+            cudaSuccess && q == cudaDriverEntryPointSuccess)
+      f = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(sym);
+    fn.store(f, std::memory_order_release);
+  }
+  return f;
+}
+
+// 16-bit rows [d2][d1][d0], s1 and s2 elements apart, read in boxes of 64 of
+// a row's elements (128 bytes, swizzled) by b1 by b2.
+bool make_map(CUtensorMap *m, int dtype, const void *base, int rank, int64_t d0, int64_t d1,
+              int64_t d2, int64_t s1, int64_t s2, int b1, int b2) {
+  auto enc = encode_fn();
+  if (!enc) return false;
+  cuuint64_t dims[3] = {(cuuint64_t)d0, (cuuint64_t)d1, (cuuint64_t)d2};
+  cuuint64_t strides[2] = {(cuuint64_t)s1 * 2, (cuuint64_t)s2 * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)b1, (cuuint32_t)b2};
+  cuuint32_t step[3] = {1, 1, 1};
+  return enc(m, dtype == TIDE_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                         : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+             (cuuint32_t)rank, const_cast<void *>(base), dims, strides, box, step,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // The checks that both entry points share; 0 or a status with its message.
 int check_heads(int dtype, int64_t hq, int64_t hkv, int64_t d, float scale, int64_t n_tokens,
                 int64_t n_seqs) {
@@ -110,7 +847,7 @@ int check_heads(int dtype, int64_t hq, int64_t hkv, int64_t d, float scale, int6
     return fail(TIDE_ERR_UNSUPPORTED, "ragged attention: dtype must be bf16 or fp16");
   if (d != 64 && d != 128)
     return fail(TIDE_ERR_UNSUPPORTED, "ragged attention: head_dim must be 64 or 128");
-  if (hkv < 1 || hq < 1 || hq % hkv || hq / hkv > 128 || hq > 65536)
+  if (hkv < 1 || hq < 1 || hq % hkv || hq / hkv > tide::ragged::kRows || hq > 65536)
     return fail(TIDE_ERR_INVALID, "ragged attention: bad heads (1 to 128 query heads per KV head)");
   if (!(scale > 0.f) || isinf(scale))
     return fail(TIDE_ERR_INVALID, "ragged attention: scale must be positive and finite");
@@ -119,14 +856,83 @@ int check_heads(int dtype, int64_t hq, int64_t hkv, int64_t d, float scale, int6
   return TIDE_OK;
 }
 
-int launch(int dtype, int64_t d, const tide::ragged::Params &p, cudaStream_t s) {
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 0;
+  return n;
+}
+
+// Units (two tiles, one KV head) that a batch may have at most.
+int64_t most_units(int64_t n_tokens, int64_t n_seqs, int64_t hq, int64_t hkv) {
+  const int64_t per = 2 * (tide::ragged::kRows / (hq / hkv));
+  const int64_t tiles = n_tokens / per + (n_seqs < n_tokens ? n_seqs : n_tokens);
+  return tiles * hkv;
+}
+
+// Splits of the keys: as many as give every SM a unit, but no split of fewer
+// than four blocks of 128 keys, whose start and join would cost more than
+// their keys.
+int64_t key_splits(int64_t n_tokens, int64_t n_seqs, int64_t hq, int64_t hkv, int64_t max_kv) {
+  const int64_t units = most_units(n_tokens, n_seqs, hq, hkv);
+  const int64_t blocks = (max_kv + tide::ragged::kKeys - 1) / tide::ragged::kKeys;
+  int64_t s = units > 0 ? 148 / units : 1;
+  if (s > blocks / 4) s = blocks / 4;
+  return s < 1 ? 1 : s;
+}
+
+template <typename T, int D, bool PAGED>
+int launch(tide::ragged::Params &p, int dtype, const void *q, int64_t q_stride, int64_t kv_rows,
+           cudaStream_t s) {
   using namespace tide::ragged;
-  auto kern = dtype == TIDE_DTYPE_BF16
-                  ? (d == 128 ? row_attention_kernel<__nv_bfloat16, 128>
-                              : row_attention_kernel<__nv_bfloat16, 64>)
-                  : (d == 128 ? row_attention_kernel<__half, 128> : row_attention_kernel<__half, 64>);
-  kern<<<(unsigned)p.batch.n_tokens, 256, 0, s>>>(p);
+  CUtensorMap mq, mk, mv;
+  const int page = 1 << p.src.page_shift;
+  const int box = PAGED && page < kKeys ? page : kKeys;
+  bool ok = make_map(&mq, dtype, q, 3, D, p.hq, p.batch.n_tokens, D, q_stride, p.group, p.tokens);
+  for (int kv = 0; kv < 2; ++kv) {
+    CUtensorMap *m = kv ? &mv : &mk;
+    const void *base = kv ? p.src.v : p.src.k;
+    ok = ok && (PAGED ? make_map(m, dtype, base, 2, D, kv_rows, 1, D, 0, box, 1)
+                      : make_map(m, dtype, base, 3, D, p.hkv, p.batch.n_tokens, D, p.src.row_stride,
+                                 1, box));
+  }
+  if (!ok) return fail(TIDE_ERR_CUDA, "ragged attention: cuTensorMapEncodeTiled failed");
+  auto kern = tile_attention_kernel<T, D, PAGED>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)Shape<D>::kSmem);
+  if (e != cudaSuccess) return report(e, "ragged attention");
+  const int64_t units =
+      most_units(p.batch.n_tokens, p.batch.n_seqs, p.hq, p.hkv) * p.splits;
+  const int sms = sm_count();
+  if (!sms) return report(cudaErrorInvalidDevice, "ragged attention");
+  kern<<<(unsigned)(units < sms ? units : sms), kThreads, Shape<D>::kSmem, s>>>(p, mq, mk, mv);
+  if (p.splits > 1) {
+    const int64_t warps = (int64_t)p.batch.n_tokens * p.hq;
+    combine_kernel<T, D><<<(unsigned)((warps + 7) / 8), 256, 0, s>>>(p);
+  }
   return report(cudaSuccess, "ragged attention");
+}
+
+template <bool PAGED>
+int dispatch(tide::ragged::Params &p, int dtype, int64_t d, const void *q, int64_t q_stride,
+             int64_t kv_rows, cudaStream_t s) {
+  if (dtype == TIDE_DTYPE_BF16)
+    return d == 128 ? launch<__nv_bfloat16, 128, PAGED>(p, dtype, q, q_stride, kv_rows, s)
+                    : launch<__nv_bfloat16, 64, PAGED>(p, dtype, q, q_stride, kv_rows, s);
+  return d == 128 ? launch<__half, 128, PAGED>(p, dtype, q, q_stride, kv_rows, s)
+                  : launch<__half, 64, PAGED>(p, dtype, q, q_stride, kv_rows, s);
+}
+
+void set_heads(tide::ragged::Params &p, int64_t hq, int64_t hkv, float scale, void *out) {
+  p.out = out;
+  p.hq = (int)hq;
+  p.hkv = (int)hkv;
+  p.group = (int)(hq / hkv);
+  p.tokens = tide::ragged::kRows / p.group;
+  p.qs = scale * tide::ragged::kLog2e;
+  p.splits = 1;
+  p.split_blocks = 1 << 24;  // all of them
 }
 
 }  // namespace
@@ -152,26 +958,19 @@ extern "C" int tide_packed_attention(int dtype, const void *q, const void *k, co
   p.batch = {cu_seqlens, nullptr, nullptr, nullptr, (int)n_seqs, 0, (int)n_tokens, (int)n_tokens,
              error_word};
   p.src = {k, v, kv_row_stride, nullptr, 0, 0, 0};
-  p.q = q;
-  p.q_stride = q_row_stride;
   p.zero_keys = zero_keys;
-  p.out = out;
-  p.hq = (int)n_q_heads;
-  p.hkv = (int)n_kv_heads;
-  p.qs = scale * tide::ragged::kLog2e;
-  return launch(dtype, head_dim, p, (cudaStream_t)stream);
+  set_heads(p, n_q_heads, n_kv_heads, scale, out);
+  return dispatch<false>(p, dtype, head_dim, q, q_row_stride, n_tokens, (cudaStream_t)stream);
 }
 
 extern "C" size_t tide_paged_attention_workspace_size(int64_t n_tokens, int64_t n_seqs,
                                                       int64_t n_q_heads, int64_t n_kv_heads,
                                                       int64_t head_dim, int64_t max_kv_len) {
-  (void)n_tokens;
-  (void)n_seqs;
-  (void)n_q_heads;
-  (void)n_kv_heads;
-  (void)head_dim;
-  (void)max_kv_len;
-  return 0;
+  if (n_tokens < 1 || n_seqs < 1 || n_kv_heads < 1 || n_q_heads < n_kv_heads || max_kv_len < 1 ||
+      n_q_heads / n_kv_heads > tide::ragged::kRows)
+    return 0;
+  const int64_t s = key_splits(n_tokens, n_seqs, n_q_heads, n_kv_heads, max_kv_len);
+  return s > 1 ? (size_t)(s * n_tokens * n_q_heads * (head_dim + 2) * 4) : 0;
 }
 
 extern "C" int tide_paged_attention(int dtype, const void *q, int64_t q_row_stride,
@@ -211,11 +1010,14 @@ extern "C" int tide_paged_attention(int dtype, const void *q, int64_t q_row_stri
   p.batch = {cu_seqlens, seq_ids, kv_lens, n_seqs_dev, (int)n_seqs, (int)n_requests,
              (int)n_tokens, (int)max_kv_len, error_word};
   p.src = {k_cache, v_cache, 0, block_tables, max_pages, (int)n_pages, shift};
-  p.q = q;
-  p.q_stride = q_row_stride;
-  p.out = out;
-  p.hq = (int)n_q_heads;
-  p.hkv = (int)n_kv_heads;
-  p.qs = scale * tide::ragged::kLog2e;
-  return launch(dtype, head_dim, p, (cudaStream_t)stream);
+  set_heads(p, n_q_heads, n_kv_heads, scale, out);
+  p.splits = (int)key_splits(n_tokens, n_seqs, n_q_heads, n_kv_heads, max_kv_len);
+  if (p.splits > 1) {
+    const int64_t blocks = (max_kv_len + tide::ragged::kKeys - 1) / tide::ragged::kKeys;
+    p.split_blocks = (int)((blocks + p.splits - 1) / p.splits);
+    p.part_o = static_cast<float *>(workspace);
+    p.part_ml = reinterpret_cast<float2 *>(p.part_o + p.splits * n_tokens * n_q_heads * head_dim);
+  }
+  return dispatch<true>(p, dtype, head_dim, q, q_row_stride, n_pages * n_kv_heads * page_size,
+                        (cudaStream_t)stream);
 }
