@@ -501,6 +501,30 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Two floats in one register pair, and the two-lane forms of fma and add.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float *a, float *b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(*a), "=f"(*b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   uint32_t r;
@@ -583,8 +607,8 @@ __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem) 
 #pragma unroll
         for (int i = 0; i < kKeys; i += 8)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) mx[q] = fmaxf(fmaxf(mx[q], s[i + 2 * q]), s[i + 2 * q + 1]);
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          for (int q = 0; q < 4; ++q) mx[q] = max3(mx[q], s[i + 2 * q], s[i + 2 * q + 1]);
+        const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
         if (j == u.b0) {  // nothing in O yet
           if (top > m) {
             l *= ex2((m - top) * p.qs);
@@ -596,6 +620,7 @@ __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem) 
             const float a = raise ? ex2((m - top) * p.qs) : 1.f;
             if (raise) m = top;
             l *= a;
+#pragma unroll 1
             for (int q = 0; q < D; q += 32) {
               uint32_t o[32];
               ptx::tmem_ld32_async(o_col + q, o);
@@ -608,21 +633,26 @@ __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem) 
           }
         }
         const float mq = m == -INFINITY ? 0.f : m * p.qs;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t qs2 = pair(p.qs, p.qs), mq2 = pair(-mq, -mq);
+        uint64_t sum0 = 0, sum1 = 0;
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          uint32_t w[32];
+        for (int q = 0; q < 4; ++q) {
+          uint32_t w[16];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float a = ex2(fmaf(s[q * 64 + 2 * i], p.qs, -mq));
-            const float b = ex2(fmaf(s[q * 64 + 2 * i + 1], p.qs, -mq));
-            sum[i & 1] += a;
-            sum[2 + (i & 1)] += b;
+          for (int i = 0; i < 16; ++i) {
+            float a, b;
+            unpair(fma2(pair(s[q * 32 + 2 * i], s[q * 32 + 2 * i + 1]), qs2, mq2), &a, &b);
+            a = ex2(a);
+            b = ex2(b);
+            if (i & 1) sum1 = add2(sum1, pair(a, b));
+            else sum0 = add2(sum0, pair(a, b));
             w[i] = pack2<T>(a, b);
           }
-          ptx::tmem_st32(s_col + q * 32, w);
+          ptx::tmem_st16(s_col + q * 16, w);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        float la, lb;
+        unpair(add2(sum0, sum1), &la, &lb);
+        l += la + lb;
         ptx::tmem_wait_st();
         ptx::tc_fence_before();
       }
@@ -645,6 +675,7 @@ __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem) 
     if (p.splits > 1 && valid)
       p.part_ml[(int64_t)u.split * p.batch.n_tokens * p.hq + at] = make_float2(m * p.qs, l);
     if (p.splits > 1 && !some) continue;  // a sum of 0: its output is not read
+#pragma unroll 1
     for (int q = 0; q < D; q += 32) {
       uint32_t o[32];
       if (some) {
@@ -718,6 +749,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   ptx::tc_fence_after();
   const uint32_t tmem = sh.tmem;
 
+  // Registers move from the four service warps to the softmax warps:
+  // 256 * 216 + 128 * 72 = 384 * 168, what the block was launched with.
+  if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
   if (warp < 4) {
     softmax_tile<T, D, PAGED>(p, sh, 0, tmem);
   } else if (warp < 8) {
