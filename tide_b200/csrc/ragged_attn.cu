@@ -359,78 +359,98 @@ __device__ void load_units(const Params &p, Shared &sh, unsigned char *q_smem,
 }
 
 // --------------------------------------------------------------- products
+// The whole warp walks through the schedule with values that are the same in
+// every lane (the shuffles tell the compiler so), and one elected lane issues:
+// the operands of tcgen05.mma live in uniform registers, and per-lane values
+// have to be moved there one by one, at 107 cycles a product instead of 68.
 template <typename T, int D>
 __device__ void issue_products(const Params &p, Shared &sh, uint32_t q_smem, uint32_t ring,
                                uint32_t tmem) {
   using S = Shape<D>;
-  const bool lead = (threadIdx.x & 31) == 0;
+  constexpr unsigned kFull = 0xffffffffu;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  uint32_t c0 = 0;  // ring count of the unit's first K block
-  uint32_t nq[2] = {0, 0}, np[2] = {0, 0};
+  tmem = __shfl_sync(kFull, tmem, 0);
+  uint32_t stage = 0, lap = 0;  // of the next K block
+  uint32_t nq = 0, np = 0;      // bit t: phases of tile t's barriers
+  const uint64_t q_desc = ptx::sw128_kmajor_desc(q_smem);
+  const uint64_t k_desc = ptx::sw128_kmajor_desc(ring);
+  const uint64_t v_desc = ptx::sw128_mnmajor_desc(ring, S::kHalf);
   for (uint32_t n = 0;; ++n) {
-    TIDE_NEXT_UNIT(u, n);
-    const int end_of[2] = {tile_end(u, p.tokens, 0), tile_end(u, p.tokens, 1)};
-    const int end = max(end_of[0], end_of[1]);
-    if (end <= u.b0) continue;
-    const int sees_of[2] = {tile_sees(u, p.tokens, 0), tile_sees(u, p.tokens, 1)};
-    auto stage_of = [&](int j, int kv) { return (c0 + 2 * (j - u.b0) + kv) % S::kStages; };
-    auto lap_of = [&](int j, int kv) { return (c0 + 2 * (j - u.b0) + kv) / S::kStages; };
-    // S_t = Q_t K_j^T over the keys that tile t sees
-    auto scores = [&](int t, int j) {
-      const int cols = min(kKeys, (sees_of[t] - j * kKeys + 31) / 32 * 32);
+    TIDE_NEXT_UNIT(w, n);
+    const int b0 = __shfl_sync(kFull, w.b0, 0);
+    const int end0 = __shfl_sync(kFull, tile_end(w, p.tokens, 0), 0);
+    const int end1 = __shfl_sync(kFull, tile_end(w, p.tokens, 1), 0);
+    const int sees0 = __shfl_sync(kFull, tile_sees(w, p.tokens, 0), 0);
+    const int sees1 = __shfl_sync(kFull, tile_sees(w, p.tokens, 1), 0);
+    const int end = max(end0, end1);
+    if (end <= b0) continue;
+    // S_t = Q_t K_j^T over the keys that tile t sees; the last tile that
+    // reads K_j frees it
+    auto scores = [&](int t, int j, uint32_t k_stage) {
+      const int cols = min(kKeys, ((t ? sees1 : sees0) - j * kKeys + 31) / 32 * 32);
       const uint32_t idesc = ptx::f16_idesc(kBf16, kRows, cols);
-      const uint64_t a = ptx::sw128_kmajor_desc(q_smem + t * S::kTile);
-      const uint64_t b = ptx::sw128_kmajor_desc(ring + stage_of(j, 0) * S::kTile);
-      if (lead) {
+      const uint64_t a = q_desc + t * (S::kTile >> 4);
+      const uint64_t b = k_desc + k_stage * (S::kTile >> 4);
+      const bool last = j + 1 == (t ? end1 : end0), frees = t == 1 || j >= end1;
+      if (ptx::elect_one()) {
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          const uint64_t off = (k / 4) * (S::kHalf >> 4) + (k % 4) * 2;
+          const uint32_t off = (k / 4) * (S::kHalf >> 4) + (k % 4) * 2;
           ptx::mma_f16_ss(tmem + t * 256, a + off, b + off, idesc, k > 0);
         }
         ptx::mma_commit(&sh.s_full[t]);
-        if (j + 1 == end_of[t]) ptx::mma_commit(&sh.q_empty[t]);
-        // the last tile that reads K_j frees it
-        if (t == 1 || j >= end_of[1]) ptx::mma_commit(&sh.kv_empty[stage_of(j, 0)]);
+        if (last) ptx::mma_commit(&sh.q_empty[t]);
+        if (frees) ptx::mma_commit(&sh.kv_empty[k_stage]);
       }
       __syncwarp();
     };
-    TIDE_WAIT(&sh.kv_full[stage_of(u.b0, 0)], lap_of(u.b0, 0) & 1);
+    TIDE_WAIT(&sh.kv_full[stage], lap & 1);
+#pragma unroll
     for (int t = 0; t < 2; ++t) {
-      if (u.b0 >= end_of[t]) continue;
-      TIDE_WAIT(&sh.q_full[t], nq[t] & 1);
-      ++nq[t];
+      if (b0 >= (t ? end1 : end0)) continue;
+      TIDE_WAIT(&sh.q_full[t], (nq >> t) & 1);
+      nq ^= 1u << t;
       ptx::tc_fence_after();
-      scores(t, u.b0);
+      scores(t, b0, stage);
     }
-    for (int j = u.b0; j < end; ++j) {
-      TIDE_WAIT(&sh.kv_full[stage_of(j, 1)], lap_of(j, 1) & 1);
+    for (int j = b0; j < end; ++j) {
+      uint32_t v_stage = stage + 1, v_lap = lap;
+      if (v_stage == S::kStages) { v_stage = 0; ++v_lap; }
+      stage = v_stage + 1, lap = v_lap;
+      if (stage == S::kStages) { stage = 0; ++lap; }
+      TIDE_WAIT(&sh.kv_full[v_stage], v_lap & 1);
       bool next_keys = false;
+#pragma unroll
       for (int t = 0; t < 2; ++t) {
-        if (j >= end_of[t]) continue;
-        TIDE_WAIT(&sh.p_full[t], np[t] & 1);
-        ++np[t];
+        const int end_t = t ? end1 : end0;
+        if (j >= end_t) continue;
+        TIDE_WAIT(&sh.p_full[t], (np >> t) & 1);
+        np ^= 1u << t;
         ptx::tc_fence_after();
         // O_t += P_t V_j over the keys that the tile sees, 16 at a time
-        const int steps = (min(kKeys, sees_of[t] - j * kKeys) + 15) / 16;
+        const int steps = (min(kKeys, (t ? sees1 : sees0) - j * kKeys) + 15) / 16;
         const uint32_t idesc = ptx::f16_idesc(kBf16, kRows, D) | ptx::kIdescMnMajorB;
-        const uint64_t b = ptx::sw128_mnmajor_desc(ring + stage_of(j, 1) * S::kTile, S::kHalf);
-        if (lead) {
-          for (int k = 0; k < steps; ++k)
-            ptx::mma_f16_ts(tmem + t * 256 + 128, tmem + t * 256 + k * 8, b + k * (2048 >> 4), idesc,
-                            j > u.b0 || k > 0);
-          if (t == 1 || j >= end_of[1]) ptx::mma_commit(&sh.kv_empty[stage_of(j, 1)]);
-          if (j + 1 >= end_of[t]) ptx::mma_commit(&sh.o_full[t]);
+        const uint64_t b = v_desc + v_stage * (S::kTile >> 4);
+        const uint32_t more = j > b0;
+        const bool last = j + 1 >= end_t, frees = t == 1 || j >= end1;
+        if (ptx::elect_one()) {
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; ++k)
+            if (k < steps)
+              ptx::mma_f16_ts(tmem + t * 256 + 128, tmem + t * 256 + k * 8, b + k * (2048 >> 4),
+                              idesc, k ? 1u : more);
+          if (frees) ptx::mma_commit(&sh.kv_empty[v_stage]);
+          if (last) ptx::mma_commit(&sh.o_full[t]);
         }
         __syncwarp();
-        if (j + 1 < end_of[t]) {
-          if (!next_keys) TIDE_WAIT(&sh.kv_full[stage_of(j + 1, 0)], lap_of(j + 1, 0) & 1);
+        if (!last) {
+          if (!next_keys) TIDE_WAIT(&sh.kv_full[stage], lap & 1);
           next_keys = true;
           ptx::tc_fence_after();
-          scores(t, j + 1);
+          scores(t, j + 1, stage);
         }
       }
     }
-    c0 += 2 * (end - u.b0);
   }
 }
 
@@ -520,6 +540,46 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// 2^x of two numbers on the FMA pipes: x = n + f with n whole and f in
+// [-1/2, 1/2], 2^f by a polynomial that is within 2^-23.6 of it relatively
+// (minimax, degree 5, by an exchange iteration), n added to the exponent.
+// x below -126 counts as -126.  The special function unit takes four of a
+// warp's exponentials a cycle, so with all of them there it would bound the
+// kernel: kPoly of 16 pairs go this way.
+__device__ __forceinline__ void ex2_poly(uint64_t x, float *a, float *b) {
+  constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to whole numbers
+  float lo, hi;
+  unpair(x, &lo, &hi);
+  x = pair(fmaxf(lo, -126.f), fmaxf(hi, -126.f));
+  const uint64_t t = add2(x, pair(kMagic, kMagic));
+  const uint64_t n = add2(t, pair(-kMagic, -kMagic));
+  const uint64_t f = fma2(n, pair(-1.f, -1.f), x);
+#ifndef POLY_DEG
+#define POLY_DEG 5
+#endif
+#if POLY_DEG == 5
+  uint64_t y = pair(0.0013276471992546789f, 0.0013276471992546789f);
+  y = fma2(y, f, pair(0.009675541334453112f, 0.009675541334453112f));
+  y = fma2(y, f, pair(0.05550713273498027f, 0.05550713273498027f));
+  y = fma2(y, f, pair(0.24022119723840024f, 0.24022119723840024f));
+  y = fma2(y, f, pair(0.6931469670647603f, 0.6931469670647603f));
+  y = fma2(y, f, pair(1.0000000716546849f, 1.0000000716546849f));
+#else
+  uint64_t y = pair(0.05517166905792616f, 0.05517166905792616f);
+  y = fma2(y, f, pair(0.2426111221932161f, 0.2426111221932161f));
+  y = fma2(y, f, pair(0.6932609854606553f, 0.6932609854606553f));
+  y = fma2(y, f, pair(0.9999280735394012f, 0.9999280735394012f));
+#endif
+  float yl, yh, tl, th;
+  unpair(y, &yl, &yh);
+  unpair(t, &tl, &th);
+  *a = __uint_as_float(__float_as_uint(yl) + (__float_as_uint(tl) << 23));
+  *b = __uint_as_float(__float_as_uint(yh) + (__float_as_uint(th) << 23));
+}
+#ifndef POLY
+#define POLY 4
+#endif
+constexpr int kPoly = POLY;
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -641,9 +701,14 @@ __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem) 
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             float a, b;
-            unpair(fma2(pair(s[q * 32 + 2 * i], s[q * 32 + 2 * i + 1]), qs2, mq2), &a, &b);
-            a = ex2(a);
-            b = ex2(b);
+            const uint64_t x = fma2(pair(s[q * 32 + 2 * i], s[q * 32 + 2 * i + 1]), qs2, mq2);
+            if ((i * kPoly) % 16 < kPoly) {
+              ex2_poly(x, &a, &b);
+            } else {
+              unpair(x, &a, &b);
+              a = ex2(a);
+              b = ex2(b);
+            }
             if (i & 1) sum1 = add2(sum1, pair(a, b));
             else sum0 = add2(sum0, pair(a, b));
             w[i] = pack2<T>(a, b);
@@ -765,7 +830,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     issue_products<T, D>(p, sh, ptx::smem_u32(q_smem), ptx::smem_u32(ring), tmem);
     __syncwarp();
     // every product done before its memory goes (after an abort too; bounded)
-    if ((threadIdx.x & 31) == 0) {
+    if (ptx::elect_one()) {
       volatile int none = 0;
       ptx::mma_commit(&sh.drain);
       ptx::mbar_wait(&sh.drain, 0, &none);
