@@ -8,9 +8,9 @@
 // A tile is 128 rows: floor(128 / G) consecutive tokens of a sequence times
 // the G query heads of one KV head, so that a key or value loaded serves all
 // heads that share it.  A unit of work is two such tiles, one behind the
-// other; a persistent CTA per SM walks over units.  Per block of 128 keys and
+// other; a persistent CTA per SM walks over units.  Per block of 64 keys and
 // tile,
-//   S[128 x 128] = Q K^T      tcgen05.mma, operands in shared memory (TMA,
+//   S[128 x 64] = Q K^T       tcgen05.mma, operands in shared memory (TMA,
 //                             128-byte swizzle), S in tensor memory;
 //   P = 2^(S qs - m)          one thread per row: running maximum m and sum l,
 //                             P rounded to the rows' 16-bit type (half a step
@@ -18,22 +18,23 @@
 //                             unrounded ones) and written over S;
 //   O[128 x D] += P V         tcgen05.mma with P from tensor memory and V as
 //                             it lies in shared memory (its MN-major operand).
-// The tensor core and the two tiles' softmax warps alternate: while one
-// tile's scores go through the exponential, the other's products run.
+// Each tile has two S buffers, so that its next scores are there when its
+// softmax warps come for them: with blocks of 128 keys and one buffer the
+// chain score product - softmax - value product of a tile was serial, at 4000
+// cycles per 128 keys of both tiles, of which the tensor core worked 2200.
+// Each tile also has a warp of its own that issues its products, in whatever
+// order they become ready, over the ends of units.
 //
 // m is only raised, and O and l rescaled, when a row's maximum has grown by
 // more than 2^8 since: weights up to 256 cost nothing (fp32 sums; 16-bit
-// floats round relatively), and O stays where it is.  The rescale needs no
-// synchronisation of its own: the commit that publishes S_j comes after the
-// product that used P_j-1 in the same instruction stream, so O is complete
-// when S_j is.
+// floats round relatively), and O stays where it is.
 //
-// Roles of the 12 warps: 0-3 and 4-7 the softmax and the output of tile 0
-// and 1; 8 finds the units; 9 loads; 10 issues the products; 11 cleans the
-// value blocks that not every row sees: a masked weight is 0, but 0 * NaN is
-// not, so rows past the last visible key are zeroed, and a value that is not
-// finite at a position that only the later rows see is zeroed, noted, and
-// added to the outputs of the rows that do see it.
+// Roles of the warps: 0-3 and 4-7 the softmax and the output of tile 0
+// and 1; 8 finds the units; 9 loads; 10 and 11 issue the tiles' products; 12
+// cleans the value blocks that not every row sees: a masked weight is 0, but
+// 0 * NaN is not, so rows past the last visible key are zeroed, and a value
+// that is not finite at a position that only the later rows see is zeroed,
+// noted, and added to the outputs of the rows that do see it.
 //
 // Order of units: by the number of keys they read, most first (the level of a
 // unit: positions before its end, in units of its size), so that the last
@@ -59,18 +60,23 @@ namespace ragged {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kRows = 128;   // rows of a tile
-constexpr int kKeys = 128;   // keys of a block
-constexpr int kThreads = 384;
+constexpr int kKeys = 64;    // keys of a block
+constexpr int kWarps = 16;   // three of them only lend their registers
+constexpr int kReaders = 12; // warps that read the units
+constexpr int kThreads = 32 * kWarps;
 constexpr int kCached = 4;   // sequences per lane that the unit search keeps in registers
 constexpr float kSlack = 8.f;  // log2 of how far a maximum may grow before a rescale
 
 template <int D>
 struct Shape {
   static constexpr int kHalves = D / 64;               // 128-byte column groups
-  static constexpr uint32_t kTile = kRows * D * 2;     // bytes of a Q tile or a K or V block
-  static constexpr uint32_t kHalf = kRows * 128;       // bytes of one column group of it
-  static constexpr int kStages = D == 128 ? 5 : 10;    // K and V blocks in flight
-  static constexpr uint32_t kSmem = (2 + kStages) * kTile + 1024;  // + alignment
+  static constexpr uint32_t kQHalf = kRows * 128;      // bytes of a column group of a Q tile
+  static constexpr uint32_t kQ = kQHalf * kHalves;     // of a Q tile
+  static constexpr uint32_t kHalf = kKeys * 128;       // of a column group of a K or V block
+  static constexpr uint32_t kBlock = kHalf * kHalves;  // of a K or V block
+  static constexpr int kStages = 8;                    // K and V blocks in flight
+  static constexpr uint32_t kStaging = 8 * 4096;       // 32 rows x 128 bytes per softmax warp
+  static constexpr uint32_t kSmem = 2 * kQ + kStages * kBlock + kStaging + 1024;  // + alignment
 };
 
 struct Params {
@@ -124,20 +130,24 @@ __device__ __forceinline__ bool cleaned_rows(const Unit &u, int sees, int j, int
   return *from < *to;
 }
 
+constexpr int kRing = 8;  // stages of every Shape
+
 struct Shared {
   uint64_t q_full[2], q_empty[2];
-  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t s_full[2][2], p_full[2][2];  // [tile][buffer]
+  uint64_t pv_done[2];                  // after every value product of a tile
+  uint64_t o_full[2];                   // after the last one of a unit
   uint64_t u_full[2], u_empty[2];
-  uint64_t drain;
-  uint64_t kv_full[10], kv_empty[10];
-  uint64_t raw_full[10];  // value blocks that have landed and are to be cleaned, in turn
+  uint64_t drain[2];
+  uint64_t kv_full[kRing], kv_empty[kRing];
+  uint64_t raw_full[kRing];  // value blocks that have landed and are to be cleaned, in turn
   Unit unit[2];
   int odd[4];       // per unit (by its number mod 4): a value of the cleaned range is not finite
   uint32_t tmem;
   int abort;
   // requested so far, for the wait after an abort
   int loaded, raw_loaded, q_loaded[2];
-  int raw[10];      // whether a stage's last copy completes on raw_full
+  int raw[kRing];   // whether a stage's last copy completes on raw_full
 };
 
 // Bounded wait of a whole warp; when it runs out the warp's role ends, and
@@ -288,10 +298,14 @@ __device__ void load_units(const Params &p, Shared &sh, unsigned char *q_smem,
   const uint32_t q_bytes = (uint32_t)(p.tokens * p.group) * 128u * S::kHalves;
   for (uint32_t n = 0;; ++n) {
     TIDE_NEXT_UNIT(u, n);
-    const int e0 = tile_end(u, p.tokens, 0), e1 = tile_end(u, p.tokens, 1);
-    const int end = max(e0, e1);
+    const int ends[2] = {tile_end(u, p.tokens, 0), tile_end(u, p.tokens, 1)};
+    const int end = max(ends[0], ends[1]);
     if (end <= u.b0) continue;
     const int sees = u.pos0 + u.n;
+    // the queries into L2 while their place in shared memory is still in use
+    if (lane < 2 * S::kHalves && ends[lane / S::kHalves] > u.b0)
+      ptx::tma_prefetch_3d(mq, lane % S::kHalves * 64, u.kvh * p.group,
+                           u.row0 + lane / S::kHalves * p.tokens);
     // the pages of a block, one per lane; the next block's are read ahead
     auto page_of = [&](int j) {
       int row = -1;
@@ -305,18 +319,6 @@ __device__ void load_units(const Params &p, Shared &sh, unsigned char *q_smem,
       }
       return row;
     };
-    auto load_q = [&](int t) {
-      if (nq[t] >= 1) TIDE_WAIT(&sh.q_empty[t], (nq[t] + 1) & 1);
-      if (lane == 0) {
-        ptx::mbar_expect_tx(&sh.q_full[t], q_bytes);
-#pragma unroll
-        for (int h = 0; h < S::kHalves; ++h)
-          ptx::tma_load_3d(q_smem + t * S::kTile + h * S::kHalf, mq, &sh.q_full[t], h * 64,
-                           u.kvh * p.group, u.row0 + t * p.tokens);
-      }
-      ++nq[t];
-      if (lane == 0) sh.q_loaded[t] = (int)nq[t];
-    };
     int row = page_of(u.b0);
     for (int j = u.b0; j < end; ++j) {
       const int next = page_of(j + 1);
@@ -325,14 +327,14 @@ __device__ void load_units(const Params &p, Shared &sh, unsigned char *q_smem,
       for (int kv = 0; kv < 2; ++kv) {
         const uint32_t stage = c % S::kStages, lap = c / S::kStages;
         if (lap >= 1) TIDE_WAIT(&sh.kv_empty[stage], (lap + 1) & 1);
-        unsigned char *dst = ring + stage * S::kTile;
+        unsigned char *dst = ring + stage * S::kBlock;
         const CUtensorMap *m = kv ? mv : mk;
         int from, to;
         const bool dirty = kv && cleaned_rows(u, sees, j, &from, &to);
         uint64_t *full = dirty ? &sh.raw_full[raw % S::kStages] : &sh.kv_full[stage];
         raw += dirty;
         if (lane == 0) {
-          ptx::mbar_expect_tx(full, PAGED ? (uint32_t)(count * box) * 128u * S::kHalves : S::kTile);
+          ptx::mbar_expect_tx(full, PAGED ? (uint32_t)(count * box) * 128u * S::kHalves : S::kBlock);
           sh.raw[stage] = dirty;
           sh.loaded = (int)c + 1;
           sh.raw_loaded = (int)raw;
@@ -346,110 +348,150 @@ __device__ void load_units(const Params &p, Shared &sh, unsigned char *q_smem,
           ptx::tma_load_3d(dst + lane * S::kHalf, m, full, lane * 64, u.kvh, u.key0 + j * kKeys);
         }
         ++c;
-        if (j == u.b0 && kv == 0) {
-          if (e0 > u.b0) load_q(0);
-          if (sh.abort) return;
-          if (e1 > u.b0) load_q(1);
-          if (sh.abort) return;
-        }
       }
+      if (j == u.b0)  // the first keys and values are on their way
+        for (int t = 0; t < 2; ++t) {
+          if (ends[t] <= u.b0) continue;
+          if (nq[t] >= 1) TIDE_WAIT(&sh.q_empty[t], (nq[t] + 1) & 1);
+          ++nq[t];
+          if (lane == 0) {
+            sh.q_loaded[t] = (int)nq[t];
+            ptx::mbar_expect_tx(&sh.q_full[t], q_bytes);
+          }
+          __syncwarp();
+          if (lane < S::kHalves)
+            ptx::tma_load_3d(q_smem + t * S::kQ + lane * S::kQHalf, mq, &sh.q_full[t], lane * 64,
+                             u.kvh * p.group, u.row0 + t * p.tokens);
+        }
       row = next;
     }
   }
 }
 
 // --------------------------------------------------------------- products
-// The whole warp walks through the schedule with values that are the same in
-// every lane (the shuffles tell the compiler so), and one elected lane issues:
-// the operands of tcgen05.mma live in uniform registers, and per-lane values
-// have to be moved there one by one, at 107 cycles a product instead of 68.
+// Tile t's products, in the order in which they become possible: a score
+// product when its K block (and Q) has landed and fewer than two are ahead of
+// the value products, a value product when its P is written.  Neither waits
+// for the other, so the next unit's first scores are made while this unit's
+// last softmax runs.  K and V blocks that the other tile alone sees are passed
+// on.  The whole warp walks through the schedule with values that are the same
+// in every lane (the shuffles tell the compiler so), and one elected lane
+// issues: the operands of tcgen05.mma live in uniform registers, and per-lane
+// values would be moved there one by one, at 107 cycles a product of 128 keys
+// instead of 80.
 template <typename T, int D>
-__device__ void issue_products(const Params &p, Shared &sh, uint32_t q_smem, uint32_t ring,
+__device__ void issue_products(const Params &p, Shared &sh, int t, uint32_t q_smem, uint32_t ring,
                                uint32_t tmem) {
   using S = Shape<D>;
   constexpr unsigned kFull = 0xffffffffu;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  tmem = __shfl_sync(kFull, tmem, 0);
-  uint32_t stage = 0, lap = 0;  // of the next K block
-  uint32_t nq = 0, np = 0;      // bit t: phases of tile t's barriers
-  const uint64_t q_desc = ptx::sw128_kmajor_desc(q_smem);
+  constexpr uint32_t kPvDesc = ptx::f16_idesc(kBf16, kRows, D) | ptx::kIdescMnMajorB;
+  t = __shfl_sync(kFull, t, 0);
+  tmem = __shfl_sync(kFull, tmem, 0) + t * 256;
+  const uint64_t q_desc = ptx::sw128_kmajor_desc(q_smem + t * S::kQ);
   const uint64_t k_desc = ptx::sw128_kmajor_desc(ring);
   const uint64_t v_desc = ptx::sw128_mnmajor_desc(ring, S::kHalf);
-  for (uint32_t n = 0;; ++n) {
-    TIDE_NEXT_UNIT(w, n);
-    const int b0 = __shfl_sync(kFull, w.b0, 0);
-    const int end0 = __shfl_sync(kFull, tile_end(w, p.tokens, 0), 0);
-    const int end1 = __shfl_sync(kFull, tile_end(w, p.tokens, 1), 0);
-    const int sees0 = __shfl_sync(kFull, tile_sees(w, p.tokens, 0), 0);
-    const int sees1 = __shfl_sync(kFull, tile_sees(w, p.tokens, 1), 0);
-    const int end = max(end0, end1);
-    if (end <= b0) continue;
-    // S_t = Q_t K_j^T over the keys that tile t sees; the last tile that
-    // reads K_j frees it
-    auto scores = [&](int t, int j, uint32_t k_stage) {
-      const int cols = min(kKeys, ((t ? sees1 : sees0) - j * kKeys + 31) / 32 * 32);
-      const uint32_t idesc = ptx::f16_idesc(kBf16, kRows, cols);
-      const uint64_t a = q_desc + t * (S::kTile >> 4);
-      const uint64_t b = k_desc + k_stage * (S::kTile >> 4);
-      const bool last = j + 1 == (t ? end1 : end0), frees = t == 1 || j >= end1;
-      if (ptx::elect_one()) {
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k / 4) * (S::kHalf >> 4) + (k % 4) * 2;
-          ptx::mma_f16_ss(tmem + t * 256, a + off, b + off, idesc, k > 0);
-        }
-        ptx::mma_commit(&sh.s_full[t]);
-        if (last) ptx::mma_commit(&sh.q_empty[t]);
-        if (frees) ptx::mma_commit(&sh.kv_empty[k_stage]);
+  auto ready = [&](uint64_t *bar, uint32_t phase) {
+    return __all_sync(kFull, ptx::mbar_test(bar, phase & 1)) != 0;
+  };
+  uint32_t n = 0, nq = 0;       // units and Q tiles taken
+  uint32_t c = 0;               // ring count of the next K block
+  uint32_t made = 0, used = 0;  // score and value products issued
+  bool open = false, done = false;
+  int j = 0, b0 = 0, end_t = 0, end = 0, sees = 0;  // of the unit that scores are made for
+  // the (up to two) value products to come: ring count of V, 16-key steps,
+  // whether O holds earlier ones, whether the unit ends
+  uint32_t v0 = 0, v1 = 0, w0 = 0, w1 = 0;
+  for (uint32_t idle = 0; !done || used != made;) {
+    bool moved = false;
+    if (!done && !open) {
+      if (ready(&sh.u_full[n & 1], n >> 1)) {
+        const Unit u = sh.unit[n & 1];
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&sh.u_empty[n & 1]);
+        ++n;
+        done = __shfl_sync(kFull, u.valid, 0) == 0;
+        b0 = j = __shfl_sync(kFull, u.b0, 0);
+        end_t = __shfl_sync(kFull, tile_end(u, p.tokens, t), 0);
+        end = max(end_t, __shfl_sync(kFull, tile_end(u, p.tokens, t ^ 1), 0));
+        sees = __shfl_sync(kFull, tile_sees(u, p.tokens, t), 0);
+        open = !done && end > b0;
+        moved = true;
       }
-      __syncwarp();
-    };
-    TIDE_WAIT(&sh.kv_full[stage], lap & 1);
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      if (b0 >= (t ? end1 : end0)) continue;
-      TIDE_WAIT(&sh.q_full[t], (nq >> t) & 1);
-      nq ^= 1u << t;
-      ptx::tc_fence_after();
-      scores(t, b0, stage);
-    }
-    for (int j = b0; j < end; ++j) {
-      uint32_t v_stage = stage + 1, v_lap = lap;
-      if (v_stage == S::kStages) { v_stage = 0; ++v_lap; }
-      stage = v_stage + 1, lap = v_lap;
-      if (stage == S::kStages) { stage = 0; ++lap; }
-      TIDE_WAIT(&sh.kv_full[v_stage], v_lap & 1);
-      bool next_keys = false;
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int end_t = t ? end1 : end0;
-        if (j >= end_t) continue;
-        TIDE_WAIT(&sh.p_full[t], (np >> t) & 1);
-        np ^= 1u << t;
+    } else if (open && made - used < 2) {
+      const uint32_t ks = c % S::kStages, vs = (c + 1) % S::kStages;
+      if (j >= end_t) {
+        // (only with no value product to come, so that no stage is tested
+        // for its next copy while this one has yet to land)
+        if (made == used && ready(&sh.kv_full[ks], c / S::kStages) &&
+            ready(&sh.kv_full[vs], (c + 1) / S::kStages)) {
+          if (ptx::elect_one()) {
+            ptx::mbar_arrive(&sh.kv_empty[ks]);
+            ptx::mbar_arrive(&sh.kv_empty[vs]);
+          }
+          __syncwarp();
+          moved = true;
+        }
+      } else if ((j > b0 || ready(&sh.q_full[t], nq)) && ready(&sh.kv_full[ks], c / S::kStages)) {
+        // S = Q K_j^T over the keys that the tile sees
+        const int keys = min(kKeys, sees - j * kKeys);
+        const uint32_t steps = (uint32_t)(keys + 15) / 16;
+        const uint32_t idesc = ptx::f16_idesc(kBf16, kRows, (int)steps * 16);
+        const uint64_t b = k_desc + ks * (S::kBlock >> 4);
+        const uint32_t d = tmem + (made & 1) * kKeys;
+        const bool last = j + 1 == end_t;
         ptx::tc_fence_after();
-        // O_t += P_t V_j over the keys that the tile sees, 16 at a time
-        const int steps = (min(kKeys, (t ? sees1 : sees0) - j * kKeys) + 15) / 16;
-        const uint32_t idesc = ptx::f16_idesc(kBf16, kRows, D) | ptx::kIdescMnMajorB;
-        const uint64_t b = v_desc + v_stage * (S::kTile >> 4);
-        const uint32_t more = j > b0;
-        const bool last = j + 1 >= end_t, frees = t == 1 || j >= end1;
         if (ptx::elect_one()) {
 #pragma unroll
-          for (int k = 0; k < kKeys / 16; ++k)
-            if (k < steps)
-              ptx::mma_f16_ts(tmem + t * 256 + 128, tmem + t * 256 + k * 8, b + k * (2048 >> 4),
-                              idesc, k ? 1u : more);
-          if (frees) ptx::mma_commit(&sh.kv_empty[v_stage]);
-          if (last) ptx::mma_commit(&sh.o_full[t]);
+          for (int k = 0; k < D / 16; ++k)
+            ptx::mma_f16_ss(d, q_desc + (k / 4) * (S::kQHalf >> 4) + (k % 4) * 2,
+                            b + (k / 4) * (S::kHalf >> 4) + (k % 4) * 2, idesc, k > 0);
+          ptx::mma_commit(&sh.s_full[t][made & 1]);
+          ptx::mma_commit(&sh.kv_empty[ks]);
+          if (last) ptx::mma_commit(&sh.q_empty[t]);
         }
         __syncwarp();
-        if (!last) {
-          if (!next_keys) TIDE_WAIT(&sh.kv_full[stage], lap & 1);
-          next_keys = true;
-          ptx::tc_fence_after();
-          scores(t, j + 1, stage);
-        }
+        if (last) ++nq;
+        v0 = v1, w0 = w1;
+        v1 = c + 1;
+        w1 = steps | (j > b0 ? 16u : 0u) | (last ? 32u : 0u);
+        if (made == used) v0 = v1, w0 = w1;
+        ++made;
+        moved = true;
       }
+      if (moved) {
+        c += 2;
+        ++j;
+        open = j < end;
+      }
+    }
+    const uint32_t v = made - used == 2 ? v0 : v1, w = made - used == 2 ? w0 : w1;
+    if (made != used && ready(&sh.p_full[t][used & 1], used >> 1) &&
+        ready(&sh.kv_full[v % S::kStages], v / S::kStages)) {
+      // O += P V_j, 16 keys at a time
+      const uint32_t vs = v % S::kStages;
+      const uint64_t b = v_desc + vs * (S::kBlock >> 4);
+      const uint32_t a = tmem + (used & 1) * kKeys;
+      ptx::tc_fence_after();
+      if (ptx::elect_one()) {
+#pragma unroll
+        for (int k = 0; k < kKeys / 16; ++k)
+          if (k < (int)(w & 15u))
+            ptx::mma_f16_ts(tmem + 128, a + k * 8, b + k * (2048 >> 4), kPvDesc, k ? 1u : w & 16u);
+        ptx::mma_commit(&sh.kv_empty[vs]);
+        ptx::mma_commit(&sh.pv_done[t]);
+        if (w & 32u) ptx::mma_commit(&sh.o_full[t]);
+      }
+      __syncwarp();
+      ++used;
+      moved = true;
+    }
+    if (moved) {
+      idle = 0;
+    } else if (++idle >= ptx::kWaitLimit || ((idle & 1023u) == 0 && __any_sync(kFull, *(volatile int *)&sh.abort))) {
+      sh.abort = 1;
+      raise_error(p.batch.err, TIDE_DEVERR_TIMEOUT);
+      return;
     }
   }
 }
@@ -479,7 +521,7 @@ __device__ void clean_values(const Params &p, Shared &sh, unsigned char *ring) {
       const uint32_t stage = (c0 + 2 * (j - u.b0) + 1) % S::kStages;
       TIDE_WAIT(&sh.raw_full[raw % S::kStages], (raw / S::kStages) & 1);
       ++raw;
-      unsigned char *v = ring + stage * S::kTile;
+      unsigned char *v = ring + stage * S::kBlock;
       const int seen = min(kKeys, sees - j * kKeys);  // rows that some token sees
       bool odd = false;
       // 8 16-byte vectors a row and column group; a swizzle moves them
@@ -543,14 +585,16 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 // 2^x of two numbers on the FMA pipes: x = n + f with n whole and f in
 // [-1/2, 1/2], 2^f by a polynomial that is within 2^-23.6 of it relatively
 // (minimax, degree 5, by an exchange iteration), n added to the exponent.
-// x below -126 counts as -126.  The special function unit takes four of a
+// x below -127, a masked score's -infinity among
+// them, counts as -127, which gives a subnormal number that is 0 in the
+// 16-bit types.  The special function unit takes four of a
 // warp's exponentials a cycle, so with all of them there it would bound the
 // kernel: kPoly of 16 pairs go this way.
 __device__ __forceinline__ void ex2_poly(uint64_t x, float *a, float *b) {
   constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to whole numbers
   float lo, hi;
   unpair(x, &lo, &hi);
-  x = pair(fmaxf(lo, -126.f), fmaxf(hi, -126.f));
+  x = pair(fmaxf(lo, -127.f), fmaxf(hi, -127.f));
   const uint64_t t = add2(x, pair(kMagic, kMagic));
   const uint64_t n = add2(t, pair(-kMagic, -kMagic));
   const uint64_t f = fma2(n, pair(-1.f, -1.f), x);
@@ -619,8 +663,31 @@ __device__ __forceinline__ void add_odd_values(const Params &p, const Unit &u, i
   }
 }
 
+// 128 bytes (eight 16-byte vectors) of each of a warp's 32 rows, row r in lane
+// r, to global memory: over shared memory, so that eight lanes write a row's
+// bytes side by side (a lane that wrote its own row would touch 32 lines an
+// instruction; the output of a unit took 4500 cycles that way).  `at` is the
+// lane's row in global memory, or NULL.
+__device__ __forceinline__ void store_rows(unsigned char *staging, const uint4 *v, unsigned char *at) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    *reinterpret_cast<uint4 *>(staging + lane * 128 + ((i ^ (lane & 7)) << 4)) = v[i];
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = i * 4 + (lane >> 3), e = lane & 7;
+    unsigned char *to = reinterpret_cast<unsigned char *>(
+        __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(at), r));
+    const uint4 x = *reinterpret_cast<const uint4 *>(staging + r * 128 + ((e ^ (r & 7)) << 4));
+    if (to) *reinterpret_cast<uint4 *>(to + e * 16) = x;
+  }
+}
+
 template <typename T, int D, bool PAGED>
-__device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem) {
+__device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem,
+                             unsigned char *staging) {
   constexpr unsigned kFull = 0xffffffffu;
   const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) & 3;
   const int r = warp * 32 + lane;                 // row of the tile
@@ -628,7 +695,7 @@ __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem) 
   const uint32_t s_col = tmem + ((uint32_t)(warp * 32) << 16) + t * 256;
   const uint32_t o_col = s_col + 128;
   const float slack = kSlack / p.qs;
-  uint32_t ns = 0, no = 0;
+  uint32_t ns = 0, no = 0;  // blocks and units so far
   for (uint32_t n = 0;; ++n) {
     TIDE_NEXT_UNIT(u, n);
     const int tokens = tile_tokens(u, p.tokens, t);
@@ -636,8 +703,9 @@ __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem) 
     const int end = tile_end(u, p.tokens, t);
     const bool valid = tok < tokens;
     const bool busy = __any_sync(kFull, valid);  // (the first token's warps always are)
-    const int sees = u.pos0 + t * p.tokens + tok + 1;  // keys this row sees
     const int last = tile_sees(u, p.tokens, t);
+    // keys this row sees (a row that is not there: as many as the last one)
+    const int sees = valid ? u.pos0 + t * p.tokens + tok + 1 : last;
     const int64_t row = u.row0 + t * p.tokens + tok;
     float m = -INFINITY, l = 0.f;
     if (p.zero_keys && valid) {  // keys of score 0 whose values add nothing
@@ -645,20 +713,19 @@ __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem) 
       if (z) m = 0.f;
       l = (float)z;
     }
-    for (int j = u.b0; j < end; ++j) {
-      TIDE_WAIT(&sh.s_full[t], ns & 1);
-      ++ns;
+    for (int j = u.b0; j < end; ++j, ++ns) {
+      const uint32_t col = s_col + (ns & 1) * kKeys;
+      TIDE_WAIT(&sh.s_full[t][ns & 1], (ns >> 1) & 1);
       if (busy) {
         ptx::tc_fence_after();
-        const int cols = min(kKeys, last - j * kKeys);  // the rest has not been computed
         uint32_t sr[kKeys];
         float *s = reinterpret_cast<float *>(sr);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) ptx::tmem_ld32_async(s_col + q * 32, sr + q * 32);
+        ptx::tmem_ld32_async(col, sr);
+        ptx::tmem_ld32_async(col + 32, sr + 32);
         ptx::tmem_wait_ld();
-#pragma unroll
-        for (int q = 0; q < 4; ++q) ptx::tmem_landed(sr + q * 32);
-        const int lim = min(sees - j * kKeys, cols);
+        ptx::tmem_landed(sr);
+        ptx::tmem_landed(sr + 32);
+        const int lim = sees - j * kKeys;  // past it: masked, or not computed
         if (__any_sync(kFull, lim < kKeys)) {
 #pragma unroll
           for (int i = 0; i < kKeys; ++i) s[i] = i < lim ? s[i] : -INFINITY;
@@ -677,6 +744,9 @@ __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem) 
         } else {
           const bool raise = top > m + slack;
           if (__any_sync(kFull, raise)) {
+            // O is complete up to the block before last; wait for the last
+            TIDE_WAIT(&sh.pv_done[t], (ns - 1) & 1);
+            ptx::tc_fence_after();
             const float a = raise ? ex2((m - top) * p.qs) : 1.f;
             if (raise) m = top;
             l *= a;
@@ -696,7 +766,7 @@ __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem) 
         const uint64_t qs2 = pair(p.qs, p.qs), mq2 = pair(-mq, -mq);
         uint64_t sum0 = 0, sum1 = 0;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < kKeys / 32; ++q) {
           uint32_t w[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -713,7 +783,7 @@ __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem) 
             else sum0 = add2(sum0, pair(a, b));
             w[i] = pack2<T>(a, b);
           }
-          ptx::tmem_st16(s_col + q * 16, w);
+          ptx::tmem_st16(col + q * 16, w);
         }
         float la, lb;
         unpair(add2(sum0, sum1), &la, &lb);
@@ -722,8 +792,9 @@ __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem) 
         ptx::tc_fence_before();
       }
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&sh.p_full[t]);
+      if (lane == 0) ptx::mbar_arrive(&sh.p_full[t][ns & 1]);
     }
+    if (m == -INFINITY) l = 0.f;  // nothing seen: drop the subnormal sums
     const bool some = end > u.b0;
     if (some) {
       TIDE_WAIT(&sh.o_full[t], no & 1);
@@ -733,40 +804,46 @@ __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem) 
     if (!busy) continue;
     const bool odd = some && sh.odd[n & 3];
     const int first = max(u.pos0 + 1, u.b0 * kKeys);
-    const int stop = min(sees, min(end * kKeys, last));
+    const int stop = valid ? min(sees, min(end * kKeys, last)) : first;
     const int64_t at = row * p.hq + u.kvh * p.group + head;
-    const bool nothing = !some || (l == 0.f);
+    const bool nothing = !some || l == 0.f;
     const float inv = nothing ? 0.f : 1.f / l;
-    if (p.splits > 1 && valid)
-      p.part_ml[(int64_t)u.split * p.batch.n_tokens * p.hq + at] = make_float2(m * p.qs, l);
-    if (p.splits > 1 && !some) continue;  // a sum of 0: its output is not read
+    if (p.splits > 1) {
+      const int64_t part = (int64_t)u.split * p.batch.n_tokens * p.hq + at;
+      if (valid) p.part_ml[part] = make_float2(m * p.qs, l);
+      if (some) {  // (else a sum of 0: its output is not read)
 #pragma unroll 1
-    for (int q = 0; q < D; q += 32) {
-      uint32_t o[32];
-      if (some) {
-        ptx::tmem_ld32_async(o_col + q, o);
-        ptx::tmem_wait_ld();
-        ptx::tmem_landed(o);
-      }
-      float *f = reinterpret_cast<float *>(o);
-      if (odd) add_odd_values<T, D, PAGED>(p, u, first, valid ? stop : first, q, f);
-      if (p.splits > 1) {
-        if (valid) {
-          float4 *dst = reinterpret_cast<float4 *>(
-              p.part_o + ((int64_t)u.split * p.batch.n_tokens * p.hq + at) * D + q);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) dst[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+        for (int q = 0; q < D; q += 32) {
+          uint32_t o[32];
+          ptx::tmem_ld32_async(o_col + q, o);
+          ptx::tmem_wait_ld();
+          ptx::tmem_landed(o);
+          if (odd) add_odd_values<T, D, PAGED>(p, u, first, stop, q, reinterpret_cast<float *>(o));
+          store_rows(staging, reinterpret_cast<const uint4 *>(o),
+                     valid ? reinterpret_cast<unsigned char *>(p.part_o + part * D + q) : nullptr);
         }
-        continue;
       }
-      uint32_t w[16];
+    } else {
+#pragma unroll 1
+      for (int q = 0; q < D; q += 64) {
+        uint32_t w[32];
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        w[i] = nothing ? 0u : pack2<T>(f[2 * i] * inv, f[2 * i + 1] * inv);
-      if (valid) {
-        uint4 *dst = reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + at * D + q);
+        for (int h = 0; h < 2; ++h) {
+          uint32_t o[32];
+          if (some) {
+            ptx::tmem_ld32_async(o_col + q + h * 32, o);
+            ptx::tmem_wait_ld();
+            ptx::tmem_landed(o);
+          }
+          float *f = reinterpret_cast<float *>(o);
+          if (odd) add_odd_values<T, D, PAGED>(p, u, first, stop, q + h * 32, f);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) dst[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+          for (int i = 0; i < 16; ++i)
+            w[h * 16 + i] = nothing ? 0u : pack2<T>(f[2 * i] * inv, f[2 * i + 1] * inv);
+        }
+        store_rows(staging, reinterpret_cast<const uint4 *>(w),
+                   valid ? reinterpret_cast<unsigned char *>(static_cast<T *>(p.out) + at * D + q)
+                         : nullptr);
       }
     }
     ptx::tc_fence_before();
@@ -782,22 +859,26 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ unsigned char dyn[];
   __shared__ Shared sh;
   unsigned char *base = dyn + ((1024u - (ptx::smem_u32(dyn) & 1023u)) & 1023u);
-  unsigned char *q_smem = base, *ring = base + 2 * S::kTile;
+  unsigned char *q_smem = base, *ring = base + 2 * S::kQ;
+  unsigned char *staging = ring + S::kStages * S::kBlock;
   const int warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
       ptx::mbar_init(&sh.q_full[t], 1);
       ptx::mbar_init(&sh.q_empty[t], 1);
-      ptx::mbar_init(&sh.s_full[t], 1);
-      ptx::mbar_init(&sh.p_full[t], 4);
+      for (int b = 0; b < 2; ++b) {
+        ptx::mbar_init(&sh.s_full[t][b], 1);
+        ptx::mbar_init(&sh.p_full[t][b], 4);
+      }
+      ptx::mbar_init(&sh.pv_done[t], 1);
       ptx::mbar_init(&sh.o_full[t], 1);
       ptx::mbar_init(&sh.u_full[t], 1);
-      ptx::mbar_init(&sh.u_empty[t], 11);
+      ptx::mbar_init(&sh.u_empty[t], kReaders);
+      ptx::mbar_init(&sh.drain[t], 1);
     }
-    ptx::mbar_init(&sh.drain, 1);
     for (int i = 0; i < S::kStages; ++i) {
       ptx::mbar_init(&sh.kv_full[i], 1);
-      ptx::mbar_init(&sh.kv_empty[i], 1);
+      ptx::mbar_init(&sh.kv_empty[i], 2);  // both tiles
       ptx::mbar_init(&sh.raw_full[i], 1);
       sh.raw[i] = 0;
     }
@@ -814,29 +895,27 @@ __global__ void __launch_bounds__(kThreads, 1)
   ptx::tc_fence_after();
   const uint32_t tmem = sh.tmem;
 
-  // Registers move from the four service warps to the softmax warps:
-  // 256 * 216 + 128 * 72 = 384 * 168, what the block was launched with.
-  if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-  else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-  if (warp < 4) {
-    softmax_tile<T, D, PAGED>(p, sh, 0, tmem);
-  } else if (warp < 8) {
-    softmax_tile<T, D, PAGED>(p, sh, 1, tmem);
+  // Registers move to the softmax warps: 256 * 176 + 256 * 80 = 512 * 128, what
+  // the block was launched with.
+  if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+  if (warp < 8) {
+    softmax_tile<T, D, PAGED>(p, sh, warp >> 2, tmem, staging + warp * 4096);
   } else if (warp == 8) {
     schedule_units(p, sh);
   } else if (warp == 9) {
     load_units<D, PAGED>(p, sh, q_smem, ring, &mq, &mk, &mv);
-  } else if (warp == 10) {
-    issue_products<T, D>(p, sh, ptx::smem_u32(q_smem), ptx::smem_u32(ring), tmem);
+  } else if (warp < 12) {
+    issue_products<T, D>(p, sh, warp - 10, ptx::smem_u32(q_smem), ptx::smem_u32(ring), tmem);
     __syncwarp();
     // every product done before its memory goes (after an abort too; bounded)
     if (ptx::elect_one()) {
       volatile int none = 0;
-      ptx::mma_commit(&sh.drain);
-      ptx::mbar_wait(&sh.drain, 0, &none);
+      ptx::mma_commit(&sh.drain[warp - 10]);
+      ptx::mbar_wait(&sh.drain[warp - 10], 0, &none);
     }
     __syncwarp();
-  } else {
+  } else if (warp == 12) {
     clean_values<T, D>(p, sh, ring);
   }
   __syncthreads();
@@ -972,13 +1051,13 @@ int64_t most_units(int64_t n_tokens, int64_t n_seqs, int64_t hq, int64_t hkv) {
 }
 
 // Splits of the keys: as many as give every SM a unit, but no split of fewer
-// than four blocks of 128 keys, whose start and join would cost more than
-// their keys.
+// than eight blocks of keys, whose start and join would cost more than their
+// keys.
 int64_t key_splits(int64_t n_tokens, int64_t n_seqs, int64_t hq, int64_t hkv, int64_t max_kv) {
   const int64_t units = most_units(n_tokens, n_seqs, hq, hkv);
   const int64_t blocks = (max_kv + tide::ragged::kKeys - 1) / tide::ragged::kKeys;
   int64_t s = units > 0 ? 148 / units : 1;
-  if (s > blocks / 4) s = blocks / 4;
+  if (s > blocks / 8) s = blocks / 8;
   return s < 1 ? 1 : s;
 }
 
