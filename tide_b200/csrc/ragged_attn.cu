@@ -8,33 +8,34 @@
 // A tile is 128 rows: floor(128 / G) consecutive tokens of a sequence times
 // the G query heads of one KV head, so that a key or value loaded serves all
 // heads that share it.  A unit of work is two such tiles, one behind the
-// other; a persistent CTA per SM walks over units.  Per block of 64 keys and
+// other; a persistent CTA per SM walks over units.  Per block of 128 keys and
 // tile,
-//   S[128 x 64] = Q K^T       tcgen05.mma, operands in shared memory (TMA,
+//   S[128 x 128] = Q K^T      tcgen05.mma, operands in shared memory (TMA,
 //                             128-byte swizzle), S in tensor memory;
 //   P = 2^(S qs - m)          one thread per row: running maximum m and sum l,
 //                             P rounded to the rows' 16-bit type (half a step
 //                             of it relative per weight; the sum l is of the
-//                             unrounded ones) and written over S;
+//                             unrounded ones) and written over a half of S;
 //   O[128 x D] += P V         tcgen05.mma with P from tensor memory and V as
 //                             it lies in shared memory (its MN-major operand).
-// Each tile has two S buffers, so that its next scores are there when its
-// softmax warps come for them: with blocks of 128 keys and one buffer the
-// chain score product - softmax - value product of a tile was serial, at 4000
-// cycles per 128 keys of both tiles, of which the tensor core worked 2200.
-// Each tile also has a warp of its own that issues its products, in whatever
-// order they become ready, over the ends of units.
+// The chain of a tile (scores, softmax, values, the next scores) is longer than
+// its share of the tensor core's time; two tiles half a period apart fill in
+// for one another.  One warp issues the products of both in turn, which keeps
+// them apart: with a warp each they fall into step and every phase waits for
+// the other tile's same phase.  The chain is cut where it can be: the value
+// product starts on three quarters of P while the last quarter's exponentials
+// run, and a unit's first scores are made while the one before is written out.
 //
 // m is only raised, and O and l rescaled, when a row's maximum has grown by
 // more than 2^8 since: weights up to 256 cost nothing (fp32 sums; 16-bit
 // floats round relatively), and O stays where it is.
 //
 // Roles of the warps: 0-3 and 4-7 the softmax and the output of tile 0
-// and 1; 8 finds the units; 9 loads; 10 and 11 issue the tiles' products; 12
-// cleans the value blocks that not every row sees: a masked weight is 0, but
-// 0 * NaN is not, so rows past the last visible key are zeroed, and a value
-// that is not finite at a position that only the later rows see is zeroed,
-// noted, and added to the outputs of the rows that do see it.
+// and 1; 8 finds the units; 9 loads; 10 issues the products; 11 cleans the
+// value blocks that not every row sees: a masked weight is 0, but 0 * NaN is
+// not, so rows past the last visible key are zeroed, and a value that is not
+// finite at a position that only the later rows see is zeroed, noted, and
+// added to the outputs of the rows that do see it.
 //
 // Order of units: by the number of keys they read, most first (the level of a
 // unit: positions before its end, in units of its size), so that the last
@@ -60,9 +61,10 @@ namespace ragged {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kRows = 128;   // rows of a tile
-constexpr int kKeys = 64;    // keys of a block
-constexpr int kWarps = 16;   // three of them only lend their registers
-constexpr int kReaders = 12; // warps that read the units
+constexpr int kKeys = 128;   // keys of a block
+constexpr int kQuarter = 32; // keys of a quarter of it
+constexpr int kWarps = 12;
+constexpr int kReaders = 11; // warps that read the units: all but the one that finds them
 constexpr int kThreads = 32 * kWarps;
 constexpr int kCached = 4;   // sequences per lane that the unit search keeps in registers
 constexpr float kSlack = 8.f;  // log2 of how far a maximum may grow before a rescale
@@ -74,7 +76,7 @@ struct Shape {
   static constexpr uint32_t kQ = kQHalf * kHalves;     // of a Q tile
   static constexpr uint32_t kHalf = kKeys * 128;       // of a column group of a K or V block
   static constexpr uint32_t kBlock = kHalf * kHalves;  // of a K or V block
-  static constexpr int kStages = 8;                    // K and V blocks in flight
+  static constexpr int kStages = D == 128 ? 4 : 8;     // K and V blocks in flight
   static constexpr uint32_t kStaging = 8 * 4096;       // 32 rows x 128 bytes per softmax warp
   static constexpr uint32_t kSmem = 2 * kQ + kStages * kBlock + kStaging + 1024;  // + alignment
 };
@@ -130,15 +132,15 @@ __device__ __forceinline__ bool cleaned_rows(const Unit &u, int sees, int j, int
   return *from < *to;
 }
 
-constexpr int kRing = 8;  // stages of every Shape
+constexpr int kRing = 8;  // the most stages of a Shape
 
 struct Shared {
   uint64_t q_full[2], q_empty[2];
-  uint64_t s_full[2][2], p_full[2][2];  // [tile][buffer]
-  uint64_t pv_done[2];                  // after every value product of a tile
-  uint64_t o_full[2];                   // after the last one of a unit
+  uint64_t s_full[2];
+  uint64_t p_full[2][2];  // [tile]: three quarters of P, the last quarter
+  uint64_t o_full[2];     // after a unit's last value product
   uint64_t u_full[2], u_empty[2];
-  uint64_t drain[2];
+  uint64_t drain;
   uint64_t kv_full[kRing], kv_empty[kRing];
   uint64_t raw_full[kRing];  // value blocks that have landed and are to be cleaned, in turn
   Unit unit[2];
@@ -348,150 +350,127 @@ __device__ void load_units(const Params &p, Shared &sh, unsigned char *q_smem,
           ptx::tma_load_3d(dst + lane * S::kHalf, m, full, lane * 64, u.kvh, u.key0 + j * kKeys);
         }
         ++c;
-      }
-      if (j == u.b0)  // the first keys and values are on their way
-        for (int t = 0; t < 2; ++t) {
-          if (ends[t] <= u.b0) continue;
-          if (nq[t] >= 1) TIDE_WAIT(&sh.q_empty[t], (nq[t] + 1) & 1);
-          ++nq[t];
-          if (lane == 0) {
-            sh.q_loaded[t] = (int)nq[t];
-            ptx::mbar_expect_tx(&sh.q_full[t], q_bytes);
+        // The queries go between the first keys and values: the products wait
+        // for Q before they free what the values need.
+        if (j == u.b0 && kv == 0)
+          for (int t = 0; t < 2; ++t) {
+            if (ends[t] <= u.b0) continue;
+            if (nq[t] >= 1) TIDE_WAIT(&sh.q_empty[t], (nq[t] + 1) & 1);
+            ++nq[t];
+            if (lane == 0) {
+              sh.q_loaded[t] = (int)nq[t];
+              ptx::mbar_expect_tx(&sh.q_full[t], q_bytes);
+            }
+            __syncwarp();
+            if (lane < S::kHalves)
+              ptx::tma_load_3d(q_smem + t * S::kQ + lane * S::kQHalf, mq, &sh.q_full[t], lane * 64,
+                               u.kvh * p.group, u.row0 + t * p.tokens);
           }
-          __syncwarp();
-          if (lane < S::kHalves)
-            ptx::tma_load_3d(q_smem + t * S::kQ + lane * S::kQHalf, mq, &sh.q_full[t], lane * 64,
-                             u.kvh * p.group, u.row0 + t * p.tokens);
-        }
+      }
       row = next;
     }
   }
 }
 
 // --------------------------------------------------------------- products
-// Tile t's products, in the order in which they become possible: a score
-// product when its K block (and Q) has landed and fewer than two are ahead of
-// the value products, a value product when its P is written.  Neither waits
-// for the other, so the next unit's first scores are made while this unit's
-// last softmax runs.  K and V blocks that the other tile alone sees are passed
-// on.  The whole warp walks through the schedule with values that are the same
-// in every lane (the shuffles tell the compiler so), and one elected lane
-// issues: the operands of tcgen05.mma live in uniform registers, and per-lane
-// values would be moved there one by one, at 107 cycles a product of 128 keys
-// instead of 80.
+// The products of both tiles, in turn: per block and tile the value product,
+// as soon as P is written, then the scores of the next block.  The last tile
+// that reads a block frees it.  What the warp does between two products is on
+// the chain of both tiles, so it is kept short.  The whole warp walks through
+// the schedule with values that are the same in every lane, and one elected
+// lane issues: the operands of tcgen05.mma live in uniform registers, and
+// per-lane values would be moved there one by one (107 cycles a product
+// instead of 80).  uniform() tells the compiler: a reduction over the warp is
+// a uniform value.
+__device__ __forceinline__ int uniform(int x) {
+  return (int)__reduce_or_sync(0xffffffffu, (unsigned)x);
+}
+
 template <typename T, int D>
-__device__ void issue_products(const Params &p, Shared &sh, int t, uint32_t q_smem, uint32_t ring,
+__device__ void issue_products(const Params &p, Shared &sh, uint32_t q_smem, uint32_t ring,
                                uint32_t tmem) {
   using S = Shape<D>;
-  constexpr unsigned kFull = 0xffffffffu;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t kPvDesc = ptx::f16_idesc(kBf16, kRows, D) | ptx::kIdescMnMajorB;
-  t = __shfl_sync(kFull, t, 0);
-  tmem = __shfl_sync(kFull, tmem, 0) + t * 256;
-  const uint64_t q_desc = ptx::sw128_kmajor_desc(q_smem + t * S::kQ);
-  const uint64_t k_desc = ptx::sw128_kmajor_desc(ring);
-  const uint64_t v_desc = ptx::sw128_mnmajor_desc(ring, S::kHalf);
-  auto ready = [&](uint64_t *bar, uint32_t phase) {
-    return __all_sync(kFull, ptx::mbar_test(bar, phase & 1)) != 0;
-  };
-  uint32_t n = 0, nq = 0;       // units and Q tiles taken
-  uint32_t c = 0;               // ring count of the next K block
-  uint32_t made = 0, used = 0;  // score and value products issued
-  bool open = false, done = false;
-  int j = 0, b0 = 0, end_t = 0, end = 0, sees = 0;  // of the unit that scores are made for
-  // the (up to two) value products to come: ring count of V, 16-key steps,
-  // whether O holds earlier ones, whether the unit ends
-  uint32_t v0 = 0, v1 = 0, w0 = 0, w1 = 0;
-  for (uint32_t idle = 0; !done || used != made;) {
-    bool moved = false;
-    if (!done && !open) {
-      if (ready(&sh.u_full[n & 1], n >> 1)) {
-        const Unit u = sh.unit[n & 1];
-        __syncwarp();
-        if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&sh.u_empty[n & 1]);
-        ++n;
-        done = __shfl_sync(kFull, u.valid, 0) == 0;
-        b0 = j = __shfl_sync(kFull, u.b0, 0);
-        end_t = __shfl_sync(kFull, tile_end(u, p.tokens, t), 0);
-        end = max(end_t, __shfl_sync(kFull, tile_end(u, p.tokens, t ^ 1), 0));
-        sees = __shfl_sync(kFull, tile_sees(u, p.tokens, t), 0);
-        open = !done && end > b0;
-        moved = true;
+  constexpr uint32_t kBlockDesc = S::kBlock >> 4;
+  tmem = (uint32_t)uniform((int)tmem);
+  const uint64_t q_desc = ptx::sw128_kmajor_desc((uint32_t)uniform((int)q_smem));
+  const uint64_t k_desc = ptx::sw128_kmajor_desc((uint32_t)uniform((int)ring));
+  const uint64_t v_desc = ptx::sw128_mnmajor_desc((uint32_t)uniform((int)ring), S::kHalf);
+  uint32_t stage = 0, lap = 0;  // of the next K block
+  uint32_t nq = 0, np = 0;      // bit t: phases of tile t's barriers
+  for (uint32_t n = 0;; ++n) {
+    TIDE_NEXT_UNIT(u, n);
+    const int b0 = uniform(u.b0);
+    const int end0 = uniform(tile_end(u, p.tokens, 0)), end1 = uniform(tile_end(u, p.tokens, 1));
+    const int sees0 = uniform(tile_sees(u, p.tokens, 0)), sees1 = uniform(tile_sees(u, p.tokens, 1));
+    const int end = max(end0, end1);
+    if (end <= b0) continue;
+    // S_t = Q_t K_j^T over the keys that the tile sees, rounded up to 16
+    auto scores = [&](int t, int j, uint32_t k_stage) {
+      const int keys = min(kKeys, (t ? sees1 : sees0) - j * kKeys);
+      const uint32_t idesc = ptx::f16_idesc(kBf16, kRows, 0) | (uint32_t)((keys + 15) / 16 * 2) << 17;
+      const uint64_t a = q_desc + t * (S::kQ >> 4), b = k_desc + k_stage * kBlockDesc;
+      if (ptx::elect_one()) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          ptx::mma_f16_ss(tmem + t * 256, a + (k / 4) * (S::kQHalf >> 4) + (k % 4) * 2,
+                          b + (k / 4) * (S::kHalf >> 4) + (k % 4) * 2, idesc, k > 0);
+        ptx::mma_commit(&sh.s_full[t]);
+        if (j + 1 == (t ? end1 : end0)) ptx::mma_commit(&sh.q_empty[t]);
+        if (t == 1 || j >= end1) ptx::mma_commit(&sh.kv_empty[k_stage]);
       }
-    } else if (open && made - used < 2) {
-      const uint32_t ks = c % S::kStages, vs = (c + 1) % S::kStages;
-      if (j >= end_t) {
-        // (only with no value product to come, so that no stage is tested
-        // for its next copy while this one has yet to land)
-        if (made == used && ready(&sh.kv_full[ks], c / S::kStages) &&
-            ready(&sh.kv_full[vs], (c + 1) / S::kStages)) {
-          if (ptx::elect_one()) {
-            ptx::mbar_arrive(&sh.kv_empty[ks]);
-            ptx::mbar_arrive(&sh.kv_empty[vs]);
-          }
-          __syncwarp();
-          moved = true;
-        }
-      } else if ((j > b0 || ready(&sh.q_full[t], nq)) && ready(&sh.kv_full[ks], c / S::kStages)) {
-        // S = Q K_j^T over the keys that the tile sees
-        const int keys = min(kKeys, sees - j * kKeys);
-        const uint32_t steps = (uint32_t)(keys + 15) / 16;
-        const uint32_t idesc = ptx::f16_idesc(kBf16, kRows, (int)steps * 16);
-        const uint64_t b = k_desc + ks * (S::kBlock >> 4);
-        const uint32_t d = tmem + (made & 1) * kKeys;
-        const bool last = j + 1 == end_t;
+      __syncwarp();
+    };
+    TIDE_WAIT(&sh.kv_full[stage], lap & 1);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      if (b0 >= (t ? end1 : end0)) continue;
+      TIDE_WAIT(&sh.q_full[t], (nq >> t) & 1);
+      nq ^= 1u << t;
+      ptx::tc_fence_after();
+      scores(t, b0, stage);
+    }
+    for (int j = b0; j < end; ++j) {
+      uint32_t v_stage = stage + 1, v_lap = lap;
+      if (v_stage == S::kStages) v_stage = 0, ++v_lap;
+      stage = v_stage + 1, lap = v_lap;
+      if (stage == S::kStages) stage = 0, ++lap;
+      TIDE_WAIT(&sh.kv_full[v_stage], v_lap & 1);
+      if (j + 1 < end) TIDE_WAIT(&sh.kv_full[stage], lap & 1);  // K of the next block
+      const uint64_t vb = v_desc + v_stage * kBlockDesc;
+      const uint32_t more = j > b0;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int end_t = t ? end1 : end0;
+        if (j >= end_t) continue;
+        // O_t += P_t V_j, 16 keys at a time: three quarters of the block as
+        // soon as they are there, then the rest
+        const int steps = (min(kKeys, (t ? sees1 : sees0) - j * kKeys) + 15) / 16;
+        const uint32_t o_col = tmem + t * 256 + kKeys, p_col = tmem + t * 256 + kKeys / 2;
+        TIDE_WAIT(&sh.p_full[t][0], (np >> t) & 1);
         ptx::tc_fence_after();
         if (ptx::elect_one()) {
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            ptx::mma_f16_ss(d, q_desc + (k / 4) * (S::kQHalf >> 4) + (k % 4) * 2,
-                            b + (k / 4) * (S::kHalf >> 4) + (k % 4) * 2, idesc, k > 0);
-          ptx::mma_commit(&sh.s_full[t][made & 1]);
-          ptx::mma_commit(&sh.kv_empty[ks]);
-          if (last) ptx::mma_commit(&sh.q_empty[t]);
+          for (int k = 0; k < 6; ++k)
+            if (k < steps)
+              ptx::mma_f16_ts(o_col, p_col + k * 8, vb + k * (2048 >> 4), kPvDesc, k ? 1u : more);
         }
         __syncwarp();
-        if (last) ++nq;
-        v0 = v1, w0 = w1;
-        v1 = c + 1;
-        w1 = steps | (j > b0 ? 16u : 0u) | (last ? 32u : 0u);
-        if (made == used) v0 = v1, w0 = w1;
-        ++made;
-        moved = true;
-      }
-      if (moved) {
-        c += 2;
-        ++j;
-        open = j < end;
-      }
-    }
-    const uint32_t v = made - used == 2 ? v0 : v1, w = made - used == 2 ? w0 : w1;
-    if (made != used && ready(&sh.p_full[t][used & 1], used >> 1) &&
-        ready(&sh.kv_full[v % S::kStages], v / S::kStages)) {
-      // O += P V_j, 16 keys at a time
-      const uint32_t vs = v % S::kStages;
-      const uint64_t b = v_desc + vs * (S::kBlock >> 4);
-      const uint32_t a = tmem + (used & 1) * kKeys;
-      ptx::tc_fence_after();
-      if (ptx::elect_one()) {
+        TIDE_WAIT(&sh.p_full[t][1], (np >> t) & 1);
+        np ^= 1u << t;
+        ptx::tc_fence_after();
+        const bool last = j + 1 == end_t;
+        if (ptx::elect_one()) {
 #pragma unroll
-        for (int k = 0; k < kKeys / 16; ++k)
-          if (k < (int)(w & 15u))
-            ptx::mma_f16_ts(tmem + 128, a + k * 8, b + k * (2048 >> 4), kPvDesc, k ? 1u : w & 16u);
-        ptx::mma_commit(&sh.kv_empty[vs]);
-        ptx::mma_commit(&sh.pv_done[t]);
-        if (w & 32u) ptx::mma_commit(&sh.o_full[t]);
+          for (int k = 6; k < 8; ++k)
+            if (k < steps) ptx::mma_f16_ts(o_col, p_col + k * 8, vb + k * (2048 >> 4), kPvDesc, 1u);
+          if (last) ptx::mma_commit(&sh.o_full[t]);
+          if (t == 1 || j >= end1) ptx::mma_commit(&sh.kv_empty[v_stage]);
+        }
+        __syncwarp();
+        if (!last) scores(t, j + 1, stage);
       }
-      __syncwarp();
-      ++used;
-      moved = true;
-    }
-    if (moved) {
-      idle = 0;
-    } else if (++idle >= ptx::kWaitLimit || ((idle & 1023u) == 0 && __any_sync(kFull, *(volatile int *)&sh.abort))) {
-      sh.abort = 1;
-      raise_error(p.batch.err, TIDE_DEVERR_TIMEOUT);
-      return;
     }
   }
 }
@@ -503,11 +482,20 @@ __device__ __forceinline__ bool odd_value(uint32_t bits16) {
   return (bits16 & kExp) == kExp;
 }
 
+template <typename P2>
+__device__ __forceinline__ P2 make_pair() {  // two zeros
+  P2 r;
+  *reinterpret_cast<uint32_t *>(&r) = 0u;
+  return r;
+}
+
 template <typename T, int D>
 __device__ void clean_values(const Params &p, Shared &sh, unsigned char *ring) {
   using S = Shape<D>;
+  using Pair = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+  constexpr int kBatch = 4;  // vectors in flight per lane
   const int lane = threadIdx.x & 31;
-  uint32_t c0 = 0, raw = 0;
+  uint32_t c0 = 0, raw = 0;  // ring count of the unit's first K block, cleaned blocks
   for (uint32_t n = 0;; ++n) {
     TIDE_NEXT_UNIT(u, n);
     const int end = max(tile_end(u, p.tokens, 0), tile_end(u, p.tokens, 1));
@@ -515,7 +503,8 @@ __device__ void clean_values(const Params &p, Shared &sh, unsigned char *ring) {
     __syncwarp();
     if (end <= u.b0) continue;
     const int sees = u.pos0 + u.n;
-    for (int j = u.b0; j < end; ++j) {
+    // (only the last blocks hold positions past the first token's own)
+    for (int j = max(u.b0, (u.pos0 + 1) / kKeys); j < end; ++j) {
       int from, to;
       if (!cleaned_rows(u, sees, j, &from, &to)) continue;
       const uint32_t stage = (c0 + 2 * (j - u.b0) + 1) % S::kStages;
@@ -523,32 +512,42 @@ __device__ void clean_values(const Params &p, Shared &sh, unsigned char *ring) {
       ++raw;
       unsigned char *v = ring + stage * S::kBlock;
       const int seen = min(kKeys, sees - j * kKeys);  // rows that some token sees
-      bool odd = false;
-      // 8 16-byte vectors a row and column group; a swizzle moves them
-      // within their row only
-      for (int e = from * 8 + lane; e < to * 8; e += 32) {
+      // a row is 8 16-byte vectors in each column group; a swizzle moves them
+      // within their 128 bytes only
+      auto vec = [&](int e) {
+        return reinterpret_cast<uint4 *>(v + (e / 8 % S::kHalves) * S::kHalf +
+                                         e / (8 * S::kHalves) * 128 + e % 8 * 16);
+      };
+      constexpr int kRowVecs = 8 * S::kHalves;
+      for (int e = max(seen, from) * kRowVecs + lane; e < to * kRowVecs; e += 32)
+        *vec(e) = make_uint4(0, 0, 0, 0);
+      // x * 0 is NaN for a NaN and for an infinity: one instruction for two
+      // values (the warp that cleans shares its scheduler with two softmax
+      // warps, and the products wait for the block)
+      Pair zero, acc;
+      zero = acc = make_pair<Pair>();
+      for (int e = from * kRowVecs + lane; e < seen * kRowVecs; e += 32 * kBatch) {
+        uint4 x[kBatch];
 #pragma unroll
-        for (int h = 0; h < S::kHalves; ++h) {
-          uint4 *at = reinterpret_cast<uint4 *>(v + h * S::kHalf) + e;
-          uint4 x = *at;
-          uint32_t *w = reinterpret_cast<uint32_t *>(&x);
-          bool change = e >= seen * 8;
-          if (change) {
-            x = make_uint4(0, 0, 0, 0);
-          } else {
+        for (int i = 0; i < kBatch; ++i) x[i] = *vec(min(e + 32 * i, seen * kRowVecs - 1));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const bool lo = odd_value<T>(w[i]), hi = odd_value<T>(w[i] >> 16);
-              if (lo) w[i] &= 0xFFFF0000u;
-              if (hi) w[i] &= 0x0000FFFFu;
-              change |= lo | hi;
-            }
-            odd |= change;
-          }
-          if (change) *at = x;
+        for (int i = 0; i < kBatch; ++i) {
+          const Pair *w = reinterpret_cast<const Pair *>(&x[i]);
+#pragma unroll
+          for (int h = 0; h < 4; ++h) acc = __hfma2(w[h], zero, acc);
         }
       }
-      if (__any_sync(0xffffffffu, odd) && lane == 0) sh.odd[n & 3] = 1;
+      const bool odd = (*reinterpret_cast<uint32_t *>(&acc) & 0x7FFF7FFFu) != 0;
+      if (__any_sync(0xffffffffu, odd)) {
+        for (int e = from * kRowVecs + lane; e < seen * kRowVecs; e += 32) {
+          uint32_t *w = reinterpret_cast<uint32_t *>(vec(e));
+          for (int h = 0; h < 4; ++h) {
+            if (odd_value<T>(w[h])) w[h] &= 0xFFFF0000u;
+            if (odd_value<T>(w[h] >> 16)) w[h] &= 0x0000FFFFu;
+          }
+        }
+        if (lane == 0) sh.odd[n & 3] = 1;
+      }
       ptx::fence_proxy_async();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(&sh.kv_full[stage]);
@@ -582,48 +581,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// 2^x of two numbers on the FMA pipes: x = n + f with n whole and f in
-// [-1/2, 1/2], 2^f by a polynomial that is within 2^-23.6 of it relatively
-// (minimax, degree 5, by an exchange iteration), n added to the exponent.
-// x below -127, a masked score's -infinity among
-// them, counts as -127, which gives a subnormal number that is 0 in the
-// 16-bit types.  The special function unit takes four of a
-// warp's exponentials a cycle, so with all of them there it would bound the
-// kernel: kPoly of 16 pairs go this way.
-__device__ __forceinline__ void ex2_poly(uint64_t x, float *a, float *b) {
-  constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to whole numbers
-  float lo, hi;
-  unpair(x, &lo, &hi);
-  x = pair(fmaxf(lo, -127.f), fmaxf(hi, -127.f));
-  const uint64_t t = add2(x, pair(kMagic, kMagic));
-  const uint64_t n = add2(t, pair(-kMagic, -kMagic));
-  const uint64_t f = fma2(n, pair(-1.f, -1.f), x);
-#ifndef POLY_DEG
-#define POLY_DEG 5
-#endif
-#if POLY_DEG == 5
-  uint64_t y = pair(0.0013276471992546789f, 0.0013276471992546789f);
-  y = fma2(y, f, pair(0.009675541334453112f, 0.009675541334453112f));
-  y = fma2(y, f, pair(0.05550713273498027f, 0.05550713273498027f));
-  y = fma2(y, f, pair(0.24022119723840024f, 0.24022119723840024f));
-  y = fma2(y, f, pair(0.6931469670647603f, 0.6931469670647603f));
-  y = fma2(y, f, pair(1.0000000716546849f, 1.0000000716546849f));
-#else
-  uint64_t y = pair(0.05517166905792616f, 0.05517166905792616f);
-  y = fma2(y, f, pair(0.2426111221932161f, 0.2426111221932161f));
-  y = fma2(y, f, pair(0.6932609854606553f, 0.6932609854606553f));
-  y = fma2(y, f, pair(0.9999280735394012f, 0.9999280735394012f));
-#endif
-  float yl, yh, tl, th;
-  unpair(y, &yl, &yh);
-  unpair(t, &tl, &th);
-  *a = __uint_as_float(__float_as_uint(yl) + (__float_as_uint(tl) << 23));
-  *b = __uint_as_float(__float_as_uint(yh) + (__float_as_uint(th) << 23));
-}
-#ifndef POLY
-#define POLY 4
-#endif
-constexpr int kPoly = POLY;
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -663,26 +620,46 @@ __device__ __forceinline__ void add_odd_values(const Params &p, const Unit &u, i
   }
 }
 
-// 128 bytes (eight 16-byte vectors) of each of a warp's 32 rows, row r in lane
-// r, to global memory: over shared memory, so that eight lanes write a row's
-// bytes side by side (a lane that wrote its own row would touch 32 lines an
-// instruction; the output of a unit took 4500 cycles that way).  `at` is the
-// lane's row in global memory, or NULL.
-__device__ __forceinline__ void store_rows(unsigned char *staging, const uint4 *v, unsigned char *at) {
+// N 16-byte vectors of each of a warp's 32 rows, row r in lane r, to global
+// memory: over shared memory, so that N lanes write a row's bytes side by side
+// (a lane that wrote its own row would touch 32 lines an instruction).  `at`
+// is the lane's row in global memory, or NULL.
+template <int N>
+__device__ __forceinline__ void store_rows(unsigned char *staging, const uint32_t *w,
+                                           unsigned char *at) {
+  constexpr int kRowsAtOnce = 32 / N;
   const int lane = threadIdx.x & 31;
   __syncwarp();
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    *reinterpret_cast<uint4 *>(staging + lane * 128 + ((i ^ (lane & 7)) << 4)) = v[i];
+  for (int i = 0; i < N; ++i)
+    *reinterpret_cast<uint4 *>(staging + lane * 128 + ((i ^ (lane & 7)) << 4)) =
+        make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
   __syncwarp();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = i * 4 + (lane >> 3), e = lane & 7;
+  for (int i = 0; i < N; ++i) {
+    const int r = i * kRowsAtOnce + lane / N, e = lane % N;
     unsigned char *to = reinterpret_cast<unsigned char *>(
         __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(at), r));
     const uint4 x = *reinterpret_cast<const uint4 *>(staging + r * 128 + ((e ^ (r & 7)) << 4));
     if (to) *reinterpret_cast<uint4 *>(to + e * 16) = x;
   }
+}
+
+// Weights of 32 scores, their sums, and their 16-bit form to tensor memory.
+template <typename T>
+__device__ __forceinline__ void weigh_quarter(const float *s, uint64_t qs2, uint64_t mq2,
+                                              uint64_t (&sum)[2], uint32_t p_col) {
+  uint32_t w[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    float a, b;
+    unpair(fma2(pair(s[2 * i], s[2 * i + 1]), qs2, mq2), &a, &b);
+    a = ex2(a);
+    b = ex2(b);
+    sum[i & 1] = add2(sum[i & 1], pair(a, b));
+    w[i] = pack2<T>(a, b);
+  }
+  ptx::tmem_st16(p_col, w);
 }
 
 template <typename T, int D, bool PAGED>
@@ -693,7 +670,7 @@ __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem,
   const int r = warp * 32 + lane;                 // row of the tile
   const int tok = r / p.group, head = r % p.group;
   const uint32_t s_col = tmem + ((uint32_t)(warp * 32) << 16) + t * 256;
-  const uint32_t o_col = s_col + 128;
+  const uint32_t p_col = s_col + kKeys / 2, o_col = s_col + kKeys;
   const float slack = kSlack / p.qs;
   uint32_t ns = 0, no = 0;  // blocks and units so far
   for (uint32_t n = 0;; ++n) {
@@ -714,87 +691,77 @@ __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem,
       l = (float)z;
     }
     for (int j = u.b0; j < end; ++j, ++ns) {
-      const uint32_t col = s_col + (ns & 1) * kKeys;
-      TIDE_WAIT(&sh.s_full[t][ns & 1], (ns >> 1) & 1);
-      if (busy) {
-        ptx::tc_fence_after();
-        uint32_t sr[kKeys];
-        float *s = reinterpret_cast<float *>(sr);
-        ptx::tmem_ld32_async(col, sr);
-        ptx::tmem_ld32_async(col + 32, sr + 32);
-        ptx::tmem_wait_ld();
-        ptx::tmem_landed(sr);
-        ptx::tmem_landed(sr + 32);
-        const int lim = sees - j * kKeys;  // past it: masked, or not computed
-        if (__any_sync(kFull, lim < kKeys)) {
-#pragma unroll
-          for (int i = 0; i < kKeys; ++i) s[i] = i < lim ? s[i] : -INFINITY;
+      TIDE_WAIT(&sh.s_full[t], ns & 1);
+      // The commit behind S_j follows the products of block j - 1 in the same
+      // stream: O is complete up to that block.
+      if (!busy) {
+        if (lane == 0) {
+          ptx::mbar_arrive(&sh.p_full[t][0]);
+          ptx::mbar_arrive(&sh.p_full[t][1]);
         }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int i = 0; i < kKeys; i += 8)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) mx[q] = max3(mx[q], s[i + 2 * q], s[i + 2 * q + 1]);
-        const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
-        if (j == u.b0) {  // nothing in O yet
-          if (top > m) {
-            l *= ex2((m - top) * p.qs);
-            m = top;
-          }
-        } else {
-          const bool raise = top > m + slack;
-          if (__any_sync(kFull, raise)) {
-            // O is complete up to the block before last; wait for the last
-            TIDE_WAIT(&sh.pv_done[t], (ns - 1) & 1);
-            ptx::tc_fence_after();
-            const float a = raise ? ex2((m - top) * p.qs) : 1.f;
-            if (raise) m = top;
-            l *= a;
-#pragma unroll 1
-            for (int q = 0; q < D; q += 32) {
-              uint32_t o[32];
-              ptx::tmem_ld32_async(o_col + q, o);
-              ptx::tmem_wait_ld();
-              ptx::tmem_landed(o);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
-              ptx::tmem_st32(o_col + q, o);
-            }
-          }
-        }
-        const float mq = m == -INFINITY ? 0.f : m * p.qs;
-        const uint64_t qs2 = pair(p.qs, p.qs), mq2 = pair(-mq, -mq);
-        uint64_t sum0 = 0, sum1 = 0;
-#pragma unroll
-        for (int q = 0; q < kKeys / 32; ++q) {
-          uint32_t w[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float a, b;
-            const uint64_t x = fma2(pair(s[q * 32 + 2 * i], s[q * 32 + 2 * i + 1]), qs2, mq2);
-            if ((i * kPoly) % 16 < kPoly) {
-              ex2_poly(x, &a, &b);
-            } else {
-              unpair(x, &a, &b);
-              a = ex2(a);
-              b = ex2(b);
-            }
-            if (i & 1) sum1 = add2(sum1, pair(a, b));
-            else sum0 = add2(sum0, pair(a, b));
-            w[i] = pack2<T>(a, b);
-          }
-          ptx::tmem_st16(col + q * 16, w);
-        }
-        float la, lb;
-        unpair(add2(sum0, sum1), &la, &lb);
-        l += la + lb;
-        ptx::tmem_wait_st();
-        ptx::tc_fence_before();
+        continue;
       }
+      ptx::tc_fence_after();
+      const int lim = sees - j * kKeys;        // keys from here on: masked, or not computed
+      uint32_t sr[kKeys];
+      float *s = reinterpret_cast<float *>(sr);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) ptx::tmem_ld32_async(s_col + q * kQuarter, sr + q * kQuarter);
+      ptx::tmem_wait_ld();
+#pragma unroll
+      for (int q = 0; q < 4; ++q) ptx::tmem_landed(sr + q * kQuarter);
+      if (__any_sync(kFull, lim < kKeys)) {
+#pragma unroll
+        for (int i = 0; i < kKeys; ++i) s[i] = i < lim ? s[i] : -INFINITY;
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < kKeys; i += 8)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) mx[q] = max3(mx[q], s[i + 2 * q], s[i + 2 * q + 1]);
+      const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+      if (j == u.b0) {  // nothing in O yet
+        if (top > m) {
+          l *= ex2((m - top) * p.qs);
+          m = top;
+        }
+      } else {
+        const bool raise = top > m + slack;
+        if (__any_sync(kFull, raise)) {
+          const float a = raise ? ex2((m - top) * p.qs) : 1.f;
+          if (raise) m = top;
+          l *= a;
+#pragma unroll 1
+          for (int q = 0; q < D; q += 16) {
+            uint32_t o[16];
+            ptx::tmem_ld16_async(o_col + q, o);
+            ptx::tmem_wait_ld();
+            ptx::tmem_landed16(o);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
+            ptx::tmem_st16(o_col + q, o);
+          }
+        }
+      }
+      const float mq = m == -INFINITY ? 0.f : m * p.qs;
+      const uint64_t qs2 = pair(p.qs, p.qs), mq2 = pair(-mq, -mq);
+      uint64_t sum[2] = {0, 0};
+      // S is in registers: P takes its upper half
+#pragma unroll
+      for (int q = 0; q < 3; ++q) weigh_quarter<T>(s + q * kQuarter, qs2, mq2, sum, p_col + q * 16);
+      ptx::tmem_wait_st();
+      ptx::tc_fence_before();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&sh.p_full[t][ns & 1]);
+      if (lane == 0) ptx::mbar_arrive(&sh.p_full[t][0]);
+      weigh_quarter<T>(s + 96, qs2, mq2, sum, p_col + 48);
+      ptx::tmem_wait_st();
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&sh.p_full[t][1]);
+      float la, lb;
+      unpair(add2(sum[0], sum[1]), &la, &lb);
+      l += la + lb;
     }
-    if (m == -INFINITY) l = 0.f;  // nothing seen: drop the subnormal sums
     const bool some = end > u.b0;
     if (some) {
       TIDE_WAIT(&sh.o_full[t], no & 1);
@@ -808,42 +775,30 @@ __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem,
     const int64_t at = row * p.hq + u.kvh * p.group + head;
     const bool nothing = !some || l == 0.f;
     const float inv = nothing ? 0.f : 1.f / l;
-    if (p.splits > 1) {
-      const int64_t part = (int64_t)u.split * p.batch.n_tokens * p.hq + at;
-      if (valid) p.part_ml[part] = make_float2(m * p.qs, l);
-      if (some) {  // (else a sum of 0: its output is not read)
+    const int64_t part = (int64_t)u.split * p.batch.n_tokens * p.hq + at;
+    if (p.splits > 1 && valid) p.part_ml[part] = make_float2(m * p.qs, l);
+    if (p.splits > 1 && !some) continue;  // (a sum of 0: its output is not read)
 #pragma unroll 1
-        for (int q = 0; q < D; q += 32) {
-          uint32_t o[32];
-          ptx::tmem_ld32_async(o_col + q, o);
-          ptx::tmem_wait_ld();
-          ptx::tmem_landed(o);
-          if (odd) add_odd_values<T, D, PAGED>(p, u, first, stop, q, reinterpret_cast<float *>(o));
-          store_rows(staging, reinterpret_cast<const uint4 *>(o),
-                     valid ? reinterpret_cast<unsigned char *>(p.part_o + part * D + q) : nullptr);
-        }
+    for (int q = 0; q < D; q += 32) {
+      uint32_t o[32];
+      if (some) {
+        ptx::tmem_ld32_async(o_col + q, o);
+        ptx::tmem_wait_ld();
+        ptx::tmem_landed(o);
       }
-    } else {
-#pragma unroll 1
-      for (int q = 0; q < D; q += 64) {
-        uint32_t w[32];
+      float *f = reinterpret_cast<float *>(o);
+      if (odd) add_odd_values<T, D, PAGED>(p, u, first, stop, q, f);
+      if (p.splits > 1) {
+        store_rows<8>(staging, o, valid ? reinterpret_cast<unsigned char *>(p.part_o + part * D + q)
+                                        : nullptr);
+      } else {
+        uint32_t w[16];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t o[32];
-          if (some) {
-            ptx::tmem_ld32_async(o_col + q + h * 32, o);
-            ptx::tmem_wait_ld();
-            ptx::tmem_landed(o);
-          }
-          float *f = reinterpret_cast<float *>(o);
-          if (odd) add_odd_values<T, D, PAGED>(p, u, first, stop, q + h * 32, f);
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            w[h * 16 + i] = nothing ? 0u : pack2<T>(f[2 * i] * inv, f[2 * i + 1] * inv);
-        }
-        store_rows(staging, reinterpret_cast<const uint4 *>(w),
-                   valid ? reinterpret_cast<unsigned char *>(static_cast<T *>(p.out) + at * D + q)
-                         : nullptr);
+        for (int i = 0; i < 16; ++i)
+          w[i] = nothing ? 0u : pack2<T>(f[2 * i] * inv, f[2 * i + 1] * inv);
+        store_rows<4>(staging, w,
+                      valid ? reinterpret_cast<unsigned char *>(static_cast<T *>(p.out) + at * D + q)
+                            : nullptr);
       }
     }
     ptx::tc_fence_before();
@@ -866,22 +821,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int t = 0; t < 2; ++t) {
       ptx::mbar_init(&sh.q_full[t], 1);
       ptx::mbar_init(&sh.q_empty[t], 1);
-      for (int b = 0; b < 2; ++b) {
-        ptx::mbar_init(&sh.s_full[t][b], 1);
-        ptx::mbar_init(&sh.p_full[t][b], 4);
-      }
-      ptx::mbar_init(&sh.pv_done[t], 1);
+      ptx::mbar_init(&sh.s_full[t], 1);
+      for (int b = 0; b < 2; ++b) ptx::mbar_init(&sh.p_full[t][b], 4);
       ptx::mbar_init(&sh.o_full[t], 1);
       ptx::mbar_init(&sh.u_full[t], 1);
       ptx::mbar_init(&sh.u_empty[t], kReaders);
-      ptx::mbar_init(&sh.drain[t], 1);
     }
     for (int i = 0; i < S::kStages; ++i) {
       ptx::mbar_init(&sh.kv_full[i], 1);
-      ptx::mbar_init(&sh.kv_empty[i], 2);  // both tiles
+      ptx::mbar_init(&sh.kv_empty[i], 1);
       ptx::mbar_init(&sh.raw_full[i], 1);
       sh.raw[i] = 0;
     }
+    ptx::mbar_init(&sh.drain, 1);
     ptx::fence_mbar_init();
     sh.abort = 0;
     sh.loaded = sh.raw_loaded = sh.q_loaded[0] = sh.q_loaded[1] = 0;
@@ -895,27 +847,27 @@ __global__ void __launch_bounds__(kThreads, 1)
   ptx::tc_fence_after();
   const uint32_t tmem = sh.tmem;
 
-  // Registers move to the softmax warps: 256 * 176 + 256 * 80 = 512 * 128, what
+  // Registers move to the softmax warps: 256 * 208 + 128 * 88 = 384 * 168, what
   // the block was launched with.
-  if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
-  else asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+  if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp < 8) {
     softmax_tile<T, D, PAGED>(p, sh, warp >> 2, tmem, staging + warp * 4096);
   } else if (warp == 8) {
     schedule_units(p, sh);
   } else if (warp == 9) {
     load_units<D, PAGED>(p, sh, q_smem, ring, &mq, &mk, &mv);
-  } else if (warp < 12) {
-    issue_products<T, D>(p, sh, warp - 10, ptx::smem_u32(q_smem), ptx::smem_u32(ring), tmem);
+  } else if (warp == 10) {
+    issue_products<T, D>(p, sh, ptx::smem_u32(q_smem), ptx::smem_u32(ring), tmem);
     __syncwarp();
     // every product done before its memory goes (after an abort too; bounded)
     if (ptx::elect_one()) {
       volatile int none = 0;
-      ptx::mma_commit(&sh.drain[warp - 10]);
-      ptx::mbar_wait(&sh.drain[warp - 10], 0, &none);
+      ptx::mma_commit(&sh.drain);
+      ptx::mbar_wait(&sh.drain, 0, &none);
     }
     __syncwarp();
-  } else if (warp == 12) {
+  } else {
     clean_values<T, D>(p, sh, ring);
   }
   __syncthreads();
@@ -1051,13 +1003,13 @@ int64_t most_units(int64_t n_tokens, int64_t n_seqs, int64_t hq, int64_t hkv) {
 }
 
 // Splits of the keys: as many as give every SM a unit, but no split of fewer
-// than eight blocks of keys, whose start and join would cost more than their
+// than four blocks of keys, whose start and join would cost more than their
 // keys.
 int64_t key_splits(int64_t n_tokens, int64_t n_seqs, int64_t hq, int64_t hkv, int64_t max_kv) {
   const int64_t units = most_units(n_tokens, n_seqs, hq, hkv);
   const int64_t blocks = (max_kv + tide::ragged::kKeys - 1) / tide::ragged::kKeys;
   int64_t s = units > 0 ? 148 / units : 1;
-  if (s > blocks / 8) s = blocks / 8;
+  if (s > blocks / 4) s = blocks / 4;
   return s < 1 ? 1 : s;
 }
 
