@@ -93,6 +93,7 @@ struct Params {
   int tokens;      // of a tile: kRows / group
   int splits;
   int split_blocks;  // key blocks of a split
+  int few;         // sequences of up to so many tokens go to the few-rows kernel
   float qs;        // scale * log2(e)
 };
 
@@ -167,7 +168,7 @@ struct Shared {
 __device__ __forceinline__ void seq_level(const Params &p, int i, int *count, int *level) {
   const Sequence s = sequence(p.batch, i);
   const int per = 2 * p.tokens;
-  *count = (s.n + per - 1) / per;
+  *count = s.n > p.few ? (s.n + per - 1) / per : 0;
   *level = max(s.kv - s.n, 0) / per;
 }
 
@@ -887,39 +888,437 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 10) ptx::tmem_dealloc(tmem, 512);
 }
 
+// --------------------------------------------------------- few rows a head
+// Sequences with so few tokens that their rows (tokens times the query heads
+// of a KV head) are at most 16 * MT: a decode step, a few drafted tokens.  Such
+// a unit reads 4 D bytes per key and does 4 D flops per key and row, so it is
+// bound by HBM, and the 128-row tiles above would leave it to one chain of
+// products and exponentials per SM.  Here a warp is on its own: it walks over
+// every fourth group of 16 keys of its CTA's share, with its own ring of TMA
+// copies (8 KB a group, three in flight) and its own running maxima, sums and
+// outputs, and the four meet once at the end.  No barrier but the ring's.
+//   S[16 MT x 16] = Q K^T   mma.sync m16n8k16, K by ldmatrix from the swizzled
+//                           copy; Q in registers;
+//   O[16 MT x D] += P V     P from the registers that held S (the accumulator
+//                           layout of one product is the operand layout of the
+//                           next), V by transposing ldmatrix.
+// (tcgen05 has nothing to give here: its rows would be 7/8 padding.)
+constexpr int kFewWarps = 4;
+constexpr int kFewStages = 3;
+constexpr int kFewKeys = 16;
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// D[16 x 8] += A[16 x 16] B[16 x 8], 16-bit operands, fp32 accumulators.
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+struct FewParams {
+  RaggedBatch batch;
+  KeySource src;
+  const void *q;
+  int64_t q_stride;
+  void *out;
+  float *part_o;    // [splits, n_seqs, few, hq, D] (splits > 1)
+  float2 *part_ml;  // [splits, n_seqs, few, hq]: maximum (scaled, base 2), sum
+  int hq, hkv, group;
+  int few;         // tokens a sequence may have: 16 MT / group
+  int splits;
+  int split_keys;  // keys of a split, a multiple of 16
+  float qs;
+};
+
+template <int D>
+struct Few {
+  static constexpr uint32_t kHalf = kFewKeys * 128;              // a 128-byte column group of 16 keys
+  static constexpr uint32_t kSide = kHalf * (D / 64);            // K or V of 16 keys
+  static constexpr uint32_t kRing = kFewStages * 2 * kSide;      // of a warp
+  static constexpr uint32_t kSmem = kFewWarps * kRing + 1024;    // + alignment
+};
+
+// Odd values among the keys that only the later rows of a unit see.  O of a
+// row gets the values it sees one by one; slow, and taken only when there is a
+// NaN or an infinity.
+// (Inlined: called, it would put O into local memory at every step.)
+template <typename T, int D, int MT>
+__device__ __forceinline__ void values_one_by_one(const unsigned char *v, const uint32_t (&pr)[MT][4],
+                                               const int (&lim)[MT][2], float (&o)[MT][D / 8][4]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int k = 0; k < kFewKeys; ++k) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      // P[row][k] sits in lane (row % 8) * 4 + (k % 8) / 2, register k / 8 * 2 + row / 8
+      const int from = (lane & ~3) + (k % 8) / 2;
+      const uint32_t pa = __shfl_sync(0xffffffffu, k < 8 ? pr[mt][0] : pr[mt][2], from);
+      const uint32_t pb = __shfl_sync(0xffffffffu, k < 8 ? pr[mt][1] : pr[mt][3], from);
+      const T *ha = reinterpret_cast<const T *>(&pa), *hb = reinterpret_cast<const T *>(&pb);
+      const float wa = Elem<T>::to_f(ha[k & 1]), wb = Elem<T>::to_f(hb[k & 1]);
+#pragma unroll
+      for (int nt = 0; nt < D / 8; ++nt) {
+        const int d = nt * 8 + (lane & 3) * 2, c = d / 8;
+        const T *x = reinterpret_cast<const T *>(v + (c / 8) * Few<D>::kHalf + k * 128 +
+                                                 (((c % 8) ^ (k & 7)) << 4)) + d % 8;
+        const float x0 = Elem<T>::to_f(x[0]), x1 = Elem<T>::to_f(x[1]);
+        // (a weight that rounded to 0 still carries an infinity)
+        if (k < lim[mt][0]) {
+          o[mt][nt][0] += isfinite(x0) ? wa * x0 : x0;
+          o[mt][nt][1] += isfinite(x1) ? wa * x1 : x1;
+        }
+        if (k < lim[mt][1]) {
+          o[mt][nt][2] += isfinite(x0) ? wb * x0 : x0;
+          o[mt][nt][3] += isfinite(x1) ? wb * x1 : x1;
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(32 * kFewWarps, 2)
+    few_rows_kernel(const __grid_constant__ FewParams p, const __grid_constant__ CUtensorMap mk,
+                    const __grid_constant__ CUtensorMap mv) {
+  using F = Few<D>;
+  constexpr unsigned kFull = 0xffffffffu;
+  constexpr int kHalves = D / 64;
+  extern __shared__ unsigned char dyn[];
+  __shared__ uint64_t full[kFewWarps][kFewStages];
+  __shared__ float s_m[kFewWarps][16 * MT], s_l[kFewWarps][16 * MT];
+  __shared__ int s_abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  ptx::grid_dependents_launch();
+  const int split = (int)(blockIdx.x % p.splits);
+  const int64_t unit = blockIdx.x / p.splits;
+  const int seq = (int)(unit / p.hkv), kvh = (int)(unit % p.hkv);
+  if (seq >= live_sequences(p.batch)) return;
+  const Sequence s = sequence(p.batch, seq);
+  if (!s.n || s.n > p.few) return;
+  const int rows = s.n * p.group;
+  const int pos0 = s.kv - s.n;  // keys before the first token's own
+  const int k0 = split * p.split_keys, k1 = p.splits > 1 ? min(s.kv, k0 + p.split_keys) : s.kv;
+  const int64_t row0 = (int64_t)s.row0 * p.hq + kvh * p.group;  // of [token, head] rows
+  const int64_t part = ((int64_t)split * p.batch.n_seqs + seq) * p.few * p.hq + kvh * p.group;
+  if (p.splits > 1 && k0 >= k1) {  // no keys: a sum of 0
+    for (int r = threadIdx.x; r < rows; r += blockDim.x)
+      p.part_ml[part + (int64_t)(r / p.group) * p.hq + r % p.group] = make_float2(-INFINITY, 0.f);
+    return;
+  }
+  unsigned char *ring = dyn + ((1024u - (ptx::smem_u32(dyn) & 1023u)) & 1023u) + warp * F::kRing;
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < kFewWarps; ++w)
+      for (int i = 0; i < kFewStages; ++i) ptx::mbar_init(&full[w][i], 1);
+    ptx::fence_mbar_init();
+    s_abort = 0;
+  }
+  __syncthreads();
+
+  // this warp's groups of 16 keys: warp, warp + 4, ... of the split's
+  const int groups = max(0, ((k1 - k0 + kFewKeys - 1) / kFewKeys - warp + kFewWarps - 1) / kFewWarps);
+  const int page = 1 << p.src.page_shift;
+  auto key_of = [&](int i) { return k0 + (warp + i * kFewWarps) * kFewKeys; };
+  // cache rows of 32 groups at a time, one per lane, the next ones read ahead
+  auto cache_rows = [&](int i0) {
+    const int i = i0 + lane;
+    if (i >= groups) return 0;
+    const int at = key_of(i);
+    const int pg = __ldg(p.src.tables + s.req * p.src.max_pages + (at >> p.src.page_shift));
+    const bool real = pg >= 0 && pg < p.src.n_pages;
+    if (!real) raise_error(p.batch.err, TIDE_DEVERR_POSITION);
+    // a row past the cache's last reads as zeros
+    return ((real ? pg : p.src.n_pages) * p.hkv + (real ? kvh : 0)) * page + (at & (page - 1));
+  };
+  int now = cache_rows(0), next = cache_rows(32);
+  auto request = [&](int i) {
+    if (i >= groups) return;
+    if ((i & 31) == 0 && i) {
+      now = next;
+      next = cache_rows(i + 32);
+    }
+    const int row = __shfl_sync(kFull, now, i & 31);
+    const int st = i % kFewStages;
+    if (lane == 0) ptx::mbar_expect_tx(&full[warp][st], 2 * F::kSide);
+    __syncwarp();
+    if (lane < 2 * kHalves)  // K, then V, a column group each
+      ptx::tma_load_2d(ring + st * 2 * F::kSide + lane * F::kHalf, lane < kHalves ? &mk : &mv,
+                       &full[warp][st], lane % kHalves * 64, row);
+    __syncwarp();
+  };
+  for (int i = 0; i < kFewStages; ++i) request(i);
+
+  // the rows of this lane: 16 mt + lane / 4, and 8 further
+  uint32_t qa[MT][D / 16][4];
+  int sees[MT][2];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = mt * 16 + h * 8 + lane / 4;
+      const bool valid = r < rows;
+      const int tok = valid ? r / p.group : s.n - 1;
+      sees[mt][h] = pos0 + tok + 1;
+      const T *q = static_cast<const T *>(p.q) + (s.row0 + tok) * p.q_stride +
+                   (int64_t)(kvh * p.group + r % p.group) * D + (lane & 3) * 2;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          qa[mt][k][e * 2 + h] = valid ? *reinterpret_cast<const uint32_t *>(q + k * 16 + e * 8) : 0u;
+    }
+  float o[MT][D / 8][4], m[MT][2], l[MT][2];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    m[mt][0] = m[mt][1] = -INFINITY;
+    l[mt][0] = l[mt][1] = 0.f;
+#pragma unroll
+    for (int nt = 0; nt < D / 8; ++nt) o[mt][nt][0] = o[mt][nt][1] = o[mt][nt][2] = o[mt][nt][3] = 0.f;
+  }
+  const float slack = kSlack / p.qs;
+  // ldmatrix addresses of this lane within a group: rows of keys, 16-byte chunks
+  const int kr = (lane & 7) + (lane >> 4) * 8, kc = (lane >> 3) & 1;  // K: key row, chunk parity
+  const int vr = lane & 15, vc = lane >> 4;                           // V (transposed)
+  int i = 0;
+  for (; i < groups; ++i) {
+    const int st = i % kFewStages;
+    if (!__all_sync(kFull, ptx::mbar_wait(&full[warp][st], (i / kFewStages) & 1, &s_abort))) {
+      raise_error(p.batch.err, TIDE_DEVERR_TIMEOUT);
+      s_abort = 1;
+      break;
+    }
+    const unsigned char *kb = ring + st * 2 * F::kSide, *vb = kb + F::kSide;
+    const uint32_t ka = ptx::smem_u32(kb) + kr * 128, va = ptx::smem_u32(vb) + vr * 128;
+    float sc[MT][2][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) sc[mt][nt][0] = sc[mt][nt][1] = sc[mt][nt][2] = sc[mt][nt][3] = 0.f;
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+      const int c = k * 2 + kc;
+      uint32_t b[4];
+      ldmatrix4(b, ka + (c / 8) * F::kHalf + (((c % 8) ^ (kr & 7)) << 4));
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        mma16816<T>(sc[mt][0], qa[mt][k], b[0], b[1]);
+        mma16816<T>(sc[mt][1], qa[mt][k], b[2], b[3]);
+      }
+    }
+    const int key = key_of(i);
+    const bool partial = key + kFewKeys > pos0 + 1;  // some row does not see all of them
+    uint32_t pr[MT][4];
+    int lim[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      float raise = 0.f, a[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        lim[mt][h] = sees[mt][h] - key;
+        float t = -INFINITY;
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float &x = sc[mt][nt][h * 2 + e];
+            if (partial && nt * 8 + (lane & 3) * 2 + e >= lim[mt][h]) x = -INFINITY;
+            t = fmaxf(t, x);
+          }
+        t = fmaxf(t, __shfl_xor_sync(kFull, t, 1));
+        t = fmaxf(t, __shfl_xor_sync(kFull, t, 2));
+        const bool up = t > m[mt][h] + slack;  // (the first keys: m is -infinity)
+        a[h] = up ? ex2((m[mt][h] - t) * p.qs) : 1.f;
+        if (up) m[mt][h] = t, raise = 1.f;
+        const float mq = m[mt][h] == -INFINITY ? 0.f : m[mt][h] * p.qs;
+        l[mt][h] *= a[h];
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+          const float x0 = ex2(fmaf(sc[mt][nt][h * 2], p.qs, -mq));
+          const float x1 = ex2(fmaf(sc[mt][nt][h * 2 + 1], p.qs, -mq));
+          l[mt][h] += x0 + x1;
+          pr[mt][nt * 2 + h] = pack2<T>(x0, x1);
+        }
+      }
+      if (__any_sync(kFull, raise != 0.f)) {
+#pragma unroll
+        for (int nt = 0; nt < D / 8; ++nt) {
+          o[mt][nt][0] *= a[0];
+          o[mt][nt][1] *= a[0];
+          o[mt][nt][2] *= a[1];
+          o[mt][nt][3] *= a[1];
+        }
+      }
+    }
+    // masked values: a weight of 0 does not silence a NaN.  Past the last key
+    // they are dropped; before it, where rows differ, odd ones are told apart.
+    const int seen = s.kv - key;  // keys of the group that exist
+    bool odd = false;
+    if (partial && s.n > 1) {
+      constexpr int kRowVecs = 8 * (D / 64);
+      for (int e = lane; e < min(seen, kFewKeys) * kRowVecs; e += 32) {
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(
+            vb + (e / 8 % (D / 64)) * F::kHalf + e / kRowVecs * 128 + e % 8 * 16);
+#pragma unroll
+        for (int h = 0; h < 4; ++h) odd |= odd_value<T>(w[h]) | odd_value<T>(w[h] >> 16);
+      }
+    }
+    if (__any_sync(kFull, odd)) {
+      values_one_by_one<T, D, MT>(vb, pr, lim, o);
+    } else {
+      // zeros for the keys past the last: rows 2 (lane % 4), + 1, and 8 further
+      uint32_t keep0 = ~0u, keep1 = ~0u;
+      if (seen < kFewKeys) {
+        const int r = (lane & 3) * 2;
+        keep0 = (r < seen ? 0xFFFFu : 0u) | (r + 1 < seen ? 0xFFFF0000u : 0u);
+        keep1 = (r + 8 < seen ? 0xFFFFu : 0u) | (r + 9 < seen ? 0xFFFF0000u : 0u);
+      }
+#pragma unroll
+      for (int nt = 0; nt < D / 8; nt += 2) {
+        const int c = nt + vc;
+        uint32_t b[4];
+        ldmatrix4_t(b, va + (c / 8) * F::kHalf + (((c % 8) ^ (vr & 7)) << 4));
+        if (seen < kFewKeys) b[0] &= keep0, b[1] &= keep1, b[2] &= keep0, b[3] &= keep1;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          mma16816<T>(o[mt][nt], pr[mt], b[0], b[1]);
+          mma16816<T>(o[mt][nt + 1], pr[mt], b[2], b[3]);
+        }
+      }
+    }
+    __syncwarp();  // the stage has been read
+    request(i + kFewStages);
+  }
+  if (i < groups && lane == 0) {  // given up: wait for the copies in flight (bounded)
+    volatile int none = 0;
+    for (int e = i; e < min(groups, i + kFewStages); ++e)
+      ptx::mbar_wait(&full[warp][e % kFewStages], (e / kFewStages) & 1, &none);
+  }
+  __syncwarp();
+
+  // the four warps' outputs meet: this warp's in its own ring
+  float *mine = reinterpret_cast<float *>(ring);  // [16 MT][D]
+  static_assert(16 * MT * D * 4 <= F::kRing, "a warp's output fits its ring");
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = mt * 16 + h * 8 + lane / 4;
+      float sum = l[mt][h];
+      sum += __shfl_xor_sync(kFull, sum, 1);
+      sum += __shfl_xor_sync(kFull, sum, 2);
+      if ((lane & 3) == 0) {
+        s_m[warp][r] = m[mt][h] * p.qs;
+        s_l[warp][r] = sum;
+      }
+#pragma unroll
+      for (int nt = 0; nt < D / 8; ++nt)
+        *reinterpret_cast<float2 *>(mine + r * D + nt * 8 + (lane & 3) * 2) =
+            make_float2(o[mt][nt][h * 2], o[mt][nt][h * 2 + 1]);
+    }
+  __syncthreads();
+  const float *all = reinterpret_cast<const float *>(ring - warp * F::kRing);
+  constexpr int kLanes = D / 4;  // lanes of a row, four columns each
+  for (int r = threadIdx.x / kLanes; r < rows; r += 32 * kFewWarps / kLanes) {
+    const int d = threadIdx.x % kLanes * 4;
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w)
+      if (s_l[w][r] != 0.f) top = fmaxf(top, s_m[w][r]);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) {
+      if (s_l[w][r] == 0.f) continue;
+      const float a = exp2f(s_m[w][r] - top);
+      const float4 y = *reinterpret_cast<const float4 *>(all + w * (F::kRing / 4) + r * D + d);
+      sum = fmaf(a, s_l[w][r], sum);
+      x.x = fmaf(a, y.x, x.x);
+      x.y = fmaf(a, y.y, x.y);
+      x.z = fmaf(a, y.z, x.z);
+      x.w = fmaf(a, y.w, x.w);
+    }
+    const int64_t at = (int64_t)(r / p.group) * p.hq + r % p.group;
+    if (p.splits > 1) {
+      if (d == 0) p.part_ml[part + at] = make_float2(top, sum);
+      *reinterpret_cast<float4 *>(p.part_o + (part + at) * D + d) = x;
+    } else {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + (row0 + at) * D + d) =
+          make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
+    }
+  }
+}
+
+// ------------------------------------------------------------------- joins
+struct Join {  // splits of the sequences of one kernel
+  const float *part_o;
+  const float2 *part_ml;
+  int splits;
+};
+
 // Joins the splits of a row and head: with M = max_s m_s,
 //   o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s,  in the order of s.
+// A sequence of up to `few` tokens has the splits of `a`, a longer one those of
+// `b`; one split is an output already.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(256)
+    combine_kernel(const __grid_constant__ RaggedBatch batch, int hq, int few, Join a, Join b, T *out) {
   constexpr int kE = D / 32;
+  ptx::grid_dependency_wait();
   const int lane = threadIdx.x & 31;
   const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (w >= (int64_t)p.batch.n_tokens * p.hq) return;
-  const int row = (int)(w / p.hq);
-  const int seq = sequence_of_row(p.batch, live_sequences(p.batch), row);
-  if (seq < 0 || !sequence(p.batch, seq).n) return;
-  const int64_t step = (int64_t)p.batch.n_tokens * p.hq;
+  if (w >= (int64_t)batch.n_tokens * hq) return;
+  const int row = (int)(w / hq);
+  const int seq = sequence_of_row(batch, live_sequences(batch), row);
+  if (seq < 0) return;
+  const Sequence s = sequence(batch, seq);
+  if (!s.n) return;
+  const bool short_one = s.n <= few;
+  const Join j = short_one ? a : b;
+  if (j.splits <= 1) return;
+  const int64_t step = (int64_t)(short_one ? (int64_t)batch.n_seqs * few : batch.n_tokens) * hq;
+  const int64_t at = short_one ? ((int64_t)seq * few + row - s.row0) * hq + w % hq : w;
   float top = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) {
-    const float2 ml = p.part_ml[s * step + w];
+  for (int i = 0; i < j.splits; ++i) {
+    const float2 ml = j.part_ml[i * step + at];
     if (ml.y != 0.f) top = fmaxf(top, ml.x);
   }
   float sum = 0.f, o[kE];
 #pragma unroll
   for (int e = 0; e < kE; ++e) o[e] = 0.f;
-  for (int s = 0; s < p.splits; ++s) {
-    const float2 ml = p.part_ml[s * step + w];
+  for (int i = 0; i < j.splits; ++i) {
+    const float2 ml = j.part_ml[i * step + at];
     if (ml.y == 0.f) continue;
-    const float a = exp2f(ml.x - top);
-    sum = fmaf(a, ml.y, sum);
-    const float *src = p.part_o + (s * step + w) * D + lane;
+    const float f = exp2f(ml.x - top);
+    sum = fmaf(f, ml.y, sum);
+    const float *src = j.part_o + (i * step + at) * D + lane * kE;
 #pragma unroll
-    for (int e = 0; e < kE; ++e) o[e] = fmaf(a, src[32 * e], o[e]);
+    for (int e = 0; e < kE; ++e) o[e] = fmaf(f, src[e], o[e]);
   }
-  T *out = static_cast<T *>(p.out) + w * D + lane;
+  T *to = out + w * D + lane * kE;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-  for (int e = 0; e < kE; ++e) out[32 * e] = Elem<T>::from_f(o[e] * inv);
+  for (int e = 0; e < kE; ++e) to[e] = Elem<T>::from_f(o[e] * inv);
 }
 
 }  // namespace ragged
@@ -1002,15 +1401,52 @@ int64_t most_units(int64_t n_tokens, int64_t n_seqs, int64_t hq, int64_t hkv) {
   return tiles * hkv;
 }
 
-// Splits of the keys: as many as give every SM a unit, but no split of fewer
-// than four blocks of keys, whose start and join would cost more than their
-// keys.
-int64_t key_splits(int64_t n_tokens, int64_t n_seqs, int64_t hq, int64_t hkv, int64_t max_kv) {
-  const int64_t units = most_units(n_tokens, n_seqs, hq, hkv);
-  const int64_t blocks = (max_kv + tide::ragged::kKeys - 1) / tide::ragged::kKeys;
-  int64_t s = units > 0 ? 148 / units : 1;
-  if (s > blocks / 4) s = blocks / 4;
-  return s < 1 ? 1 : s;
+// How a paged call is cut up.  Sequences of up to `few` tokens (rows that fit
+// the few-rows kernel) and longer ones go to a kernel each; a call that cannot
+// have the one or the other does not launch it.
+struct Plan {
+  int mt;                // 16-row groups of the few-rows kernel; 0: none
+  int few;               // tokens
+  bool tiles;            // whether the tile kernel runs
+  int few_splits, split_keys;
+  int splits, split_blocks;
+  size_t few_bytes, bytes;  // workspace
+};
+
+Plan plan_paged(bool one_token, int64_t n_tokens, int64_t n_seqs, int64_t hq, int64_t hkv, int64_t d,
+                int64_t max_kv) {
+  using namespace tide::ragged;
+  Plan p{};
+  const int64_t group = hq / hkv;
+  // a decode step whose heads fit 16 rows; else up to 32 rows
+  p.mt = one_token && group <= 16 ? 1 : group <= 32 ? 2 : 0;
+  p.few = (int)(p.mt * 16 / group);
+  if (one_token) p.few = 1;
+  if (n_tokens < p.few) p.few = (int)n_tokens;
+  if (n_seqs == 1 && n_tokens > p.few) p.mt = p.few = 0;  // (one sequence: its length is known)
+  p.tiles = !p.mt || (!one_token && n_tokens > p.few);
+  const int64_t rows = n_tokens * hq;
+  // Few rows: splits that give every SM its two CTAs about twice over (they
+  // are of different lengths), of 256 keys at least.
+  const int64_t units = n_seqs * hkv;
+  int64_t s = p.mt ? (4 * 148 + units - 1) / units : 1;
+  if (s > max_kv / 256) s = max_kv / 256;
+  if (s < 1) s = 1;
+  const int64_t keys = (max_kv + s - 1) / s;
+  p.split_keys = (int)((keys + 63) / 64 * 64);
+  p.few_splits = (int)s;
+  p.few_bytes = s > 1 ? (size_t)(s * n_seqs * p.few * hq * (d + 2) * 4 + 15) / 16 * 16 : 0;
+  // Tiles: as many as give every SM a unit, of four blocks of keys at least
+  // (below that the start and the join of a split cost more than its keys).
+  const int64_t tile_units = most_units(n_tokens, n_seqs, hq, hkv);
+  const int64_t blocks = (max_kv + kKeys - 1) / kKeys;
+  int64_t t = p.tiles && tile_units > 0 ? 148 / tile_units : 1;
+  if (t > blocks / 4) t = blocks / 4;
+  if (t < 1) t = 1;
+  p.splits = (int)t;
+  p.split_blocks = (int)((blocks + t - 1) / t);
+  p.bytes = p.few_bytes + (t > 1 ? (size_t)(t * rows * (d + 2) * 4) : 0);
+  return p;
 }
 
 template <typename T, int D, bool PAGED>
@@ -1038,11 +1474,41 @@ int launch(tide::ragged::Params &p, int dtype, const void *q, int64_t q_stride, 
   const int sms = sm_count();
   if (!sms) return report(cudaErrorInvalidDevice, "ragged attention");
   kern<<<(unsigned)(units < sms ? units : sms), kThreads, Shape<D>::kSmem, s>>>(p, mq, mk, mv);
-  if (p.splits > 1) {
-    const int64_t warps = (int64_t)p.batch.n_tokens * p.hq;
-    combine_kernel<T, D><<<(unsigned)((warps + 7) / 8), 256, 0, s>>>(p);
-  }
   return report(cudaSuccess, "ragged attention");
+}
+
+template <typename T, int D, int MT>
+int launch_few(const tide::ragged::FewParams &p, int dtype, int64_t kv_rows, cudaStream_t s) {
+  using namespace tide::ragged;
+  CUtensorMap mk, mv;
+  if (!make_map(&mk, dtype, p.src.k, 2, D, kv_rows, 1, D, 0, kFewKeys, 1) ||
+      !make_map(&mv, dtype, p.src.v, 2, D, kv_rows, 1, D, 0, kFewKeys, 1))
+    return fail(TIDE_ERR_CUDA, "paged_attention: cuTensorMapEncodeTiled failed");
+  auto kern = few_rows_kernel<T, D, MT>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)Few<D>::kSmem);
+  if (e != cudaSuccess) return report(e, "paged_attention");
+  const int64_t ctas = (int64_t)p.batch.n_seqs * p.hkv * p.splits;
+  kern<<<(unsigned)ctas, 32 * kFewWarps, Few<D>::kSmem, s>>>(p, mk, mv);
+  return report(cudaSuccess, "paged_attention");
+}
+
+template <typename T, int D>
+int launch_join(const tide::RaggedBatch &b, int hq, int few, const tide::ragged::Join &x,
+                const tide::ragged::Join &y, void *out, cudaStream_t s) {
+  const int64_t warps = (int64_t)b.n_tokens * hq;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((warps + 7) / 8), 1, 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];  // its launch overlaps the tail of the kernel before
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return report(cudaLaunchKernelEx(&cfg, tide::ragged::combine_kernel<T, D>, b, hq, few, x, y,
+                                   static_cast<T *>(out)),
+                "paged_attention");
 }
 
 template <bool PAGED>
@@ -1064,6 +1530,7 @@ void set_heads(tide::ragged::Params &p, int64_t hq, int64_t hkv, float scale, vo
   p.qs = scale * tide::ragged::kLog2e;
   p.splits = 1;
   p.split_blocks = 1 << 24;  // all of them
+  p.few = 0;
 }
 
 }  // namespace
@@ -1100,8 +1567,11 @@ extern "C" size_t tide_paged_attention_workspace_size(int64_t n_tokens, int64_t 
   if (n_tokens < 1 || n_seqs < 1 || n_kv_heads < 1 || n_q_heads < n_kv_heads || max_kv_len < 1 ||
       n_q_heads / n_kv_heads > tide::ragged::kRows)
     return 0;
-  const int64_t s = key_splits(n_tokens, n_seqs, n_q_heads, n_kv_heads, max_kv_len);
-  return s > 1 ? (size_t)(s * n_tokens * n_q_heads * (head_dim + 2) * 4) : 0;
+  // (cu_seqlens or not: the larger need of the two)
+  const size_t one = plan_paged(true, n_tokens, n_seqs, n_q_heads, n_kv_heads, head_dim, max_kv_len).bytes;
+  const size_t many =
+      plan_paged(false, n_tokens, n_seqs, n_q_heads, n_kv_heads, head_dim, max_kv_len).bytes;
+  return one > many ? one : many;
 }
 
 extern "C" int tide_paged_attention(int dtype, const void *q, int64_t q_row_stride,
@@ -1137,18 +1607,70 @@ extern "C" int tide_paged_attention(int dtype, const void *q, int64_t q_row_stri
     return fail(TIDE_ERR_WORKSPACE, "paged_attention: workspace missing, too small or misaligned");
   int shift = 0;
   while ((1 << shift) < page_size) ++shift;
+  const int64_t kv_rows = n_pages * n_kv_heads * page_size;
+  cudaStream_t st = (cudaStream_t)stream;
+  const Plan plan = plan_paged(!cu_seqlens, n_tokens, n_seqs, n_q_heads, n_kv_heads, head_dim, max_kv_len);
+  const int64_t rows = n_tokens * n_q_heads;
+  unsigned char *ws = static_cast<unsigned char *>(workspace);
   tide::ragged::Params p{};
   p.batch = {cu_seqlens, seq_ids, kv_lens, n_seqs_dev, (int)n_seqs, (int)n_requests,
              (int)n_tokens, (int)max_kv_len, error_word};
   p.src = {k_cache, v_cache, 0, block_tables, max_pages, (int)n_pages, shift};
   set_heads(p, n_q_heads, n_kv_heads, scale, out);
-  p.splits = (int)key_splits(n_tokens, n_seqs, n_q_heads, n_kv_heads, max_kv_len);
-  if (p.splits > 1) {
-    const int64_t blocks = (max_kv_len + tide::ragged::kKeys - 1) / tide::ragged::kKeys;
-    p.split_blocks = (int)((blocks + p.splits - 1) / p.splits);
-    p.part_o = static_cast<float *>(workspace);
-    p.part_ml = reinterpret_cast<float2 *>(p.part_o + p.splits * n_tokens * n_q_heads * head_dim);
+  p.few = plan.mt ? plan.few : 0;
+  tide::ragged::Join few_join{nullptr, nullptr, 1}, join{nullptr, nullptr, 1};
+  if (plan.few_splits > 1)
+    few_join = {reinterpret_cast<float *>(ws),
+                reinterpret_cast<float2 *>(ws + plan.few_splits * n_seqs * plan.few * n_q_heads *
+                                                    head_dim * 4),
+                plan.few_splits};
+  if (plan.splits > 1) {
+    unsigned char *at = ws + plan.few_bytes;
+    join = {reinterpret_cast<float *>(at),
+            reinterpret_cast<float2 *>(at + plan.splits * rows * head_dim * 4), plan.splits};
+    p.splits = plan.splits;
+    p.split_blocks = plan.split_blocks;
+    p.part_o = const_cast<float *>(join.part_o);
+    p.part_ml = const_cast<float2 *>(join.part_ml);
   }
-  return dispatch<true>(p, dtype, head_dim, q, q_row_stride, n_pages * n_kv_heads * page_size,
-                        (cudaStream_t)stream);
+  if (plan.tiles)
+    if (int rc = dispatch<true>(p, dtype, head_dim, q, q_row_stride, kv_rows, st)) return rc;
+  if (plan.mt) {
+    tide::ragged::FewParams f{};
+    f.batch = p.batch;
+    f.src = p.src;
+    f.q = q;
+    f.q_stride = q_row_stride;
+    f.out = out;
+    f.part_o = const_cast<float *>(few_join.part_o);
+    f.part_ml = const_cast<float2 *>(few_join.part_ml);
+    f.hq = p.hq;
+    f.hkv = p.hkv;
+    f.group = p.group;
+    f.few = plan.few;
+    f.splits = plan.few_splits;
+    f.split_keys = plan.split_keys;
+    f.qs = p.qs;
+    int rc;
+    if (dtype == TIDE_DTYPE_BF16)
+      rc = head_dim == 128 ? (plan.mt == 1 ? launch_few<__nv_bfloat16, 128, 1>(f, dtype, kv_rows, st)
+                                           : launch_few<__nv_bfloat16, 128, 2>(f, dtype, kv_rows, st))
+                           : (plan.mt == 1 ? launch_few<__nv_bfloat16, 64, 1>(f, dtype, kv_rows, st)
+                                           : launch_few<__nv_bfloat16, 64, 2>(f, dtype, kv_rows, st));
+    else
+      rc = head_dim == 128 ? (plan.mt == 1 ? launch_few<__half, 128, 1>(f, dtype, kv_rows, st)
+                                           : launch_few<__half, 128, 2>(f, dtype, kv_rows, st))
+                           : (plan.mt == 1 ? launch_few<__half, 64, 1>(f, dtype, kv_rows, st)
+                                           : launch_few<__half, 64, 2>(f, dtype, kv_rows, st));
+    if (rc) return rc;
+  }
+  if (few_join.splits > 1 || join.splits > 1) {
+    if (dtype == TIDE_DTYPE_BF16)
+      return head_dim == 128
+                 ? launch_join<__nv_bfloat16, 128>(p.batch, p.hq, p.few, few_join, join, out, st)
+                 : launch_join<__nv_bfloat16, 64>(p.batch, p.hq, p.few, few_join, join, out, st);
+    return head_dim == 128 ? launch_join<__half, 128>(p.batch, p.hq, p.few, few_join, join, out, st)
+                           : launch_join<__half, 64>(p.batch, p.hq, p.few, few_join, join, out, st);
+  }
+  return TIDE_OK;
 }
