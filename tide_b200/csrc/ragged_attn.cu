@@ -886,14 +886,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   ptx::tc_fence_after();
   if (warp == 10) ptx::tmem_dealloc(tmem, 512);
+  // Launched over the tail of the few-rows kernel, on which it does not
+  // depend: what comes after this kernel comes after that one too.
+  if (threadIdx.x == 0) ptx::grid_dependency_wait();
 }
 
 // --------------------------------------------------------- few rows a head
-// Sequences with so few tokens that their rows (tokens times the query heads
-// of a KV head) are at most 16 * MT: a decode step, a few drafted tokens.  Such
-// a unit reads 4 D bytes per key and does 4 D flops per key and row, so it is
-// bound by HBM, and the 128-row tiles above would leave it to one chain of
-// products and exponentials per SM.  Here a warp is on its own: it walks over
+// Sequences with few rows (tokens times the query heads of a KV head): a
+// decode step, a few drafted tokens.  Such a unit reads 4 D bytes per key and
+// does 4 D flops per key and row, so it is bound by HBM, and the 128-row tiles
+// above would leave it to one chain of products and exponentials per SM.  A
+// CTA takes 16 MT rows; a sequence with more (up to four such groups) has
+// several, which share their keys through L2.  A warp is on its own: it walks over
 // every fourth group of 16 keys of its CTA's share, with its own ring of TMA
 // copies (8 KB a group, three in flight) and its own running maxima, sums and
 // outputs, and the four meet once at the end.  No barrier but the ring's.
@@ -946,7 +950,9 @@ struct FewParams {
   float *part_o;    // [splits, n_seqs, few, hq, D] (splits > 1)
   float2 *part_ml;  // [splits, n_seqs, few, hq]: maximum (scaled, base 2), sum
   int hq, hkv, group;
-  int few;         // tokens a sequence may have: 16 MT / group
+  int few;         // tokens a sequence may have
+  int tokens;      // of a CTA: 16 MT / group
+  int parts;       // CTAs that share a sequence's tokens
   int splits;
   int split_keys;  // keys of a split, a multiple of 16
   float qs;
@@ -1011,17 +1017,26 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2)
   __shared__ int s_abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   ptx::grid_dependents_launch();
-  const int split = (int)(blockIdx.x % p.splits);
-  const int64_t unit = blockIdx.x / p.splits;
+  const int of_parts = (int)(blockIdx.x % p.parts);
+  const int split = (int)(blockIdx.x / p.parts % p.splits);
+  const int64_t unit = blockIdx.x / p.parts / p.splits;
   const int seq = (int)(unit / p.hkv), kvh = (int)(unit % p.hkv);
   if (seq >= live_sequences(p.batch)) return;
-  const Sequence s = sequence(p.batch, seq);
-  if (!s.n || s.n > p.few) return;
+  Sequence s = sequence(p.batch, seq);
+  const int tok0 = of_parts * p.tokens;  // this CTA's tokens from here on
+  if (s.n > p.few || tok0 >= s.n) return;
+  {  // as a sequence of its own, which ends with its last token
+    const int rest = s.n - tok0 - p.tokens;
+    s.row0 += tok0;
+    s.n = rest > 0 ? p.tokens : s.n - tok0;
+    s.kv -= max(rest, 0);
+  }
   const int rows = s.n * p.group;
   const int pos0 = s.kv - s.n;  // keys before the first token's own
   const int k0 = split * p.split_keys, k1 = p.splits > 1 ? min(s.kv, k0 + p.split_keys) : s.kv;
   const int64_t row0 = (int64_t)s.row0 * p.hq + kvh * p.group;  // of [token, head] rows
-  const int64_t part = ((int64_t)split * p.batch.n_seqs + seq) * p.few * p.hq + kvh * p.group;
+  const int64_t part =
+      (((int64_t)split * p.batch.n_seqs + seq) * p.few + tok0) * p.hq + kvh * p.group;
   if (p.splits > 1 && k0 >= k1) {  // no keys: a sum of 0
     for (int r = threadIdx.x; r < rows; r += blockDim.x)
       p.part_ml[part + (int64_t)(r / p.group) * p.hq + r % p.group] = make_float2(-INFINITY, 0.f);
@@ -1270,55 +1285,66 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2)
 }
 
 // ------------------------------------------------------------------- joins
-struct Join {  // splits of the sequences of one kernel
-  const float *part_o;
-  const float2 *part_ml;
-  int splits;
-};
-
-// Joins the splits of a row and head: with M = max_s m_s,
-//   o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s,  in the order of s.
-// A sequence of up to `few` tokens has the splits of `a`, a longer one those of
-// `b`; one split is an output already.
-template <typename T, int D>
-__global__ void __launch_bounds__(256)
-    combine_kernel(const __grid_constant__ RaggedBatch batch, int hq, int few, Join a, Join b, T *out) {
+// Joins the splits of a row and head, a CTA for each: with M = max_s m_s,
+//   o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s,
+// warp w over the splits w, w + 4, ..., the four sums in the order of w.
+// FEW: the rows are [sequence, token below few]; else the packed rows of the
+// sequences with more tokens than that.
+template <typename T, int D, bool FEW>
+__global__ void __launch_bounds__(128)
+    join_kernel(const __grid_constant__ RaggedBatch batch, int hq, int few, int splits,
+                const float *__restrict__ part_o, const float2 *__restrict__ part_ml, T *out) {
   constexpr int kE = D / 32;
+  __shared__ float s_top[4], s_sum[4], s_o[4][D];
   ptx::grid_dependency_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (w >= (int64_t)batch.n_tokens * hq) return;
-  const int row = (int)(w / hq);
-  const int seq = sequence_of_row(batch, live_sequences(batch), row);
-  if (seq < 0) return;
-  const Sequence s = sequence(batch, seq);
-  if (!s.n) return;
-  const bool short_one = s.n <= few;
-  const Join j = short_one ? a : b;
-  if (j.splits <= 1) return;
-  const int64_t step = (int64_t)(short_one ? (int64_t)batch.n_seqs * few : batch.n_tokens) * hq;
-  const int64_t at = short_one ? ((int64_t)seq * few + row - s.row0) * hq + w % hq : w;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t at = blockIdx.x;
+  const int64_t step = (int64_t)(FEW ? (int64_t)batch.n_seqs * few : batch.n_tokens) * hq;
+  const int live = live_sequences(batch);
+  int64_t row;
+  if (FEW) {
+    const int seq = (int)(at / hq / few), tok = (int)(at / hq % few);
+    if (seq >= live) return;
+    const Sequence s = sequence(batch, seq);
+    if (s.n > few || tok >= s.n) return;
+    row = s.row0 + tok;
+  } else {
+    row = at / hq;
+    const int seq = sequence_of_row(batch, live, (int)row);
+    if (seq < 0 || sequence(batch, seq).n <= few) return;
+  }
   float top = -INFINITY;
-  for (int i = 0; i < j.splits; ++i) {
-    const float2 ml = j.part_ml[i * step + at];
+  for (int i = threadIdx.x; i < splits; i += 128) {
+    const float2 ml = part_ml[i * step + at];
     if (ml.y != 0.f) top = fmaxf(top, ml.x);
   }
+#pragma unroll
+  for (int e = 16; e; e >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, e));
+  if (lane == 0) s_top[warp] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
   float sum = 0.f, o[kE];
 #pragma unroll
   for (int e = 0; e < kE; ++e) o[e] = 0.f;
-  for (int i = 0; i < j.splits; ++i) {
-    const float2 ml = j.part_ml[i * step + at];
-    if (ml.y == 0.f) continue;
+#pragma unroll 4
+  for (int i = warp; i < splits; i += 4) {
+    const float2 ml = part_ml[i * step + at];
+    if (ml.y == 0.f) continue;  // (its output was not written)
     const float f = exp2f(ml.x - top);
     sum = fmaf(f, ml.y, sum);
-    const float *src = j.part_o + (i * step + at) * D + lane * kE;
+    const float *src = part_o + (i * step + at) * D + lane * kE;
 #pragma unroll
     for (int e = 0; e < kE; ++e) o[e] = fmaf(f, src[e], o[e]);
   }
-  T *to = out + w * D + lane * kE;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  if (lane == 0) s_sum[warp] = sum;
 #pragma unroll
-  for (int e = 0; e < kE; ++e) to[e] = Elem<T>::from_f(o[e] * inv);
+  for (int e = 0; e < kE; ++e) s_o[warp][lane * kE + e] = o[e];
+  __syncthreads();
+  if (threadIdx.x >= D) return;
+  const int d = threadIdx.x;
+  sum = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+  const float x = (s_o[0][d] + s_o[1][d]) + (s_o[2][d] + s_o[3][d]);
+  out[(row * hq + at % hq) * D + d] = Elem<T>::from_f(sum == 0.f ? 0.f : x / sum);
 }
 
 }  // namespace ragged
@@ -1405,8 +1431,8 @@ int64_t most_units(int64_t n_tokens, int64_t n_seqs, int64_t hq, int64_t hkv) {
 // the few-rows kernel) and longer ones go to a kernel each; a call that cannot
 // have the one or the other does not launch it.
 struct Plan {
-  int mt;                // 16-row groups of the few-rows kernel; 0: none
-  int few;               // tokens
+  int mt;                // 16-row groups of a CTA of the few-rows kernel; 0: none
+  int few, tokens, parts;
   bool tiles;            // whether the tile kernel runs
   int few_splits, split_keys;
   int splits, split_blocks;
@@ -1418,19 +1444,25 @@ Plan plan_paged(bool one_token, int64_t n_tokens, int64_t n_seqs, int64_t hq, in
   using namespace tide::ragged;
   Plan p{};
   const int64_t group = hq / hkv;
-  // a decode step whose heads fit 16 rows; else up to 32 rows
+  // a decode step whose heads fit 16 rows; else 32 rows a CTA
   p.mt = one_token && group <= 16 ? 1 : group <= 32 ? 2 : 0;
-  p.few = (int)(p.mt * 16 / group);
-  if (one_token) p.few = 1;
+  p.tokens = (int)(p.mt * 16 / group);
+  // Up to 128 rows (a tile of the other kernel) are few.  The lengths are on
+  // the device: with as many tokens as make most sequences long, all of them
+  // go to the tiles, with one sequence its length is known.
+  p.few = one_token ? 1 : 4 * p.tokens;
+  if (!one_token && (n_tokens > n_seqs * 2 * p.few || (n_seqs == 1 && n_tokens > p.few))) p.mt = 0;
+  if (!p.mt) p.few = 0;
   if (n_tokens < p.few) p.few = (int)n_tokens;
-  if (n_seqs == 1 && n_tokens > p.few) p.mt = p.few = 0;  // (one sequence: its length is known)
   p.tiles = !p.mt || (!one_token && n_tokens > p.few);
+  p.parts = p.mt ? (p.few + p.tokens - 1) / p.tokens : 0;
   const int64_t rows = n_tokens * hq;
-  // Few rows: splits that give every SM its two CTAs about twice over (they
-  // are of different lengths), of 256 keys at least.
+  // Few rows: splits of 512 keys at least, as long as the CTAs that an SM
+  // holds (two) are not taken eight times over: sequences differ in length,
+  // and the more pieces, the evener the end.
   const int64_t units = n_seqs * hkv;
-  int64_t s = p.mt ? (4 * 148 + units - 1) / units : 1;
-  if (s > max_kv / 256) s = max_kv / 256;
+  int64_t s = p.mt ? (16 * 148 + units - 1) / units : 1;
+  if (s > (max_kv + 511) / 512) s = (max_kv + 511) / 512;
   if (s < 1) s = 1;
   const int64_t keys = (max_kv + s - 1) / s;
   p.split_keys = (int)((keys + 63) / 64 * 64);
@@ -1451,7 +1483,7 @@ Plan plan_paged(bool one_token, int64_t n_tokens, int64_t n_seqs, int64_t hq, in
 
 template <typename T, int D, bool PAGED>
 int launch(tide::ragged::Params &p, int dtype, const void *q, int64_t q_stride, int64_t kv_rows,
-           cudaStream_t s) {
+           bool behind_few, cudaStream_t s) {
   using namespace tide::ragged;
   CUtensorMap mq, mk, mv;
   const int page = 1 << p.src.page_shift;
@@ -1473,8 +1505,17 @@ int launch(tide::ragged::Params &p, int dtype, const void *q, int64_t q_stride, 
       most_units(p.batch.n_tokens, p.batch.n_seqs, p.hq, p.hkv) * p.splits;
   const int sms = sm_count();
   if (!sms) return report(cudaErrorInvalidDevice, "ragged attention");
-  kern<<<(unsigned)(units < sms ? units : sms), kThreads, Shape<D>::kSmem, s>>>(p, mq, mk, mv);
-  return report(cudaSuccess, "ragged attention");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(units < sms ? units : sms), 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = Shape<D>::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = behind_few ? 1 : 0;
+  return report(cudaLaunchKernelEx(&cfg, kern, p, mq, mk, mv), "ragged attention");
 }
 
 template <typename T, int D, int MT>
@@ -1488,37 +1529,58 @@ int launch_few(const tide::ragged::FewParams &p, int dtype, int64_t kv_rows, cud
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        (int)Few<D>::kSmem);
   if (e != cudaSuccess) return report(e, "paged_attention");
-  const int64_t ctas = (int64_t)p.batch.n_seqs * p.hkv * p.splits;
+  const int64_t ctas = (int64_t)p.batch.n_seqs * p.hkv * p.splits * p.parts;
   kern<<<(unsigned)ctas, 32 * kFewWarps, Few<D>::kSmem, s>>>(p, mk, mv);
   return report(cudaSuccess, "paged_attention");
 }
 
-template <typename T, int D>
-int launch_join(const tide::RaggedBatch &b, int hq, int few, const tide::ragged::Join &x,
-                const tide::ragged::Join &y, void *out, cudaStream_t s) {
-  const int64_t warps = (int64_t)b.n_tokens * hq;
+template <typename T, int D, bool FEW>
+int launch_join(const tide::RaggedBatch &b, int hq, int few, int splits, const float *part_o,
+                const float2 *part_ml, void *out, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((warps + 7) / 8), 1, 1);
-  cfg.blockDim = dim3(256, 1, 1);
+  cfg.gridDim = dim3((unsigned)((FEW ? (int64_t)b.n_seqs * few : b.n_tokens) * hq), 1, 1);
+  cfg.blockDim = dim3(128, 1, 1);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];  // its launch overlaps the tail of the kernel before
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return report(cudaLaunchKernelEx(&cfg, tide::ragged::combine_kernel<T, D>, b, hq, few, x, y,
-                                   static_cast<T *>(out)),
+  return report(cudaLaunchKernelEx(&cfg, tide::ragged::join_kernel<T, D, FEW>, b, hq, few, splits,
+                                   part_o, part_ml, static_cast<T *>(out)),
                 "paged_attention");
 }
 
-template <bool PAGED>
-int dispatch(tide::ragged::Params &p, int dtype, int64_t d, const void *q, int64_t q_stride,
-             int64_t kv_rows, cudaStream_t s) {
-  if (dtype == TIDE_DTYPE_BF16)
-    return d == 128 ? launch<__nv_bfloat16, 128, PAGED>(p, dtype, q, q_stride, kv_rows, s)
-                    : launch<__nv_bfloat16, 64, PAGED>(p, dtype, q, q_stride, kv_rows, s);
-  return d == 128 ? launch<__half, 128, PAGED>(p, dtype, q, q_stride, kv_rows, s)
-                  : launch<__half, 64, PAGED>(p, dtype, q, q_stride, kv_rows, s);
+// The paged call of one element type and head dimension, as planned.
+template <typename T, int D>
+int run_paged(const Plan &plan, tide::ragged::Params &p, int dtype, const void *q, int64_t q_stride,
+              int64_t kv_rows, unsigned char *ws, cudaStream_t s) {
+  const int64_t few_rows = (int64_t)p.batch.n_seqs * plan.few * p.hq;
+  const int64_t rows = (int64_t)p.batch.n_tokens * p.hq;
+  float *few_o = reinterpret_cast<float *>(ws);
+  float2 *few_ml = reinterpret_cast<float2 *>(ws + plan.few_splits * few_rows * D * 4);
+  p.few = plan.few;
+  if (plan.splits > 1) {
+    p.splits = plan.splits;
+    p.split_blocks = plan.split_blocks;
+    p.part_o = reinterpret_cast<float *>(ws + plan.few_bytes);
+    p.part_ml = reinterpret_cast<float2 *>(ws + plan.few_bytes + plan.splits * rows * D * 4);
+  }
+  int rc;
+  if (plan.mt) {
+    tide::ragged::FewParams f{p.batch, p.src,  q,     q_stride,  p.out,       few_o,
+                              few_ml,  p.hq,   p.hkv, p.group,   plan.few,    plan.tokens,
+                              plan.parts, plan.few_splits, plan.split_keys, p.qs};
+    rc = plan.mt == 1 ? launch_few<T, D, 1>(f, dtype, kv_rows, s) : launch_few<T, D, 2>(f, dtype, kv_rows, s);
+    if (rc) return rc;
+  }
+  if (plan.tiles && (rc = launch<T, D, true>(p, dtype, q, q_stride, kv_rows, plan.mt != 0, s))) return rc;
+  if (plan.mt && plan.few_splits > 1 &&
+      (rc = launch_join<T, D, true>(p.batch, p.hq, plan.few, plan.few_splits, few_o, few_ml, p.out, s)))
+    return rc;
+  if (plan.splits > 1)
+    return launch_join<T, D, false>(p.batch, p.hq, plan.few, plan.splits, p.part_o, p.part_ml, p.out, s);
+  return TIDE_OK;
 }
 
 void set_heads(tide::ragged::Params &p, int64_t hq, int64_t hkv, float scale, void *out) {
@@ -1558,7 +1620,13 @@ extern "C" int tide_packed_attention(int dtype, const void *q, const void *k, co
   p.src = {k, v, kv_row_stride, nullptr, 0, 0, 0};
   p.zero_keys = zero_keys;
   set_heads(p, n_q_heads, n_kv_heads, scale, out);
-  return dispatch<false>(p, dtype, head_dim, q, q_row_stride, n_tokens, (cudaStream_t)stream);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == TIDE_DTYPE_BF16)
+    return head_dim == 128
+               ? launch<__nv_bfloat16, 128, false>(p, dtype, q, q_row_stride, n_tokens, false, st)
+               : launch<__nv_bfloat16, 64, false>(p, dtype, q, q_row_stride, n_tokens, false, st);
+  return head_dim == 128 ? launch<__half, 128, false>(p, dtype, q, q_row_stride, n_tokens, false, st)
+                         : launch<__half, 64, false>(p, dtype, q, q_row_stride, n_tokens, false, st);
 }
 
 extern "C" size_t tide_paged_attention_workspace_size(int64_t n_tokens, int64_t n_seqs,
@@ -1610,67 +1678,15 @@ extern "C" int tide_paged_attention(int dtype, const void *q, int64_t q_row_stri
   const int64_t kv_rows = n_pages * n_kv_heads * page_size;
   cudaStream_t st = (cudaStream_t)stream;
   const Plan plan = plan_paged(!cu_seqlens, n_tokens, n_seqs, n_q_heads, n_kv_heads, head_dim, max_kv_len);
-  const int64_t rows = n_tokens * n_q_heads;
   unsigned char *ws = static_cast<unsigned char *>(workspace);
   tide::ragged::Params p{};
   p.batch = {cu_seqlens, seq_ids, kv_lens, n_seqs_dev, (int)n_seqs, (int)n_requests,
              (int)n_tokens, (int)max_kv_len, error_word};
   p.src = {k_cache, v_cache, 0, block_tables, max_pages, (int)n_pages, shift};
   set_heads(p, n_q_heads, n_kv_heads, scale, out);
-  p.few = plan.mt ? plan.few : 0;
-  tide::ragged::Join few_join{nullptr, nullptr, 1}, join{nullptr, nullptr, 1};
-  if (plan.few_splits > 1)
-    few_join = {reinterpret_cast<float *>(ws),
-                reinterpret_cast<float2 *>(ws + plan.few_splits * n_seqs * plan.few * n_q_heads *
-                                                    head_dim * 4),
-                plan.few_splits};
-  if (plan.splits > 1) {
-    unsigned char *at = ws + plan.few_bytes;
-    join = {reinterpret_cast<float *>(at),
-            reinterpret_cast<float2 *>(at + plan.splits * rows * head_dim * 4), plan.splits};
-    p.splits = plan.splits;
-    p.split_blocks = plan.split_blocks;
-    p.part_o = const_cast<float *>(join.part_o);
-    p.part_ml = const_cast<float2 *>(join.part_ml);
-  }
-  if (plan.tiles)
-    if (int rc = dispatch<true>(p, dtype, head_dim, q, q_row_stride, kv_rows, st)) return rc;
-  if (plan.mt) {
-    tide::ragged::FewParams f{};
-    f.batch = p.batch;
-    f.src = p.src;
-    f.q = q;
-    f.q_stride = q_row_stride;
-    f.out = out;
-    f.part_o = const_cast<float *>(few_join.part_o);
-    f.part_ml = const_cast<float2 *>(few_join.part_ml);
-    f.hq = p.hq;
-    f.hkv = p.hkv;
-    f.group = p.group;
-    f.few = plan.few;
-    f.splits = plan.few_splits;
-    f.split_keys = plan.split_keys;
-    f.qs = p.qs;
-    int rc;
-    if (dtype == TIDE_DTYPE_BF16)
-      rc = head_dim == 128 ? (plan.mt == 1 ? launch_few<__nv_bfloat16, 128, 1>(f, dtype, kv_rows, st)
-                                           : launch_few<__nv_bfloat16, 128, 2>(f, dtype, kv_rows, st))
-                           : (plan.mt == 1 ? launch_few<__nv_bfloat16, 64, 1>(f, dtype, kv_rows, st)
-                                           : launch_few<__nv_bfloat16, 64, 2>(f, dtype, kv_rows, st));
-    else
-      rc = head_dim == 128 ? (plan.mt == 1 ? launch_few<__half, 128, 1>(f, dtype, kv_rows, st)
-                                           : launch_few<__half, 128, 2>(f, dtype, kv_rows, st))
-                           : (plan.mt == 1 ? launch_few<__half, 64, 1>(f, dtype, kv_rows, st)
-                                           : launch_few<__half, 64, 2>(f, dtype, kv_rows, st));
-    if (rc) return rc;
-  }
-  if (few_join.splits > 1 || join.splits > 1) {
-    if (dtype == TIDE_DTYPE_BF16)
-      return head_dim == 128
-                 ? launch_join<__nv_bfloat16, 128>(p.batch, p.hq, p.few, few_join, join, out, st)
-                 : launch_join<__nv_bfloat16, 64>(p.batch, p.hq, p.few, few_join, join, out, st);
-    return head_dim == 128 ? launch_join<__half, 128>(p.batch, p.hq, p.few, few_join, join, out, st)
-                           : launch_join<__half, 64>(p.batch, p.hq, p.few, few_join, join, out, st);
-  }
-  return TIDE_OK;
+  if (dtype == TIDE_DTYPE_BF16)
+    return head_dim == 128 ? run_paged<__nv_bfloat16, 128>(plan, p, dtype, q, q_row_stride, kv_rows, ws, st)
+                           : run_paged<__nv_bfloat16, 64>(plan, p, dtype, q, q_row_stride, kv_rows, ws, st);
+  return head_dim == 128 ? run_paged<__half, 128>(plan, p, dtype, q, q_row_stride, kv_rows, ws, st)
+                         : run_paged<__half, 64>(plan, p, dtype, q, q_row_stride, kv_rows, ws, st);
 }
