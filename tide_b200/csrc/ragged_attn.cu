@@ -896,17 +896,19 @@ __global__ void __launch_bounds__(kThreads, 1)
 // decode step, a few drafted tokens.  Such a unit reads 4 D bytes per key and
 // does 4 D flops per key and row, so it is bound by HBM, and the 128-row tiles
 // above would leave it to one chain of products and exponentials per SM.  A
-// CTA takes 16 MT rows; a sequence with more (up to four such groups) has
+// CTA takes 8 NT rows; a sequence with more (up to four such groups) has
 // several, which share their keys through L2.  A warp is on its own: it walks over
 // every fourth group of 16 keys of its CTA's share, with its own ring of TMA
 // copies (8 KB a group, three in flight) and its own running maxima, sums and
 // outputs, and the four meet once at the end.  No barrier but the ring's.
-//   S[16 MT x 16] = Q K^T   mma.sync m16n8k16, K by ldmatrix from the swizzled
-//                           copy; Q in registers;
-//   O[16 MT x D] += P V     P from the registers that held S (the accumulator
-//                           layout of one product is the operand layout of the
-//                           next), V by transposing ldmatrix.
-// (tcgen05 has nothing to give here: its rows would be 7/8 padding.)
+//   S^T[16 x 8 NT] = K Q^T   mma.sync m16n8k16, K by ldmatrix from the swizzled
+//                            copy, Q in registers;
+//   O^T[D x 8 NT] += V^T P^T V by transposing ldmatrix, P from the registers
+//                            that held S, each 8 x 8 of it transposed.
+// The rows are the narrow side of the products, so they are padded to 8 only:
+// these products run at some 32 cycles each per SM partition (tcgen05 has
+// nothing to give here, its rows would be padding), which with rows padded to
+// 16 was more than the time that the keys of 32 rows take to arrive.
 constexpr int kFewWarps = 4;
 constexpr int kFewStages = 3;
 constexpr int kFewKeys = 16;
@@ -951,8 +953,8 @@ struct FewParams {
   float2 *part_ml;  // [splits, n_seqs, few, hq]: maximum (scaled, base 2), sum
   int hq, hkv, group;
   int few;         // tokens a sequence may have
-  int tokens;      // of a CTA: 16 MT / group
-  int parts;       // CTAs that share a sequence's tokens
+  int tokens;      // of a CTA: 8 NT / group
+  int pieces;      // pieces of up to `tokens` tokens that the sequences may have
   int splits;
   int split_keys;  // keys of a split, a multiple of 16
   float qs;
@@ -966,64 +968,59 @@ struct Few {
   static constexpr uint32_t kSmem = kFewWarps * kRing + 1024;    // + alignment
 };
 
-// Odd values among the keys that only the later rows of a unit see.  O of a
-// row gets the values it sees one by one; slow, and taken only when there is a
-// NaN or an infinity.
-// (Inlined: called, it would put O into local memory at every step.)
-template <typename T, int D, int MT>
-__device__ __forceinline__ void values_one_by_one(const unsigned char *v, const uint32_t (&pr)[MT][4],
-                                               const int (&lim)[MT][2], float (&o)[MT][D / 8][4]) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll 1
-  for (int k = 0; k < kFewKeys; ++k) {
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      // P[row][k] sits in lane (row % 8) * 4 + (k % 8) / 2, register k / 8 * 2 + row / 8
-      const int from = (lane & ~3) + (k % 8) / 2;
-      const uint32_t pa = __shfl_sync(0xffffffffu, k < 8 ? pr[mt][0] : pr[mt][2], from);
-      const uint32_t pb = __shfl_sync(0xffffffffu, k < 8 ? pr[mt][1] : pr[mt][3], from);
-      const T *ha = reinterpret_cast<const T *>(&pa), *hb = reinterpret_cast<const T *>(&pb);
-      const float wa = Elem<T>::to_f(ha[k & 1]), wb = Elem<T>::to_f(hb[k & 1]);
-#pragma unroll
-      for (int nt = 0; nt < D / 8; ++nt) {
-        const int d = nt * 8 + (lane & 3) * 2, c = d / 8;
-        const T *x = reinterpret_cast<const T *>(v + (c / 8) * Few<D>::kHalf + k * 128 +
-                                                 (((c % 8) ^ (k & 7)) << 4)) + d % 8;
-        const float x0 = Elem<T>::to_f(x[0]), x1 = Elem<T>::to_f(x[1]);
-        // (a weight that rounded to 0 still carries an infinity)
-        if (k < lim[mt][0]) {
-          o[mt][nt][0] += isfinite(x0) ? wa * x0 : x0;
-          o[mt][nt][1] += isfinite(x1) ? wa * x1 : x1;
-        }
-        if (k < lim[mt][1]) {
-          o[mt][nt][2] += isfinite(x0) ? wb * x0 : x0;
-          o[mt][nt][3] += isfinite(x1) ? wb * x1 : x1;
-        }
-      }
-    }
-  }
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
 }
 
-template <typename T, int D, int MT>
-__global__ void __launch_bounds__(32 * kFewWarps, 2)
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(32 * kFewWarps, NT <= 2 ? 3 : 2)
     few_rows_kernel(const __grid_constant__ FewParams p, const __grid_constant__ CUtensorMap mk,
                     const __grid_constant__ CUtensorMap mv) {
   using F = Few<D>;
   constexpr unsigned kFull = 0xffffffffu;
-  constexpr int kHalves = D / 64;
+  constexpr int kHalves = D / 64, kRowsMost = 8 * NT;
   extern __shared__ unsigned char dyn[];
   __shared__ uint64_t full[kFewWarps][kFewStages];
-  __shared__ float s_m[kFewWarps][16 * MT], s_l[kFewWarps][16 * MT];
+  __shared__ float s_m[kFewWarps][kRowsMost], s_l[kFewWarps][kRowsMost];
   __shared__ int s_abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   ptx::grid_dependents_launch();
-  const int of_parts = (int)(blockIdx.x % p.parts);
-  const int split = (int)(blockIdx.x / p.parts % p.splits);
-  const int64_t unit = blockIdx.x / p.parts / p.splits;
-  const int seq = (int)(unit / p.hkv), kvh = (int)(unit % p.hkv);
-  if (seq >= live_sequences(p.batch)) return;
+  const int split = (int)(blockIdx.x % p.splits);
+  const int64_t unit = blockIdx.x / p.splits;
+  const int kvh = (int)(unit % p.hkv);
+  const int live = live_sequences(p.batch);
+  int seq = (int)(unit / p.hkv), tok0 = 0;  // this CTA's tokens from tok0 on
+  if (p.few > p.tokens) {
+    // pieces of the sequences, counted in their order, 32 sequences at a time
+    int rest = seq, found = -1;
+    for (int b = 0; b < live && found < 0; b += 32) {
+      int mine = 0;
+      if (b + lane < live) {
+        const int n = __ldg(p.batch.cu + b + lane + 1) - __ldg(p.batch.cu + b + lane);
+        mine = n > 0 && n <= p.few ? (n + p.tokens - 1) / p.tokens : 0;
+      }
+      int upto = mine;
+#pragma unroll
+      for (int w = 1; w < 32; w *= 2) {
+        const int x = __shfl_up_sync(kFull, upto, w);
+        if (lane >= w) upto += x;
+      }
+      const unsigned past = __ballot_sync(kFull, upto > rest);
+      if (past) {
+        const int at = __ffs(past) - 1;
+        found = b + at;
+        tok0 = (rest - __shfl_sync(kFull, upto - mine, at)) * p.tokens;
+      } else {
+        rest -= __shfl_sync(kFull, upto, 31);
+      }
+    }
+    if (found < 0) return;
+    seq = found;
+  }
+  if (seq >= live) return;
   Sequence s = sequence(p.batch, seq);
-  const int tok0 = of_parts * p.tokens;  // this CTA's tokens from here on
   if (s.n > p.few || tok0 >= s.n) return;
   {  // as a sequence of its own, which ends with its last token
     const int rest = s.n - tok0 - p.tokens;
@@ -1032,6 +1029,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2)
     s.kv -= max(rest, 0);
   }
   const int rows = s.n * p.group;
+  const int tiles = (rows + 7) / 8;  // 8-row groups that there are
   const int pos0 = s.kv - s.n;  // keys before the first token's own
   const int k0 = split * p.split_keys, k1 = p.splits > 1 ? min(s.kv, k0 + p.split_keys) : s.kv;
   const int64_t row0 = (int64_t)s.row0 * p.hq + kvh * p.group;  // of [token, head] rows
@@ -1084,37 +1082,40 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2)
   };
   for (int i = 0; i < kFewStages; ++i) request(i);
 
-  // the rows of this lane: 16 mt + lane / 4, and 8 further
-  uint32_t qa[MT][D / 16][4];
-  int sees[MT][2];
+  // Q^T: columns are rows 8 nt + lane / 4; the statistics of a column are kept
+  // by the lanes whose accumulators belong to it, columns 8 nt + 2 (lane % 4)
+  // and one further
+  uint32_t qb[NT][D / 16][2];
+  int sees[NT][2];
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = nt * 8 + lane / 4;
+    const bool valid = r < rows;
+    const T *q = static_cast<const T *>(p.q) + (s.row0 + (valid ? r / p.group : 0)) * p.q_stride +
+                 (int64_t)(kvh * p.group + r % p.group) * D + (lane & 3) * 2;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = mt * 16 + h * 8 + lane / 4;
-      const bool valid = r < rows;
-      const int tok = valid ? r / p.group : s.n - 1;
-      sees[mt][h] = pos0 + tok + 1;
-      const T *q = static_cast<const T *>(p.q) + (s.row0 + tok) * p.q_stride +
-                   (int64_t)(kvh * p.group + r % p.group) * D + (lane & 3) * 2;
+    for (int k = 0; k < D / 16; ++k)
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k)
+      for (int e = 0; e < 2; ++e)
+        qb[nt][k][e] = valid ? *reinterpret_cast<const uint32_t *>(q + k * 16 + e * 8) : 0u;
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          qa[mt][k][e * 2 + h] = valid ? *reinterpret_cast<const uint32_t *>(q + k * 16 + e * 8) : 0u;
+    for (int e = 0; e < 2; ++e) {
+      const int c = nt * 8 + (lane & 3) * 2 + e;
+      sees[nt][e] = pos0 + (c < rows ? c / p.group : s.n - 1) + 1;
     }
-  float o[MT][D / 8][4], m[MT][2], l[MT][2];
+  }
+  float o[NT][D / 16][4], m[NT][2], l[NT][2];
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    m[mt][0] = m[mt][1] = -INFINITY;
-    l[mt][0] = l[mt][1] = 0.f;
+  for (int nt = 0; nt < NT; ++nt) {
+    m[nt][0] = m[nt][1] = -INFINITY;
+    l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
-    for (int nt = 0; nt < D / 8; ++nt) o[mt][nt][0] = o[mt][nt][1] = o[mt][nt][2] = o[mt][nt][3] = 0.f;
+    for (int d = 0; d < D / 16; ++d) o[nt][d][0] = o[nt][d][1] = o[nt][d][2] = o[nt][d][3] = 0.f;
   }
   const float slack = kSlack / p.qs;
   // ldmatrix addresses of this lane within a group: rows of keys, 16-byte chunks
-  const int kr = (lane & 7) + (lane >> 4) * 8, kc = (lane >> 3) & 1;  // K: key row, chunk parity
-  const int vr = lane & 15, vc = lane >> 4;                           // V (transposed)
+  const int kr = lane & 15, kc = lane >> 4;                             // K: [key][dim]
+  const int vr = (lane & 7) + (lane >> 4) * 8, vc = (lane >> 3) & 1;    // V, transposed
   int i = 0;
   for (; i < groups; ++i) {
     const int st = i % kFewStages;
@@ -1125,103 +1126,112 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2)
     }
     const unsigned char *kb = ring + st * 2 * F::kSide, *vb = kb + F::kSide;
     const uint32_t ka = ptx::smem_u32(kb) + kr * 128, va = ptx::smem_u32(vb) + vr * 128;
-    float sc[MT][2][4];
+    float sc[NT][4];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt) sc[mt][nt][0] = sc[mt][nt][1] = sc[mt][nt][2] = sc[mt][nt][3] = 0.f;
+    for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
       const int c = k * 2 + kc;
-      uint32_t b[4];
-      ldmatrix4(b, ka + (c / 8) * F::kHalf + (((c % 8) ^ (kr & 7)) << 4));
+      uint32_t a[4];
+      ldmatrix4(a, ka + (c / 8) * F::kHalf + (((c % 8) ^ (kr & 7)) << 4));
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        mma16816<T>(sc[mt][0], qa[mt][k], b[0], b[1]);
-        mma16816<T>(sc[mt][1], qa[mt][k], b[2], b[3]);
-      }
+      for (int nt = 0; nt < NT; ++nt)
+        if (nt < tiles) mma16816<T>(sc[nt], a, qb[nt][k][0], qb[nt][k][1]);
     }
     const int key = key_of(i);
     const bool partial = key + kFewKeys > pos0 + 1;  // some row does not see all of them
-    uint32_t pr[MT][4];
-    int lim[MT][2];
+    uint32_t pt[NT][2];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      float raise = 0.f, a[2];
+    for (int nt = 0; nt < NT; ++nt) {
+      if (nt >= tiles) continue;
+      float a[2], x[4];
+      bool raise = false;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        lim[mt][h] = sees[mt][h] - key;
-        float t = -INFINITY;
+      for (int e = 0; e < 2; ++e) {
+        // keys lane / 4 and 8 further
+        const int lim = sees[nt][e] - key - lane / 4;
+        if (partial && lim <= 0) sc[nt][e] = -INFINITY;
+        if (partial && lim <= 8) sc[nt][2 + e] = -INFINITY;
+        float t = fmaxf(sc[nt][e], sc[nt][2 + e]);
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float &x = sc[mt][nt][h * 2 + e];
-            if (partial && nt * 8 + (lane & 3) * 2 + e >= lim[mt][h]) x = -INFINITY;
-            t = fmaxf(t, x);
-          }
-        t = fmaxf(t, __shfl_xor_sync(kFull, t, 1));
-        t = fmaxf(t, __shfl_xor_sync(kFull, t, 2));
-        const bool up = t > m[mt][h] + slack;  // (the first keys: m is -infinity)
-        a[h] = up ? ex2((m[mt][h] - t) * p.qs) : 1.f;
-        if (up) m[mt][h] = t, raise = 1.f;
-        const float mq = m[mt][h] == -INFINITY ? 0.f : m[mt][h] * p.qs;
-        l[mt][h] *= a[h];
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          const float x0 = ex2(fmaf(sc[mt][nt][h * 2], p.qs, -mq));
-          const float x1 = ex2(fmaf(sc[mt][nt][h * 2 + 1], p.qs, -mq));
-          l[mt][h] += x0 + x1;
-          pr[mt][nt * 2 + h] = pack2<T>(x0, x1);
-        }
+        for (int w = 4; w < 32; w *= 2) t = fmaxf(t, __shfl_xor_sync(kFull, t, w));
+        const bool up = t > m[nt][e] + slack;  // (the first keys: m is -infinity)
+        a[e] = up ? ex2((m[nt][e] - t) * p.qs) : 1.f;
+        if (up) m[nt][e] = t;
+        raise |= up;
+        const float mq = m[nt][e] == -INFINITY ? 0.f : m[nt][e] * p.qs;
+        x[e] = ex2(fmaf(sc[nt][e], p.qs, -mq));
+        x[2 + e] = ex2(fmaf(sc[nt][2 + e], p.qs, -mq));
+        l[nt][e] = fmaf(l[nt][e], a[e], x[e] + x[2 + e]);
       }
-      if (__any_sync(kFull, raise != 0.f)) {
+      pt[nt][0] = transpose8x8(pack2<T>(x[0], x[1]));
+      pt[nt][1] = transpose8x8(pack2<T>(x[2], x[3]));
+      if (__any_sync(kFull, raise)) {
 #pragma unroll
-        for (int nt = 0; nt < D / 8; ++nt) {
-          o[mt][nt][0] *= a[0];
-          o[mt][nt][1] *= a[0];
-          o[mt][nt][2] *= a[1];
-          o[mt][nt][3] *= a[1];
+        for (int d = 0; d < D / 16; ++d) {
+          o[nt][d][0] *= a[0];
+          o[nt][d][1] *= a[1];
+          o[nt][d][2] *= a[0];
+          o[nt][d][3] *= a[1];
         }
       }
     }
-    // masked values: a weight of 0 does not silence a NaN.  Past the last key
-    // they are dropped; before it, where rows differ, odd ones are told apart.
+    // Masked values: a weight of 0 does not silence a NaN.  Past the last key
+    // they are dropped; before it, where rows differ, odd ones are taken out,
+    // and added to the rows that do see them.
     const int seen = s.kv - key;  // keys of the group that exist
-    bool odd = false;
-    if (partial && s.n > 1) {
-      constexpr int kRowVecs = 8 * (D / 64);
-      for (int e = lane; e < min(seen, kFewKeys) * kRowVecs; e += 32) {
-        const uint32_t *w = reinterpret_cast<const uint32_t *>(
-            vb + (e / 8 % (D / 64)) * F::kHalf + e / kRowVecs * 128 + e % 8 * 16);
-#pragma unroll
-        for (int h = 0; h < 4; ++h) odd |= odd_value<T>(w[h]) | odd_value<T>(w[h] >> 16);
+    if (seen < kFewKeys || (partial && s.n > 1)) {
+      unsigned char *v = ring + st * 2 * F::kSide + F::kSide;
+      constexpr int kRowVecs = 8 * kHalves;
+      auto word = [&](int e) {  // word e of the group: keys, then 16-byte vectors
+        return reinterpret_cast<uint32_t *>(v + (e / 32 % kHalves) * F::kHalf +
+                                            e / (4 * kRowVecs) * 128 + e % 32 * 4);
+      };
+      bool odd = false;
+      for (int e = lane; e < kFewKeys * kRowVecs * 4; e += 32) {
+        uint32_t *w = word(e);
+        if (e / (4 * kRowVecs) >= seen) *w = 0u;
+        else odd |= odd_value<T>(*w) | odd_value<T>(*w >> 16);
       }
-    }
-    if (__any_sync(kFull, odd)) {
-      values_one_by_one<T, D, MT>(vb, pr, lim, o);
-    } else {
-      // zeros for the keys past the last: rows 2 (lane % 4), + 1, and 8 further
-      uint32_t keep0 = ~0u, keep1 = ~0u;
-      if (seen < kFewKeys) {
-        const int r = (lane & 3) * 2;
-        keep0 = (r < seen ? 0xFFFFu : 0u) | (r + 1 < seen ? 0xFFFF0000u : 0u);
-        keep1 = (r + 8 < seen ? 0xFFFFu : 0u) | (r + 9 < seen ? 0xFFFF0000u : 0u);
-      }
+      if (__any_sync(kFull, odd)) {
+        // rare: key by key, 16-byte chunk and row of the warp's own layout
+#pragma unroll 1
+        for (int k = 0; k < min(seen, kFewKeys); ++k) {
 #pragma unroll
-      for (int nt = 0; nt < D / 8; nt += 2) {
-        const int c = nt + vc;
-        uint32_t b[4];
-        ldmatrix4_t(b, va + (c / 8) * F::kHalf + (((c % 8) ^ (vr & 7)) << 4));
-        if (seen < kFewKeys) b[0] &= keep0, b[1] &= keep1, b[2] &= keep0, b[3] &= keep1;
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          mma16816<T>(o[mt][nt], pr[mt], b[0], b[1]);
-          mma16816<T>(o[mt][nt + 1], pr[mt], b[2], b[3]);
+            for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int dim = d * 16 + h * 8 + lane / 4, c = dim / 8;
+                const float x = Elem<T>::to_f(*reinterpret_cast<const T *>(
+                    v + (c / 8) * F::kHalf + k * 128 + (((c % 8) ^ (k & 7)) << 4) + dim % 8 * 2));
+                if (!isfinite(x)) {
+                  if (key + k < sees[nt][0]) o[nt][d][h * 2] += x;
+                  if (key + k < sees[nt][1]) o[nt][d][h * 2 + 1] += x;
+                }
+              }
+        }
+        __syncwarp();
+        for (int e = lane; e < kFewKeys * kRowVecs * 4; e += 32) {
+          uint32_t *w = word(e);
+          if (odd_value<T>(*w)) *w &= 0xFFFF0000u;
+          if (odd_value<T>(*w >> 16)) *w &= 0x0000FFFFu;
         }
       }
+      __syncwarp();
+    }
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) {
+      const int c = d * 2 + vc;
+      uint32_t a[4];
+      ldmatrix4_t(a, va + (c / 8) * F::kHalf + (((c % 8) ^ (vr & 7)) << 4));
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        if (nt < tiles) mma16816<T>(o[nt][d], a, pt[nt][0], pt[nt][1]);
     }
     __syncwarp();  // the stage has been read
+    ptx::fence_proxy_async();
     request(i + kFewStages);
   }
   if (i < groups && lane == 0) {  // given up: wait for the copies in flight (bounded)
@@ -1231,25 +1241,27 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2)
   }
   __syncwarp();
 
-  // the four warps' outputs meet: this warp's in its own ring
-  float *mine = reinterpret_cast<float *>(ring);  // [16 MT][D]
-  static_assert(16 * MT * D * 4 <= F::kRing, "a warp's output fits its ring");
+  // the four warps' outputs meet: this warp's in its own ring, [row][D + 4]
+  constexpr int kPitch = D + 4;  // (4: eight lanes of a column write to eight places)
+  float *mine = reinterpret_cast<float *>(ring);
+  static_assert(kRowsMost * kPitch * 4 <= F::kRing, "a warp's output fits its ring");
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = mt * 16 + h * 8 + lane / 4;
-      float sum = l[mt][h];
-      sum += __shfl_xor_sync(kFull, sum, 1);
-      sum += __shfl_xor_sync(kFull, sum, 2);
-      if ((lane & 3) == 0) {
-        s_m[warp][r] = m[mt][h] * p.qs;
+    for (int e = 0; e < 2; ++e) {
+      const int r = nt * 8 + (lane & 3) * 2 + e;
+      float sum = l[nt][e];
+#pragma unroll
+      for (int w = 4; w < 32; w *= 2) sum += __shfl_xor_sync(kFull, sum, w);
+      if (lane < 4) {
+        s_m[warp][r] = m[nt][e] * p.qs;
         s_l[warp][r] = sum;
       }
 #pragma unroll
-      for (int nt = 0; nt < D / 8; ++nt)
-        *reinterpret_cast<float2 *>(mine + r * D + nt * 8 + (lane & 3) * 2) =
-            make_float2(o[mt][nt][h * 2], o[mt][nt][h * 2 + 1]);
+      for (int d = 0; d < D / 16; ++d) {
+        mine[r * kPitch + d * 16 + lane / 4] = o[nt][d][e];
+        mine[r * kPitch + d * 16 + 8 + lane / 4] = o[nt][d][2 + e];
+      }
     }
   __syncthreads();
   const float *all = reinterpret_cast<const float *>(ring - warp * F::kRing);
@@ -1265,7 +1277,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2)
     for (int w = 0; w < kFewWarps; ++w) {
       if (s_l[w][r] == 0.f) continue;
       const float a = exp2f(s_m[w][r] - top);
-      const float4 y = *reinterpret_cast<const float4 *>(all + w * (F::kRing / 4) + r * D + d);
+      const float4 y = *reinterpret_cast<const float4 *>(all + w * (F::kRing / 4) + r * kPitch + d);
       sum = fmaf(a, s_l[w][r], sum);
       x.x = fmaf(a, y.x, x.x);
       x.y = fmaf(a, y.y, x.y);
@@ -1285,66 +1297,95 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2)
 }
 
 // ------------------------------------------------------------------- joins
-// Joins the splits of a row and head, a CTA for each: with M = max_s m_s,
-//   o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s,
-// warp w over the splits w, w + 4, ..., the four sums in the order of w.
+// Joins the splits of a row and head: with M = max_s m_s,
+//   o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.
+// `per` warps of the CTA's eight share a row: eight splits each at a time, whose
+// loads are all in flight before the first is used (a join is latency), with a
+// running maximum; then the warps' results in their order.
 // FEW: the rows are [sequence, token below few]; else the packed rows of the
 // sequences with more tokens than that.
 template <typename T, int D, bool FEW>
-__global__ void __launch_bounds__(128)
-    join_kernel(const __grid_constant__ RaggedBatch batch, int hq, int few, int splits,
+__global__ void __launch_bounds__(256)
+    join_kernel(const __grid_constant__ RaggedBatch batch, int hq, int few, int splits, int per,
                 const float *__restrict__ part_o, const float2 *__restrict__ part_ml, T *out) {
-  constexpr int kE = D / 32;
-  __shared__ float s_top[4], s_sum[4], s_o[4][D];
+  constexpr int kE = D / 32, kBatch = 8;
+  __shared__ float s_m[8], s_l[8], s_o[8][D];
   ptx::grid_dependency_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t at = blockIdx.x;
   const int64_t step = (int64_t)(FEW ? (int64_t)batch.n_seqs * few : batch.n_tokens) * hq;
+  const int64_t at = (int64_t)blockIdx.x * (8 / per) + warp / per;
   const int live = live_sequences(batch);
-  int64_t row;
-  if (FEW) {
-    const int seq = (int)(at / hq / few), tok = (int)(at / hq % few);
-    if (seq >= live) return;
-    const Sequence s = sequence(batch, seq);
-    if (s.n > few || tok >= s.n) return;
-    row = s.row0 + tok;
-  } else {
-    row = at / hq;
-    const int seq = sequence_of_row(batch, live, (int)row);
-    if (seq < 0 || sequence(batch, seq).n <= few) return;
+  int64_t row = -1;
+  if (at < step) {
+    if (FEW) {
+      const int seq = (int)(at / hq / few), tok = (int)(at / hq % few);
+      if (seq < live) {
+        const Sequence s = sequence(batch, seq);
+        if (s.n <= few && tok < s.n) row = s.row0 + tok;
+      }
+    } else {
+      const int seq = sequence_of_row(batch, live, (int)(at / hq));
+      if (seq >= 0 && sequence(batch, seq).n > few) row = at / hq;
+    }
   }
-  float top = -INFINITY;
-  for (int i = threadIdx.x; i < splits; i += 128) {
-    const float2 ml = part_ml[i * step + at];
-    if (ml.y != 0.f) top = fmaxf(top, ml.x);
-  }
-#pragma unroll
-  for (int e = 16; e; e >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, e));
-  if (lane == 0) s_top[warp] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
-  float sum = 0.f, o[kE];
+  float m = -INFINITY, l = 0.f, o[kE];
 #pragma unroll
   for (int e = 0; e < kE; ++e) o[e] = 0.f;
-#pragma unroll 4
-  for (int i = warp; i < splits; i += 4) {
-    const float2 ml = part_ml[i * step + at];
-    if (ml.y == 0.f) continue;  // (its output was not written)
-    const float f = exp2f(ml.x - top);
-    sum = fmaf(f, ml.y, sum);
-    const float *src = part_o + (i * step + at) * D + lane * kE;
+  if (row >= 0) {
+    for (int i0 = warp % per; i0 < splits; i0 += per * kBatch) {
+      float2 ml[kBatch];
+      float x[kBatch][kE];
 #pragma unroll
-    for (int e = 0; e < kE; ++e) o[e] = fmaf(f, src[e], o[e]);
+      for (int b = 0; b < kBatch; ++b) {
+        const int i = i0 + b * per;
+        ml[b] = i < splits ? part_ml[i * step + at] : make_float2(-INFINITY, 0.f);
+        const float *src = part_o + (min(i, splits - 1) * step + at) * D + lane * kE;
+#pragma unroll
+        for (int e = 0; e < kE; ++e) x[b][e] = src[e];  // (not written where the sum is 0)
+      }
+      float top = m;
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) top = ml[b].y != 0.f ? fmaxf(top, ml[b].x) : top;
+      const float a = l != 0.f ? exp2f(m - top) : 0.f;
+      l *= a;
+#pragma unroll
+      for (int e = 0; e < kE; ++e) o[e] = l != 0.f ? o[e] * a : 0.f;
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        if (ml[b].y == 0.f) continue;
+        const float f = exp2f(ml[b].x - top);
+        l = fmaf(f, ml[b].y, l);
+#pragma unroll
+        for (int e = 0; e < kE; ++e) o[e] = fmaf(f, x[b][e], o[e]);
+      }
+      m = top;
+    }
   }
-  if (lane == 0) s_sum[warp] = sum;
+  if (per > 1) {
+    if (lane == 0) s_m[warp] = m, s_l[warp] = l;
 #pragma unroll
-  for (int e = 0; e < kE; ++e) s_o[warp][lane * kE + e] = o[e];
-  __syncthreads();
-  if (threadIdx.x >= D) return;
-  const int d = threadIdx.x;
-  sum = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
-  const float x = (s_o[0][d] + s_o[1][d]) + (s_o[2][d] + s_o[3][d]);
-  out[(row * hq + at % hq) * D + d] = Elem<T>::from_f(sum == 0.f ? 0.f : x / sum);
+    for (int e = 0; e < kE; ++e) s_o[warp][lane * kE + e] = o[e];
+    __syncthreads();
+    if (warp % per) return;
+    float top = -INFINITY;
+    for (int w = warp; w < warp + per; ++w)
+      if (s_l[w] != 0.f) top = fmaxf(top, s_m[w]);
+    l = 0.f;
+#pragma unroll
+    for (int e = 0; e < kE; ++e) o[e] = 0.f;
+    for (int w = warp; w < warp + per; ++w) {
+      if (s_l[w] == 0.f) continue;
+      const float f = exp2f(s_m[w] - top);
+      l = fmaf(f, s_l[w], l);
+#pragma unroll
+      for (int e = 0; e < kE; ++e) o[e] = fmaf(f, s_o[w][lane * kE + e], o[e]);
+    }
+  }
+  if (row < 0) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T *to = out + (row * hq + at % hq) * D + lane * kE;
+#pragma unroll
+  for (int e = 0; e < kE; ++e) to[e] = Elem<T>::from_f(o[e] * inv);
 }
 
 }  // namespace ragged
@@ -1431,8 +1472,9 @@ int64_t most_units(int64_t n_tokens, int64_t n_seqs, int64_t hq, int64_t hkv) {
 // the few-rows kernel) and longer ones go to a kernel each; a call that cannot
 // have the one or the other does not launch it.
 struct Plan {
-  int mt;                // 16-row groups of a CTA of the few-rows kernel; 0: none
-  int few, tokens, parts;
+  int nt;                // 8-row groups of a CTA of the few-rows kernel; 0: none
+  int few, tokens;
+  int64_t pieces;        // of up to `tokens` tokens, at most
   bool tiles;            // whether the tile kernel runs
   int few_splits, split_keys;
   int splits, split_blocks;
@@ -1444,26 +1486,29 @@ Plan plan_paged(bool one_token, int64_t n_tokens, int64_t n_seqs, int64_t hq, in
   using namespace tide::ragged;
   Plan p{};
   const int64_t group = hq / hkv;
-  // a decode step whose heads fit 16 rows; else 32 rows a CTA
-  p.mt = one_token && group <= 16 ? 1 : group <= 32 ? 2 : 0;
-  p.tokens = (int)(p.mt * 16 / group);
-  // Up to 128 rows (a tile of the other kernel) are few.  The lengths are on
-  // the device: with as many tokens as make most sequences long, all of them
-  // go to the tiles, with one sequence its length is known.
-  p.few = one_token ? 1 : 4 * p.tokens;
-  if (!one_token && (n_tokens > n_seqs * 2 * p.few || (n_seqs == 1 && n_tokens > p.few))) p.mt = 0;
-  if (!p.mt) p.few = 0;
+  // Rows of a CTA of the few-rows kernel: 8 for a decode step whose heads fit
+  // them, else 16, else 32.
+  p.nt = one_token && group <= 8 ? 1 : group <= 16 ? 2 : group <= 32 ? 4 : 0;
+  p.tokens = (int)(p.nt * 8 / group);
+  // The lengths are on the device; few is what two CTAs take.  mma.sync bounds
+  // that kernel from some 16 rows on (16 requests of 1 to 9 tokens and 4 heads
+  // each over up to 2100 keys: 54 us there, 41 us as tiles), so with more on
+  // average every sequence goes to the tiles; with one sequence its length is
+  // known.
+  p.few = one_token ? 1 : 2 * p.tokens;
+  if (!one_token && (n_tokens * group > n_seqs * 16 || (n_seqs == 1 && n_tokens > p.few))) p.nt = 0;
+  if (!p.nt) p.few = 0;
   if (n_tokens < p.few) p.few = (int)n_tokens;
-  p.tiles = !p.mt || (!one_token && n_tokens > p.few);
-  p.parts = p.mt ? (p.few + p.tokens - 1) / p.tokens : 0;
+  p.tiles = !p.nt || (!one_token && n_tokens > p.few);
+  p.pieces = n_seqs + (p.few > p.tokens ? n_tokens / p.tokens : 0);
   const int64_t rows = n_tokens * hq;
   // Few rows: splits of 512 keys at least, as long as the CTAs that an SM
   // holds (two) are not taken eight times over: sequences differ in length,
   // and the more pieces, the evener the end.
-  const int64_t units = n_seqs * hkv;
-  int64_t s = p.mt ? (16 * 148 + units - 1) / units : 1;
+  const int64_t units = p.pieces * hkv;
+  int64_t s = p.nt ? (16 * 148 + units - 1) / units : 1;
   if (s > (max_kv + 511) / 512) s = (max_kv + 511) / 512;
-  if (s < 1) s = 1;
+  if (s < 1 || units >= 4 * 148) s = 1;
   const int64_t keys = (max_kv + s - 1) / s;
   p.split_keys = (int)((keys + 63) / 64 * 64);
   p.few_splits = (int)s;
@@ -1518,18 +1563,18 @@ int launch(tide::ragged::Params &p, int dtype, const void *q, int64_t q_stride, 
   return report(cudaLaunchKernelEx(&cfg, kern, p, mq, mk, mv), "ragged attention");
 }
 
-template <typename T, int D, int MT>
+template <typename T, int D, int NT>
 int launch_few(const tide::ragged::FewParams &p, int dtype, int64_t kv_rows, cudaStream_t s) {
   using namespace tide::ragged;
   CUtensorMap mk, mv;
   if (!make_map(&mk, dtype, p.src.k, 2, D, kv_rows, 1, D, 0, kFewKeys, 1) ||
       !make_map(&mv, dtype, p.src.v, 2, D, kv_rows, 1, D, 0, kFewKeys, 1))
     return fail(TIDE_ERR_CUDA, "paged_attention: cuTensorMapEncodeTiled failed");
-  auto kern = few_rows_kernel<T, D, MT>;
+  auto kern = few_rows_kernel<T, D, NT>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        (int)Few<D>::kSmem);
   if (e != cudaSuccess) return report(e, "paged_attention");
-  const int64_t ctas = (int64_t)p.batch.n_seqs * p.hkv * p.splits * p.parts;
+  const int64_t ctas = (int64_t)p.pieces * p.hkv * p.splits;
   kern<<<(unsigned)ctas, 32 * kFewWarps, Few<D>::kSmem, s>>>(p, mk, mv);
   return report(cudaSuccess, "paged_attention");
 }
@@ -1538,8 +1583,10 @@ template <typename T, int D, bool FEW>
 int launch_join(const tide::RaggedBatch &b, int hq, int few, int splits, const float *part_o,
                 const float2 *part_ml, void *out, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((FEW ? (int64_t)b.n_seqs * few : b.n_tokens) * hq), 1, 1);
-  cfg.blockDim = dim3(128, 1, 1);
+  const int64_t rows = (int64_t)(FEW ? (int64_t)b.n_seqs * few : b.n_tokens) * hq;
+  const int per = splits <= 8 ? 1 : splits <= 16 ? 2 : splits <= 32 ? 4 : 8;
+  cfg.gridDim = dim3((unsigned)((rows * per + 7) / 8), 1, 1);
+  cfg.blockDim = dim3(256, 1, 1);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];  // its launch overlaps the tail of the kernel before
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1547,7 +1594,7 @@ int launch_join(const tide::RaggedBatch &b, int hq, int few, int splits, const f
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return report(cudaLaunchKernelEx(&cfg, tide::ragged::join_kernel<T, D, FEW>, b, hq, few, splits,
-                                   part_o, part_ml, static_cast<T *>(out)),
+                                   per, part_o, part_ml, static_cast<T *>(out)),
                 "paged_attention");
 }
 
@@ -1567,15 +1614,17 @@ int run_paged(const Plan &plan, tide::ragged::Params &p, int dtype, const void *
     p.part_ml = reinterpret_cast<float2 *>(ws + plan.few_bytes + plan.splits * rows * D * 4);
   }
   int rc;
-  if (plan.mt) {
+  if (plan.nt) {
     tide::ragged::FewParams f{p.batch, p.src,  q,     q_stride,  p.out,       few_o,
                               few_ml,  p.hq,   p.hkv, p.group,   plan.few,    plan.tokens,
-                              plan.parts, plan.few_splits, plan.split_keys, p.qs};
-    rc = plan.mt == 1 ? launch_few<T, D, 1>(f, dtype, kv_rows, s) : launch_few<T, D, 2>(f, dtype, kv_rows, s);
+                              (int)plan.pieces, plan.few_splits, plan.split_keys, p.qs};
+    rc = plan.nt == 1   ? launch_few<T, D, 1>(f, dtype, kv_rows, s)
+         : plan.nt == 2 ? launch_few<T, D, 2>(f, dtype, kv_rows, s)
+                        : launch_few<T, D, 4>(f, dtype, kv_rows, s);
     if (rc) return rc;
   }
-  if (plan.tiles && (rc = launch<T, D, true>(p, dtype, q, q_stride, kv_rows, plan.mt != 0, s))) return rc;
-  if (plan.mt && plan.few_splits > 1 &&
+  if (plan.tiles && (rc = launch<T, D, true>(p, dtype, q, q_stride, kv_rows, plan.nt != 0, s))) return rc;
+  if (plan.nt && plan.few_splits > 1 &&
       (rc = launch_join<T, D, true>(p.batch, p.hq, plan.few, plan.few_splits, few_o, few_ml, p.out, s)))
     return rc;
   if (plan.splits > 1)
