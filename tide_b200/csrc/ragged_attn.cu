@@ -39,8 +39,13 @@
 //
 // Order of units: by the number of keys they read, most first (the level of a
 // unit: positions before its end, in units of its size), so that the last
-// ones to start are short.  A sequence's level range and the rank within a
+// ones to start are short; dealt to the CTAs to and fro, so that none gets the
+// longest of every round.  A sequence's level range and the rank within a
 // level come from counting over the sequences, so no list of units is built.
+// Where the sequences' keys and values exceed what L2 holds, this goes group by
+// group of consecutive sequences that fit: over all sixteen prompts of a 16 x
+// 2048 prefill at once (134 MB) the kernel read 1.6 GB from HBM instead of 0.4
+// and took 606 us instead of 570, at 15 % more power than it has.
 //
 // Long contexts with few rows are split over the keys (paged caches only):
 // the splits' unnormalised outputs, maxima and sums go to the workspace and
@@ -94,6 +99,7 @@ struct Params {
   int splits;
   int split_blocks;  // key blocks of a split
   int few;         // sequences of up to so many tokens go to the few-rows kernel
+  int64_t group_keys;  // keys whose rows, of all KV heads, L2 holds
   float qs;        // scale * log2(e)
 };
 
@@ -177,55 +183,83 @@ __device__ void schedule_units(const Params &p, Shared &sh) {
   const int lane = threadIdx.x & 31;
   const int live = live_sequences(p.batch);
   int cnt[kCached], lvl[kCached];
-  int top = 0;
 #pragma unroll
   for (int k = 0; k < kCached; ++k) {
     cnt[k] = lvl[k] = 0;
     if (lane + 32 * k < live) seq_level(p, lane + 32 * k, &cnt[k], &lvl[k]);
-    top = max(top, cnt[k] + lvl[k]);
   }
-  for (int i = lane + 32 * kCached; i < live; i += 32) {
-    int c, l;
-    seq_level(p, i, &c, &l);
-    top = max(top, c + l);
-  }
-  top = __reduce_max_sync(kFull, top);
-  auto units_from = [&](int x) {  // units of level x and above
+  int s0 = 0, s1 = 0;  // the group: sequences [s0, s1)
+  auto units_from = [&](int x) {  // its units of level x and above
     int c = 0;
 #pragma unroll
-    for (int k = 0; k < kCached; ++k) c += min(max(cnt[k] + lvl[k] - x, 0), cnt[k]);
-    for (int i = lane + 32 * kCached; i < live; i += 32) {
-      int n, l;
-      seq_level(p, i, &n, &l);
+    for (int k = 0; k < kCached; ++k)
+      if (lane + 32 * k >= s0 && lane + 32 * k < s1) c += min(max(cnt[k] + lvl[k] - x, 0), cnt[k]);
+    for (int i = max(s0 & ~31, 32 * kCached) + lane; i < s1; i += 32) {
+      int n = 0, l = 0;
+      if (i >= s0) seq_level(p, i, &n, &l);
       c += min(max(n + l - x, 0), n);
     }
     return (int)__reduce_add_sync(kFull, (unsigned)c);
   };
-  const int total = units_from(0);
   const int per_rank = p.hkv * p.splits;
-  int x = top, above = 0, upto = 0;  // level, units above it, units of it and above
+  int64_t base = 0;                  // units (of one KV head and split) before the group
+  int total = 0;                     // in the group
+  int x = 0, above = 0, upto = 0;    // level, the group's units above it, of it and above
   uint32_t n = 0;
-  for (int64_t u = blockIdx.x;; u += gridDim.x, ++n) {
+  for (int64_t round = 0;; ++round, ++n) {
+    const int64_t u =
+        round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
     const int slot = n & 1;
     const int64_t rank = u / per_rank;
+    while (rank - base >= total && s1 < live) {  // the next group
+      base += total;
+      s0 = s1;
+      int64_t keys = 0;
+      int top = 0;
+      for (;;) {
+        const int i = s1 + lane;
+        const int mine = i < live ? sequence(p.batch, i).kv : 0;
+        int64_t sum = mine;
+#pragma unroll
+        for (int w = 1; w < 32; w *= 2) {
+          const int64_t y = __shfl_up_sync(kFull, sum, w);
+          if (lane >= w) sum += y;
+        }
+        const bool in = i < live && (keys + sum <= p.group_keys || i == s0);
+        const int many = __popc(__ballot_sync(kFull, in));
+        if (in) {
+          int c, l;
+          seq_level(p, i, &c, &l);
+          top = max(top, c + l);
+        }
+        keys += __shfl_sync(kFull, sum, 31);
+        s1 += many;
+        if (many < 32) break;
+      }
+      x = __reduce_max_sync(kFull, top);
+      above = upto = 0;
+      total = units_from(0);
+    }
     Unit w{};
-    if (rank < total) {
-      if (rank >= upto) {  // units_from(lo) > rank >= units_from(hi)
+    if (rank - base < total) {
+      const int in_group = (int)(rank - base);
+      if (in_group >= upto) {  // units_from(lo) > in_group >= units_from(hi)
         int lo = 0, hi = x;
         while (hi - lo > 1) {
           const int mid = (lo + hi) >> 1;
-          if (units_from(mid) > rank) lo = mid;
+          if (units_from(mid) > in_group) lo = mid;
           else hi = mid;
         }
         x = lo;
         upto = units_from(lo);
         above = units_from(hi);
       }
-      int r = (int)rank - above;  // the r-th sequence with a unit of level x
+      int r = in_group - above;  // the r-th sequence of the group with a unit of level x
       int seq = -1, level = 0;
 #pragma unroll
       for (int k = 0; k < kCached; ++k) {
-        const bool has = lvl[k] <= x && x < lvl[k] + cnt[k];
+        const int i = lane + 32 * k;
+        const bool has = i >= s0 && i < s1 && lvl[k] <= x && x < lvl[k] + cnt[k];
         const unsigned who = __ballot_sync(kFull, has);
         if (seq < 0) {
           if (r < __popc(who)) {
@@ -238,9 +272,9 @@ __device__ void schedule_units(const Params &p, Shared &sh) {
           }
         }
       }
-      for (int b = 32 * kCached; seq < 0 && b < live; b += 32) {
+      for (int b = max(s0 & ~31, 32 * kCached); seq < 0 && b < s1; b += 32) {
         int c = 0, l = 0;
-        if (b + lane < live) seq_level(p, b + lane, &c, &l);
+        if (b + lane >= s0 && b + lane < s1) seq_level(p, b + lane, &c, &l);
         const bool has = l <= x && x < l + c;
         const unsigned who = __ballot_sync(kFull, has);
         if (r < __popc(who)) {
@@ -1632,7 +1666,7 @@ int run_paged(const Plan &plan, tide::ragged::Params &p, int dtype, const void *
   return TIDE_OK;
 }
 
-void set_heads(tide::ragged::Params &p, int64_t hq, int64_t hkv, float scale, void *out) {
+void set_heads(tide::ragged::Params &p, int64_t hq, int64_t hkv, int64_t d, float scale, void *out) {
   p.out = out;
   p.hq = (int)hq;
   p.hkv = (int)hkv;
@@ -1642,6 +1676,7 @@ void set_heads(tide::ragged::Params &p, int64_t hq, int64_t hkv, float scale, vo
   p.splits = 1;
   p.split_blocks = 1 << 24;  // all of them
   p.few = 0;
+  p.group_keys = (64 << 20) / (hkv * d * 4);  // half of the 126 MB
 }
 
 }  // namespace
@@ -1668,7 +1703,7 @@ extern "C" int tide_packed_attention(int dtype, const void *q, const void *k, co
              error_word};
   p.src = {k, v, kv_row_stride, nullptr, 0, 0, 0};
   p.zero_keys = zero_keys;
-  set_heads(p, n_q_heads, n_kv_heads, scale, out);
+  set_heads(p, n_q_heads, n_kv_heads, head_dim, scale, out);
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == TIDE_DTYPE_BF16)
     return head_dim == 128
@@ -1732,7 +1767,7 @@ extern "C" int tide_paged_attention(int dtype, const void *q, int64_t q_row_stri
   p.batch = {cu_seqlens, seq_ids, kv_lens, n_seqs_dev, (int)n_seqs, (int)n_requests,
              (int)n_tokens, (int)max_kv_len, error_word};
   p.src = {k_cache, v_cache, 0, block_tables, max_pages, (int)n_pages, shift};
-  set_heads(p, n_q_heads, n_kv_heads, scale, out);
+  set_heads(p, n_q_heads, n_kv_heads, head_dim, scale, out);
   if (dtype == TIDE_DTYPE_BF16)
     return head_dim == 128 ? run_paged<__nv_bfloat16, 128>(plan, p, dtype, q, q_row_stride, kv_rows, ws, st)
                            : run_paged<__nv_bfloat16, 64>(plan, p, dtype, q, q_row_stride, kv_rows, ws, st);
