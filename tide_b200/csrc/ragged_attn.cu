@@ -8,7 +8,7 @@
 // A tile is 128 rows: floor(128 / G) consecutive tokens of a sequence times
 // the G query heads of one KV head, so that a key or value loaded serves all
 // heads that share it.  A unit of work is two such tiles, one behind the
-// other; a persistent CTA per SM walks over units.  Per block of 128 keys and
+// other; a CTA per SM walks over units.  Per block of 128 keys and
 // tile,
 //   S[128 x 128] = Q K^T      tcgen05.mma, operands in shared memory (TMA,
 //                             128-byte swizzle), S in tensor memory;
@@ -39,8 +39,9 @@
 //
 // Order of units: by the number of keys they read, most first (the level of a
 // unit: positions before its end, in units of its size), so that the last
-// ones to start are short; dealt to the CTAs to and fro, so that none gets the
-// longest of every round.  A sequence's level range and the rank within a
+// ones to start are short.  The grid has a CTA per unit; those that run take
+// over the ones that have yet to start (cluster launch control), one ahead.  A
+// sequence's level range and the rank within a
 // level come from counting over the sequences, so no list of units is built.
 // Where the sequences' keys and values exceed what L2 holds, this goes group by
 // group of consecutive sequences that fit: over all sixteen prompts of a 16 x
@@ -148,6 +149,8 @@ struct Shared {
   uint64_t o_full[2];     // after a unit's last value product
   uint64_t u_full[2], u_empty[2];
   uint64_t drain;
+  uint64_t taken;   // the answer to a request for another CTA's unit
+  __align__(16) unsigned char answer[16];
   uint64_t kv_full[kRing], kv_empty[kRing];
   uint64_t raw_full[kRing];  // value blocks that have landed and are to be cleaned, in turn
   Unit unit[2];
@@ -178,6 +181,29 @@ __device__ __forceinline__ void seq_level(const Params &p, int i, int *count, in
   *level = max(s.kv - s.n, 0) / per;
 }
 
+// The unit of a CTA that has yet to start, which then does not; *more is false
+// when there is none.  False when the wait ran out.
+__device__ __forceinline__ bool next_unit(const Params &p, Shared &sh, int64_t *u, uint32_t *asked,
+                                          bool *more) {
+  if ((threadIdx.x & 31) == 0) {
+    ptx::mbar_expect_tx(&sh.taken, 16);
+    ptx::clc_try_cancel(sh.answer, &sh.taken);
+  }
+  __syncwarp();
+  if (!__all_sync(0xffffffffu, ptx::mbar_wait(&sh.taken, *asked & 1, &sh.abort))) {
+    sh.abort = 1;
+    raise_error(p.batch.err, TIDE_DEVERR_TIMEOUT);
+    return false;
+  }
+  ++*asked;
+  uint32_t cta = 0;
+  *more = ptx::clc_canceled(sh.answer, &cta);
+  *u = cta;
+  ptx::fence_proxy_async();  // read before the next answer is written
+  __syncwarp();
+  return true;
+}
+
 __device__ void schedule_units(const Params &p, Shared &sh) {
   constexpr unsigned kFull = 0xffffffffu;
   const int lane = threadIdx.x & 31;
@@ -187,6 +213,18 @@ __device__ void schedule_units(const Params &p, Shared &sh) {
   for (int k = 0; k < kCached; ++k) {
     cnt[k] = lvl[k] = 0;
     if (lane + 32 * k < live) seq_level(p, lane + 32 * k, &cnt[k], &lvl[k]);
+  }
+  int64_t units_in_all = 0;  // of one KV head and split
+  {
+    int c = 0;
+#pragma unroll
+    for (int k = 0; k < kCached; ++k) c += cnt[k];
+    for (int i = lane + 32 * kCached; i < live; i += 32) {
+      int n, l;
+      seq_level(p, i, &n, &l);
+      c += n;
+    }
+    units_in_all = __reduce_add_sync(kFull, (unsigned)c);
   }
   int s0 = 0, s1 = 0;  // the group: sequences [s0, s1)
   auto units_from = [&](int x) {  // its units of level x and above
@@ -205,12 +243,21 @@ __device__ void schedule_units(const Params &p, Shared &sh) {
   int64_t base = 0;                  // units (of one KV head and split) before the group
   int total = 0;                     // in the group
   int x = 0, above = 0, upto = 0;    // level, the group's units above it, of it and above
-  uint32_t n = 0;
-  for (int64_t round = 0;; ++round, ++n) {
-    const int64_t u =
-        round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+  int top_level = 0;
+  uint32_t asked = 0;
+  bool more = true;
+  int64_t u = blockIdx.x;
+  for (uint32_t n = 0;; ++n) {
     const int slot = n & 1;
+    // every warp has taken up the unit before: time for another one (sooner,
+    // and at the end one CTA would hold what another could run)
+    if (n > 0) TIDE_WAIT(&sh.u_empty[slot ^ 1], ((n - 1) >> 1) & 1);
+    if (n > 0 && !next_unit(p, sh, &u, &asked, &more)) return;
+    // a CTA without a unit takes over what else there is without one
+    while (more && u / per_rank >= units_in_all)
+      if (!next_unit(p, sh, &u, &asked, &more)) return;
     const int64_t rank = u / per_rank;
+    if (rank < base) s1 = total = 0, base = 0;  // (should they ever come out of order)
     while (rank - base >= total && s1 < live) {  // the next group
       base += total;
       s0 = s1;
@@ -236,13 +283,14 @@ __device__ void schedule_units(const Params &p, Shared &sh) {
         s1 += many;
         if (many < 32) break;
       }
-      x = __reduce_max_sync(kFull, top);
+      x = top_level = __reduce_max_sync(kFull, top);
       above = upto = 0;
       total = units_from(0);
     }
     Unit w{};
-    if (rank - base < total) {
+    if (more && rank < units_in_all) {
       const int in_group = (int)(rank - base);
+      if (in_group < above) x = top_level, above = upto = 0;
       if (in_group >= upto) {  // units_from(lo) > in_group >= units_from(hi)
         int lo = 0, hi = x;
         while (hi - lo > 1) {
@@ -300,7 +348,6 @@ __device__ void schedule_units(const Params &p, Shared &sh) {
       w.b0 = w.split * p.split_blocks;
       w.b1 = w.b0 + p.split_blocks;
     }
-    if (n >= 2) TIDE_WAIT(&sh.u_empty[slot], ((n >> 1) + 1) & 1);
     if (lane == 0) {
       sh.unit[slot] = w;
       ptx::mbar_arrive(&sh.u_full[slot]);
@@ -869,6 +916,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       sh.raw[i] = 0;
     }
     ptx::mbar_init(&sh.drain, 1);
+    ptx::mbar_init(&sh.taken, 1);
     ptx::fence_mbar_init();
     sh.abort = 0;
     sh.loaded = sh.raw_loaded = sh.q_loaded[0] = sh.q_loaded[1] = 0;
@@ -1487,14 +1535,6 @@ int check_heads(int dtype, int64_t hq, int64_t hkv, int64_t d, float scale, int6
   return TIDE_OK;
 }
 
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 0;
-  return n;
-}
-
 // Units (two tiles, one KV head) that a batch may have at most.
 int64_t most_units(int64_t n_tokens, int64_t n_seqs, int64_t hq, int64_t hkv) {
   const int64_t per = 2 * (tide::ragged::kRows / (hq / hkv));
@@ -1547,13 +1587,19 @@ Plan plan_paged(bool one_token, int64_t n_tokens, int64_t n_seqs, int64_t hq, in
   p.split_keys = (int)((keys + 63) / 64 * 64);
   p.few_splits = (int)s;
   p.few_bytes = s > 1 ? (size_t)(s * n_seqs * p.few * hq * (d + 2) * 4 + 15) / 16 * 16 : 0;
-  // Tiles: as many as give every SM a unit, of four blocks of keys at least
-  // (below that the start and the join of a split cost more than its keys).
+  // Tiles: the number of splits whose rounds over the SMs end soonest.  A block
+  // of keys takes a unit about 1.8 us, starting and ending it 4 us, and a
+  // split's outputs go to HBM and back (8 (d + 2) bytes a row at 6.5 TB/s).
   const int64_t tile_units = most_units(n_tokens, n_seqs, hq, hkv);
   const int64_t blocks = (max_kv + kKeys - 1) / kKeys;
-  int64_t t = p.tiles && tile_units > 0 ? 148 / tile_units : 1;
-  if (t > blocks / 4) t = blocks / 4;
-  if (t < 1) t = 1;
+  int64_t t = 1;
+  double best = 0;
+  for (int64_t i = 1; p.tiles && i <= 32 && (i == 1 || i * 4 <= blocks); ++i) {
+    const double rounds = (double)((tile_units * i + 147) / 148);
+    const double us = rounds * (1.8 * (double)((blocks + i - 1) / i) + 4.0) +
+                      (i > 1 ? 4.0 + 8.0 * (double)(rows * i * (d + 2)) / 6.5e6 : 0.0);
+    if (i == 1 || us < best) best = us, t = i;
+  }
   p.splits = (int)t;
   p.split_blocks = (int)((blocks + t - 1) / t);
   p.bytes = p.few_bytes + (t > 1 ? (size_t)(t * rows * (d + 2) * 4) : 0);
@@ -1582,10 +1628,9 @@ int launch(tide::ragged::Params &p, int dtype, const void *q, int64_t q_stride, 
   if (e != cudaSuccess) return report(e, "ragged attention");
   const int64_t units =
       most_units(p.batch.n_tokens, p.batch.n_seqs, p.hq, p.hkv) * p.splits;
-  const int sms = sm_count();
-  if (!sms) return report(cudaErrorInvalidDevice, "ragged attention");
+  if (units > INT32_MAX) return fail(TIDE_ERR_INVALID, "ragged attention: too many rows and heads");
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(units < sms ? units : sms), 1, 1);
+  cfg.gridDim = dim3((unsigned)units, 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.dynamicSmemBytes = Shape<D>::kSmem;
   cfg.stream = s;

@@ -387,6 +387,31 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity
   }
   return false;
 }
+// Cluster launch control: asks that a CTA of this grid that has yet to start
+// be cancelled; the 16-byte answer (16-byte aligned) arrives on `bar`.
+__device__ __forceinline__ void clc_try_cancel(void *answer, uint64_t *bar) {
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], "
+      "[%1];" ::"r"(smem_u32(answer)),
+      "r"(smem_u32(bar))
+      : "memory");
+}
+// Whether one was, and its index in x.
+__device__ __forceinline__ bool clc_canceled(const void *answer, uint32_t *cta) {
+  uint32_t ok, x;
+  asm volatile(
+      "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+      : "=r"(ok), "=r"(x)
+      : "r"(smem_u32(answer))
+      : "memory");
+  *cta = x;
+  return ok != 0;
+}
 __device__ __forceinline__ void fence_cluster() {
   asm volatile("fence.acq_rel.cluster;" ::: "memory");
 }
