@@ -23,6 +23,7 @@
 #include <stdio.h>
 
 #include "ragged.cuh"
+#include "tc_ptx.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -33,6 +34,7 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxRequests = 8192;
 constexpr int kClusterCtas = 8;
+constexpr int kRun = 4;  // tokens that a thread takes in a row where there are many
 // New tokens from which a cluster shares the writing; below, one CTA.
 constexpr int64_t kClusterTokens = 4096;
 
@@ -90,31 +92,33 @@ __device__ __forceinline__ void block_scan(long long (&v)[3], long long (&carry)
   __syncthreads();
 }
 
-__global__ void __launch_bounds__(kThreads) page_tables_kernel(Params p) {
+__global__ void __launch_bounds__(kThreads) page_tables_kernel(const __grid_constant__ Params p) {
   extern __shared__ int32_t dyn[];
   // per request: packed token offset, tokens held, first new page's rank (-1:
-  // no page was to be had), where its returned pages go
+  // no page was to be had), where its returned pages go and how many they are
   int32_t *s_cu = dyn;                    // [n_req + 1]
   int32_t *s_ctx = s_cu + p.n_req + 1;    // [n_req]
   int32_t *s_rank = s_ctx + p.n_req;      // [n_req]
-  int32_t *s_push = s_rank + p.n_req;     // [n_req]
+  int32_t *s_push = s_rank + p.n_req;     // [n_req] (only with `done`)
+  int32_t *s_back = s_push + p.n_req;     // [n_req]
+  int32_t *s_gone = s_back + p.n_req;     // the requests that return pages, in any order
   __shared__ long long s_sum[kWarps][3];
   __shared__ long long s_taken;
+  __shared__ int s_n_gone;
   cg::cluster_group cluster = cg::this_cluster();
   const int cta = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31;
   const bool first = cta == 0;  // the CTA that reports
   const int64_t room = p.max_pages * p.page;
-
-  int n_free = __ldcg(p.n_free);
-  if (n_free < 0 || n_free > p.n_pages) {
-    if (first && tid == 0) raise_error(p.err, TIDE_DEVERR_COUNT);
-    n_free = min(max(n_free, 0), p.n_pages);
-  }
   if (tid == 0) {
     s_taken = 0;
+    s_n_gone = 0;
     s_cu[0] = 0;
   }
+  ptx::grid_dependency_wait();
+  int n_free = __ldcg(p.n_free);  // (used when the lengths have come too)
+  const bool bad_free = n_free < 0 || n_free > p.n_pages;
+  n_free = min(max(n_free, 0), p.n_pages);
   __syncthreads();
 
   // 1. prefix sums; the pages of the requests that are done, a share per CTA
@@ -144,25 +148,31 @@ __global__ void __launch_bounds__(kThreads) page_tables_kernel(Params p) {
       // (then no later one's do, so their ranks are not used)
       const bool past = v[0] > p.n_slots;
       s_rank[r] = wide || past ? -1 : (int32_t)(v[1] - need);
-      s_push[r] = (int32_t)min((long long)n_free + v[2] - back, (long long)p.n_pages);
+      if (back) {
+        s_push[r] = (int32_t)min((long long)n_free + v[2] - back, (long long)p.n_pages);
+        s_back[r] = back;
+        s_gone[atomicAdd(&s_n_gone, 1)] = r;
+      }
       if (first && wide) raise_error(p.err, TIDE_DEVERR_PAGES);
       if (first && past) raise_error(p.err, TIDE_DEVERR_COUNT);
     }
   }
+  if (first && tid == 0 && bad_free) raise_error(p.err, TIDE_DEVERR_COUNT);
   __syncthreads();
-  if (p.done)  // a warp per request that is done, shared by the CTAs
-    for (int r = cta * kWarps + (tid >> 5); r < p.n_req; r += ctas * kWarps) {
-      if (__ldg(p.done + r) == 0) continue;
-      const int back = (int)min((int64_t)ceil_div(max(__ldcg(p.ctx + r), 0), p.page), p.max_pages);
-      for (int j = tid & 31; j < back; j += 32) {
-        if ((long long)s_push[r] + j < p.n_pages)
-          p.free_pages[s_push[r] + j] = __ldcg(p.tables + (int64_t)r * p.max_pages + j);
-        else
-          raise_error(p.err, TIDE_DEVERR_PAGES);
-      }
+  // a warp per request that returns pages, shared by the CTAs by its number
+  for (int i = tid >> 5; i < s_n_gone; i += kWarps) {
+    const int r = s_gone[i];
+    if (r % ctas != cta) continue;
+    for (int j = lane; j < s_back[r]; j += 32) {
+      if ((long long)s_push[r] + j < p.n_pages)
+        p.free_pages[s_push[r] + j] = __ldcg(p.tables + (int64_t)r * p.max_pages + j);
+      else
+        raise_error(p.err, TIDE_DEVERR_PAGES);
     }
+  }
   const long long avail = min((long long)n_free + carry[2], (long long)p.n_pages);
   // which requests got their pages; how many pages are taken
+  int taken = 0;
   for (int r = tid; r < p.n_req; r += kThreads) {
     const int ctx = s_ctx[r], add = s_cu[r + 1] - s_cu[r];
     if (s_rank[r] < 0 || !add) continue;
@@ -172,9 +182,11 @@ __global__ void __launch_bounds__(kThreads) page_tables_kernel(Params p) {
       s_rank[r] = -1;
       if (first) raise_error(p.err, TIDE_DEVERR_PAGES);
     } else if (need) {
-      atomicMax((unsigned long long *)&s_taken, (unsigned long long)upto);  // order-free
+      taken = max(taken, (int)upto);  // (no more than the pages there are)
     }
   }
+  taken = __reduce_max_sync(0xffffffffu, taken);
+  if (lane == 0 && taken) atomicMax((unsigned long long *)&s_taken, (unsigned long long)taken);
   cluster.sync();  // (also a block barrier) see the header
 
   // 2. tables, lengths, offsets, free count
@@ -188,35 +200,43 @@ __global__ void __launch_bounds__(kThreads) page_tables_kernel(Params p) {
     p.cu[0] = 0;
     *p.n_free_out = (int32_t)(avail - s_taken);
   }
-  // 3. slots and positions, a token per thread; a token that opens a page
-  // writes its table entry
-  for (int64_t t = me; t < p.n_slots; t += all) {
-    int64_t slot = -1, pos = 0;
-    if (t < carry[0]) {
-      int lo = 0, hi = p.n_req;  // s_cu[lo] <= t < s_cu[hi]
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (s_cu[mid] <= t) lo = mid;
+  // 3. slots and positions, runs of tokens per thread (one search and a page
+  // or two for a run); a token that opens a page writes its table entry
+  const int run = p.n_slots >= (int64_t)kRun * all ? kRun : 1;
+  for (int64_t t0 = (int64_t)me * run; t0 < p.n_slots; t0 += (int64_t)all * run) {
+    int r = 0, at = -1, page = 0;  // request, page of its table that `page` is
+    if (t0 < carry[0]) {
+      int hi = p.n_req;  // s_cu[r] <= t0 < s_cu[hi]
+      while (hi - r > 1) {
+        const int mid = (r + hi) >> 1;
+        if (s_cu[mid] <= t0) r = mid;
         else hi = mid;
       }
-      const int ctx = s_ctx[lo], rank = s_rank[lo];
-      pos = ctx + (t - s_cu[lo]);
-      if (rank >= 0) {
-        const int pg = (int)(pos / p.page), off = (int)(pos % p.page);
-        const int have = ceil_div(ctx, p.page);
-        int32_t *entry = p.tables + (int64_t)lo * p.max_pages + pg;
-        int page;
-        if (pg < have) {
-          page = __ldcg(entry);
-        } else {
-          page = __ldcg(p.free_pages + (avail - 1 - rank - (pg - have)));
-          if (off == 0) *entry = page;
-        }
-        slot = (int64_t)page * p.page + off;
-      }
     }
-    p.slots[t] = slot;
-    p.positions[t] = pos;
+    for (int i = 0; i < run; ++i) {
+      const int64_t t = t0 + i;
+      if (t >= p.n_slots) break;
+      int64_t slot = -1, pos = 0;
+      if (t < carry[0]) {
+        while (s_cu[r + 1] <= t) ++r, at = -1;  // (past requests without new tokens)
+        const int ctx = s_ctx[r], rank = s_rank[r];
+        pos = ctx + (t - s_cu[r]);
+        if (rank >= 0) {
+          const int pg = (int)(pos / p.page), off = (int)(pos - (int64_t)pg * p.page);
+          if (pg != at) {
+            const int have = ceil_div(ctx, p.page);
+            int32_t *entry = p.tables + (int64_t)r * p.max_pages + pg;
+            page = pg < have ? __ldcg(entry)
+                             : __ldcg(p.free_pages + (avail - 1 - rank - (pg - have)));
+            if (pg >= have && off == 0) *entry = page;
+            at = pg;
+          }
+          slot = (int64_t)page * p.page + off;
+        }
+      }
+      p.slots[t] = slot;
+      p.positions[t] = pos;
+    }
   }
 }
 
@@ -229,7 +249,9 @@ __global__ void __launch_bounds__(256)
                         int64_t n_rows, int hkv, uint4 *__restrict__ kc, uint4 *__restrict__ vc,
                         int64_t n_pages, int page, int32_t *err) {
   constexpr int kVecs = D / 8;  // 16-byte vectors of a head
+  constexpr int kFlight = 4;    // of a lane's, loaded before the first is stored
   const int lane = threadIdx.x & 31;
+  ptx::grid_dependency_wait();
   int64_t live = n_rows;
   if (n_dev) live = min((int64_t)max(__ldg(n_dev), 0), n_rows);
   const int64_t warps = (int64_t)gridDim.x * (blockDim.x / 32);
@@ -250,13 +272,20 @@ __global__ void __launch_bounds__(256)
     const int64_t dst = (pg * hkv * page + slot % page) * kVecs;  // head 0
     const int64_t head = (int64_t)page * kVecs;
     const int n = hkv * kVecs;
-    for (int e = lane; e < n; e += 32) {
-      const int64_t to = dst + (e / kVecs) * head + e % kVecs;
-      const uint4 zero = make_uint4(0, 0, 0, 0);
-      const uint4 a = k_new ? k_new[i * row_vecs + e] : zero;
-      const uint4 b = v_new ? v_new[i * row_vecs + e] : zero;
-      kc[to] = a;
-      vc[to] = b;
+    for (int e0 = lane; e0 < n; e0 += 32 * kFlight) {
+      uint4 a[kFlight], b[kFlight];
+#pragma unroll
+      for (int f = 0; f < kFlight; ++f) {
+        const int e = e0 + 32 * f;
+        a[f] = b[f] = make_uint4(0, 0, 0, 0);
+        if (k_new && e < n) a[f] = k_new[i * row_vecs + e], b[f] = v_new[i * row_vecs + e];
+      }
+#pragma unroll
+      for (int f = 0; f < kFlight; ++f) {
+        const int e = e0 + 32 * f;
+        const int64_t to = dst + (e / kVecs) * head + e % kVecs;
+        if (e < n) kc[to] = a[f], vc[to] = b[f];
+      }
     }
   }
 }
@@ -301,10 +330,10 @@ extern "C" int tide_page_tables(const int32_t *context_lens, const int32_t *new_
   Params p{context_lens, new_lens,  done,       (int)n_requests, free_pages, n_free,
            (int)n_pages, block_tables, max_pages, (int)page_size,  n_free_out, kv_lens,
            cu_seqlens,   slot_map,  positions,  n_slots,         error_word};
-  const size_t smem = (4 * (size_t)n_requests + 1) * sizeof(int32_t);
-  cudaError_t e = cudaFuncSetAttribute(page_tables_kernel,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)((4 * (size_t)kMaxRequests + 1) * sizeof(int32_t)));
+  const size_t smem = ((done ? 6 : 3) * (size_t)n_requests + 1) * sizeof(int32_t);
+  static std::atomic<uint64_t> set{0};
+  cudaError_t e = tide::allow_smem(page_tables_kernel,
+                                   (int)((6 * (size_t)kMaxRequests + 1) * sizeof(int32_t)), set);
   if (e != cudaSuccess) return report(e, "page_tables");
   const unsigned ctas = n_slots >= kClusterTokens ? kClusterCtas : 1;
   cudaLaunchConfig_t cfg = {};
@@ -312,13 +341,15 @@ extern "C" int tide_page_tables(const int32_t *context_lens, const int32_t *new_
   cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = (cudaStream_t)stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ctas;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   return report(cudaLaunchKernelEx(&cfg, page_tables_kernel, p), "page_tables");
 }
 
@@ -348,10 +379,19 @@ extern "C" int tide_paged_append(int dtype, const void *k_new, const void *v_new
   if (blocks > 148 * 32) blocks = 148 * 32;
   cudaStream_t s = (cudaStream_t)stream;
   auto kern = head_dim == 128 ? paged_append_kernel<128> : paged_append_kernel<64>;
-  kern<<<(unsigned)blocks, 256, 0, s>>>(
-      static_cast<const uint4 *>(k_new), static_cast<const uint4 *>(v_new), kv_row_stride / 8,
-      slot_map, n_slot_map, row_ids, n_rows_dev, n_rows, (int)n_kv_heads,
-      static_cast<uint4 *>(k_cache), static_cast<uint4 *>(v_cache), n_pages, (int)page_size,
-      error_word);
-  return report(cudaSuccess, "paged_append");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks, 1, 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return report(cudaLaunchKernelEx(&cfg, kern, static_cast<const uint4 *>(k_new),
+                                   static_cast<const uint4 *>(v_new), kv_row_stride / 8, slot_map,
+                                   n_slot_map, row_ids, n_rows_dev, n_rows, (int)n_kv_heads,
+                                   static_cast<uint4 *>(k_cache), static_cast<uint4 *>(v_cache),
+                                   n_pages, (int)page_size, error_word),
+                "paged_append");
 }

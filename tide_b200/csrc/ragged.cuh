@@ -2,6 +2,8 @@
 // the attention kernels over packed sequences and over a paged cache.
 #pragma once
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace tide {
@@ -85,6 +87,20 @@ struct KeySource {
   int n_pages;
   int page_shift;          // log2(page_size)
 };
+
+// The kernel's dynamic shared memory limit, raised once on every device (`set`
+// has a bit for each that has it; beyond 64 devices it is raised every time).
+template <typename K>
+inline cudaError_t allow_smem(K kern, int bytes, std::atomic<uint64_t> &set) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (set.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) set.fetch_or(bit, std::memory_order_acq_rel);
+  return e;
+}
 
 void set_last_error(const char *msg);
 

@@ -101,6 +101,8 @@ struct Params {
   int split_blocks;  // key blocks of a split
   int few;         // sequences of up to so many tokens go to the few-rows kernel
   int64_t group_keys;  // keys whose rows, of all KV heads, L2 holds
+  int take_over;   // whether there are more CTAs than run at once
+  int behind_few;  // launched over the few-rows kernel of the same call
   float qs;        // scale * log2(e)
 };
 
@@ -245,17 +247,22 @@ __device__ void schedule_units(const Params &p, Shared &sh) {
   int x = 0, above = 0, upto = 0;    // level, the group's units above it, of it and above
   int top_level = 0;
   uint32_t asked = 0;
-  bool more = true;
+  bool more = true;  // this CTA has a unit
   int64_t u = blockIdx.x;
   for (uint32_t n = 0;; ++n) {
     const int slot = n & 1;
     // every warp has taken up the unit before: time for another one (sooner,
     // and at the end one CTA would hold what another could run)
-    if (n > 0) TIDE_WAIT(&sh.u_empty[slot ^ 1], ((n - 1) >> 1) & 1);
-    if (n > 0 && !next_unit(p, sh, &u, &asked, &more)) return;
-    // a CTA without a unit takes over what else there is without one
-    while (more && u / per_rank >= units_in_all)
+    if (n > 0 && !p.take_over) more = false;
+    if (n > 0 && more) {
+      TIDE_WAIT(&sh.u_empty[slot ^ 1], ((n - 1) >> 1) & 1);
       if (!next_unit(p, sh, &u, &asked, &more)) return;
+    }
+    // a CTA without a unit takes over what else there is without one
+    while (more && u / per_rank >= units_in_all) {
+      if (!p.take_over) more = false;
+      else if (!next_unit(p, sh, &u, &asked, &more)) return;
+    }
     const int64_t rank = u / per_rank;
     if (rank < base) s1 = total = 0, base = 0;  // (should they ever come out of order)
     while (rank - base >= total && s1 < live) {  // the next group
@@ -929,6 +936,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = sh.tmem;
+  // Up to here this overlaps the kernel before.  (Over the few-rows kernel of
+  // the same call, which waits before it lets this one start, there is nothing
+  // more to wait for.)
+  if (!p.behind_few) ptx::grid_dependency_wait();
 
   // Registers move to the softmax warps: 256 * 208 + 128 * 88 = 384 * 168, what
   // the block was launched with.
@@ -968,9 +979,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   ptx::tc_fence_after();
   if (warp == 10) ptx::tmem_dealloc(tmem, 512);
-  // Launched over the tail of the few-rows kernel, on which it does not
-  // depend: what comes after this kernel comes after that one too.
-  if (threadIdx.x == 0) ptx::grid_dependency_wait();
+  // what comes after this kernel comes after the few-rows kernel too
+  if (p.behind_few && threadIdx.x == 0) ptx::grid_dependency_wait();
 }
 
 // --------------------------------------------------------- few rows a head
@@ -1068,6 +1078,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, NT <= 2 ? 3 : 2)
   __shared__ float s_m[kFewWarps][kRowsMost], s_l[kFewWarps][kRowsMost];
   __shared__ int s_abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  ptx::grid_dependency_wait();
   ptx::grid_dependents_launch();
   const int split = (int)(blockIdx.x % p.splits);
   const int64_t unit = blockIdx.x / p.splits;
@@ -1623,8 +1634,8 @@ int launch(tide::ragged::Params &p, int dtype, const void *q, int64_t q_stride, 
   }
   if (!ok) return fail(TIDE_ERR_CUDA, "ragged attention: cuTensorMapEncodeTiled failed");
   auto kern = tile_attention_kernel<T, D, PAGED>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)Shape<D>::kSmem);
+  static std::atomic<uint64_t> set{0};  // per device
+  cudaError_t e = tide::allow_smem(kern, (int)Shape<D>::kSmem, set);
   if (e != cudaSuccess) return report(e, "ragged attention");
   const int64_t units =
       most_units(p.batch.n_tokens, p.batch.n_seqs, p.hq, p.hkv) * p.splits;
@@ -1638,7 +1649,9 @@ int launch(tide::ragged::Params &p, int dtype, const void *q, int64_t q_stride, 
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = behind_few ? 1 : 0;
+  cfg.numAttrs = 1;
+  p.take_over = units > 148;
+  p.behind_few = behind_few;
   return report(cudaLaunchKernelEx(&cfg, kern, p, mq, mk, mv), "ragged attention");
 }
 
@@ -1650,12 +1663,21 @@ int launch_few(const tide::ragged::FewParams &p, int dtype, int64_t kv_rows, cud
       !make_map(&mv, dtype, p.src.v, 2, D, kv_rows, 1, D, 0, kFewKeys, 1))
     return fail(TIDE_ERR_CUDA, "paged_attention: cuTensorMapEncodeTiled failed");
   auto kern = few_rows_kernel<T, D, NT>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)Few<D>::kSmem);
+  static std::atomic<uint64_t> set{0};  // per device
+  cudaError_t e = tide::allow_smem(kern, (int)Few<D>::kSmem, set);
   if (e != cudaSuccess) return report(e, "paged_attention");
   const int64_t ctas = (int64_t)p.pieces * p.hkv * p.splits;
-  kern<<<(unsigned)ctas, 32 * kFewWarps, Few<D>::kSmem, s>>>(p, mk, mv);
-  return report(cudaSuccess, "paged_attention");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas, 1, 1);
+  cfg.blockDim = dim3(32 * kFewWarps, 1, 1);
+  cfg.dynamicSmemBytes = Few<D>::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return report(cudaLaunchKernelEx(&cfg, kern, p, mk, mv), "paged_attention");
 }
 
 template <typename T, int D, bool FEW>
