@@ -8,36 +8,33 @@
 // and a request gets its pages iff upto_r <= free pages: page j of its new
 // ones is entry free - 1 - (upto_r - need_r + j) of the stack.  So three
 // prefix sums over the requests (tokens, pages needed, pages returned) give
-// every output in parallel, without an atomic: the result does not depend on
-// the order of threads.
-// All lengths are a few KB, so every CTA of the one cluster scans all of them
-// itself (no exchange), and the CTAs share the writing.  Two cluster barriers
-// order what may alias or overlap: the first lies between the last read of
-// the lengths, the free count and the old tables and the first write of their
-// successors; it also makes the pages returned by one CTA visible to the
-// others, which may hand them out again at once.
+// every output in parallel, and the result does not depend on the order of
+// threads.  The lengths are a few KB, so this is one CTA, all latency; its
+// barrier lies between the last read of what the outputs may alias or
+// overlap (the lengths, the free count, the tables of requests that start
+// over) and the first write of those, and makes the returned pages visible to
+// the threads that hand them out again.
+// Up to a slot per thread it writes the slot map and the positions too; more
+// tokens are work for many SMs (65536 of them on a cluster of eight took 14 us,
+// bound by the issue of its eight SMs): slot_map_kernel follows, started over
+// the first one's tail.  What that one cannot see from the outputs, whether a
+// request found its pages, it reads from the sign of the slot of the request's
+// first token, which the first kernel has written as it will be.
 //
 // paged_append_kernel copies 2 * kv_heads * head_dim elements per row: bound
 // by HBM, or by latency for a decode step's rows.
-#include <cooperative_groups.h>
 #include <stdio.h>
 
 #include "ragged.cuh"
 #include "tc_ptx.cuh"
 
-namespace cg = cooperative_groups;
-
 namespace tide {
 namespace pages {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
+static_assert(kWarps == 32, "a lane per warp in the block scan");
 constexpr int kMaxRequests = 8192;
-constexpr int kClusterCtas = 8;
-constexpr int kRun = 4;  // tokens that a thread takes in a row where there are many
-// New tokens from which a cluster shares the writing; below, one CTA.
-constexpr int64_t kClusterTokens = 4096;
-
 struct Params {
   const int32_t *ctx, *add, *done;
   int n_req;
@@ -76,39 +73,40 @@ __device__ __forceinline__ void block_scan(long long (&v)[3], long long (&carry)
 #pragma unroll
     for (int k = 0; k < 3; ++k) s_sum[warp][k] = v[k];
   __syncthreads();
-  long long before[3] = {0, 0, 0}, total[3] = {0, 0, 0};
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w)
-#pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      if (w < warp) before[k] += s_sum[w][k];
-      total[k] += s_sum[w][k];
-    }
-#pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    v[k] += before[k] + carry[k];
-    carry[k] += total[k];
+  for (int k = 0; k < 3; ++k) {  // the warps' sums, one per lane
+    const long long own = s_sum[lane][k];
+    const long long upto = warp_inclusive(own, lane);
+    v[k] += carry[k] + __shfl_sync(0xffffffffu, upto - own, warp);
+    carry[k] += __shfl_sync(0xffffffffu, upto, 31);
   }
   __syncthreads();
 }
 
+// The request of packed new token t < cu[n]: cu[r] <= t < cu[r + 1].
+__device__ __forceinline__ int request_of(const int32_t *cu, int n, int t) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cu[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
 __global__ void __launch_bounds__(kThreads) page_tables_kernel(const __grid_constant__ Params p) {
   extern __shared__ int32_t dyn[];
-  // per request: packed token offset, tokens held, first new page's rank (-1:
-  // no page was to be had), where its returned pages go and how many they are
+  // per request: packed token offset, tokens held, new pages up to and with its
+  // own; with `done`, where its returned pages go and how many they are
   int32_t *s_cu = dyn;                    // [n_req + 1]
   int32_t *s_ctx = s_cu + p.n_req + 1;    // [n_req]
-  int32_t *s_rank = s_ctx + p.n_req;      // [n_req]
-  int32_t *s_push = s_rank + p.n_req;     // [n_req] (only with `done`)
+  int32_t *s_upto = s_ctx + p.n_req;      // [n_req]; its sign: no page was to be had
+  int32_t *s_push = s_upto + p.n_req;     // [n_req]
   int32_t *s_back = s_push + p.n_req;     // [n_req]
   int32_t *s_gone = s_back + p.n_req;     // the requests that return pages, in any order
   __shared__ long long s_sum[kWarps][3];
-  __shared__ long long s_taken;
-  __shared__ int s_n_gone;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int cta = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
+  __shared__ int s_taken, s_n_gone;
   const int tid = threadIdx.x, lane = tid & 31;
-  const bool first = cta == 0;  // the CTA that reports
   const int64_t room = p.max_pages * p.page;
   if (tid == 0) {
     s_taken = 0;
@@ -129,7 +127,7 @@ __global__ void __launch_bounds__(kThreads) page_tables_kernel(const __grid_cons
     int held = in ? __ldcg(p.ctx + r) : 0, add = in ? __ldcg(p.add + r) : 0;
     const bool gone = in && p.done && __ldg(p.done + r) != 0;
     if (held < 0 || add < 0 || add > p.n_slots) {
-      if (first) raise_error(p.err, TIDE_DEVERR_COUNT);
+      raise_error(p.err, TIDE_DEVERR_COUNT);
       held = max(held, 0);
       if (add < 0 || add > p.n_slots) add = 0;
     }
@@ -143,26 +141,24 @@ __global__ void __launch_bounds__(kThreads) page_tables_kernel(const __grid_cons
     if (in) {
       s_cu[r + 1] = (int32_t)min(v[0], (long long)INT32_MAX);
       s_ctx[r] = ctx;
-      // the rank is checked against the free pages below, when they are
-      // known; a request whose tokens do not fit in n_slots gets none either
-      // (then no later one's do, so their ranks are not used)
+      // checked against the free pages below, when they are known; a request
+      // whose tokens do not fit in n_slots gets none either (nor do those of
+      // any later one)
       const bool past = v[0] > p.n_slots;
-      s_rank[r] = wide || past ? -1 : (int32_t)(v[1] - need);
+      s_upto[r] = wide || past ? ~(int32_t)v[1] : (int32_t)v[1];
       if (back) {
         s_push[r] = (int32_t)min((long long)n_free + v[2] - back, (long long)p.n_pages);
         s_back[r] = back;
         s_gone[atomicAdd(&s_n_gone, 1)] = r;
       }
-      if (first && wide) raise_error(p.err, TIDE_DEVERR_PAGES);
-      if (first && past) raise_error(p.err, TIDE_DEVERR_COUNT);
+      if (wide) raise_error(p.err, TIDE_DEVERR_PAGES);
+      if (past) raise_error(p.err, TIDE_DEVERR_COUNT);
     }
   }
-  if (first && tid == 0 && bad_free) raise_error(p.err, TIDE_DEVERR_COUNT);
+  if (tid == 0 && bad_free) raise_error(p.err, TIDE_DEVERR_COUNT);
   __syncthreads();
-  // a warp per request that returns pages, shared by the CTAs by its number
-  for (int i = tid >> 5; i < s_n_gone; i += kWarps) {
+  for (int i = tid >> 5; i < s_n_gone; i += kWarps) {  // a warp per request that returns pages
     const int r = s_gone[i];
-    if (r % ctas != cta) continue;
     for (int j = lane; j < s_back[r]; j += 32) {
       if ((long long)s_push[r] + j < p.n_pages)
         p.free_pages[s_push[r] + j] = __ldcg(p.tables + (int64_t)r * p.max_pages + j);
@@ -174,70 +170,94 @@ __global__ void __launch_bounds__(kThreads) page_tables_kernel(const __grid_cons
   // which requests got their pages; how many pages are taken
   int taken = 0;
   for (int r = tid; r < p.n_req; r += kThreads) {
-    const int ctx = s_ctx[r], add = s_cu[r + 1] - s_cu[r];
-    if (s_rank[r] < 0 || !add) continue;
+    const int ctx = s_ctx[r], add = s_cu[r + 1] - s_cu[r], upto = s_upto[r];
+    if (upto < 0 || !add) continue;
     const int need = ceil_div(ctx + add, p.page) - ceil_div(ctx, p.page);
-    const long long upto = (long long)s_rank[r] + need;
     if (need && upto > avail) {
-      s_rank[r] = -1;
-      if (first) raise_error(p.err, TIDE_DEVERR_PAGES);
+      s_upto[r] = ~upto;
+      raise_error(p.err, TIDE_DEVERR_PAGES);
     } else if (need) {
-      taken = max(taken, (int)upto);  // (no more than the pages there are)
+      taken = max(taken, upto);
     }
   }
   taken = __reduce_max_sync(0xffffffffu, taken);
-  if (lane == 0 && taken) atomicMax((unsigned long long *)&s_taken, (unsigned long long)taken);
-  cluster.sync();  // (also a block barrier) see the header
+  if (lane == 0 && taken) atomicMax(&s_taken, taken);
+  __syncthreads();  // see the header
 
-  // 2. tables, lengths, offsets, free count
-  const int all = ctas * kThreads, me = cta * kThreads + tid;
-  for (int r = me; r < p.n_req; r += all) {
-    const int ctx = s_ctx[r], add = s_cu[r + 1] - s_cu[r], rank = s_rank[r];
-    p.kv[r] = rank < 0 ? ctx : ctx + add;
+  // 2. lengths, offsets, free count, the first slot of every request, and the
+  // table entries of the new pages, a page per thread (those of the requests
+  // that got theirs are the first `taken`)
+  for (int r = tid; r < p.n_req; r += kThreads) {
+    const int ctx = s_ctx[r], add = s_cu[r + 1] - s_cu[r], upto = s_upto[r];
+    p.kv[r] = upto < 0 ? ctx : ctx + add;
     p.cu[r + 1] = s_cu[r + 1];
+    if (add && p.n_slots > kThreads && s_cu[r] < p.n_slots) {
+      int64_t slot = -1;
+      if (upto >= 0) {
+        const int pg = ctx / p.page, have = ceil_div(ctx, p.page);
+        const int need = ceil_div(ctx + add, p.page) - have;
+        const int page = pg < have ? __ldcg(p.tables + (int64_t)r * p.max_pages + pg)
+                                   : __ldcg(p.free_pages + (avail - 1 - (upto - need)));
+        slot = (int64_t)page * p.page + ctx % p.page;
+      }
+      p.slots[s_cu[r]] = slot;
+    }
   }
-  if (me == 0) {
+  if (tid == 0) {
     p.cu[0] = 0;
     *p.n_free_out = (int32_t)(avail - s_taken);
   }
-  // 3. slots and positions, runs of tokens per thread (one search and a page
-  // or two for a run); a token that opens a page writes its table entry
-  const int run = p.n_slots >= (int64_t)kRun * all ? kRun : 1;
-  for (int64_t t0 = (int64_t)me * run; t0 < p.n_slots; t0 += (int64_t)all * run) {
-    int r = 0, at = -1, page = 0;  // request, page of its table that `page` is
-    if (t0 < carry[0]) {
-      int hi = p.n_req;  // s_cu[r] <= t0 < s_cu[hi]
-      while (hi - r > 1) {
-        const int mid = (r + hi) >> 1;
-        if (s_cu[mid] <= t0) r = mid;
-        else hi = mid;
-      }
+  for (int k = tid; k < s_taken; k += kThreads) {
+    int lo = 0, hi = p.n_req;  // the first request with more than k pages up to it
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1, upto = s_upto[mid];
+      if ((upto < 0 ? ~upto : upto) > k) hi = mid;
+      else lo = mid + 1;
     }
-    for (int i = 0; i < run; ++i) {
-      const int64_t t = t0 + i;
-      if (t >= p.n_slots) break;
-      int64_t slot = -1, pos = 0;
-      if (t < carry[0]) {
-        while (s_cu[r + 1] <= t) ++r, at = -1;  // (past requests without new tokens)
-        const int ctx = s_ctx[r], rank = s_rank[r];
-        pos = ctx + (t - s_cu[r]);
-        if (rank >= 0) {
-          const int pg = (int)(pos / p.page), off = (int)(pos - (int64_t)pg * p.page);
-          if (pg != at) {
-            const int have = ceil_div(ctx, p.page);
-            int32_t *entry = p.tables + (int64_t)r * p.max_pages + pg;
-            page = pg < have ? __ldcg(entry)
-                             : __ldcg(p.free_pages + (avail - 1 - rank - (pg - have)));
-            if (pg >= have && off == 0) *entry = page;
-            at = pg;
-          }
-          slot = (int64_t)page * p.page + off;
-        }
-      }
-      p.slots[t] = slot;
-      p.positions[t] = pos;
+    const int have = ceil_div(s_ctx[lo], p.page);
+    const int need = ceil_div(s_ctx[lo] + (s_cu[lo + 1] - s_cu[lo]), p.page) - have;
+    p.tables[(int64_t)lo * p.max_pages + have + (k - (s_upto[lo] - need))] =
+        __ldcg(p.free_pages + (avail - 1 - k));
+  }
+  if (tid >= p.n_slots || p.n_slots > kThreads) return;  // (slot_map_kernel follows)
+  int64_t slot = -1, pos = 0;
+  if (tid < s_cu[p.n_req]) {
+    const int r = request_of(s_cu, p.n_req, tid), ctx = s_ctx[r], upto = s_upto[r];
+    pos = (int64_t)ctx + (tid - s_cu[r]);
+    if (upto >= 0) {
+      const uint32_t at = (uint32_t)pos / (uint32_t)p.page;
+      const int have = ceil_div(ctx, p.page);
+      const int need = ceil_div(ctx + (s_cu[r + 1] - s_cu[r]), p.page) - have;
+      const int page = (int)at < have
+                           ? __ldcg(p.tables + (int64_t)r * p.max_pages + at)
+                           : __ldcg(p.free_pages + (avail - 1 - (upto - need) - ((int)at - have)));
+      slot = (int64_t)page * p.page + (uint32_t)pos % (uint32_t)p.page;
     }
   }
+  p.slots[tid] = slot;
+  p.positions[tid] = pos;
+}
+
+// 3. Slots and positions where a thread per token is more than one CTA, from
+// the lengths and tables that the step leaves.
+__global__ void __launch_bounds__(256) slot_map_kernel(const __grid_constant__ Params p) {
+  ptx::grid_dependency_wait();
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t >= p.n_slots) return;
+  int64_t slot = -1, pos = 0;
+  if (t < __ldcg(p.cu + p.n_req)) {
+    const int r = request_of(p.cu, p.n_req, (int)t);
+    const int start = p.cu[r], len = __ldcg(p.kv + r);
+    const bool granted = __ldcg(p.slots + start) >= 0;
+    pos = (int64_t)(granted ? len - (p.cu[r + 1] - start) : len) + (t - start);
+    if (granted) {
+      const uint32_t at = (uint32_t)pos / (uint32_t)p.page;
+      slot = (int64_t)__ldcg(p.tables + (int64_t)r * p.max_pages + at) * p.page +
+             (uint32_t)pos % (uint32_t)p.page;
+    }
+  }
+  p.slots[t] = slot;
+  p.positions[t] = pos;
 }
 
 // A warp per row: its 2 * hkv * d / 8 16-byte vectors, keys then values.
@@ -335,22 +355,24 @@ extern "C" int tide_page_tables(const int32_t *context_lens, const int32_t *new_
   cudaError_t e = tide::allow_smem(page_tables_kernel,
                                    (int)((6 * (size_t)kMaxRequests + 1) * sizeof(int32_t)), set);
   if (e != cudaSuccess) return report(e, "page_tables");
-  const unsigned ctas = n_slots >= kClusterTokens ? kClusterCtas : 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas, 1, 1);
+  cfg.gridDim = dim3(1, 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = (cudaStream_t)stream;
-  cudaLaunchAttribute attr[2];
+  cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = ctas;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  return report(cudaLaunchKernelEx(&cfg, page_tables_kernel, p), "page_tables");
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, page_tables_kernel, p);
+  if (e == cudaSuccess && n_slots > kThreads) {
+    cfg.gridDim = dim3((unsigned)((n_slots + 255) / 256), 1, 1);
+    cfg.blockDim = dim3(256, 1, 1);
+    cfg.dynamicSmemBytes = 0;
+    e = cudaLaunchKernelEx(&cfg, slot_map_kernel, p);
+  }
+  return report(e, "page_tables");
 }
 
 extern "C" int tide_paged_append(int dtype, const void *k_new, const void *v_new,
