@@ -17,12 +17,16 @@ masked).  Attention itself runs over the whole [batch, seq] layout (zeros
 in the exited rows), so its cost does not shrink; the projections and the
 MLP, which dominate a layer, run on the active rows only.
 
+With padding in the input, or on request, attention runs on the active rows
+too, packed by sequence (tide_packed_attention): each prompt's survivors are a
+ragged sequence, and the zero keys of the tokens that have exited before one
+are a number per row instead of rows.  Padding takes part in nothing.
+
 Supported layer families: Llama-style decoder layers (q/k/v/o projections,
 optional per-head q/k RMSNorm as in Qwen3, rotary embeddings, gated MLP) and
-GPT-2 blocks.  Inputs without padding only.  For 16-bit Llama-family models
-the layers' elementwise work (RMSNorms with the residual adds, q/k norm +
-rotary, SiLU gate) runs on fused kernels that round where the HF modules
-round (tide_b200/csrc/decode_layer.cu); projections stay the modules' own.
+GPT-2 blocks.  For 16-bit Llama-family models the layers' elementwise work
+(RMSNorms with the residual adds, q/k norm + rotary, SiLU gate) runs on fused
+kernels that round where the HF modules round (tide_b200/csrc/decode_layer.cu); projections stay the modules' own.
 
 LiveDecoder does the same for decoding: per-row exits whose later layers
 skip the row, a KV cache addressed by slot, and steps free of host reads,
@@ -30,6 +34,7 @@ each one CUDA-graph replay.
 """
 from __future__ import annotations
 
+from dataclasses import dataclass
 from typing import Callable, Optional
 
 import torch
@@ -42,13 +47,45 @@ def _rotate_half(x: torch.Tensor) -> torch.Tensor:
     return torch.cat((-x[..., h:], x[..., :h]), dim=-1)
 
 
+@dataclass
+class _Packed:
+    """The active rows as packed sequences: their offsets, and for each row
+    how many tokens before it have exited (their keys and values are zero)."""
+    cu_seqlens: torch.Tensor           # int32 [B + 1]
+    zero_keys: Optional[torch.Tensor]  # int32 [n]; None: none
+    error_word: torch.Tensor
+
+    @staticmethod
+    def of(pos: torch.Tensor, B: int, S: int, order: torch.Tensor, first: "Optional[_Packed]",
+           error_word: torch.Tensor) -> "_Packed":
+        """For rows at token indices pos (ascending), order[t] being token t's
+        place among the batch's tokens without padding and `first` the packing
+        before any exit (None: this is it)."""
+        bounds = torch.arange(B + 1, device=pos.device, dtype=pos.dtype) * S
+        cu = torch.searchsorted(pos, bounds).to(torch.int32)
+        if first is None:
+            return _Packed(cu, None, error_word)
+        seq = torch.div(pos, S, rounding_mode="floor")
+        rank = torch.arange(pos.numel(), device=pos.device) - cu[seq]
+        gone = order[pos] - first.cu_seqlens[seq] - rank
+        return _Packed(cu, gone.to(torch.int32), error_word)
+
+
 def _attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pos: Optional[torch.Tensor],
-            B: int, S: int, scale: float) -> torch.Tensor:
+            B: int, S: int, scale: float, packed: Optional[_Packed] = None) -> torch.Tensor:
     """Causal attention of the active rows q/k/v [n, heads, d] (token index
     b * S + s in `pos`; None = all B * S tokens in order) over the whole
-    [B, S] layout, exited tokens' keys and values being zeros.  Returns
+    [B, S] layout, exited tokens' keys and values being zeros; with `packed`
+    over the active rows alone, the zeros counted.  Returns
     [n, heads_q * d]."""
     n, nh, d = q.shape
+    if packed is not None:
+        from tide_b200 import _native
+
+        out = torch.empty(n, nh, d, dtype=q.dtype, device=q.device)
+        _native.ops().packed_attention(q, k, v, packed.cu_seqlens, packed.zero_keys, out, scale,
+                                       packed.error_word)
+        return out.view(n, nh * d)
     nkv = k.shape[1]
     if pos is not None:
         qf = q.new_zeros(B * S, nh, d)
@@ -84,7 +121,7 @@ class _LlamaFamily:
         return self.embed(ids).reshape(ids.numel(), -1)
 
     def layer(self, i: int, h: torch.Tensor, pos: Optional[torch.Tensor], seq_pos: torch.Tensor,
-              B: int, S: int) -> torch.Tensor:
+              B: int, S: int, packed: Optional[_Packed] = None) -> torch.Tensor:
         layer = self.layers[i]
         attn = layer.self_attn
         d = attn.head_dim
@@ -100,7 +137,7 @@ class _LlamaFamily:
         cos, sin = cos[0].unsqueeze(1), sin[0].unsqueeze(1)
         q = q * cos + _rotate_half(q) * sin
         k = k * cos + _rotate_half(k) * sin
-        o = _attend(q, k, v, pos, B, S, float(attn.scaling))
+        o = _attend(q, k, v, pos, B, S, float(attn.scaling), packed)
         h = h + attn.o_proj(o)
         return h + layer.mlp(layer.post_attention_layernorm(h))
 
@@ -243,7 +280,8 @@ class _LlamaFamily:
         return out, total
 
     def layer_fused(self, i: int, h: torch.Tensor, pos: Optional[torch.Tensor],
-                    seq_pos: torch.Tensor, B: int, S: int) -> torch.Tensor:
+                    seq_pos: torch.Tensor, B: int, S: int,
+                    packed: Optional[_Packed] = None) -> torch.Tensor:
         """layer() of the live prefill on the fused kernels: the input norm,
         the q/k norms with the rotary embedding at each row's own position,
         the residual add with the post-attention norm, and the SiLU gate are
@@ -263,9 +301,9 @@ class _LlamaFamily:
         # q, k and v land at their tokens' places in [B * S] buffers (a one-
         # position "cache" per token, the tokens' indices as slots): the
         # exited tokens' keys and values stay zero, their queries are never
-        # read back.  With every token active the rows are the tokens and v
-        # is written onto itself.
-        if pos is None:
+        # read back.  With every token active, or attention on the active rows
+        # alone, the rows stay where they are and v is written onto itself.
+        if pos is None or packed is not None:
             slots = torch.arange(n, dtype=torch.int32, device=h.device)
             q_full = torch.empty(n, hq, 128, dtype=q.dtype, device=q.device)
             k_full = torch.empty(n, hkv, 1, 128, dtype=k.dtype, device=k.device)
@@ -282,8 +320,8 @@ class _LlamaFamily:
                          0, None, seq_pos.long().contiguous(), slots, None, q_full,
                          k_full, v_full, None)
         o = _attend(q_full, k_full.view(-1, hkv, 128), v_full.view(-1, hkv, 128), None, B, S,
-                    float(attn.scaling))
-        if pos is not None:
+                    float(attn.scaling), packed)
+        if pos is not None and packed is None:
             o = o.index_select(0, pos)
         x2, h1 = self.rms_norm(layer.post_attention_layernorm, h, None, delta=attn.o_proj(o))
         mlp = layer.mlp
@@ -348,8 +386,11 @@ class _GPT2Family:
         p = torch.arange(S, device=ids.device)
         return (self.wte(ids) + self.wpe(p)[None]).reshape(B * S, -1)
 
+    def head_dim(self) -> int:
+        return self.wte.embedding_dim // self.layers[0].attn.num_heads
+
     def layer(self, i: int, h: torch.Tensor, pos: Optional[torch.Tensor], seq_pos: torch.Tensor,
-              B: int, S: int) -> torch.Tensor:
+              B: int, S: int, packed: Optional[_Packed] = None) -> torch.Tensor:
         blk = self.layers[i]
         attn = blk.attn
         n, H = h.shape
@@ -359,7 +400,7 @@ class _GPT2Family:
         scale = (d ** -0.5) if attn.scale_attn_weights else 1.0
         if getattr(attn, "scale_attn_by_inverse_layer_idx", False):
             scale /= float(i + 1)
-        o = _attend(q.view(n, nh, d), k.view(n, nh, d), v.view(n, nh, d), pos, B, S, scale)
+        o = _attend(q.view(n, nh, d), k.view(n, nh, d), v.view(n, nh, d), pos, B, S, scale, packed)
         h = h + attn.c_proj(o)
         return h + blk.mlp(blk.ln_2(h))
 
@@ -380,31 +421,51 @@ def family_of(model: nn.Module):
 @torch.no_grad()
 def live_forward(runtime, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor],
                  on_checkpoint: Optional[Callable[[int, int], None]] = None,
-                 fused_layers: bool = True):
+                 fused_layers: bool = True, packed: bool = False):
     """The live forward of TIDERuntime (see the module docstring): returns
     (out_buf [B*S, H] of final-normed rows at their token positions,
     ExitStats, exit_layer [B*S] int32).  One host read-back of the survivor
     count per checkpoint (the next layers' shapes depend on it).  Llama-
     family layers of a 16-bit model run on the fused elementwise kernels when
-    they are ones those reproduce (fused_layers=False: the modules)."""
+    they are ones those reproduce (fused_layers=False: the modules).
+    With padding (zeros in attention_mask, left or right; a token's position is
+    its place in the row, as in the model's own forward), or packed=True,
+    attention runs on the active rows alone (16-bit models with a head
+    dimension of 64 or 128); padding enters no layer, its rows of out_buf are
+    zero and it is not counted."""
     from tide_b200.scheduler import ExitStats
 
-    if attention_mask is not None and not bool(attention_mask.bool().all()):
-        raise NotImplementedError("live early exit takes inputs without padding")
     fam = runtime._live_family()
     B, S = input_ids.shape
     N = B * S
     dev = input_ids.device
+    padded = attention_mask is not None and not bool(attention_mask.bool().all())
+    if padded and attention_mask.shape != input_ids.shape:
+        raise ValueError("attention_mask must be [batch, seq]")
     h = fam.embed_tokens(input_ids)
     H = h.shape[1]
     dtype = h.dtype
+    packed = packed or padded
+    if packed and (dtype not in (torch.bfloat16, torch.float16) or fam.head_dim() not in (64, 128)):
+        raise NotImplementedError("live early exit takes inputs with padding, or packed ones, for "
+                                  "bf16 and fp16 models with a head dimension of 64 or 128")
     seq_all = torch.arange(S, device=dev).repeat(B)
     out_buf = torch.zeros(N, H, dtype=dtype, device=dev)
     exit_layer = torch.full((N,), -1, dtype=torch.int32, device=dev)
-    stats = ExitStats(total_tokens=N)
+    # the active rows' token indices (None: all tokens, in order)
+    pos = attention_mask.to(dev).reshape(-1).bool().nonzero()[:, 0] if padded else None
+    if padded:
+        h = h.index_select(0, pos)  # (a row's own position went in with its embedding)
+    stats = ExitStats(total_tokens=h.shape[0])
     routers = {L for L in runtime.routers if L >= runtime.config.min_layers}
     thr = runtime.config.exit_threshold
-    pos = None  # all tokens, in order
+    order = first = rows = None
+    if packed:
+        err = runtime._runner.error_word
+        at = torch.arange(N, device=dev) if pos is None else pos
+        order = torch.zeros(N, dtype=torch.int64, device=dev)
+        order[at] = torch.arange(at.numel(), device=dev)
+        first = rows = _Packed.of(at, B, S, order, None, err)
     pos_out = [torch.empty(N, dtype=torch.int64, device=dev) for _ in range(2)]
     exit_pos = torch.empty(N, dtype=torch.int64, device=dev)
     counts = torch.zeros(2, dtype=torch.int32, device=dev)
@@ -414,7 +475,9 @@ def live_forward(runtime, input_ids: torch.Tensor, attention_mask: Optional[torc
     n_ck = 0
     for i in range(len(fam.layers)):
         seq_pos = seq_all if pos is None else pos % S
-        h = layer_fn(i, h, pos, seq_pos, B, S)
+        if h.shape[0] == 0:
+            break
+        h = layer_fn(i, h, pos, seq_pos, B, S, rows)
         if i not in routers:
             continue
         nxt = pos_out[n_ck % 2]
@@ -431,6 +494,8 @@ def live_forward(runtime, input_ids: torch.Tensor, attention_mask: Optional[torc
             on_checkpoint(i, n_surv)
         pos = nxt[:n_surv]
         h = comp[:n_surv]  # the survivors, compacted by the kernel: the next layer's input
+        if packed:
+            rows = _Packed.of(pos, B, S, order, first, err)
         if n_surv == 0:
             break
     n_rem = h.shape[0]
@@ -557,14 +622,13 @@ class LiveDecoder:
 
         rt, fam, B = self.rt, self.fam, b.B
         norm = rt._norm
-        h = fam.embed_tokens(b.tokens.view(B, 1))
-        length = self.pos + 1
+        self._begin(b)
+        h = self._embed(b)
         rows, slots, n_live = b.rows0, b.slots0, b.n0
         b.exit_layer.fill_(-1)
         thr = rt.config.exit_threshold
         for i in range(len(fam.layers)):
-            layer_fn = fam.decode_layer_fused if self.fused else fam.decode_layer
-            h = layer_fn(i, h, slots, n_live, self.pos, length, self.k[i], self.v[i], self.err)
+            h = self._layer(b, i, h, rows, slots, n_live)
             if i not in b.ck:
                 continue
             comp, rows_out, slots_out, exit_pos, counts = b.ck[i]
@@ -584,25 +648,57 @@ class LiveDecoder:
         _native.ops().norm_scatter_rows(last, rows, n_live, b.out_buf, norm.weight, norm.bias,
                                         norm.kind, norm.eps, self.err)
         self.remaining_dev += n_live
-        self.pos += 1
+        self._end(b)
         return rt._lm_head(b.out_buf)
+
+    # ---- what a step does to the cache (a decoder with another cache has its own)
+    def _begin(self, b: _StepBuffers) -> None:
+        self._after = self.pos + 1  # positions with this step's
+
+    def _embed(self, b: _StepBuffers) -> torch.Tensor:
+        return self.fam.embed_tokens(b.tokens.view(b.B, 1))
+
+    def _layer(self, b: _StepBuffers, i: int, h: torch.Tensor, rows: torch.Tensor,
+               slots: torch.Tensor, n_live: torch.Tensor) -> torch.Tensor:
+        layer_fn = self.fam.decode_layer_fused if self.fused else self.fam.decode_layer
+        return layer_fn(i, h, slots, n_live, self.pos, self._after, self.k[i], self.v[i], self.err)
+
+    def _end(self, b: _StepBuffers) -> None:
+        self.pos += 1
+
+    def _undo(self, saved) -> None:
+        """Take a step's effects on the cache back (saved: what _state() gave
+        before it)."""
+        for kc, vc in zip(self.k, self.v):
+            kc[:, :, saved].zero_()
+            vc[:, :, saved].zero_()
+        self.length = saved
+
+    def _state(self):
+        return self._length
+
+    def _prepare(self, b: _StepBuffers) -> None:
+        """Before a step, recorded or not: its checks and its device inputs."""
+        if self._length >= self.max_len:
+            raise RuntimeError("the live decoder's cache is full")
+
+    def _advanced(self, b: _StepBuffers) -> None:
+        """After a step: the lengths as the host knows them."""
+        self._length += 1
 
     def _capture(self, b: _StepBuffers) -> None:
         """Record b's step as a CUDA graph.  One eager step first (library
         handles, workspaces, folded routers), on a side stream; its effects
         are undone (the position's cache entries, the counters) before the
         capture, which runs nothing."""
-        p = self._length
+        saved = self._state()
         counters = (self.exits_dev.clone(), self.remaining_dev.clone())
         s = torch.cuda.Stream(device=self.dev)
         s.wait_stream(torch.cuda.current_stream(self.dev))
         with torch.cuda.stream(s):
             self._body(b)
         torch.cuda.current_stream(self.dev).wait_stream(s)
-        for kc, vc in zip(self.k, self.v):
-            kc[:, :, p].zero_()
-            vc[:, :, p].zero_()
-        self.length = p
+        self._undo(saved)
         self.exits_dev.copy_(counters[0])
         self.remaining_dev.copy_(counters[1])
         b.graph = torch.cuda.CUDAGraph()
@@ -617,14 +713,13 @@ class LiveDecoder:
         `stats` (an ExitStats) counts the step's tokens; its exits stay on
         the device until read_stats()."""
         B = tokens.shape[0]
-        if self._length >= self.max_len:
-            raise RuntimeError("the live decoder's cache is full")
         if B > self.n_slots:
             raise ValueError("more rows than cache slots")
         b = self._bufs.get(B)
         if b is None:
             H = self.fam.embed.embedding_dim
             b = self._bufs[B] = _StepBuffers(B, H, self.dtype, self.dev, self._checkpoints())
+        self._prepare(b)
         b.tokens.copy_(tokens.reshape(B))
         if self.graph:
             # the threshold is a constant of the recorded step: record again
@@ -636,7 +731,7 @@ class LiveDecoder:
             logits = b.logits
         else:
             logits = self._body(b)
-        self._length += 1
+        self._advanced(b)
         self.last_exit_layer = b.exit_layer[:B]
         if stats is not None:
             stats.total_tokens += B

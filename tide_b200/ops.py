@@ -120,4 +120,5 @@ class CheckpointRunner:
         if e:
             self.error_word.zero_()
             raise RuntimeError(f"tide_b200 kernel reported device error bits 0x{e:x} "
-                               "(1: exit position out of range, 2: wait timeout, 4: bad row count)")
+                               "(1: exit position out of range, 2: wait timeout, 4: bad row count, "
+                               "8: no free page)")

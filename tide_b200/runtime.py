@@ -180,7 +180,8 @@ class TIDERuntime(nn.Module):
         if host[-1]:
             self._runner.error_word.zero_()
             raise RuntimeError(f"tide_b200 kernel reported device error bits 0x{host[-1]:x} "
-                               "(1: position out of range, 2: wait timeout, 4: bad row count)")
+                               "(1: position out of range, 2: wait timeout, 4: bad row count, "
+                               "8: no free page)")
         stats = ExitStats(total_tokens=N)
         exit_layer = torch.full((N,), -1, dtype=torch.int32, device=counts.device)
         remaining = N
@@ -235,7 +236,8 @@ class TIDERuntime(nn.Module):
         return self._family
 
     def forward(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor] = None,
-                logits_to_keep: int = 0, live: Optional[bool] = None, **kwargs) -> torch.Tensor:
+                logits_to_keep: int = 0, live: Optional[bool] = None, packed: bool = False,
+                **kwargs) -> torch.Tensor:
         """Early-exit forward: logits [B, S, V].  By default the reference's
         post-hoc exit over the model's hidden states (runtime.py:134-192),
         with one host synchronisation per call (the exit counts, after the
@@ -243,17 +245,21 @@ class TIDERuntime(nn.Module):
         while the caller goes on).  With live=True (or config.live_compaction) the
         layers after each checkpoint run only on the tokens still active
         (tide_b200/live.py; logits then differ from the post-hoc ones by
-        design, through the exited tokens' zero-padded K/V).  After a call,
-        last_stats holds the ExitStats and last_exit_layer [B, S] the layer
-        each token exited at (-1: ran every layer).  `logits_to_keep` > 0
-        keeps only the last that many positions ([B, logits_to_keep, V]), so
+        design, through the exited tokens' zero-padded K/V); with padding in
+        attention_mask, or packed=True, their attention too runs on the active
+        tokens only, packed by sequence, and padding takes part in nothing (its
+        logits are those of a zero row, and last_stats does not count it).
+        After a call, last_stats holds the ExitStats and last_exit_layer [B, S]
+        the layer each token exited at (-1: ran every layer, or padding).
+        `logits_to_keep` > 0 keeps only the last that many positions
+        ([B, logits_to_keep, V]), so
         lm_head runs on the rows whose logits are used, e.g. 1 before
         sampling."""
         B, S = input_ids.shape
         if live if live is not None else self.config.live_compaction:
             from tide_b200.live import live_forward
 
-            out_buf, stats, exit_layer = live_forward(self, input_ids, attention_mask)
+            out_buf, stats, exit_layer = live_forward(self, input_ids, attention_mask, packed=packed)
             if self._learned_exits():
                 for layer in stats.exits_per_layer:
                     self._project_exits(out_buf, layer, (exit_layer == layer).nonzero()[:, 0])
@@ -307,7 +313,10 @@ class TIDERuntime(nn.Module):
         exit are skipped for it (tide_b200.live.LiveDecoder: its own KV cache
         addressed by slot, exited rows' later keys and values zero-padded,
         each step one CUDA graph replay unless live_graph=False);
-        Llama-family models with head_dim 128, bf16/fp16."""
+        Llama-family models with head_dim 128, bf16/fp16.  With paged=True as
+        well they decode on a paged cache (tide_b200.paged.PagedLiveDecoder),
+        each row from the tokens that `attention_mask` (zeros: padding, left
+        or right) leaves of it; the other modes take no mask."""
         eos = kwargs.get("eos_token_id", 2)
         B = input_ids.shape[0]
         dev = input_ids.device
@@ -316,10 +325,15 @@ class TIDERuntime(nn.Module):
         gen_stats = ExitStats(total_tokens=0)
         if live:
             from tide_b200.live import LiveDecoder
+            from tide_b200.paged import PagedLiveDecoder
 
-            dec = LiveDecoder(self, B, input_ids.shape[1] + max_new_tokens + 1,
-                              graph=kwargs.get("live_graph", True))
-            next_logits = dec.prefill(input_ids)
+            room, graph = input_ids.shape[1] + max_new_tokens + 1, kwargs.get("live_graph", True)
+            if kwargs.get("paged", False):
+                dec = PagedLiveDecoder(self, B, room, graph=graph)
+                next_logits = dec.prefill(input_ids, kwargs.get("attention_mask"))
+            else:
+                dec = LiveDecoder(self, B, room, graph=graph)
+                next_logits = dec.prefill(input_ids)
             for _ in range(max_new_tokens):
                 nxt = sample_next_token(next_logits, temperature, top_k, top_p)
                 generated = torch.cat([generated, nxt], dim=-1)
