@@ -709,39 +709,60 @@ __device__ __forceinline__ void add_odd_values(const Params &p, const Unit &u, i
   }
 }
 
-// N 16-byte vectors of each of a warp's 32 rows, row r in lane r, to global
-// memory: over shared memory, so that N lanes write a row's bytes side by side
-// (a lane that wrote its own row would touch 32 lines an instruction).  `at`
-// is the lane's row in global memory, or NULL.
+// Rows of a warp to global memory, N 16-byte vectors of each of its 32 rows at
+// a time, row r in lane r: over shared memory, so that N lanes write a row's
+// bytes side by side (a lane that wrote its own row would touch 32 lines an
+// instruction).  The places are found once, and the loads from shared memory
+// are all issued before the first store (one after the other, behind stores
+// that might have been to the same place, they made a unit's end 4700 cycles
+// long).
 template <int N>
-__device__ __forceinline__ void store_rows(unsigned char *staging, const uint32_t *w,
-                                           unsigned char *at) {
-  constexpr int kRowsAtOnce = 32 / N;
-  const int lane = threadIdx.x & 31;
-  __syncwarp();
+struct RowStore {
+  static constexpr int kRowsAtOnce = 32 / N;
+  unsigned char *to[N];
+
+  // at: this lane's row in global memory, or NULL
+  __device__ __forceinline__ explicit RowStore(unsigned char *at) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    *reinterpret_cast<uint4 *>(staging + lane * 128 + ((i ^ (lane & 7)) << 4)) =
-        make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int r = i * kRowsAtOnce + lane / N, e = lane % N;
-    unsigned char *to = reinterpret_cast<unsigned char *>(
-        __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(at), r));
-    const uint4 x = *reinterpret_cast<const uint4 *>(staging + r * 128 + ((e ^ (r & 7)) << 4));
-    if (to) *reinterpret_cast<uint4 *>(to + e * 16) = x;
+    for (int i = 0; i < N; ++i) {
+      unsigned char *a = reinterpret_cast<unsigned char *>(__shfl_sync(
+          0xffffffffu, reinterpret_cast<unsigned long long>(at), i * kRowsAtOnce + lane / N));
+      to[i] = a ? a + lane % N * 16 : nullptr;
+    }
   }
-}
+  // w to the bytes from `offset` on of each row
+  __device__ __forceinline__ void operator()(uint32_t staging, const uint32_t *w, int offset) const {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      ptx::sts128(staging + lane * 128 + ((i ^ (lane & 7)) << 4), w + 4 * i);
+    __syncwarp();
+    uint4 x[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = i * kRowsAtOnce + lane / N;
+      x[i] = ptx::lds128(staging + r * 128 + ((lane % N ^ (r & 7)) << 4));
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (to[i]) *reinterpret_cast<uint4 *>(to[i] + offset) = x[i];
+  }
+};
 
 // Weights of 32 scores, their sums, and their 16-bit form to tensor memory.
-template <typename T>
+// MORE: also the largest of the first MORE scores, in the shadow of the
+// exponentials (16 lanes a cycle per SM, eight cycles for a warp's).
+template <typename T, int MORE>
 __device__ __forceinline__ void weigh_quarter(const float *s, uint64_t qs2, uint64_t mq2,
-                                              uint64_t (&sum)[2], uint32_t p_col) {
+                                              uint64_t (&sum)[2], uint32_t p_col, float (&mx)[2]) {
   uint32_t w[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     float a, b;
+    if (MORE) mx[i & 1] = max3(mx[i & 1], s[2 * i], s[2 * i + 1]);
+    if (MORE > 32) mx[i & 1] = max3(mx[i & 1], s[32 + 2 * i], s[32 + 2 * i + 1]);
     unpair(fma2(pair(s[2 * i], s[2 * i + 1]), qs2, mq2), &a, &b);
     a = ex2(a);
     b = ex2(b);
@@ -753,7 +774,7 @@ __device__ __forceinline__ void weigh_quarter(const float *s, uint64_t qs2, uint
 
 template <typename T, int D, bool PAGED>
 __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem,
-                             unsigned char *staging) {
+                             uint32_t staging) {
   constexpr unsigned kFull = 0xffffffffu;
   const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) & 3;
   const int r = warp * 32 + lane;                 // row of the tile
@@ -803,46 +824,58 @@ __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem,
 #pragma unroll
         for (int i = 0; i < kKeys; ++i) s[i] = i < lim ? s[i] : -INFINITY;
       }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int i = 0; i < kKeys; i += 8)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) mx[q] = max3(mx[q], s[i + 2 * q], s[i + 2 * q + 1]);
-      const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+      // Weights of three quarters against the maximum as it was, and the
+      // maximum beside them: a block rarely has a score more than kSlack above
+      // it, and if it has they are weighed once more.  (With the maximum first
+      // each block's chain was 250 of 3350 cycles longer.)
+      uint64_t sum[2], qs2, mq2;
+      float mx[2];
+      auto weigh = [&] {  // S is in registers: P takes its upper half
+        const float mq = m == -INFINITY ? 0.f : m * p.qs;
+        qs2 = pair(p.qs, p.qs), mq2 = pair(-mq, -mq);
+        sum[0] = sum[1] = 0;
+        mx[0] = mx[1] = -INFINITY;
+        weigh_quarter<T, 32>(s, qs2, mq2, sum, p_col, mx);
+        weigh_quarter<T, 32>(s + 32, qs2, mq2, sum, p_col + 16, mx);
+        weigh_quarter<T, 64>(s + 64, qs2, mq2, sum, p_col + 32, mx);
+      };
       if (j == u.b0) {  // nothing in O yet
+        mx[0] = mx[1] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kKeys; i += 4)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) mx[q] = max3(mx[q], s[i + 2 * q], s[i + 2 * q + 1]);
+        const float top = fmaxf(mx[0], mx[1]);
         if (top > m) {
           l *= ex2((m - top) * p.qs);
           m = top;
         }
-      } else {
-        const bool raise = top > m + slack;
-        if (__any_sync(kFull, raise)) {
-          const float a = raise ? ex2((m - top) * p.qs) : 1.f;
-          if (raise) m = top;
-          l *= a;
+      }
 #pragma unroll 1
-          for (int q = 0; q < D; q += 16) {
-            uint32_t o[16];
-            ptx::tmem_ld16_async(o_col + q, o);
-            ptx::tmem_wait_ld();
-            ptx::tmem_landed16(o);
+      for (;;) {
+        weigh();
+        const float top = fmaxf(mx[0], mx[1]);
+        const bool raise = top > m + slack;  // (never in a unit's first block)
+        if (!__any_sync(kFull, raise)) break;
+        const float a = raise ? ex2((m - top) * p.qs) : 1.f;
+        if (raise) m = top;
+        l *= a;
+#pragma unroll 1
+        for (int q = 0; q < D; q += 16) {
+          uint32_t o[16];
+          ptx::tmem_ld16_async(o_col + q, o);
+          ptx::tmem_wait_ld();
+          ptx::tmem_landed16(o);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
-            ptx::tmem_st16(o_col + q, o);
-          }
+          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
+          ptx::tmem_st16(o_col + q, o);
         }
       }
-      const float mq = m == -INFINITY ? 0.f : m * p.qs;
-      const uint64_t qs2 = pair(p.qs, p.qs), mq2 = pair(-mq, -mq);
-      uint64_t sum[2] = {0, 0};
-      // S is in registers: P takes its upper half
-#pragma unroll
-      for (int q = 0; q < 3; ++q) weigh_quarter<T>(s + q * kQuarter, qs2, mq2, sum, p_col + q * 16);
       ptx::tmem_wait_st();
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(&sh.p_full[t][0]);
-      weigh_quarter<T>(s + 96, qs2, mq2, sum, p_col + 48);
+      weigh_quarter<T, 0>(s + 96, qs2, mq2, sum, p_col + 48, mx);
       ptx::tmem_wait_st();
       ptx::tc_fence_before();
       __syncwarp();
@@ -852,6 +885,11 @@ __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem,
       l += la + lb;
     }
     const bool some = end > u.b0;
+    const int64_t at = row * p.hq + u.kvh * p.group + head;
+    const bool nothing = !some || l == 0.f;
+    const float inv = nothing ? 0.f : 1.f / l;
+    const int64_t part = (int64_t)u.split * p.batch.n_tokens * p.hq + at;
+    if (p.splits > 1 && valid) p.part_ml[part] = make_float2(m * p.qs, l);
     if (some) {
       TIDE_WAIT(&sh.o_full[t], no & 1);
       ++no;
@@ -861,33 +899,35 @@ __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem,
     const bool odd = some && sh.odd[n & 3];
     const int first = max(u.pos0 + 1, u.b0 * kKeys);
     const int stop = valid ? min(sees, min(end * kKeys, last)) : first;
-    const int64_t at = row * p.hq + u.kvh * p.group + head;
-    const bool nothing = !some || l == 0.f;
-    const float inv = nothing ? 0.f : 1.f / l;
-    const int64_t part = (int64_t)u.split * p.batch.n_tokens * p.hq + at;
-    if (p.splits > 1 && valid) p.part_ml[part] = make_float2(m * p.qs, l);
-    if (p.splits > 1 && !some) continue;  // (a sum of 0: its output is not read)
-#pragma unroll 1
-    for (int q = 0; q < D; q += 32) {
-      uint32_t o[32];
+    auto output = [&](int q, uint32_t(&o)[32]) {
       if (some) {
         ptx::tmem_ld32_async(o_col + q, o);
         ptx::tmem_wait_ld();
         ptx::tmem_landed(o);
       }
-      float *f = reinterpret_cast<float *>(o);
-      if (odd) add_odd_values<T, D, PAGED>(p, u, first, stop, q, f);
-      if (p.splits > 1) {
-        store_rows<8>(staging, o, valid ? reinterpret_cast<unsigned char *>(p.part_o + part * D + q)
-                                        : nullptr);
-      } else {
-        uint32_t w[16];
+      if (odd) add_odd_values<T, D, PAGED>(p, u, first, stop, q, reinterpret_cast<float *>(o));
+    };
+    if (p.splits > 1) {
+      if (!some) continue;  // (a sum of 0: its output is not read)
+      const RowStore<8> store(valid ? reinterpret_cast<unsigned char *>(p.part_o + part * D) : nullptr);
+#pragma unroll 1
+      for (int q = 0; q < D; q += 32) {
+        uint32_t o[32];
+        output(q, o);
+        store(staging, o, q * 4);
+      }
+    } else {
+      const RowStore<4> store(
+          valid ? reinterpret_cast<unsigned char *>(static_cast<T *>(p.out) + at * D) : nullptr);
+#pragma unroll 1
+      for (int q = 0; q < D; q += 32) {
+        uint32_t o[32], w[16];
+        output(q, o);
+        const float *f = reinterpret_cast<const float *>(o);
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           w[i] = nothing ? 0u : pack2<T>(f[2 * i] * inv, f[2 * i + 1] * inv);
-        store_rows<4>(staging, w,
-                      valid ? reinterpret_cast<unsigned char *>(static_cast<T *>(p.out) + at * D + q)
-                            : nullptr);
+        store(staging, w, q * 2);
       }
     }
     ptx::tc_fence_before();
@@ -946,7 +986,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
   else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp < 8) {
-    softmax_tile<T, D, PAGED>(p, sh, warp >> 2, tmem, staging + warp * 4096);
+    softmax_tile<T, D, PAGED>(p, sh, warp >> 2, tmem, ptx::smem_u32(staging + warp * 4096));
   } else if (warp == 8) {
     schedule_units(p, sh);
   } else if (warp == 9) {

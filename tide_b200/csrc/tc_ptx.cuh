@@ -173,6 +173,19 @@ __device__ __forceinline__ void tc_fence_after() {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
 
+__device__ __forceinline__ void sts128(uint32_t at, const uint32_t *w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]),
+               "r"(w[2]), "r"(w[3])
+               : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+  uint4 x;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+               : "r"(at)
+               : "memory");
+  return x;
+}
 // True in one lane of a converged warp, the same one every time.
 __device__ __forceinline__ bool elect_one() {
   uint32_t e;
