@@ -102,6 +102,7 @@ struct Params {
   int few;         // sequences of up to so many tokens go to the few-rows kernel
   int64_t group_keys;  // keys whose rows, of all KV heads, L2 holds
   int take_over;   // whether there are more CTAs than run at once
+  int boxes;       // whether a warp's 32 rows are a box of the output's map
   int behind_few;  // launched over the few-rows kernel of the same call
   float qs;        // scale * log2(e)
 };
@@ -720,10 +721,10 @@ template <int N>
 struct RowStore {
   static constexpr int kRowsAtOnce = 32 / N;
   unsigned char *to[N];
+  int lane;
 
   // at: this lane's row in global memory, or NULL
-  __device__ __forceinline__ explicit RowStore(unsigned char *at) {
-    const int lane = threadIdx.x & 31;
+  __device__ __forceinline__ RowStore(unsigned char *at, int lane) : lane(lane) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       unsigned char *a = reinterpret_cast<unsigned char *>(__shfl_sync(
@@ -733,7 +734,6 @@ struct RowStore {
   }
   // w to the bytes from `offset` on of each row
   __device__ __forceinline__ void operator()(uint32_t staging, const uint32_t *w, int offset) const {
-    const int lane = threadIdx.x & 31;
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -774,7 +774,7 @@ __device__ __forceinline__ void weigh_quarter(const float *s, uint64_t qs2, uint
 
 template <typename T, int D, bool PAGED>
 __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem,
-                             uint32_t staging) {
+                             uint32_t stage, const CUtensorMap *mo) {
   constexpr unsigned kFull = 0xffffffffu;
   const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) & 3;
   const int r = warp * 32 + lane;                 // row of the tile
@@ -840,12 +840,12 @@ __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem,
         weigh_quarter<T, 64>(s + 64, qs2, mq2, sum, p_col + 32, mx);
       };
       if (j == u.b0) {  // nothing in O yet
-        mx[0] = mx[1] = -INFINITY;
+        float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < kKeys; i += 4)
+        for (int i = 0; i < kKeys; i += 8)
 #pragma unroll
-          for (int q = 0; q < 2; ++q) mx[q] = max3(mx[q], s[i + 2 * q], s[i + 2 * q + 1]);
-        const float top = fmaxf(mx[0], mx[1]);
+          for (int q = 0; q < 4; ++q) x[q] = max3(x[q], s[i + 2 * q], s[i + 2 * q + 1]);
+        const float top = fmaxf(max3(x[0], x[1], x[2]), x[3]);
         if (top > m) {
           l *= ex2((m - top) * p.qs);
           m = top;
@@ -907,9 +907,18 @@ __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem,
       }
       if (odd) add_odd_values<T, D, PAGED>(p, u, first, stop, q, reinterpret_cast<float *>(o));
     };
+    // (The addresses below are worked out here: kept over the loop above they
+    // would cost it registers.)
+    int me = lane;
+    uint32_t staging = stage;
+    asm volatile("" : "+r"(me), "+r"(staging));
+    // copies out of the staging that the unit before left in flight
+    if (lane == 0) ptx::bulk_wait_read(0);
+    __syncwarp();
     if (p.splits > 1) {
       if (!some) continue;  // (a sum of 0: its output is not read)
-      const RowStore<8> store(valid ? reinterpret_cast<unsigned char *>(p.part_o + part * D) : nullptr);
+      const RowStore<8> store(valid ? reinterpret_cast<unsigned char *>(p.part_o + part * D) : nullptr,
+                              me);
 #pragma unroll 1
       for (int q = 0; q < D; q += 32) {
         uint32_t o[32];
@@ -917,8 +926,13 @@ __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem,
         store(staging, o, q * 4);
       }
     } else {
+      // When all 32 rows are there, and they are whole tokens' heads, or heads
+      // of one token: copies of 32 columns, two of them in flight, from 64-byte
+      // rows swizzled as the copy expects.
+      const bool box = p.boxes && __all_sync(kFull, valid);
+      const int tok0 = __shfl_sync(kFull, (int)row, 0), head0 = __shfl_sync(kFull, u.kvh * p.group + head, 0);
       const RowStore<4> store(
-          valid ? reinterpret_cast<unsigned char *>(static_cast<T *>(p.out) + at * D) : nullptr);
+          valid ? reinterpret_cast<unsigned char *>(static_cast<T *>(p.out) + at * D) : nullptr, me);
 #pragma unroll 1
       for (int q = 0; q < D; q += 32) {
         uint32_t o[32], w[16];
@@ -927,7 +941,22 @@ __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem,
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           w[i] = nothing ? 0u : pack2<T>(f[2 * i] * inv, f[2 * i + 1] * inv);
-        store(staging, w, q * 2);
+        if (box) {
+          const uint32_t half = (q & 32) * 64;
+          if (lane == 0) ptx::bulk_wait_read(1);
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            ptx::sts128(staging + half + me * 64 + ((i ^ ((me >> 1) & 3)) << 4), w + 4 * i);
+          ptx::fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            ptx::tma_store_3d(mo, staging + half, q, head0, tok0);
+            ptx::bulk_commit();
+          }
+        } else {
+          store(staging, w, q * 2);
+        }
       }
     }
     ptx::tc_fence_before();
@@ -938,7 +967,8 @@ template <typename T, int D, bool PAGED>
 __global__ void __launch_bounds__(kThreads, 1)
     tile_attention_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap mq,
                           const __grid_constant__ CUtensorMap mk,
-                          const __grid_constant__ CUtensorMap mv) {
+                          const __grid_constant__ CUtensorMap mv,
+                          const __grid_constant__ CUtensorMap mo) {
   using S = Shape<D>;
   extern __shared__ unsigned char dyn[];
   __shared__ Shared sh;
@@ -986,7 +1016,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
   else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp < 8) {
-    softmax_tile<T, D, PAGED>(p, sh, warp >> 2, tmem, ptx::smem_u32(staging + warp * 4096));
+    softmax_tile<T, D, PAGED>(p, sh, warp >> 2, tmem, ptx::smem_u32(staging + warp * 4096), &mo);
+    if ((threadIdx.x & 31) == 0) ptx::bulk_wait_all();
   } else if (warp == 8) {
     schedule_units(p, sh);
   } else if (warp == 9) {
@@ -1553,20 +1584,21 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return f;
 }
 
-// 16-bit rows [d2][d1][d0], s1 and s2 elements apart, read in boxes of 64 of
-// a row's elements (128 bytes, swizzled) by b1 by b2.
+// 16-bit rows [d2][d1][d0], s1 and s2 elements apart, in boxes of 64 of a
+// row's elements (128 bytes, swizzled; or 32, 64 bytes) by b1 by b2.
 bool make_map(CUtensorMap *m, int dtype, const void *base, int rank, int64_t d0, int64_t d1,
-              int64_t d2, int64_t s1, int64_t s2, int b1, int b2) {
+              int64_t d2, int64_t s1, int64_t s2, int b1, int b2, int b0 = 64) {
   auto enc = encode_fn();
   if (!enc) return false;
   cuuint64_t dims[3] = {(cuuint64_t)d0, (cuuint64_t)d1, (cuuint64_t)d2};
   cuuint64_t strides[2] = {(cuuint64_t)s1 * 2, (cuuint64_t)s2 * 2};
-  cuuint32_t box[3] = {64, (cuuint32_t)b1, (cuuint32_t)b2};
+  cuuint32_t box[3] = {(cuuint32_t)b0, (cuuint32_t)b1, (cuuint32_t)b2};
   cuuint32_t step[3] = {1, 1, 1};
   return enc(m, dtype == TIDE_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                          : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
              (cuuint32_t)rank, const_cast<void *>(base), dims, strides, box, step,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_INTERLEAVE_NONE,
+             b0 == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -1661,7 +1693,7 @@ template <typename T, int D, bool PAGED>
 int launch(tide::ragged::Params &p, int dtype, const void *q, int64_t q_stride, int64_t kv_rows,
            bool behind_few, cudaStream_t s) {
   using namespace tide::ragged;
-  CUtensorMap mq, mk, mv;
+  CUtensorMap mq, mk, mv, mo;
   const int page = 1 << p.src.page_shift;
   const int box = PAGED && page < kKeys ? page : kKeys;
   bool ok = make_map(&mq, dtype, q, 3, D, p.hq, p.batch.n_tokens, D, q_stride, p.group, p.tokens);
@@ -1671,6 +1703,14 @@ int launch(tide::ragged::Params &p, int dtype, const void *q, int64_t q_stride, 
     ok = ok && (PAGED ? make_map(m, dtype, base, 2, D, kv_rows, 1, D, 0, box, 1)
                       : make_map(m, dtype, base, 3, D, p.hkv, p.batch.n_tokens, D, p.src.row_stride,
                                  1, box));
+  }
+  p.boxes = 32 % p.group == 0 || p.group % 32 == 0;
+  if (p.boxes && p.splits == 1) {
+    const int heads = p.group < 32 ? p.group : 32;
+    ok = ok && make_map(&mo, dtype, p.out, 3, D, p.hq, p.batch.n_tokens, D, (int64_t)p.hq * D, heads,
+                        32 / heads, 32);
+  } else {
+    mo = mq;  // (not used)
   }
   if (!ok) return fail(TIDE_ERR_CUDA, "ragged attention: cuTensorMapEncodeTiled failed");
   auto kern = tile_attention_kernel<T, D, PAGED>;
@@ -1692,7 +1732,7 @@ int launch(tide::ragged::Params &p, int dtype, const void *q, int64_t q_stride, 
   cfg.numAttrs = 1;
   p.take_over = units > 148;
   p.behind_few = behind_few;
-  return report(cudaLaunchKernelEx(&cfg, kern, p, mq, mk, mv), "ragged attention");
+  return report(cudaLaunchKernelEx(&cfg, kern, p, mq, mk, mv, mo), "ragged attention");
 }
 
 template <typename T, int D, int NT>

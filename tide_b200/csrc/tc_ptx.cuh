@@ -126,6 +126,15 @@ __device__ __forceinline__ void bulk_store(void *dst, const void *src, uint32_t 
                "r"(smem_u32(src)), "r"(bytes), "l"(policy)
                : "memory");
 }
+// 3-D tiled store shared -> global, of this thread's open bulk group.
+__device__ __forceinline__ void tma_store_3d(const void *tmap, uint32_t src, int c0, int c1,
+                                             int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+          reinterpret_cast<uint64_t>(tmap)),
+      "r"(src), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
 __device__ __forceinline__ void bulk_commit() {
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
