@@ -1149,7 +1149,15 @@ __global__ void __launch_bounds__(32 * kFewWarps, NT <= 2 ? 3 : 2)
   __shared__ float s_m[kFewWarps][kRowsMost], s_l[kFewWarps][kRowsMost];
   __shared__ int s_abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  ptx::grid_dependency_wait();
+  if (threadIdx.x == 0) {
+    ptx::prefetch_tmap(&mk);
+    ptx::prefetch_tmap(&mv);
+    for (int w = 0; w < kFewWarps; ++w)
+      for (int i = 0; i < kFewStages; ++i) ptx::mbar_init(&full[w][i], 1);
+    ptx::fence_mbar_init();
+    s_abort = 0;
+  }
+  ptx::grid_dependency_wait();  // up to here this overlaps the kernel before
   ptx::grid_dependents_launch();
   const int split = (int)(blockIdx.x % p.splits);
   const int64_t unit = blockIdx.x / p.splits;
@@ -1205,12 +1213,6 @@ __global__ void __launch_bounds__(32 * kFewWarps, NT <= 2 ? 3 : 2)
     return;
   }
   unsigned char *ring = dyn + ((1024u - (ptx::smem_u32(dyn) & 1023u)) & 1023u) + warp * F::kRing;
-  if (threadIdx.x == 0) {
-    for (int w = 0; w < kFewWarps; ++w)
-      for (int i = 0; i < kFewStages; ++i) ptx::mbar_init(&full[w][i], 1);
-    ptx::fence_mbar_init();
-    s_abort = 0;
-  }
   __syncthreads();
 
   // this warp's groups of 16 keys: warp, warp + 4, ... of the split's
@@ -1474,7 +1476,6 @@ __global__ void __launch_bounds__(256)
                 const float *__restrict__ part_o, const float2 *__restrict__ part_ml, T *out) {
   constexpr int kE = D / 32, kBatch = 8;
   __shared__ float s_m[8], s_l[8], s_o[8][D];
-  ptx::grid_dependency_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t step = (int64_t)(FEW ? (int64_t)batch.n_seqs * few : batch.n_tokens) * hq;
   const int64_t at = (int64_t)blockIdx.x * (8 / per) + warp / per;
@@ -1492,6 +1493,9 @@ __global__ void __launch_bounds__(256)
       if (seq >= 0 && sequence(batch, seq).n > few) row = at / hq;
     }
   }
+  // The kernels before waited for what made the batch before they let this one
+  // start; what they themselves write comes now.
+  ptx::grid_dependency_wait();
   float m = -INFINITY, l = 0.f, o[kE];
 #pragma unroll
   for (int e = 0; e < kE; ++e) o[e] = 0.f;
