@@ -1663,12 +1663,18 @@ Plan plan_paged(bool one_token, int64_t n_tokens, int64_t n_seqs, int64_t hq, in
   p.tiles = !p.nt || (!one_token && n_tokens > p.few);
   p.pieces = n_seqs + (p.few > p.tokens ? n_tokens / p.tokens : 0);
   const int64_t rows = n_tokens * hq;
-  // Few rows: splits of 512 keys at least, as long as the CTAs that an SM
-  // holds (two) are not taken eight times over: sequences differ in length,
-  // and the more pieces, the evener the end.
+  // Few rows.  Up to a quarter as many units as CTAs that run at once (two an
+  // SM): one round of them, with splits of 128 keys at least (3 requests of 9000
+  // to 40000 keys, 8 KV heads: 51 us; with up to eight rounds of splits of 512
+  // 57; one of 1000: 7.9 and 10.9).  More units: up to eight rounds, since
+  // sequences differ in length, and the more pieces, the evener the end (16
+  // requests of up to 16000: 98 us in one round, 88 in eight).
+  constexpr int64_t kSlots = 2 * 148;
   const int64_t units = p.pieces * hkv;
-  int64_t s = p.nt ? (16 * 148 + units - 1) / units : 1;
-  if (s > (max_kv + 511) / 512) s = (max_kv + 511) / 512;
+  const bool one_round = units * 4 <= kSlots;
+  const int64_t least = one_round ? 128 : 512;
+  int64_t s = !p.nt ? 1 : one_round ? kSlots / units : (8 * kSlots + units - 1) / units;
+  if (s > (max_kv + least - 1) / least) s = (max_kv + least - 1) / least;
   if (s < 1 || units >= 4 * 148) s = 1;
   const int64_t keys = (max_kv + s - 1) / s;
   p.split_keys = (int)((keys + 63) / 64 * 64);
