@@ -1766,11 +1766,12 @@ int launch_few(const tide::ragged::FewParams &p, int dtype, int64_t kv_rows, cud
   if (!make_map(&mk, dtype, p.src.k, 2, D, kv_rows, 1, D, 0, kFewKeys, 1) ||
       !make_map(&mv, dtype, p.src.v, 2, D, kv_rows, 1, D, 0, kFewKeys, 1))
     return fail(TIDE_ERR_CUDA, "paged_attention: cuTensorMapEncodeTiled failed");
+  const int64_t ctas = (int64_t)p.pieces * p.hkv * p.splits;
+  if (ctas > INT32_MAX) return fail(TIDE_ERR_INVALID, "paged_attention: too many sequences and heads");
   auto kern = few_rows_kernel<T, D, NT>;
   static std::atomic<uint64_t> set{0};  // per device
   cudaError_t e = tide::allow_smem(kern, (int)Few<D>::kSmem, set);
   if (e != cudaSuccess) return report(e, "paged_attention");
-  const int64_t ctas = (int64_t)p.pieces * p.hkv * p.splits;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas, 1, 1);
   cfg.blockDim = dim3(32 * kFewWarps, 1, 1);
