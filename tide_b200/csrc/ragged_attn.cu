@@ -188,16 +188,18 @@ struct Shared {
   } while (0)
 
 // ------------------------------------------------------------------ units
-__device__ __forceinline__ void seq_level(const Params &p, int i, int *count, int *level) {
+// Units of sequence i, the level of its first one, and its keys.
+__device__ __forceinline__ int seq_level(const Params &p, int i, int *count, int *level) {
   const Sequence s = sequence(p.batch, i);
-  const int per = 2 * p.tokens;
-  *count = s.n > p.few ? (s.n + per - 1) / per : 0;
-  *level = max(s.kv - s.n, 0) / per;
+  const unsigned per = 2 * p.tokens;
+  *count = s.n > p.few ? (int)((s.n + per - 1) / per) : 0;
+  *level = (int)((unsigned)max(s.kv - s.n, 0) / per);
+  return s.kv;
 }
 
 // The unit of a CTA that has yet to start, which then does not; *more is false
 // when there is none.  False when the wait ran out.
-__device__ __forceinline__ bool next_unit(const Params &p, Shared &sh, int64_t *u, uint32_t *asked,
+__device__ __forceinline__ bool next_unit(const Params &p, Shared &sh, uint32_t *u, uint32_t *asked,
                                           bool *more) {
   if ((threadIdx.x & 31) == 0) {
     ptx::mbar_expect_tx(&sh.taken, 16);
@@ -223,22 +225,30 @@ __device__ void schedule_units(const Params &p, Shared &sh) {
   const int lane = threadIdx.x & 31;
   const int live = live_sequences(p.batch);
   int cnt[kCached], lvl[kCached];
-#pragma unroll
-  for (int k = 0; k < kCached; ++k) {
-    cnt[k] = lvl[k] = 0;
-    if (lane + 32 * k < live) seq_level(p, lane + 32 * k, &cnt[k], &lvl[k]);
-  }
-  int64_t units_in_all = 0;  // of one KV head and split
+  uint32_t units_in_all = 0;  // of one KV head and split
+  int64_t keys_in_all = 0;
+  int top = 0;
   {
-    int c = 0;
+    unsigned c = 0, low = 0, high = 0;  // (keys: their low and high 16 bits)
+    auto add = [&](int i, int *n, int *l) {
+      const unsigned kv = (unsigned)seq_level(p, i, n, l);
+      c += *n;
+      low += kv & 0xffff;
+      high += kv >> 16;
+      top = max(top, *n + *l);
+    };
 #pragma unroll
-    for (int k = 0; k < kCached; ++k) c += cnt[k];
+    for (int k = 0; k < kCached; ++k) {
+      cnt[k] = lvl[k] = 0;
+      if (lane + 32 * k < live) add(lane + 32 * k, &cnt[k], &lvl[k]);
+    }
     for (int i = lane + 32 * kCached; i < live; i += 32) {
       int n, l;
-      seq_level(p, i, &n, &l);
-      c += n;
+      add(i, &n, &l);
     }
-    units_in_all = __reduce_add_sync(kFull, (unsigned)c);
+    units_in_all = __reduce_add_sync(kFull, c);
+    keys_in_all = (int64_t)__reduce_add_sync(kFull, low) + ((int64_t)__reduce_add_sync(kFull, high) << 16);
+    top = __reduce_max_sync(kFull, top);
   }
   int s0 = 0, s1 = 0;  // the group: sequences [s0, s1)
   auto units_from = [&](int x) {  // its units of level x and above
@@ -253,14 +263,19 @@ __device__ void schedule_units(const Params &p, Shared &sh) {
     }
     return (int)__reduce_add_sync(kFull, (unsigned)c);
   };
-  const int per_rank = p.hkv * p.splits;
-  int64_t base = 0;                  // units (of one KV head and split) before the group
+  const uint32_t per_rank = p.hkv * p.splits;
+  int base = 0;                      // units (of one KV head and split) before the group
   int total = 0;                     // in the group
   int x = 0, above = 0, upto = 0;    // level, the group's units above it, of it and above
   int top_level = 0;
+  if (keys_in_all <= p.group_keys) {  // one group: all of them
+    s1 = live;
+    total = (int)units_in_all;
+    x = top_level = top;
+  }
   uint32_t asked = 0;
   bool more = true;  // this CTA has a unit
-  int64_t u = blockIdx.x;
+  uint32_t u = blockIdx.x;
   for (uint32_t n = 0;; ++n) {
     const int slot = n & 1;
     // every warp has taken up the unit before: time for another one (sooner,
@@ -275,13 +290,13 @@ __device__ void schedule_units(const Params &p, Shared &sh) {
       if (!p.take_over) more = false;
       else if (!next_unit(p, sh, &u, &asked, &more)) return;
     }
-    const int64_t rank = u / per_rank;
+    const int rank = (int)(u / per_rank);
     if (rank < base) s1 = total = 0, base = 0;  // (should they ever come out of order)
     while (rank - base >= total && s1 < live) {  // the next group
       base += total;
       s0 = s1;
       int64_t keys = 0;
-      int top = 0;
+      int most = 0;
       for (;;) {
         const int i = s1 + lane;
         const int mine = i < live ? sequence(p.batch, i).kv : 0;
@@ -296,19 +311,19 @@ __device__ void schedule_units(const Params &p, Shared &sh) {
         if (in) {
           int c, l;
           seq_level(p, i, &c, &l);
-          top = max(top, c + l);
+          most = max(most, c + l);
         }
         keys += __shfl_sync(kFull, sum, 31);
         s1 += many;
         if (many < 32) break;
       }
-      x = top_level = __reduce_max_sync(kFull, top);
+      x = top_level = __reduce_max_sync(kFull, most);
       above = upto = 0;
       total = units_from(0);
     }
     Unit w{};
-    if (more && rank < units_in_all) {
-      const int in_group = (int)(rank - base);
+    if (more && rank < (int)units_in_all) {
+      const int in_group = rank - base;
       if (in_group < above) x = top_level, above = upto = 0;
       if (in_group >= upto) {  // units_from(lo) > in_group >= units_from(hi)
         int lo = 0, hi = x;
