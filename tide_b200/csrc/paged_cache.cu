@@ -118,6 +118,7 @@ __global__ void __launch_bounds__(kThreads) page_tables_kernel(const __grid_cons
     s_cu[0] = 0;
   }
   ptx::grid_dependency_wait();
+  if (tid == 0) ptx::grid_dependents_launch();
   int n_free = __ldcg(p.n_free);  // (used when the lengths have come too)
   const bool bad_free = n_free < 0 || n_free > p.n_pages;
   n_free = min(max(n_free, 0), p.n_pages);
@@ -246,6 +247,7 @@ __global__ void __launch_bounds__(kThreads) page_tables_kernel(const __grid_cons
 // the lengths and tables that the step leaves.
 __global__ void __launch_bounds__(256) slot_map_kernel(const __grid_constant__ Params p) {
   ptx::grid_dependency_wait();
+  ptx::grid_dependents_launch();
   const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (t >= p.n_slots) return;
   int64_t slot = -1, pos = 0;
@@ -276,6 +278,7 @@ __global__ void __launch_bounds__(256)
   constexpr int kFlight = 4;    // of a lane's, loaded before the first is stored
   const int lane = threadIdx.x & 31;
   ptx::grid_dependency_wait();
+  ptx::grid_dependents_launch();
   int64_t live = n_rows;
   if (n_dev) live = min((int64_t)max(__ldg(n_dev), 0), n_rows);
   const int64_t warps = (int64_t)gridDim.x * (blockDim.x / 32);

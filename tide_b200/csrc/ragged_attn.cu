@@ -1036,6 +1036,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // the same call, which waits before it lets this one start, there is nothing
   // more to wait for.)
   if (!p.behind_few) ptx::grid_dependency_wait();
+  if (threadIdx.x == 0) ptx::grid_dependents_launch();
 
   // Registers move to the softmax warps: 256 * 208 + 128 * 88 = 384 * 168, what
   // the block was launched with.
@@ -1525,6 +1526,7 @@ __global__ void __launch_bounds__(256)
   // The kernels before waited for what made the batch before they let this one
   // start; what they themselves write comes now.
   ptx::grid_dependency_wait();
+  ptx::grid_dependents_launch();
   float m = -INFINITY, l = 0.f, o[kE];
 #pragma unroll
   for (int e = 0; e < kE; ++e) o[e] = 0.f;
