@@ -56,8 +56,12 @@
 // level come from counting over the sequences, so no list of units is built.
 // Where the sequences' keys and values exceed what L2 holds, this goes group by
 // group of consecutive sequences that fit: over all sixteen prompts of a 16 x
-// 2048 prefill at once (134 MB) the kernel read 1.6 GB from HBM instead of 0.4
-// and took 606 us instead of 577, at its power limit.
+// 2048 prefill at once (134 MB) the kernel read 1.6 GB from HBM instead of 0.7
+// and took 606 us instead of 577, at its power limit.  A batch of up to 64 MB is
+// one group; the groups of a larger one have 48 MB, so that the queries and
+// outputs that stream past leave them there (16 x 2048 at the power limit: 637
+// us with 64 MB, 621 with 48, 621 with 32, 639 with 24; 32 x 2048: 1272, 1248,
+// 1244, 1266; 20 of 200 to 4000: 984, 983, 1000, 1007).
 //
 // Long contexts with few rows are split over the keys (paged caches only):
 // the splits' unnormalised outputs, maxima and sums go to the workspace and
@@ -111,7 +115,7 @@ struct Params {
   int splits;
   int split_blocks;  // key blocks of a split
   int few;         // sequences of up to so many tokens go to the few-rows kernel
-  int64_t group_keys;  // keys whose rows, of all KV heads, L2 holds
+  int64_t group_keys;  // keys whose rows, of all KV heads, are 64 MB (half of L2)
   int take_over;   // whether there are more CTAs than run at once
   int boxes;       // whether a warp's 32 rows are a box of the output's map
   int behind_few;  // launched over the few-rows kernel of the same call
@@ -306,7 +310,7 @@ __device__ void schedule_units(const Params &p, Shared &sh) {
           const int64_t y = __shfl_up_sync(kFull, sum, w);
           if (lane >= w) sum += y;
         }
-        const bool in = i < live && (keys + sum <= p.group_keys || i == s0);
+        const bool in = i < live && (keys + sum <= p.group_keys / 4 * 3 || i == s0);
         const int many = __popc(__ballot_sync(kFull, in));
         if (in) {
           int c, l;
@@ -1865,7 +1869,7 @@ void set_heads(tide::ragged::Params &p, int64_t hq, int64_t hkv, int64_t d, floa
   p.splits = 1;
   p.split_blocks = 1 << 24;  // all of them
   p.few = 0;
-  p.group_keys = (64 << 20) / (hkv * d * 4);  // half of the 126 MB
+  p.group_keys = (64 << 20) / (hkv * d * 4);
 }
 
 }  // namespace
