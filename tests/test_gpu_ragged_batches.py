@@ -209,3 +209,35 @@ def test_bad_arguments_leave_the_stream_usable():
             call()
     out = run_packed(q, k, v, [8])
     check_attention(out, *packed_reference(q, k, v, [8], None, 0.125), 8, 64, torch.bfloat16)
+
+
+def test_rows_that_overlap_are_refused():
+    """An expanded tensor's rows lie in one place (stride 0)."""
+    q, k, v = rows(8, 4, 2, 64, torch.bfloat16, 1, False)
+    same = {n: t[:1].expand(8, -1, -1) for n, t in (("q", q), ("k", k), ("v", v))}
+    out, cu = torch.zeros_like(q), i32([0, 8])
+    for a in ((same["q"], k, v), (q, same["k"], same["v"])):
+        with pytest.raises(RuntimeError, match="overlap"):
+            _native.ops().packed_attention(*a, cu, None, out, 0.125, None)
+    kc = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16, device=DEV)
+    slots = torch.arange(8, device=DEV)
+    with pytest.raises(RuntimeError, match="overlap"):
+        _native.ops().paged_append(same["k"], same["v"], slots, None, None, kc, kc.clone(), None)
+    with pytest.raises(RuntimeError, match="overlap"):
+        _native.ops().paged_attention(same["q"], kc, kc, i32([[0]] * 8), i32([1] * 8), None, None, out,
+                                      16, 0.125, None)
+    assert not out.any() and not kc.any()
+
+
+@pytest.mark.parametrize("group,hkv,d", [(2, 3, 128), (32, 2, 64), (64, 1, 128), (96, 2, 64), (16, 1, 128)])
+def test_packed_attention_whole_tiles(group, hkv, d):
+    """Sequences that fill tiles (their outputs leave as boxes) and do not."""
+    lens = [128, 200, 1, 64]
+    q, k, v = rows(sum(lens), group * hkv, hkv, d, torch.bfloat16, group)
+    out = torch.full_like(q.contiguous(), 7.0)
+    tail = torch.full((3, *out.shape[1:]), 7.0, dtype=out.dtype, device=DEV)
+    out = torch.cat([out, tail])
+    _native.ops().packed_attention(torch.cat([q, q[:3]]), torch.cat([k, k[:3]]), torch.cat([v, v[:3]]),
+                                   i32(starts(lens)), None, out, d ** -0.5, None)
+    check_attention(out[:-3], *packed_reference(q, k, v, lens, None, d ** -0.5), 200, d, torch.bfloat16)
+    assert bool((out[-3:] == 7).all())

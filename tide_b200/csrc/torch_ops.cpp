@@ -603,7 +603,11 @@ int64_t packed_heads(const at::Tensor &t, const char *name) {
   TORCH_CHECK(t.is_cuda() && t.dim() == 3, name, " must be a CUDA tensor [n, heads, d]");
   TORCH_CHECK((t.size(2) <= 1 || t.stride(2) == 1) && (t.size(1) <= 1 || t.stride(1) == t.size(2)),
               name, ": heads must be packed in each row");
-  return t.size(0) <= 1 ? t.size(1) * t.size(2) : t.stride(0);
+  const int64_t width = t.size(1) * t.size(2);
+  // (an expanded tensor's rows all lie in one place: stride 0, which the C entry
+  // points take for packed rows)
+  TORCH_CHECK(t.size(0) <= 1 || t.stride(0) >= width, name, ": rows must not overlap");
+  return t.size(0) <= 1 ? width : t.stride(0);
 }
 
 void check_paged_caches(const at::Tensor &k_cache, const at::Tensor &v_cache, int64_t hkv, int64_t d,
