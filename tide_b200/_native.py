@@ -17,6 +17,7 @@ EXT_PATH = PKG / "_C.so"
 _lock = threading.Lock()
 _lib = None
 _ops_loaded = False
+_namespace = None  # torch.ops.tide, once the operators are registered
 
 
 class NativeMissing(RuntimeError):
@@ -38,14 +39,17 @@ def lib() -> ctypes.CDLL:
 
 def ops():
     """torch.ops.tide with the CUDA operators registered, loaded once."""
-    global _ops_loaded
+    global _ops_loaded, _namespace
+    if _namespace is not None:  # (without the lock: half a microsecond of a call)
+        return _namespace
     with _lock:
         if not _ops_loaded:
             if not EXT_PATH.exists():
                 raise NativeMissing(f"{EXT_PATH} is missing: build it with `python tide_b200/build.py`")
             torch.ops.load_library(str(EXT_PATH))
             _ops_loaded = True
-    return torch.ops.tide
+        _namespace = torch.ops.tide
+    return _namespace
 
 
 def require_cuda(t: torch.Tensor, what: str) -> None:
