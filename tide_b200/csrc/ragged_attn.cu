@@ -56,7 +56,7 @@
 // level come from counting over the sequences, so no list of units is built.
 // Where the sequences' keys and values exceed what L2 holds, this goes group by
 // group of consecutive sequences that fit: over all sixteen prompts of a 16 x
-// 2048 prefill at once (134 MB) the kernel read 1.6 GB from HBM instead of 0.7
+// 2048 prefill at once (134 MB) the kernel read 1.6 GB from HBM instead of 0.5
 // and took 606 us instead of 577, at its power limit.  A batch of up to 64 MB is
 // one group; the groups of a larger one have 48 MB, so that the queries and
 // outputs that stream past leave them there (16 x 2048 at the power limit: 637
