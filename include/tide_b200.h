@@ -305,8 +305,8 @@ int tide_silu_mul(int dtype, const void *gate, const void *up, void *out, int64_
  * left as they were, and sets TIDE_DEVERR_POSITION; a page outside
  * [0, n_pages) reads as zeros and sets it too.  A NaN or infinity in a value
  * row reaches the tokens that see that row, and no others (the weights are
- * rounded to the rows' type: an infinity whose weight rounds to 0, below 2^-24
- * of the largest in fp16, arrives as a NaN). */
+ * rounded to the rows' type: an infinity whose weight rounds to 0, 2^-32 of the
+ * largest or less in fp16, arrives as a NaN). */
 int tide_packed_attention(int dtype, const void *q, const void *k, const void *v,
                           int64_t q_row_stride, int64_t kv_row_stride, const int32_t *cu_seqlens,
                           int64_t n_seqs, const int32_t *zero_keys, void *out, int64_t n_tokens,

@@ -12,10 +12,10 @@
 // tile,
 //   S[128 x 128] = Q K^T      tcgen05.mma, operands in shared memory (TMA,
 //                             128-byte swizzle), S in tensor memory;
-//   P = 2^(S qs - m)          one thread per row: running maximum m and sum l,
-//                             P rounded to the rows' 16-bit type (half a step
-//                             of it relative per weight; the sum l is of the
-//                             unrounded ones) and written over a half of S;
+//   P = 2^(S qs - m + c)      one thread per row: running maximum m and sum l,
+//                             P rounded to the rows' 16-bit type (the sum l is
+//                             of the unrounded ones) and written over a half of
+//                             S; c = 7 for fp16, 0 for bf16 (kLift);
 //   O[128 x D] += P V         tcgen05.mma with P from tensor memory and V as
 //                             it lies in shared memory (its MN-major operand).
 // The chain of a tile (scores, softmax, values, the next scores) is longer than
@@ -27,10 +27,17 @@
 // run, and a unit's first scores are made while the one before is written out.
 //
 // m is only raised, and O and l rescaled, when a row's maximum has grown by
-// more than 2^8 since: weights up to 256 cost nothing (fp32 sums; 16-bit
-// floats round relatively), and O stays where it is.  So a block's weights are
-// made with m as it was, its maximum beside them, and made again in the rare
-// case that m is raised.
+// more than 2^8 since: larger weights cost nothing (fp32 sums), and O stays
+// where it is.  So a block's weights are made with m as it was, its maximum
+// beside them, and made again in the rare case that m is raised.
+//
+// A weight is off by half a step of its 16-bit type, relatively, as long as it
+// is a normal number there.  For bf16 that is any weight that 32 bits hold.
+// fp16 ends at 2^-14: a row whose largest weight lies on a key of small value
+// takes its output from the others, and weights of 2^-25 and below, 40000 of
+// which are 1e-3 of the row, would be rounded to nothing.  So fp16 weights, and
+// with them l and the zero keys' share of it, are 2^7 times as large: the
+// largest 2^(8 + 7), and half a subnormal step 2^-32 of a weight at m.
 //
 // What bounds it: that chain.  The products take 1390 cycles of a tile's 3130
 // per block (16 of 67 cycles, and the latency of two commits), the softmax the
@@ -89,6 +96,11 @@ constexpr int kReaders = 11; // warps that read the units: all but the one that 
 constexpr int kThreads = 32 * kWarps;
 constexpr int kCached = 4;   // sequences per lane that the unit search keeps in registers
 constexpr float kSlack = 8.f;  // log2 of how far a maximum may grow before a rescale
+// log2 of what the weights, and their sums, are multiplied by (see above)
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f;
+template <typename T>
+constexpr float kLifted = std::is_same<T, __half>::value ? 128.f : 1.f;  // 2^kLift
 
 template <int D>
 struct Shape {
@@ -715,6 +727,18 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+// The same for weights.  Those of fp16 stop at its largest number: scores past
+// 2^24, which 32 bits hold to a step of 2 and more, may be that much above m + 8.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+  } else {
+    return pack2<T>(lo, hi);
+  }
+}
 
 // The values that the cleaner zeroed in the positions that this row sees, for
 // the columns [d0, d0 + 32): weight > 0 times a NaN or infinity is itself.
@@ -797,7 +821,7 @@ __device__ __forceinline__ void weigh_quarter(const float *s, uint64_t qs2, uint
     a = ex2(a);
     b = ex2(b);
     sum[i & 1] = add2(sum[i & 1], pair(a, b));
-    w[i] = pack2<T>(a, b);
+    w[i] = pack_weights<T>(a, b);
   }
   ptx::tmem_st16(p_col, w);
 }
@@ -828,7 +852,7 @@ __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem,
     if (p.zero_keys && valid) {  // keys of score 0 whose values add nothing
       const int z = max(__ldg(p.zero_keys + row), 0);
       if (z) m = 0.f;
-      l = (float)z;
+      l = (float)z * kLifted<T>;
     }
     for (int j = u.b0; j < end; ++j, ++ns) {
       TIDE_WAIT(&sh.s_full[t], ns & 1);
@@ -861,7 +885,7 @@ __device__ void softmax_tile(const Params &p, Shared &sh, int t, uint32_t tmem,
       uint64_t sum[2], qs2, mq2;
       float mx[2];
       auto weigh = [&] {  // S is in registers: P takes its upper half
-        const float mq = m == -INFINITY ? 0.f : m * p.qs;
+        const float mq = (m == -INFINITY ? 0.f : m * p.qs) - kLift<T>;
         qs2 = pair(p.qs, p.qs), mq2 = pair(-mq, -mq);
         sum[0] = sum[1] = 0;
         mx[0] = mx[1] = -INFINITY;
@@ -1359,13 +1383,13 @@ __global__ void __launch_bounds__(32 * kFewWarps, NT <= 2 ? 3 : 2)
         a[e] = up ? ex2((m[nt][e] - t) * p.qs) : 1.f;
         if (up) m[nt][e] = t;
         raise |= up;
-        const float mq = m[nt][e] == -INFINITY ? 0.f : m[nt][e] * p.qs;
+        const float mq = (m[nt][e] == -INFINITY ? 0.f : m[nt][e] * p.qs) - kLift<T>;
         x[e] = ex2(fmaf(sc[nt][e], p.qs, -mq));
         x[2 + e] = ex2(fmaf(sc[nt][2 + e], p.qs, -mq));
         l[nt][e] = fmaf(l[nt][e], a[e], x[e] + x[2 + e]);
       }
-      pt[nt][0] = transpose8x8(pack2<T>(x[0], x[1]));
-      pt[nt][1] = transpose8x8(pack2<T>(x[2], x[3]));
+      pt[nt][0] = transpose8x8(pack_weights<T>(x[0], x[1]));
+      pt[nt][1] = transpose8x8(pack_weights<T>(x[2], x[3]));
       if (__any_sync(kFull, raise)) {
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) {
