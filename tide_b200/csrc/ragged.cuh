@@ -34,6 +34,14 @@ __device__ __forceinline__ int live_sequences(const RaggedBatch &b) {
   return min(max(n, 0), b.n_seqs);
 }
 
+// Rows [*row0, *end) of sequence i; false for bounds that are out of order or
+// outside the rows.
+__device__ __forceinline__ bool sequence_bounds(const RaggedBatch &b, int i, int *row0, int *end) {
+  *row0 = __ldg(b.cu + i);
+  *end = __ldg(b.cu + i + 1);
+  return *row0 >= 0 && *end >= *row0 && *end <= b.n_tokens;
+}
+
 // Sequence i of the batch; one with bad bounds, request or length is empty
 // and raises TIDE_DEVERR_POSITION.
 __device__ __forceinline__ Sequence sequence(const RaggedBatch &b, int i) {
@@ -41,12 +49,11 @@ __device__ __forceinline__ Sequence sequence(const RaggedBatch &b, int i) {
   s.row0 = i;
   s.n = 1;
   if (b.cu) {
-    s.row0 = __ldg(b.cu + i);
-    const int end = __ldg(b.cu + i + 1);
-    s.n = end - s.row0;
-    if (s.row0 < 0 || end < s.row0 || end > b.n_tokens) {
+    int end;
+    const bool good = sequence_bounds(b, i, &s.row0, &end);
+    s.n = good ? end - s.row0 : 0;
+    if (!good) {
       raise_error(b.err, TIDE_DEVERR_POSITION);
-      s.n = 0;
       s.row0 = 0;
     }
   }
@@ -64,18 +71,29 @@ __device__ __forceinline__ Sequence sequence(const RaggedBatch &b, int i) {
   return s;
 }
 
-// The sequence that holds packed row `row`, or -1: the last one whose start
-// is at or before it (a scan, so that offsets out of order cannot hide one).
+// The sequence that holds packed row `row`, or -1; the same for a whole warp.
+// Offsets in order: the last sequence whose start is at or before the row.  Where
+// that one does not hold it (a row of no sequence, or offsets out of order, among
+// which such a search can miss the row's), the first of all that does.
 __device__ __forceinline__ int sequence_of_row(const RaggedBatch &b, int live, int row) {
   if (!b.cu) return row < live ? row : -1;
+  auto holds = [&](int i) {
+    int row0, end;
+    return sequence_bounds(b, i, &row0, &end) && row0 <= row && row < end;
+  };
   int lo = 0, hi = live;  // cu[lo] <= row < cu[hi], if sorted
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (__ldg(b.cu + mid) <= row) lo = mid;
     else hi = mid;
   }
-  if (lo >= live) return -1;
-  return __ldg(b.cu + lo) <= row && row < __ldg(b.cu + lo + 1) ? lo : -1;
+  if (lo < live && holds(lo)) return lo;
+  const int lane = threadIdx.x & 31;
+  for (int base = 0; base < live; base += 32) {
+    const unsigned who = __ballot_sync(0xffffffffu, base + lane < live && holds(base + lane));
+    if (who) return base + __ffs(who) - 1;
+  }
+  return -1;
 }
 
 // Where the keys are: rows of a packed tensor, or pages.
