@@ -49,3 +49,13 @@ def test_rows_behind_the_last_sequence_and_a_start_past_the_first_row(max_kv):
     ref = [x[20:60] for x in paged_reference(q, kc, vc, tables, lens, new, ids, 128 ** -0.5)]
     check_attention(out[20:60], *ref, max(lens), 128, q.dtype)
     assert bool((out[:20] == 7).all()) and bool((out[60:] == 7).all()) and int(err) == 0
+
+
+@pytest.mark.parametrize("max_kv", [104, 4000])
+@pytest.mark.parametrize("cu,fine", [
+    ([0, 1, 5000], [0]), ([0, 1, -3], [0]), ([2, 1, 2], [1]), ([-1, 1, 2], [1]), ([0, 1, 3], [0])], ids=str)
+def test_few_rows_flag_a_bad_sequence(max_kv, cu, fine):
+    """Sequences of which two CTAs take one each, and no other kernel runs."""
+    new = [1, 1]
+    case = paged_case(new, [100, 60], 16, 1, 128, torch.bfloat16, 16, 5)
+    served(*case[:4], case[4], new, case[5], cu, max_kv, fine)

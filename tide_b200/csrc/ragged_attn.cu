@@ -1228,8 +1228,12 @@ __global__ void __launch_bounds__(32 * kFewWarps, NT <= 2 ? 3 : 2)
     for (int b = 0; b < live && found < 0; b += 32) {
       int mine = 0;
       if (b + lane < live) {
-        const int n = __ldg(p.batch.cu + b + lane + 1) - __ldg(p.batch.cu + b + lane);
-        mine = n > 0 && n <= p.few ? (n + p.tokens - 1) / p.tokens : 0;
+        int row, end;
+        const bool good = sequence_bounds(p.batch, b + lane, &row, &end);
+        // (one that has no piece here, and with that no CTA to flag it)
+        if (!good) raise_error(p.batch.err, TIDE_DEVERR_POSITION);
+        const int n = good ? end - row : 0;
+        mine = n <= p.few ? (n + p.tokens - 1) / p.tokens : 0;
       }
       int upto = mine;
 #pragma unroll
