@@ -316,7 +316,16 @@ class TIDERuntime(nn.Module):
         Llama-family models with head_dim 128, bf16/fp16.  With paged=True as
         well they decode on a paged cache (tide_b200.paged.PagedLiveDecoder),
         each row from the tokens that `attention_mask` (zeros: padding, left
-        or right) leaves of it; the other modes take no mask."""
+        or right) leaves of it.  live=True without paged=True refuses a mask
+        with zeros; the reference's loop, which takes no mask, warns that the
+        padding counts as tokens there."""
+        paged, mask = kwargs.get("paged", False), kwargs.get("attention_mask")
+        if mask is not None and not (live and paged) and not bool(mask.bool().all()):
+            if live:
+                raise ValueError("generate(live=True) takes an attention_mask with zeros on the paged "
+                                 "cache only: pass paged=True")
+            logger.warning("generate takes an attention_mask with live=True and paged=True only: "
+                           "its padding counts as tokens here")
         eos = kwargs.get("eos_token_id", 2)
         B = input_ids.shape[0]
         dev = input_ids.device
@@ -328,9 +337,9 @@ class TIDERuntime(nn.Module):
             from tide_b200.paged import PagedLiveDecoder
 
             room, graph = input_ids.shape[1] + max_new_tokens + 1, kwargs.get("live_graph", True)
-            if kwargs.get("paged", False):
+            if paged:
                 dec = PagedLiveDecoder(self, B, room, graph=graph)
-                next_logits = dec.prefill(input_ids, kwargs.get("attention_mask"))
+                next_logits = dec.prefill(input_ids, mask)
             else:
                 dec = LiveDecoder(self, B, room, graph=graph)
                 next_logits = dec.prefill(input_ids)
