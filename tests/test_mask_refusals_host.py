@@ -59,3 +59,10 @@ def test_generate_says_that_padding_counts_as_tokens(monkeypatch, per_row):
     with pytest.raises(Reached):
         generate(attention_mask=MASK, per_row_exit=per_row)
     assert len(said) == 1 and "padding" in said[0]
+
+
+def test_generate_refuses_the_paged_cache_without_live():
+    with pytest.raises(ValueError, match="live=True"):
+        generate(paged=True)
+    with pytest.raises(Reached):
+        generate(paged=False)

@@ -320,6 +320,8 @@ class TIDERuntime(nn.Module):
         with zeros; the reference's loop, which takes no mask, warns that the
         padding counts as tokens there."""
         paged, mask = kwargs.get("paged", False), kwargs.get("attention_mask")
+        if paged and not live:
+            raise ValueError("generate(paged=True) is a form of live decoding: pass live=True")
         if mask is not None and not (live and paged) and not bool(mask.bool().all()):
             if live:
                 raise ValueError("generate(live=True) takes an attention_mask with zeros on the paged "
