@@ -66,3 +66,18 @@ def test_generate_refuses_the_paged_cache_without_live():
         generate(paged=True)
     with pytest.raises(Reached):
         generate(paged=False)
+
+
+@pytest.mark.parametrize("config,kw", [({}, {}), ({}, dict(live=False)),
+                                       (dict(live_compaction=True), dict(live=False))])
+def test_forward_refuses_packed_without_live(config, kw):
+    with pytest.raises(ValueError, match="live"):
+        forward(config, packed=True, **kw)
+    with pytest.raises(Reached):
+        forward(config, packed=False, **kw)
+
+
+@pytest.mark.parametrize("config,kw", [({}, dict(live=True)), (dict(live_compaction=True), {})])
+def test_forward_takes_packed_with_live(config, kw):
+    with pytest.raises(Reached):
+        forward(config, packed=True, **kw)

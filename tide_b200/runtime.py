@@ -256,7 +256,12 @@ class TIDERuntime(nn.Module):
         lm_head runs on the rows whose logits are used, e.g. 1 before
         sampling."""
         B, S = input_ids.shape
-        if live if live is not None else self.config.live_compaction:
+        if live is None:
+            live = self.config.live_compaction
+        if packed and not live:
+            raise ValueError("packed=True is a form of the live forward: pass live=True (or set "
+                             "config.live_compaction)")
+        if live:
             from tide_b200.live import live_forward
 
             out_buf, stats, exit_layer = live_forward(self, input_ids, attention_mask, packed=packed)
