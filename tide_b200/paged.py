@@ -198,6 +198,7 @@ class PagedLiveDecoder(LiveDecoder):
                              "new_lens adds up to")
         lens = self._take([0 if o else n for o, n in zip(over, self.lengths)], new)
         n = sum(new)
+        tokens = tokens.reshape(1, -1).to(self.dev)
         slot_map = torch.empty(max(n, 1), dtype=torch.int64, device=self.dev)
         positions = torch.empty_like(slot_map)
         self.cache.advance(self._i32(new), slot_map, positions, self._i32([int(o) for o in over]))
@@ -205,7 +206,7 @@ class PagedLiveDecoder(LiveDecoder):
         if n == 0:
             return None
         places = torch.arange(n, dtype=torch.int32, device=self.dev)
-        h = self.fam.embed_tokens(tokens.view(1, -1).to(self.dev))
+        h = self.fam.embed_tokens(tokens)
         for i in range(len(self.fam.layers)):
             q, k, v = self._qkv(i, h, positions, places, None)
             self.cache.append(i, k, v, slot_map)
