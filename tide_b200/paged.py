@@ -189,7 +189,9 @@ class PagedLiveDecoder(LiveDecoder):
         every request r, after the requests with done[r] have given their
         pages back and started over; every layer, no exits.  Returns the
         logits of each request's last new token [n_requests, V] (zeros for one
-        without any), or None when there are no tokens at all."""
+        without any), or None when there are no tokens at all.  Raises if a
+        kernel has flagged a device error (what the call has added to the
+        requests is then not to be used: they start over with done)."""
         new = [int(n) for n in new_lens]
         over = [False] * self.n_slots if done is None else [bool(d) for d in done]
         if len(new) != self.n_slots or len(over) != self.n_slots or min(new) < 0 \
@@ -214,7 +216,9 @@ class PagedLiveDecoder(LiveDecoder):
             h = self._rest(i, h, o, None)
         got = [r for r in range(self.n_slots) if new[r]]
         ends = torch.cumsum(torch.tensor(new), 0)[got] - 1
-        logits = self.rt._lm_head(self.fam.norm(h.index_select(0, ends.to(self.dev))))
+        ends = ends.to(self.dev)  # (waits for the layers)
+        self.runner.check_errors()
+        logits = self.rt._lm_head(self.fam.norm(h.index_select(0, ends)))
         if len(got) == self.n_slots:
             return logits
         full = logits.new_zeros(self.n_slots, logits.shape[1])
