@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(kThreads) page_tables_kernel(const __grid_cons
   n_free = min(max(n_free, 0), p.n_pages);
   __syncthreads();
 
-  // 1. prefix sums; the pages of the requests that are done, a share per CTA
+  // 1. prefix sums; the pages of the requests that are done, a warp a request
   long long carry[3] = {0, 0, 0};  // tokens, pages needed, pages returned
   for (int base = 0; base < p.n_req; base += kThreads) {
     const int r = base + tid;

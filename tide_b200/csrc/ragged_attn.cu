@@ -42,11 +42,13 @@
 // What bounds it: that chain.  The products take 1390 cycles of a tile's 3130
 // per block (16 of 67 cycles, and the latency of two commits), the softmax the
 // rest (128 exponentials a row and thread, at 16 a cycle and SM); the tensor
-// cores work 65 % of the time.  A GPU at its power limit then runs this at some
-// 1.6 GHz.  bf16, 32 query heads on 8 KV heads of 128: 16 prompts of 2048 in 533
-// us (1030 TFLOP/s), one of 16384 in 1.72 to 1.88 ms (1280 to 1170), 2048 tokens
-// over 26003 paged keys in 780 us (1160); a unit costs 4000 cycles besides its
-// blocks.
+// cores work 65 % of the time while a unit's blocks go by, and 50 % of the whole
+// prefill below (a unit costs 4000 cycles besides its blocks, and half of a
+// diagonal block is masked).  A GPU at its power limit runs this at 1.6 to 1.7
+// GHz, which it reaches after a few calls.  bf16, 32 query heads on 8 KV heads
+// of 128, four calls in a row and 2000: 16 prompts of 2048 in 532 and 620 us
+// (1030 and 887 TFLOP/s), one of 16384 in 1.72 and 1.99 ms (1280 and 1105), 2048
+// tokens over 26003 paged keys in 800 and 895 us (1130 and 1010).
 //
 // Roles of the warps: 0-3 and 4-7 the softmax and the output of tile 0
 // and 1; 8 finds the units; 9 loads; 10 issues the products; 11 cleans the
@@ -127,7 +129,8 @@ struct Params {
   int splits;
   int split_blocks;  // key blocks of a split
   int few;         // sequences of up to so many tokens go to the few-rows kernel
-  int64_t group_keys;  // keys whose rows, of all KV heads, are 64 MB (half of L2)
+  int64_t group_keys;  // keys whose rows, of all KV heads, are 64 MB: up to so many are
+                       // one group; three quarters of them are a group of a larger batch
   int take_over;   // whether there are more CTAs than run at once
   int boxes;       // whether a warp's 32 rows are a box of the output's map
   int behind_few;  // launched over the few-rows kernel of the same call
@@ -1114,8 +1117,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // decode step, a few drafted tokens.  Such a unit reads 4 D bytes per key and
 // does 4 D flops per key and row, so it is bound by HBM, and the 128-row tiles
 // above would leave it to one chain of products and exponentials per SM.  A
-// CTA takes 8 NT rows; a sequence with more (up to four such groups) has
-// several, which share their keys through L2.  A warp is on its own: it walks over
+// CTA takes 8 NT rows; a sequence with more, up to twice as many, has two, which
+// share their keys through L2.  A warp is on its own: it walks over
 // every fourth group of 16 keys of its CTA's share, with its own ring of TMA
 // copies (8 KB a group, three in flight) and its own running maxima, sums and
 // outputs, and the four meet once at the end.  No barrier but the ring's.
