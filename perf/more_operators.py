@@ -91,7 +91,7 @@ def draw(rng):
             c.update(tokens=_log(rng, 1, 32768), spare=_log(rng, 1, 300))
         if op == "append":
             c.update(live=rng.choice([1.0, 0.6]), hq=hq, norm=rng.random() < 0.5,
-                     rotate=rng.random() < 0.8, far=_log(rng, 1, 130000))
+                     rotate=rng.random() < 0.8, far=rng.choice([0, _log(rng, 1, 130000)]))
         if op == "read":
             c.update(hole=rng.choice([0.0, 0.1]))
         if op != "attend" or _fits(c):
@@ -249,6 +249,12 @@ def _filled(pages, c, g):
     return cache
 
 
+def _paged_slots(n, pages, page, g):
+    """The slots of n tokens that fill pages of the pool one after the other."""
+    at = torch.randperm(pages, generator=g, device=DEV)[:-(-n // page)]
+    return (at[:, None] * page + torch.arange(page, device=DEV)).view(-1)[:n]
+
+
 def _prepare_append(c, g):
     dt, d, hq, hkv, m = DTYPES[c["dtype"]], c["d"], c["hq"], c["hkv"], c["tokens"]
     n = _alive(c, m)
@@ -256,14 +262,17 @@ def _prepare_append(c, g):
     # q, k and v: column slices of one projection's output
     x = torch.cat([torch.randn(n, hq * d, generator=g, device=DEV), _keys((n, hkv * d), g),
                    torch.randn(n, hkv * d, generator=g, device=DEV)], 1).to(dt)
-    slots = torch.randperm(pages * c["page"], generator=g, device=DEV)[:m]
+    if c["far"]:  # a token each of many requests
+        slots = torch.randperm(pages * c["page"], generator=g, device=DEV)[:m]
+    else:  # prompts: page after page
+        slots = _paged_slots(m, pages, c["page"], g)
     rows = None
     if n < m:  # the rows that are still active, in order
         rows = torch.randperm(m, generator=g, device=DEV)[:n].sort()[0].to(torch.int32)
     freq = 1.0 / (500000.0 ** (torch.arange(0, d, 2, device=DEV).double() / d))
     w = [(1 + 0.2 * torch.randn(d, generator=g, device=DEV)).to(dt) for _ in range(2)]
     start = torch.randint(0, c["far"] + 1, (m,), generator=g, device=DEV)
-    where = torch.arange(m, device=DEV) % 2048 if c["far"] == 0 else start
+    where = start if c["far"] else torch.arange(m, device=DEV) % 2048
     # the slots whose tokens this pass has written, which it reads back
     mine = slots if rows is None else slots[rows.long()]
     return dict(
@@ -280,8 +289,7 @@ def _prepare_append(c, g):
 def _prepare_read(c, g):
     dt, n = DTYPES[c["dtype"]], c["tokens"]
     pages = -(-n // c["page"]) + c["spare"]
-    slots = torch.randperm(pages, generator=g, device=DEV)[:-(-n // c["page"])]
-    slots = (slots[:, None] * c["page"] + torch.arange(c["page"], device=DEV)).view(-1)[:n]
+    slots = _paged_slots(n, pages, c["page"], g)
     if c["hole"]:
         slots = torch.where(torch.rand(n, generator=g, device=DEV) < c["hole"], -1, slots)
     return dict(cache=_filled(pages, c, g), mine=slots.contiguous(),
