@@ -340,6 +340,79 @@ int tide_paged_append(int dtype, const void *k_new, const void *v_new, int64_t k
                       int64_t head_dim, void *k_cache, void *v_cache, int64_t n_pages,
                       int64_t page_size, int32_t *error_word, tide_stream_t stream);
 
+/* ---- a paged cache in 4 bits -------------------------------------------- */
+/*
+ * The same pages with keys and values in 4.5 bits each, for bf16 and fp16 rows.
+ * A group is 32 neighbouring channels of a token's key or value in one head;
+ * it has codes c and a zero point z in 0..15 and a scale s, and stands for
+ * (c - z) s, which both 16-bit types hold exactly.  With lo and hi the group's
+ * least and largest value, 0 among them, and t = (hi - lo) / 15:
+ *   s = t rounded up to four significant bits (0 for a group of zeros, else at
+ *   least 2^-120, 2^-21 for fp16 rows),  z = round(-lo / s),
+ *   c = min(max(round(x / s) + z, 0), 15)    (ties to even).
+ * So a value is off by s / 2 at most (by s where s / 2 more would pass the rows'
+ * largest number), and zero is held as zero.  A group with a value that is not
+ * finite reads as NaN.
+ *
+ * The cache is [n_pages, n_kv_heads, page_size / 16, 18 head_dim] bytes.  The 18
+ * head_dim bytes of 16 tokens of a head: the codes of the keys
+ * [16, head_dim / 2], of the values, the scales of the keys [head_dim / 32,
+ * token % 4, token / 4] of 16 bits, of the values.  Eight channels are 32 bits
+ * (little-endian), four each, lowest first channels 0, 2, 4, 6, 1, 3, 5, 7.  A
+ * scale is a bf16 with z in its last four bits.  All bytes zero is a cache of
+ * zeros.
+ *
+ * tide_paged_append_q4: keys and values of new tokens into it, as
+ * tide_paged_append, with what comes before on the way.  Row i is entry m =
+ * row_ids[i] (i when NULL) of slot_map and positions.  k_new row i, with its
+ * heads' RMSNorm (k_norm_weight [head_dim] of the rows' type, or NULL: none)
+ * and turned by its position (inv_freq [head_dim / 2] fp32, or NULL: not),
+ *   y = x * rsqrt(mean(x^2) + eps) * w,
+ *   out[j] = y[j] cos a - y[j + d/2] sin a,  out[j + d/2] = y[j + d/2] cos a +
+ *   y[j] sin a,  a = positions[m] * inv_freq[j],  cos and sin times
+ *   attention_scaling,
+ * goes to slot slot_map[m] with v_new row i as it is.  q row i (optional, with
+ * q_norm_weight) is treated likewise and goes to row i of q_out [n_rows,
+ * n_q_heads, head_dim], whatever its slot; rows not below *n_rows_dev, and
+ * those of a row id outside [0, n_slot_map), are left.  Nothing is rounded on
+ * the way: q once to its type, k once to 32 bits before its codes are made, the
+ * angle being taken in 64 bits.  q, k_new and v_new all NULL write zeros.
+ * Slots and row ids as in tide_paged_append; no slot may be named twice in a
+ * call.  page_size a multiple of 16.
+ *
+ * tide_paged_read_q4: the key and value at slots[i] to row i of k_out and v_out
+ * [n_rows, n_kv_heads, head_dim]; a row with slot -1 is left as it was, one
+ * with a slot outside the cache too (TIDE_DEVERR_POSITION).
+ *
+ * tide_paged_attention_q4: tide_paged_attention over it, with the same
+ * arguments and rules.  A key or value group that reads as NaN reaches the tokens
+ * that see it, and no others. */
+int tide_paged_append_q4(int dtype, const void *q, int64_t q_row_stride, const void *k_new,
+                         const void *v_new, int64_t kv_row_stride, const void *q_norm_weight,
+                         const void *k_norm_weight, float eps, const float *inv_freq,
+                         float attention_scaling, const int64_t *positions,
+                         const int64_t *slot_map, int64_t n_slot_map, const int32_t *row_ids,
+                         const int32_t *n_rows_dev, int64_t n_rows, int64_t n_q_heads,
+                         int64_t n_kv_heads, int64_t head_dim, void *q_out, void *cache,
+                         int64_t n_pages, int64_t page_size, int32_t *error_word,
+                         tide_stream_t stream);
+int tide_paged_read_q4(int dtype, const void *cache, int64_t n_pages, int64_t page_size,
+                       const int64_t *slots, int64_t n_rows, int64_t n_kv_heads, int64_t head_dim,
+                       void *k_out, void *v_out, int32_t *error_word, tide_stream_t stream);
+size_t tide_paged_attention_q4_workspace_size(int64_t n_tokens, int64_t n_seqs, int64_t n_requests,
+                                              int64_t n_q_heads, int64_t n_kv_heads,
+                                              int64_t head_dim, int64_t max_kv_len);
+int tide_paged_attention_q4(int dtype, const void *q, int64_t q_row_stride, const void *cache,
+                            int64_t n_pages, int64_t page_size, const int32_t *block_tables,
+                            int64_t max_pages, int64_t n_requests, const int32_t *kv_lens,
+                            const int32_t *cu_seqlens, const int32_t *seq_ids, int64_t n_seqs,
+                            const int32_t *n_seqs_dev, void *out, int64_t n_tokens,
+                            int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim,
+                            int64_t max_kv_len, float scale, void *workspace,
+                            size_t workspace_bytes, int32_t *error_word, tide_stream_t stream);
+
+/* ---- page bookkeeping --------------------------------------------------- */
+
 /* The page bookkeeping of one step, from the requests' lengths:
  *   1. a request with done[r] != 0 (optional) gives back the pages of its
  *      context_lens[r] positions and starts over from length 0;

@@ -1,0 +1,127 @@
+"""The 4-bit cache without a GPU: its entry points reject bad arguments before any
+device call, and the format's restatement keeps its promises."""
+import pytest
+import torch
+
+from tests import q4_helpers as Q
+from tide_b200 import _native, capi
+
+P = 1 << 20  # an aligned address that no call below follows
+BAD, NOT_HERE, ALIGN = capi.ERR_INVALID, capi.ERR_UNSUPPORTED, capi.ERR_ALIGNMENT
+
+
+def append(**kw):
+    a = dict(dtype=capi.DTYPE_BF16, q=P, qs=0, k=P, v=P, stride=0, qw=None, kw=None, eps=1e-6, freq=P,
+             scaling=1.0, pos=P, slots=P, n_map=8, ids=None, live=None, n=8, hq=8, hkv=2, d=128,
+             q_out=P, cache=P, n_pages=4, page=16, err=None)
+    a.update(kw)
+    return _native.lib().tide_paged_append_q4(*a.values(), None)
+
+
+def read(**kw):
+    a = dict(dtype=capi.DTYPE_F16, cache=P, n_pages=4, page=16, slots=P, n=8, hkv=2, d=64, k=P, v=P,
+             err=None)
+    a.update(kw)
+    return _native.lib().tide_paged_read_q4(*a.values(), None)
+
+
+def attend(**kw):
+    a = dict(dtype=capi.DTYPE_BF16, q=P, qs=0, cache=P, n_pages=16, page=16, tables=P, width=8,
+             n_req=4, lens=P, cu=P, ids=None, n_seqs=2, live=None, out=P, n=8, hq=8, hkv=2, d=128,
+             max_kv=100, scale=0.1, ws=P, ws_bytes=1 << 40, err=None)
+    a.update(kw)
+    return _native.lib().tide_paged_attention_q4(*a.values(), None)
+
+
+@pytest.mark.parametrize("kw,rc", [
+    (dict(dtype=capi.DTYPE_F32), NOT_HERE), (dict(d=96), NOT_HERE), (dict(page=24), BAD),
+    (dict(page=0), BAD), (dict(n_pages=0), BAD), (dict(n_pages=1 << 31), BAD), (dict(hkv=0), BAD),
+    (dict(n=-1), BAD), (dict(n_map=7), BAD), (dict(n_map=-1, ids=P), BAD), (dict(hq=0), BAD),
+    (dict(qs=8 * 128 - 8), BAD), (dict(qs=8 * 128 + 4), BAD), (dict(stride=2 * 128 - 8), BAD),
+    (dict(stride=2 * 128 + 2), BAD), (dict(v=None), BAD), (dict(k=None), BAD),
+    (dict(k=None, v=None), BAD), (dict(q_out=None), BAD), (dict(pos=None), BAD), (dict(slots=None), BAD),
+    (dict(cache=None), BAD), (dict(cache=P + 8), ALIGN), (dict(q=P + 2), ALIGN), (dict(k=P + 8), ALIGN),
+    (dict(q_out=P + 4), ALIGN)])
+def test_append_refusals(kw, rc):
+    assert append(**kw) == rc
+    assert _native.lib().tide_last_error()
+
+
+@pytest.mark.parametrize("kw,rc", [
+    (dict(dtype=capi.DTYPE_F32), NOT_HERE), (dict(d=80), NOT_HERE), (dict(page=8), BAD),
+    (dict(n_pages=0), BAD), (dict(n=-1), BAD), (dict(hkv=0), BAD), (dict(slots=None), BAD),
+    (dict(k=None), BAD), (dict(v=P + 8), ALIGN), (dict(cache=P + 2), ALIGN)])
+def test_read_refusals(kw, rc):
+    assert read(**kw) == rc
+    assert _native.lib().tide_last_error()
+
+
+@pytest.mark.parametrize("kw,rc", [
+    (dict(dtype=capi.DTYPE_F32), NOT_HERE), (dict(d=256), NOT_HERE), (dict(hq=9), BAD),
+    (dict(hq=258), BAD), (dict(hkv=0), BAD), (dict(page=48), NOT_HERE), (dict(page=8), NOT_HERE),
+    (dict(max_kv=129), BAD), (dict(max_kv=-1), BAD), (dict(n_pages=0), NOT_HERE),
+    (dict(scale=0.0), BAD), (dict(scale=float("nan")), BAD), (dict(scale=float("inf")), BAD),
+    (dict(cu=None), BAD), (dict(n_seqs=5), BAD), (dict(n=-1), BAD), (dict(tables=None), BAD),
+    (dict(lens=None), BAD), (dict(out=None), BAD), (dict(cache=P + 8), ALIGN), (dict(q=P + 8), ALIGN),
+    (dict(qs=1020), BAD), (dict(ws=None), capi.ERR_WORKSPACE), (dict(ws_bytes=16), capi.ERR_WORKSPACE),
+    (dict(ws=P + 4), capi.ERR_WORKSPACE)])
+def test_attention_refusals(kw, rc):
+    kw = dict(dict(n=1000, max_kv=100), **kw)
+    assert attend(**kw) == rc
+    assert _native.lib().tide_last_error()
+
+
+def test_empty_calls_do_nothing():
+    assert append(n=0, q=None, k=None, v=None, slots=None) == capi.OK
+    assert read(n=0, cache=None) == capi.OK
+    assert attend(n=0, q=None) == capi.OK
+    assert attend(n_seqs=0, q=None) == capi.OK
+
+
+def test_operators_are_registered_and_have_no_cpu_kernel():
+    ops = _native.ops()
+    cache = torch.zeros(2, 1, 1, 18 * 64, dtype=torch.uint8)
+    k = torch.zeros(3, 1, 64, dtype=torch.float16)
+    slots = torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(NotImplementedError):
+        ops.paged_read_q4(cache, slots, k, k.clone(), None)
+    for name in ("paged_append_q4", "paged_attention_q4"):
+        assert hasattr(ops, name), name
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_values_are_near_and_of_the_rows_type(dtype):
+    """Within half a step of what was put in, exactly a number of the rows' type,
+    zero staying zero, for groups of one sign, of two, and of tiny numbers."""
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(40, 128, generator=g) * torch.logspace(-6, 3, 40)[:, None]
+    x[::3] = x[::3].abs()
+    x[1::5, 32:64] = 0
+    x = x.to(dtype)
+    c, z, s = Q.quantise(x, dtype)
+    v = Q.values(x, dtype)
+    assert torch.equal(v, v.to(dtype).double())
+    assert bool(((v - x.double()).abs().unflatten(-1, (-1, 32)) <= s[..., None] / 2).all())
+    assert bool((v[x == 0] == 0).all())
+    assert int(c.min()) >= 0 and int(c.max()) <= 15 and int(z.min()) >= 0 and int(z.max()) <= 15
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_packing_is_the_documented_layout(d):
+    g = torch.Generator().manual_seed(4)
+    k, v = (torch.randn(2, 3, 32, d, generator=g).to(torch.bfloat16) for _ in range(2))
+    cache = Q.pack(k, v, torch.bfloat16)
+    assert cache.shape == (2, 3, 2, 18 * d)
+    for page, head, token in ((0, 0, 0), (1, 2, 31), (1, 0, 18), (0, 1, 7)):
+        got = Q.token_values(cache, page, head, token, d)
+        for x, y in zip((k, v), got):
+            assert Q.values(x[page, head, token], torch.bfloat16).tolist() == y
+
+
+def test_numbers_next_to_the_types_largest_stay_finite():
+    x = torch.full((1, 64), 65504.0, dtype=torch.float16)
+    x[0, 40] = -65504.0
+    assert bool(Q.values(x, torch.float16).half().isfinite().all())
+    y = torch.full((1, 64), torch.finfo(torch.bfloat16).max, dtype=torch.bfloat16)
+    y[0, 3] = -y[0, 3]
+    assert bool(Q.values(y, torch.bfloat16).to(torch.bfloat16).isfinite().all())

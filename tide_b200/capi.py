@@ -64,6 +64,12 @@ PROTOTYPES = {
                                        p, p, i64, i64, i64, i64, i64, f32, p, sz, p, p]),
     "tide_paged_append": (C.c_int, [C.c_int, p, p, i64, p, i64, p, p, i64, i64, i64, p, p, i64,
                                     i64, p, p]),
+    "tide_paged_append_q4": (C.c_int, [C.c_int, p, i64, p, p, i64, p, p, f32, p, f32, p, p, i64, p, p,
+                                       i64, i64, i64, i64, p, p, i64, i64, p, p]),
+    "tide_paged_read_q4": (C.c_int, [C.c_int, p, i64, i64, p, i64, i64, i64, p, p, p, p]),
+    "tide_paged_attention_q4_workspace_size": (sz, [i64, i64, i64, i64, i64, i64, i64]),
+    "tide_paged_attention_q4": (C.c_int, [C.c_int, p, i64, p, i64, i64, p, i64, i64, p, p, p, i64, p, p,
+                                          i64, i64, i64, i64, i64, f32, p, sz, p, p]),
     "tide_page_tables": (C.c_int, [p, p, p, i64, p, p, i64, p, i64, i64, p, p, p, p, p, i64, p,
                                    p]),
     "tide_router_fold": (C.c_int, [C.c_int, p, p, p, i64, i64, p, p, p, p, p]),

@@ -712,6 +712,132 @@ void paged_append(const std::optional<at::Tensor> &k_new, const std::optional<at
       const_cast<int32_t *>(err), cur_stream(k_cache)));
 }
 
+// A cache in 4 bits [n_pages, kv_heads, page_size / 16, 18 d] of bytes.
+int64_t q4_head_dim(const at::Tensor &cache) {
+  check_cuda_contig(cache, "cache");
+  TORCH_CHECK(cache.scalar_type() == at::kByte && cache.dim() == 4 && cache.size(3) % 18 == 0,
+              "cache must be uint8 [n_pages, kv_heads, page_size / 16, 18 * head_dim]");
+  return cache.size(3) / 18;
+}
+
+void paged_append_q4(const std::optional<at::Tensor> &q, const std::optional<at::Tensor> &k_new,
+                     const std::optional<at::Tensor> &v_new, const at::Tensor &slot_map,
+                     const std::optional<at::Tensor> &row_ids, const std::optional<at::Tensor> &n_rows_dev,
+                     const std::optional<at::Tensor> &positions, const std::optional<at::Tensor> &inv_freq,
+                     double attention_scaling, const std::optional<at::Tensor> &q_norm_weight,
+                     const std::optional<at::Tensor> &k_norm_weight, double eps,
+                     const std::optional<at::Tensor> &q_out, const at::Tensor &cache,
+                     const std::optional<at::Tensor> &error_word) {
+  const int64_t d = q4_head_dim(cache), hkv = cache.size(1);
+  const auto dev = cache.device();
+  auto given = [](const std::optional<at::Tensor> &t) { return t.has_value() && t->defined(); };
+  check_cuda_contig(slot_map, "slot_map");
+  TORCH_CHECK(slot_map.scalar_type() == at::kLong && slot_map.device() == dev, "slot_map must be int64");
+  const bool rows = given(k_new);
+  TORCH_CHECK(rows == given(v_new), "k_new and v_new: both or neither");
+  TORCH_CHECK(rows || !given(q), "q comes with k_new and v_new");
+  TORCH_CHECK(given(q) == given(q_out), "q and q_out: both or neither");
+  int64_t n = given(row_ids) ? row_ids->numel() : slot_map.numel(), stride = 0, q_stride = 0, hq = 0;
+  at::ScalarType dt = at::kBFloat16;  // (zeros are the same for both)
+  if (rows) {
+    dt = k_new->scalar_type();
+    stride = packed_heads(*k_new, "k_new");
+    TORCH_CHECK(packed_heads(*v_new, "v_new") == stride, "k_new and v_new must share a row stride");
+    TORCH_CHECK(v_new->sizes() == k_new->sizes() && k_new->size(1) == hkv && k_new->size(2) == d,
+                "k_new, v_new must be [n, kv_heads, d]");
+    TORCH_CHECK(v_new->scalar_type() == dt && k_new->device() == dev && v_new->device() == dev,
+                "new rows must share dtype, and the cache's device");
+    n = k_new->size(0);
+  }
+  TORCH_CHECK(given(row_ids) || slot_map.numel() >= n, "slot_map must have an entry for every row");
+  if (given(q)) {
+    q_stride = packed_heads(*q, "q");
+    hq = q->size(1);
+    TORCH_CHECK(q->size(0) == n && q->size(2) == d && q->scalar_type() == dt && q->device() == dev,
+                "q must be [n, heads, d], of the keys' dtype and device");
+    check_cuda_contig(*q_out, "q_out");
+    TORCH_CHECK(q_out->sizes() == q->sizes() && q_out->scalar_type() == dt && q_out->device() == dev,
+                "q_out must be like q");
+  }
+  const float *freq = nullptr;
+  const int64_t *pos = nullptr;
+  if (given(inv_freq)) {
+    check_cuda_contig(*inv_freq, "inv_freq");
+    TORCH_CHECK(inv_freq->scalar_type() == at::kFloat && inv_freq->numel() == d / 2 && inv_freq->device() == dev,
+                "inv_freq must be fp32 with head_dim / 2 entries");
+    TORCH_CHECK(given(positions), "inv_freq comes with positions");
+    check_cuda_contig(*positions, "positions");
+    TORCH_CHECK(positions->scalar_type() == at::kLong && positions->numel() >= slot_map.numel() &&
+                positions->device() == dev, "positions must be int64, an entry for every one of slot_map");
+    freq = inv_freq->data_ptr<float>();
+    pos = positions->data_ptr<int64_t>();
+  }
+  for (const auto *w : {&q_norm_weight, &k_norm_weight}) {
+    if (!given(*w)) continue;
+    check_cuda_contig(**w, "norm weight");
+    TORCH_CHECK((*w)->scalar_type() == dt && (*w)->numel() == d && (*w)->device() == dev,
+                "norm weights must be [head_dim] of the rows' dtype");
+  }
+  const int32_t *ids = opt_i32(row_ids, "row_ids", n, dev);
+  const int32_t *live = opt_i32(n_rows_dev, "n_rows_dev", 1, dev);
+  const int32_t *err = opt_i32(error_word, "error_word", 1, dev);
+  const c10::cuda::CUDAGuard guard(dev);
+  TIDE_CHECK_OK(tide_paged_append_q4(
+      to_dtype(dt, "paged_append_q4"), opt_ptr(q), q_stride, opt_ptr(k_new), opt_ptr(v_new), stride,
+      opt_ptr(q_norm_weight), opt_ptr(k_norm_weight), (float)eps, freq, (float)attention_scaling, pos,
+      slot_map.data_ptr<int64_t>(), slot_map.numel(), ids, live, n, hq, hkv, d, opt_mut(q_out),
+      cache.data_ptr(), cache.size(0), cache.size(2) * 16, const_cast<int32_t *>(err), cur_stream(cache)));
+}
+
+void paged_read_q4(const at::Tensor &cache, const at::Tensor &slots, const at::Tensor &k_out,
+                   const at::Tensor &v_out, const std::optional<at::Tensor> &error_word) {
+  const int64_t d = q4_head_dim(cache);
+  const auto dev = cache.device();
+  check_cuda_contig(slots, "slots");
+  TORCH_CHECK(slots.scalar_type() == at::kLong && slots.device() == dev, "slots must be int64");
+  check_cuda_contig(k_out, "k_out");
+  check_out(v_out, k_out);
+  TORCH_CHECK(k_out.dim() == 3 && k_out.size(0) == slots.numel() && k_out.size(1) == cache.size(1) &&
+              k_out.size(2) == d && k_out.device() == dev, "k_out and v_out must be [n, kv_heads, head_dim]");
+  const int32_t *err = opt_i32(error_word, "error_word", 1, dev);
+  const c10::cuda::CUDAGuard guard(dev);
+  TIDE_CHECK_OK(tide_paged_read_q4(to_dtype(k_out.scalar_type(), "paged_read_q4"), cache.data_ptr(),
+                                   cache.size(0), cache.size(2) * 16, slots.data_ptr<int64_t>(),
+                                   slots.numel(), cache.size(1), d, k_out.data_ptr(), v_out.data_ptr(),
+                                   const_cast<int32_t *>(err), cur_stream(cache)));
+}
+
+void paged_attention_q4(const at::Tensor &q, const at::Tensor &cache, const at::Tensor &block_tables,
+                        const at::Tensor &kv_lens, const std::optional<at::Tensor> &cu_seqlens,
+                        const std::optional<at::Tensor> &seq_ids, const at::Tensor &out,
+                        int64_t max_kv_len, double scale, const std::optional<at::Tensor> &error_word,
+                        const std::optional<at::Tensor> &n_seqs_dev) {
+  const int64_t qs = packed_heads(q, "q");
+  const auto dev = q.device();
+  TORCH_CHECK(q4_head_dim(cache) == q.size(2), "q and cache must share a head dimension");
+  TORCH_CHECK(cache.device() == dev, "rows and cache must share a device");
+  check_out(out, q);
+  TORCH_CHECK(block_tables.dim() == 2, "block_tables must be [n_requests, max_pages]");
+  const int32_t *bt = i32(block_tables, "block_tables", 0, dev);
+  const int64_t n_req = std::min(block_tables.size(0), kv_lens.numel());
+  const int32_t *lens = i32(kv_lens, "kv_lens", 0, dev);
+  const int32_t *cu = opt_i32(cu_seqlens, "cu_seqlens", 1, dev);
+  const int64_t n_seqs = cu ? cu_seqlens->numel() - 1 : q.size(0);
+  const int32_t *ids = opt_i32(seq_ids, "seq_ids", n_seqs, dev);
+  const int32_t *live = opt_i32(n_seqs_dev, "n_seqs_dev", 1, dev);
+  const int32_t *err = opt_i32(error_word, "error_word", 1, dev);
+  const c10::cuda::CUDAGuard guard(dev);
+  const int64_t need = (int64_t)tide_paged_attention_q4_workspace_size(
+      q.size(0), n_seqs, n_req, q.size(1), cache.size(1), q.size(2), max_kv_len);
+  at::Tensor ws;  // of the current stream's allocator, so of this call alone
+  if (need) ws = at::empty({need}, q.options().dtype(at::kByte));
+  TIDE_CHECK_OK(tide_paged_attention_q4(
+      to_dtype(q.scalar_type(), "paged_attention_q4"), q.data_ptr(), qs, cache.data_ptr(), cache.size(0),
+      cache.size(2) * 16, bt, block_tables.size(1), n_req, lens, cu, ids, n_seqs, live, out.data_ptr(),
+      q.size(0), q.size(1), cache.size(1), q.size(2), max_kv_len, (float)scale,
+      need ? ws.data_ptr() : nullptr, (size_t)need, const_cast<int32_t *>(err), cur_stream(q)));
+}
+
 void page_tables(const at::Tensor &context_lens, const at::Tensor &new_lens,
                  const std::optional<at::Tensor> &done, const at::Tensor &free_pages,
                  const at::Tensor &n_free, const at::Tensor &block_tables, int64_t page_size,
@@ -914,6 +1040,15 @@ TORCH_LIBRARY(tide, m) {
         "float scale, Tensor(b!)? error_word, Tensor? n_seqs_dev=None) -> ()");
   m.def("paged_append(Tensor? k_new, Tensor? v_new, Tensor slot_map, Tensor? row_ids, "
         "Tensor? n_rows_dev, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!)? error_word) -> ()");
+  m.def("paged_append_q4(Tensor? q, Tensor? k_new, Tensor? v_new, Tensor slot_map, Tensor? row_ids, "
+        "Tensor? n_rows_dev, Tensor? positions, Tensor? inv_freq, float attention_scaling, "
+        "Tensor? q_norm_weight, Tensor? k_norm_weight, float eps, Tensor(a!)? q_out, "
+        "Tensor(b!) cache, Tensor(c!)? error_word) -> ()");
+  m.def("paged_read_q4(Tensor cache, Tensor slots, Tensor(a!) k_out, Tensor(b!) v_out, "
+        "Tensor(c!)? error_word) -> ()");
+  m.def("paged_attention_q4(Tensor q, Tensor cache, Tensor block_tables, Tensor kv_lens, "
+        "Tensor? cu_seqlens, Tensor? seq_ids, Tensor(a!) out, int max_kv_len, float scale, "
+        "Tensor(b!)? error_word, Tensor? n_seqs_dev=None) -> ()");
   m.def("page_tables(Tensor context_lens, Tensor new_lens, Tensor? done, Tensor(a!) free_pages, "
         "Tensor n_free, Tensor(b!) block_tables, int page_size, Tensor(c!) n_free_out, "
         "Tensor(d!) kv_lens, Tensor(e!) cu_seqlens, Tensor(f!) slot_map, Tensor(g!) positions, "
@@ -948,6 +1083,9 @@ TORCH_LIBRARY_IMPL(tide, CUDA, m) {
   m.impl("packed_attention", &packed_attention);
   m.impl("paged_attention", &paged_attention);
   m.impl("paged_append", &paged_append);
+  m.impl("paged_append_q4", &paged_append_q4);
+  m.impl("paged_read_q4", &paged_read_q4);
+  m.impl("paged_attention_q4", &paged_attention_q4);
   m.impl("page_tables", &page_tables);
   m.impl("router_fold", &router_fold);
   m.impl("checkpoint", &checkpoint);
