@@ -41,8 +41,8 @@ NVCC_FLAGS = ARCH + ["-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC,-O3"
 CU_SOURCES = ["capi.cu", "tc_checkpoint.cu", "tc_route_pair.cu", "tc_fused.cu", "move_bulk.cu",
               "noalloc.cu", "decode_attn.cu", "decode_layer.cu", "paged_cache.cu", "ragged_attn.cu",
               "paged_q4.cu"]
-HEADERS = ["common.cuh", "move_bulk.cuh", "paged_q4.cuh", "ragged.cuh", "simt_kernels.cuh", "tc_checkpoint.cuh",
-           "tc_ptx.cuh"]
+HEADERS = ["attn_math.cuh", "common.cuh", "move_bulk.cuh", "paged_q4.cuh", "ragged.cuh", "simt_kernels.cuh",
+           "tc_checkpoint.cuh", "tc_ptx.cuh"]
 
 
 def _run(cmd: list[str], verbose: bool) -> None:

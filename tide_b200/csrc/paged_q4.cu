@@ -4,6 +4,7 @@
 #include <math.h>
 #include <stdio.h>
 
+#include "attn_math.cuh"
 #include "paged_q4.cuh"
 #include "ragged.cuh"
 #include "tc_ptx.cuh"
@@ -354,6 +355,7 @@ struct OpenParams {
   void *k, *v;
   int64_t wide;  // pages of a sequence in k and v
   int32_t *out_tables, *out_live;
+  int few;       // sequences of up to so many rows are not needed
 };
 constexpr int kOpenPage = 128;  // tokens of a 16-bit page
 constexpr int kOpenTokens = 64; // of a CTA
@@ -372,7 +374,11 @@ __global__ void __launch_bounds__(256) open_kernel(const __grid_constant__ OpenP
   if (i >= live) return;
   const int seq = p.first + i;
   const int req = p.batch.seq_ids ? __ldg(p.batch.seq_ids + seq) : seq;
-  // (a bad request or length is the attention's to flag)
+  // (bad bounds, a bad request or length are the attention's to flag)
+  if (p.few) {
+    int row0, end;
+    if (!p.batch.cu || !sequence_bounds(p.batch, seq, &row0, &end) || end - row0 <= p.few) return;
+  }
   if (req < 0 || req >= p.batch.n_requests) return;
   if (tok0 % kOpenPage == 0 && threadIdx.x == 0)
     p.out_tables[req * p.wide + tok0 / kOpenPage] = i * (int)p.wide + tok0 / kOpenPage;
@@ -394,6 +400,412 @@ __global__ void __launch_bounds__(256) open_kernel(const __grid_constant__ OpenP
       const uint32_t s = *reinterpret_cast<const uint16_t *>(block + L::scale(side, word / 4, at % kBlock));
       reinterpret_cast<uint4 *>(side ? p.v : p.k)[to] =
           real ? value8<T>(w, pars<T>(s | s << 16)) : make_uint4(0, 0, 0, 0);
+    }
+  }
+}
+
+// --------------------------------------------------- attention of few rows
+// Sequences with few rows (tokens times the query heads of a KV head).  A CTA
+// takes 8 NT rows of a sequence, or of a split of its keys; its four warps walk
+// over every fourth block of 16 tokens each on their own, with their own ring of
+// bulk copies (a block is one copy), running maxima, sums and outputs, and meet
+// once at the end.  The rows are the narrow side of the products:
+//   S^T[16 x 8 NT] = K Q^T,   O^T[D x 8 NT] += V^T P^T    (mma.sync m16n8k16).
+// A lane makes its operands in registers from the codes, each exactly the value
+// that they stand for, so nothing is staged as 16 bits.  The order of the
+// tokens of a block, and of the channels, is free in both products, and chosen
+// so that a lane reads what it needs in wide pieces without bank conflicts:
+//   row g of S is token kappa(g) = g / 2 + 4 (g % 2), row g + 8 the one 8 further;
+//   k-elements of lane t (of four) of S are the D / 4 channels from D / 4 t on, in
+//   one scale group;
+//   rows g and g + 8 of O's tiles are the D / 8 channels from D / 8 g on, their
+//   k-elements of lane t the tokens t, t + 4, t + 8, t + 12, whose scales lie side
+//   by side and whose pairs of codes come from two words' halves.
+constexpr int kFewWarps = 4;
+
+template <int D, int NT>
+struct Few {
+  static constexpr int kStages = NT <= 2 ? 6 : 8;
+  static constexpr int kRing = kStages * Layout<D>::kBytes;  // of a warp
+  static constexpr int kSmem = kFewWarps * kRing;
+  static constexpr int kCtas = NT == 1 ? 4 : NT == 2 ? 3 : 2;  // of an SM
+};
+
+struct FewParams {
+  RaggedBatch batch;
+  const unsigned char *cache;
+  const int32_t *tables;
+  int64_t max_pages;
+  int n_pages, page_shift;
+  const void *q;
+  int64_t q_stride;
+  void *out;
+  float *part_o;    // [splits, n_seqs, few, hq, D] (splits > 1)
+  float2 *part_ml;  // [splits, n_seqs, few, hq]: maximum (scaled, base 2), sum
+  int hq, hkv, group;
+  int few;         // tokens a sequence may have
+  int tokens;      // of a CTA: 8 NT / group
+  int pieces;      // pieces of up to `tokens` tokens that the sequences may have
+  int splits;
+  int split_keys;  // keys of a split, a multiple of 16
+  float qs;
+};
+
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
+  return __byte_perm(a, b, sel);
+}
+
+// The weights as they meet the values, for the sum that divides them.
+template <typename T>
+__device__ __forceinline__ float2 unpack_weights(uint32_t x) {
+  if constexpr (std::is_same<T, __half>::value)
+    return __half22float2(as_pair<T>(x));
+  else
+    return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+}
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
+    few_rows_kernel(const __grid_constant__ FewParams p) {
+  using namespace ragged;
+  using L = Layout<D>;
+  using F = Few<D, NT>;
+  constexpr unsigned kFull = 0xffffffffu;
+  constexpr int kRowsMost = 8 * NT, kSteps = D / 16;
+  constexpr int kKWords = D / 32;  // words of a lane's channels in a key
+  constexpr int kVWords = D / 64;  // in a value
+  extern __shared__ __align__(128) unsigned char dyn[];
+  __shared__ uint64_t full[kFewWarps][F::kStages];
+  __shared__ float s_m[kFewWarps][kRowsMost], s_l[kFewWarps][kRowsMost];
+  __shared__ int s_abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < kFewWarps; ++w)
+      for (int i = 0; i < F::kStages; ++i) ptx::mbar_init(&full[w][i], 1);
+    ptx::fence_mbar_init();
+    s_abort = 0;
+  }
+  ptx::grid_dependency_wait();  // up to here this overlaps the kernel before
+  ptx::grid_dependents_launch();
+  const int split = (int)(blockIdx.x % p.splits);
+  const int64_t unit = blockIdx.x / p.splits;
+  const int kvh = (int)(unit % p.hkv);
+  const int live = live_sequences(p.batch);
+  int seq = (int)(unit / p.hkv), tok0 = 0;  // this CTA's tokens from tok0 on
+  if (p.few > p.tokens && !find_piece(p.batch, live, p.few, p.tokens, &seq, &tok0)) return;
+  if (seq >= live) return;
+  Sequence s = sequence(p.batch, seq);
+  if (s.n > p.few || tok0 >= s.n) return;
+  {  // as a sequence of its own, which ends with its last token
+    const int rest = s.n - tok0 - p.tokens;
+    s.row0 += tok0;
+    s.n = rest > 0 ? p.tokens : s.n - tok0;
+    s.kv -= max(rest, 0);
+  }
+  const int rows = s.n * p.group;
+  const int tiles = (rows + 7) / 8;  // 8-row groups that there are
+  const int pos0 = s.kv - s.n;       // keys before the first token's own
+  const int k0 = split * p.split_keys, k1 = p.splits > 1 ? min(s.kv, k0 + p.split_keys) : s.kv;
+  const int64_t row0 = (int64_t)s.row0 * p.hq + kvh * p.group;  // of [token, head] rows
+  const int64_t part =
+      (((int64_t)split * p.batch.n_seqs + seq) * p.few + tok0) * p.hq + kvh * p.group;
+  if (p.splits > 1 && k0 >= k1) {  // no keys: a sum of 0
+    for (int r = threadIdx.x; r < rows; r += blockDim.x)
+      p.part_ml[part + (int64_t)(r / p.group) * p.hq + r % p.group] = make_float2(-INFINITY, 0.f);
+    return;
+  }
+  unsigned char *ring = dyn + warp * F::kRing;
+  __syncthreads();
+
+  // this warp's blocks: warp, warp + 4, ... of the split's
+  const int blocks = max(0, ((k1 - k0 + kBlock - 1) / kBlock - warp + kFewWarps - 1) / kFewWarps);
+  const int page = 1 << p.page_shift;
+  auto key_of = [&](int i) { return k0 + (warp + i * kFewWarps) * kBlock; };
+  // where 32 blocks at a time are in the cache, one per lane, the next ones read
+  // ahead; -1: a page outside it
+  auto places = [&](int i0) {
+    const int i = i0 + lane;
+    if (i >= blocks) return -1;
+    const int at = key_of(i);
+    const int pg = __ldg(p.tables + s.req * p.max_pages + (at >> p.page_shift));
+    if (pg < 0 || pg >= p.n_pages) {
+      raise_error(p.batch.err, TIDE_DEVERR_POSITION);
+      return -1;
+    }
+    return (pg * p.hkv + kvh) * (page / kBlock) + (at & (page - 1)) / kBlock;
+  };
+  const uint64_t once = l2_evict_first_policy();
+  int now = places(0), next = places(32);
+  auto request = [&](int i) {
+    if (i >= blocks) return;
+    if ((i & 31) == 0 && i) {
+      now = next;
+      next = places(i + 32);
+    }
+    const int place = __shfl_sync(kFull, now, i & 31);
+    const int st = i % F::kStages;
+    unsigned char *to = ring + st * L::kBytes;
+    if (place >= 0) {
+      if (lane == 0) {
+        ptx::mbar_expect_tx(&full[warp][st], L::kBytes);
+        ptx::bulk_load(to, p.cache + (int64_t)place * L::kBytes, L::kBytes, &full[warp][st], once);
+      }
+    } else {  // reads as zeros
+      for (int e = lane; e < L::kBytes / 16; e += 32) reinterpret_cast<uint4 *>(to)[e] = make_uint4(0, 0, 0, 0);
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&full[warp][st]);
+    }
+    __syncwarp();
+  };
+  for (int i = 0; i < F::kStages; ++i) request(i);
+
+  // Q^T: columns are rows 8 nt + g; the statistics of a column are kept by the
+  // lanes whose accumulators belong to it, columns 8 nt + 2 t and one further
+  uint32_t qb[NT][kSteps][2];
+  int sees[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = nt * 8 + g;
+    const bool valid = r < rows;
+    const T *q = static_cast<const T *>(p.q) + (s.row0 + (valid ? r / p.group : 0)) * p.q_stride +
+                 (int64_t)(kvh * p.group + (valid ? r % p.group : 0)) * D + t * (D / 4);
+#pragma unroll
+    for (int w = 0; w < kKWords; ++w) {
+      const uint4 x = valid ? *reinterpret_cast<const uint4 *>(q + 8 * w) : make_uint4(0, 0, 0, 0);
+      qb[nt][2 * w][0] = x.x;
+      qb[nt][2 * w][1] = x.y;
+      qb[nt][2 * w + 1][0] = x.z;
+      qb[nt][2 * w + 1][1] = x.w;
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int c = nt * 8 + t * 2 + e;
+      sees[nt][e] = pos0 + (c < rows ? c / p.group : s.n - 1) + 1;
+    }
+  }
+  float o[NT][kSteps][4], m[NT][2], l[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    m[nt][0] = m[nt][1] = -INFINITY;
+    l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+    for (int d = 0; d < kSteps; ++d) o[nt][d][0] = o[nt][d][1] = o[nt][d][2] = o[nt][d][3] = 0.f;
+  }
+  const float slack = kSlack / p.qs;
+  const int kappa = (g >> 1) + 4 * (g & 1);
+  int i = 0;
+  for (; i < blocks; ++i) {
+    const int st = i % F::kStages;
+    if (!__all_sync(kFull, ptx::mbar_wait(&full[warp][st], (i / F::kStages) & 1, &s_abort))) {
+      raise_error(p.batch.err, TIDE_DEVERR_TIMEOUT);
+      s_abort = 1;
+      break;
+    }
+    const unsigned char *b = ring + st * L::kBytes;
+    const int key = key_of(i);
+    const int seen = s.kv - key;                   // keys of the block that exist
+    const bool partial = key + kBlock > pos0 + 1;  // some row does not see all of them
+    // the block's words and scales of this lane
+    uint32_t kw[2][kKWords], vw[4][kVWords];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const unsigned char *at = b + L::codes(0, kappa + 8 * h) + t * (D / 8);
+      if constexpr (D == 128) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(at);
+        kw[h][0] = x.x, kw[h][1] = x.y, kw[h][2] = x.z, kw[h][3] = x.w;
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2 *>(at);
+        kw[h][0] = x.x, kw[h][1] = x.y;
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const unsigned char *at = b + L::codes(1, t + 4 * h) + g * (D / 16);
+      if constexpr (D == 128) {
+        const uint2 x = *reinterpret_cast<const uint2 *>(at);
+        vw[h][0] = x.x, vw[h][1] = x.y;
+      } else {
+        vw[h][0] = *reinterpret_cast<const uint32_t *>(at);
+      }
+    }
+    const int v_group = g * (D / 8) / kGroup;
+    const uint2 ks = *reinterpret_cast<const uint2 *>(b + L::scale(0, t * (D / 4) / kGroup, g >> 1));
+    uint2 vs = *reinterpret_cast<const uint2 *>(b + L::scale(1, v_group, t));
+    // Masked values: a weight of 0 does not silence a NaN.  Past the last key a
+    // token's scales are dropped; before it, where rows differ, those that are
+    // NaN are, and added to the rows that do see them.
+    if (seen < kBlock) {
+      if (t >= seen) vs.x &= 0xffff0000u;
+      if (t + 4 >= seen) vs.x &= 0x0000ffffu;
+      if (t + 8 >= seen) vs.y &= 0xffff0000u;
+      if (t + 12 >= seen) vs.y &= 0x0000ffffu;
+    }
+    if (partial && s.n > 1) {
+      auto odd = [](uint32_t x) { return (x & 0x7f80u) == 0x7f80u; };
+      if (__any_sync(kFull, odd(vs.x) || odd(vs.x >> 16) || odd(vs.y) || odd(vs.y >> 16))) {
+        // rare: token by token
+#pragma unroll 1
+        for (int k = 0; k < min(seen, kBlock); ++k) {
+          if (!odd(*reinterpret_cast<const uint16_t *>(b + L::scale(1, v_group, k)))) continue;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int d = 0; d < kSteps; ++d)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (key + k < sees[nt][e & 1]) o[nt][d][e] += NAN;
+        }
+        if (odd(vs.x)) vs.x &= 0xffff0000u;
+        if (odd(vs.x >> 16)) vs.x &= 0x0000ffffu;
+        if (odd(vs.y)) vs.y &= 0xffff0000u;
+        if (odd(vs.y >> 16)) vs.y &= 0x0000ffffu;
+      }
+    }
+    __syncwarp();  // the stage has been read
+    ptx::fence_proxy_async();
+    request(i + F::kStages);
+
+    float sc[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+    {
+      const uint32_t both = g & 1 ? 0x3232u : 0x1010u;
+      const Pars<T> p0 = pars<T>(prmt(ks.x, 0u, both)), p1 = pars<T>(prmt(ks.y, 0u, both));
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) {
+        const int sh = 8 * (k & 1);
+        const uint32_t w0 = kw[0][k / 2] >> sh, w1 = kw[1][k / 2] >> sh;
+        const uint32_t a[4] = {value2<T>(w0, p0), value2<T>(w1, p1), value2<T>(w0 >> 4, p0),
+                               value2<T>(w1 >> 4, p1)};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          if (nt < tiles) mma16816<T>(sc[nt], a, qb[nt][k][0], qb[nt][k][1]);
+      }
+    }
+    uint32_t pt[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      if (nt >= tiles) continue;
+      bool raise = false;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        // tokens kappa and 8 further
+        if (partial) {
+          const int lim = sees[nt][e] - key - kappa;
+          if (lim <= 0) sc[nt][e] = -INFINITY;
+          if (lim <= 8) sc[nt][2 + e] = -INFINITY;
+        }
+        raise |= fmaxf(sc[nt][e], sc[nt][2 + e]) > m[nt][e] + slack;  // (the first keys: m is -infinity)
+      }
+      if (__any_sync(kFull, raise)) {
+        float a[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float top = fmaxf(sc[nt][e], sc[nt][2 + e]);
+#pragma unroll
+          for (int w = 4; w < 32; w *= 2) top = fmaxf(top, __shfl_xor_sync(kFull, top, w));
+          const bool up = top > m[nt][e] + slack;
+          a[e] = up ? ex2((m[nt][e] - top) * p.qs) : 1.f;
+          if (up) m[nt][e] = top;
+          l[nt][e] *= a[e];
+        }
+#pragma unroll
+        for (int d = 0; d < kSteps; ++d) {
+          o[nt][d][0] *= a[0];
+          o[nt][d][1] *= a[1];
+          o[nt][d][2] *= a[0];
+          o[nt][d][3] *= a[1];
+        }
+      }
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float mq = (m[nt][e] == -INFINITY ? 0.f : m[nt][e] * p.qs) - kLift<T>;
+        x[e] = ex2(fmaf(sc[nt][e], p.qs, -mq));
+        x[2 + e] = ex2(fmaf(sc[nt][2 + e], p.qs, -mq));
+      }
+      const uint32_t w0 = pack_weights<T>(x[0], x[1]), w1 = pack_weights<T>(x[2], x[3]);
+      const float2 f0 = unpack_weights<T>(w0), f1 = unpack_weights<T>(w1);
+      l[nt][0] += f0.x + f1.x;
+      l[nt][1] += f0.y + f1.y;
+      pt[nt][0] = transpose8x8(w0);
+      pt[nt][1] = transpose8x8(w1);
+    }
+    {
+      const Pars<T> p0 = pars<T>(vs.x), p1 = pars<T>(vs.y);
+#pragma unroll
+      for (int w = 0; w < kVWords; ++w) {
+        const uint32_t lo0 = prmt(vw[0][w], vw[1][w], 0x5410u), hi0 = prmt(vw[0][w], vw[1][w], 0x7632u);
+        const uint32_t lo1 = prmt(vw[2][w], vw[3][w], 0x5410u), hi1 = prmt(vw[2][w], vw[3][w], 0x7632u);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t a[4] = {value2<T>(lo0 >> 4 * k, p0), value2<T>(hi0 >> 4 * k, p0),
+                                 value2<T>(lo1 >> 4 * k, p1), value2<T>(hi1 >> 4 * k, p1)};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            if (nt < tiles) mma16816<T>(o[nt][4 * w + k], a, pt[nt][0], pt[nt][1]);
+        }
+      }
+    }
+  }
+  if (i < blocks && lane == 0) {  // given up: wait for the copies in flight (bounded)
+    volatile int none = 0;
+    for (int e = i; e < min(blocks, i + F::kStages); ++e)
+      ptx::mbar_wait(&full[warp][e % F::kStages], (e / F::kStages) & 1, &none);
+  }
+  __syncwarp();
+
+  // the four warps' outputs meet: this warp's in its own ring, [row][D + 4]
+  constexpr int kPitch = D + 4;
+  float *mine = reinterpret_cast<float *>(ring);
+  static_assert(kRowsMost * kPitch * 4 <= F::kRing, "a warp's output fits its ring");
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = nt * 8 + t * 2 + e;
+      float sum = l[nt][e];
+#pragma unroll
+      for (int w = 4; w < 32; w *= 2) sum += __shfl_xor_sync(kFull, sum, w);
+      if (g == 0) {
+        s_m[warp][r] = m[nt][e] * p.qs;
+        s_l[warp][r] = sum;
+      }
+#pragma unroll
+      for (int d = 0; d < kSteps; ++d)
+        *reinterpret_cast<float2 *>(mine + r * kPitch + g * (D / 8) + 2 * d) =
+            make_float2(o[nt][d][e], o[nt][d][2 + e]);
+    }
+  __syncthreads();
+  const float *all = reinterpret_cast<const float *>(dyn);
+  constexpr int kLanes = D / 4;  // lanes of a row, four columns each
+  for (int r = threadIdx.x / kLanes; r < rows; r += 32 * kFewWarps / kLanes) {
+    const int d = threadIdx.x % kLanes * 4;
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w)
+      if (s_l[w][r] != 0.f) top = fmaxf(top, s_m[w][r]);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) {
+      if (s_l[w][r] == 0.f) continue;
+      const float a = exp2f(s_m[w][r] - top);
+      const float4 y = *reinterpret_cast<const float4 *>(all + w * (F::kRing / 4) + r * kPitch + d);
+      sum = fmaf(a, s_l[w][r], sum);
+      x.x = fmaf(a, y.x, x.x);
+      x.y = fmaf(a, y.y, x.y);
+      x.z = fmaf(a, y.z, x.z);
+      x.w = fmaf(a, y.w, x.w);
+    }
+    const int64_t at = (int64_t)(r / p.group) * p.hq + r % p.group;
+    if (p.splits > 1) {
+      if (d == 0) p.part_ml[part + at] = make_float2(top, sum);
+      *reinterpret_cast<float4 *>(p.part_o + (part + at) * D + d) = x;
+    } else {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + (row0 + at) * D + d) =
+          make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
     }
   }
 }
@@ -448,33 +860,82 @@ int append(const tide::q4::AppendParams &p, cudaStream_t s) {
   return start("paged_append_q4", append_kernel<T, D, 1>, p.n_rows, 256, 0, s, p);
 }
 
-// How a call of the many-rows path is cut up: sequences a round, so that the
-// 16-bit pages of a round stay within 1 GB (or are one sequence's).
-struct Rounds {
-  int64_t wide;   // 16-bit pages of a sequence
-  int64_t seqs;   // of a round
-  size_t side;    // bytes of the keys' (or values') pages
-  size_t tables, inner, bytes;
+// How an attention call is cut up.  Sequences of up to `few` tokens go to the
+// few-rows kernel, longer ones as 16-bit pages to the tiles; a call that cannot
+// have the one or the other does not launch it.
+struct Plan {
+  int nt;           // 8-row groups of a CTA of the few-rows kernel; 0: none
+  int few, tokens;
+  int64_t pieces;   // of up to `tokens` tokens, at most
+  int splits, split_keys;
+  bool tiles;       // whether the tiles run: in rounds of sequences, so that the
+  int64_t wide;     // 16-bit pages of a round stay within 256 MB (or are one
+  int64_t seqs;     // sequence's): pages of a sequence, sequences of a round
+  size_t few_bytes, side, tables, inner, bytes;  // workspace
 };
 
-Rounds rounds_of(bool one_token, int64_t n_tokens, int64_t n_seqs, int64_t n_requests, int64_t hq,
-                 int64_t hkv, int64_t d, int64_t max_kv) {
-  Rounds r{};
-  r.wide = (max_kv + tide::q4::kOpenPage - 1) / tide::q4::kOpenPage;
-  if (r.wide < 1) r.wide = 1;
-  const int64_t page = tide::q4::kOpenPage * hkv * d * 2;
-  r.seqs = (1ll << 29) / (page * r.wide);
-  if (r.seqs < 1) r.seqs = 1;
-  if (r.seqs > n_seqs) r.seqs = n_seqs;
-  r.side = (size_t)(r.seqs * r.wide * page);
-  r.tables = (size_t)((n_requests * r.wide * 4 + 16 + 15) / 16 * 16);  // and the live count
-  for (const int64_t n : {r.seqs, n_seqs % r.seqs}) {  // (the last round may be a smaller one)
-    const size_t inner =
-        tide_paged_attention_workspace_size(one_token ? n : n_tokens, n, hq, hkv, d, max_kv);
-    if (inner > r.inner) r.inner = inner;
+Plan plan_of(bool one_token, int64_t n_tokens, int64_t n_seqs, int64_t n_requests, int64_t hq,
+             int64_t hkv, int64_t d, int64_t max_kv) {
+  Plan p{};
+  const int64_t group = hq / hkv;
+  p.nt = group <= 8 ? 1 : group <= 16 ? 2 : group <= 32 ? 4 : 0;
+  if (!one_token) {
+    const int64_t rows = (n_tokens * group + n_seqs - 1) / n_seqs;  // of a sequence, on average
+    if (p.nt && p.nt < 2 && rows > 8) p.nt = 2;
+    if (p.nt && p.nt < 4 && rows > 16) p.nt = 4;
+    if (rows > 32 || (n_seqs == 1 && rows > 64)) p.nt = 0;
   }
-  r.bytes = 2 * r.side + r.tables + r.inner;
-  return r;
+  p.tokens = (int)(p.nt * 8 / group);
+  p.few = !p.nt ? 0 : one_token ? 1 : 2 * p.tokens;
+  if (n_tokens < p.few) p.few = (int)n_tokens;
+  p.tiles = !p.nt || (!one_token && n_tokens > p.few);
+  p.pieces = n_seqs + (p.few > p.tokens ? n_tokens / p.tokens : 0);
+  // Splits of the few-rows kernel, as paged_attention's: one round of CTAs where
+  // there are few units, else up to eight, for an even end.
+  const int64_t slots = 148 * (p.nt == 1 ? 4 : p.nt == 2 ? 3 : 2);
+  const int64_t units = p.pieces * hkv;
+  const bool one_round = units * 4 <= slots;
+  const int64_t least = one_round ? 128 : 512;
+  int64_t s = !p.nt ? 1 : one_round ? slots / units : (8 * slots + units - 1) / units;
+  if (s > (max_kv + least - 1) / least) s = (max_kv + least - 1) / least;
+  if (s < 1 || units >= 2 * slots) s = 1;
+  p.splits = (int)s;
+  p.split_keys = (int)(((max_kv + s - 1) / s + 63) / 64 * 64);
+  p.few_bytes = s > 1 ? (size_t)(s * n_seqs * p.few * hq * (d + 2) * 4 + 15) / 16 * 16 : 0;
+  p.bytes = p.few_bytes;
+  if (!p.tiles) return p;
+  p.wide = (max_kv + tide::q4::kOpenPage - 1) / tide::q4::kOpenPage;
+  if (p.wide < 1) p.wide = 1;
+  const int64_t page = tide::q4::kOpenPage * hkv * d * 2;
+  p.seqs = (1ll << 27) / (page * p.wide);
+  if (p.seqs < 1) p.seqs = 1;
+  if (p.seqs > n_seqs) p.seqs = n_seqs;
+  p.side = (size_t)(p.seqs * p.wide * page);
+  p.tables = (size_t)((n_requests * p.wide * 4 + 16 + 15) / 16 * 16);  // and the live count
+  for (const int64_t n : {p.seqs, n_seqs % p.seqs}) {  // (the last round may be a smaller one)
+    const size_t inner =
+        tide::paged_tiles_workspace_size(one_token ? n : n_tokens, n, hq, hkv, d, max_kv);
+    if (inner > p.inner) p.inner = inner;
+  }
+  p.bytes += 2 * p.side + p.tables + p.inner;
+  return p;
+}
+
+template <typename T, int D, int NT>
+int launch_few(const tide::q4::FewParams &p, cudaStream_t s) {
+  using namespace tide::q4;
+  using F = Few<D, NT>;
+  auto kern = few_rows_kernel<T, D, NT>;
+  static std::atomic<uint64_t> set{0};  // per device
+  const cudaError_t e = tide::allow_smem(kern, F::kSmem, set);
+  if (e != cudaSuccess) return report(e, "paged_attention_q4");
+  return start("paged_attention_q4", kern, (int64_t)p.pieces * p.hkv * p.splits, 32 * kFewWarps, F::kSmem,
+               s, p);
+}
+
+template <typename T, int D>
+int few_rows(int nt, const tide::q4::FewParams &p, cudaStream_t s) {
+  return nt == 1 ? launch_few<T, D, 1>(p, s) : nt == 2 ? launch_few<T, D, 2>(p, s) : launch_few<T, D, 4>(p, s);
 }
 
 template <typename T, int D>
@@ -567,8 +1028,8 @@ extern "C" size_t tide_paged_attention_q4_workspace_size(int64_t n_tokens, int64
       max_kv_len < 0 || n_q_heads / n_kv_heads > 128)
     return 0;
   // (cu_seqlens or not: the larger need of the two)
-  const size_t one = rounds_of(true, n_tokens, n_seqs, n_requests, n_q_heads, n_kv_heads, head_dim, max_kv_len).bytes;
-  const size_t many = rounds_of(false, n_tokens, n_seqs, n_requests, n_q_heads, n_kv_heads, head_dim, max_kv_len).bytes;
+  const size_t one = plan_of(true, n_tokens, n_seqs, n_requests, n_q_heads, n_kv_heads, head_dim, max_kv_len).bytes;
+  const size_t many = plan_of(false, n_tokens, n_seqs, n_requests, n_q_heads, n_kv_heads, head_dim, max_kv_len).bytes;
   return one > many ? one : many;
 }
 
@@ -596,6 +1057,8 @@ extern "C" int tide_paged_attention_q4(int dtype, const void *q, int64_t q_row_s
     return fail(TIDE_ERR_INVALID, "paged_attention_q4: bad row stride (rows overlap, or not a multiple of 8)");
   if (bad_cache(n_pages, page_size, n_kv_heads) || (page_size & (page_size - 1)))
     return fail(TIDE_ERR_UNSUPPORTED, "paged_attention_q4: page_size must be a power of two of at least 16");
+  if (n_pages * n_kv_heads > INT32_MAX / (page_size / 16))
+    return fail(TIDE_ERR_INVALID, "paged_attention_q4: more than 2^31 blocks of 16 tokens");
   if (max_pages < 0 || n_requests < 0 || n_requests > INT32_MAX || max_kv_len < 0 ||
       max_kv_len > INT32_MAX / 2 || (max_kv_len + page_size - 1) / page_size > max_pages)
     return fail(TIDE_ERR_INVALID, "paged_attention_q4: bad sizes (block table, max_kv_len)");
@@ -611,43 +1074,56 @@ extern "C" int tide_paged_attention_q4(int dtype, const void *q, int64_t q_row_s
   if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
     return fail(TIDE_ERR_WORKSPACE, "paged_attention_q4: workspace missing, too small or misaligned");
   const cudaStream_t st = (cudaStream_t)stream;
+  const bool bf16 = dtype == TIDE_DTYPE_BF16, wide = head_dim == 128;
   unsigned char *ws = static_cast<unsigned char *>(workspace);
-  const Rounds r = rounds_of(!cu_seqlens, n_tokens, n_seqs, n_requests, n_q_heads, n_kv_heads, head_dim, max_kv_len);
-  int32_t *live = reinterpret_cast<int32_t *>(ws + 2 * r.side);
+  const Plan plan =
+      plan_of(!cu_seqlens, n_tokens, n_seqs, n_requests, n_q_heads, n_kv_heads, head_dim, max_kv_len);
+  int shift = 0;
+  while ((1 << shift) < page_size) ++shift;
+  const tide::RaggedBatch batch{cu_seqlens, seq_ids, kv_lens, n_seqs_dev, (int)n_seqs, (int)n_requests,
+                                (int)n_tokens, (int)max_kv_len, error_word};
+  int rc = TIDE_OK;
+  if (plan.nt) {
+    float *part_o = reinterpret_cast<float *>(ws);
+    const int64_t part_rows = plan.splits * n_seqs * plan.few * n_q_heads;
+    float2 *part_ml = reinterpret_cast<float2 *>(part_o + part_rows * head_dim);
+    const tide::q4::FewParams f{batch, static_cast<const unsigned char *>(cache), block_tables, max_pages,
+                                (int)n_pages, shift, q, q_row_stride, out, part_o, part_ml, (int)n_q_heads,
+                                (int)n_kv_heads, (int)(n_q_heads / n_kv_heads), plan.few, plan.tokens,
+                                (int)plan.pieces, plan.splits, plan.split_keys,
+                                scale * tide::ragged::kLog2e};
+    rc = bf16 ? (wide ? few_rows<__nv_bfloat16, 128>(plan.nt, f, st) : few_rows<__nv_bfloat16, 64>(plan.nt, f, st))
+              : (wide ? few_rows<__half, 128>(plan.nt, f, st) : few_rows<__half, 64>(plan.nt, f, st));
+    if (!rc && plan.splits > 1)
+      rc = tide::join_few_rows(dtype, head_dim, batch, (int)n_q_heads, plan.few, plan.splits, part_o, part_ml,
+                               out, st);
+  }
+  if (rc || !plan.tiles) return rc;
+  ws += plan.few_bytes;
+  int32_t *live = reinterpret_cast<int32_t *>(ws + 2 * plan.side);
   int32_t *tables = live + 4;
-  for (int64_t i = 0; i < n_seqs; i += r.seqs) {
-    const int64_t n = n_seqs - i < r.seqs ? n_seqs - i : r.seqs;
-    tide::q4::OpenParams p{};
-    p.batch = {cu_seqlens, seq_ids, kv_lens, n_seqs_dev, (int)n_seqs, (int)n_requests, (int)n_tokens,
-               (int)max_kv_len, error_word};
-    p.first = (int)i;
-    p.n = (int)n;
-    p.cache = static_cast<const unsigned char *>(cache);
-    p.tables = block_tables;
-    p.max_pages = max_pages;
-    p.n_pages = (int)n_pages;
-    p.page = (int)page_size;
-    p.hkv = (int)n_kv_heads;
-    p.k = ws;
-    p.v = ws + r.side;
-    p.wide = r.wide;
-    p.out_tables = tables;
-    p.out_live = live;
-    int rc = dtype == TIDE_DTYPE_BF16
-                 ? (head_dim == 128 ? open<__nv_bfloat16, 128>(p, st) : open<__nv_bfloat16, 64>(p, st))
-                 : (head_dim == 128 ? open<__half, 128>(p, st) : open<__half, 64>(p, st));
+  for (int64_t i = 0; i < n_seqs; i += plan.seqs) {
+    const int64_t n = n_seqs - i < plan.seqs ? n_seqs - i : plan.seqs;
+    const tide::q4::OpenParams o{batch, (int)i, (int)n, static_cast<const unsigned char *>(cache),
+                                 block_tables, max_pages, (int)n_pages, (int)page_size, (int)n_kv_heads, ws,
+                                 ws + plan.side, plan.wide, tables, live, plan.few};
+    rc = bf16 ? (wide ? open<__nv_bfloat16, 128>(o, st) : open<__nv_bfloat16, 64>(o, st))
+              : (wide ? open<__half, 128>(o, st) : open<__half, 64>(o, st));
     if (rc) return rc;
     // sequence i of this round is request i of the call where none are named
     const int64_t skip = seq_ids ? 0 : i;
     const int64_t row = cu_seqlens ? 0 : i;
-    rc = tide_paged_attention(
-        dtype, static_cast<const unsigned char *>(q) + row * q_row_stride * 2, q_row_stride, p.k, p.v,
-        r.seqs * r.wide, tide::q4::kOpenPage, tables + skip * r.wide, r.wide, n_requests - skip,
-        kv_lens + skip, cu_seqlens ? cu_seqlens + i : nullptr, seq_ids ? seq_ids + i : nullptr, n,
-        n_seqs_dev ? live : nullptr,
-        static_cast<unsigned char *>(out) + row * n_q_heads * head_dim * 2, cu_seqlens ? n_tokens : n,
-        n_q_heads, n_kv_heads, head_dim, max_kv_len, scale, ws + 2 * r.side + r.tables, r.inner,
-        error_word, stream);
+    const tide::RaggedBatch part{cu_seqlens ? cu_seqlens + i : nullptr, seq_ids ? seq_ids + i : nullptr,
+                                 kv_lens + skip, n_seqs_dev ? live : nullptr, (int)n,
+                                 (int)(n_requests - skip), (int)(cu_seqlens ? n_tokens : n),
+                                 (int)max_kv_len, error_word};
+    const tide::KeySource src{ws, ws + plan.side, 0, tables + skip * plan.wide, plan.wide,
+                              (int)(plan.seqs * plan.wide), 7};
+    static_assert(tide::q4::kOpenPage == 1 << 7, "");
+    rc = tide::paged_tiles(dtype, head_dim, part, src, plan.few,
+                           static_cast<const unsigned char *>(q) + row * q_row_stride * 2, q_row_stride,
+                           static_cast<unsigned char *>(out) + row * n_q_heads * head_dim * 2, n_q_heads,
+                           n_kv_heads, scale, ws + 2 * plan.side + plan.tables, st);
     if (rc) return rc;
   }
   return TIDE_OK;

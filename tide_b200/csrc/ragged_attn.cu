@@ -83,13 +83,13 @@
 #include <atomic>
 #include <type_traits>
 
+#include "attn_math.cuh"
 #include "ragged.cuh"
 #include "tc_ptx.cuh"
 
 namespace tide {
 namespace ragged {
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kRows = 128;   // rows of a tile
 constexpr int kKeys = 128;   // keys of a block
 constexpr int kQuarter = 32; // keys of a quarter of it
@@ -97,13 +97,6 @@ constexpr int kWarps = 12;
 constexpr int kReaders = 11; // warps that read the units: all but the one that finds them
 constexpr int kThreads = 32 * kWarps;
 constexpr int kCached = 4;   // sequences per lane that the unit search keeps in registers
-constexpr float kSlack = 8.f;  // log2 of how far a maximum may grow before a rescale
-// log2 of what the weights, and their sums, are multiplied by (see above)
-template <typename T>
-constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f;
-template <typename T>
-constexpr float kLifted = std::is_same<T, __half>::value ? 128.f : 1.f;  // 2^kLift
-
 template <int D>
 struct Shape {
   static constexpr int kHalves = D / 64;               // 128-byte column groups
@@ -692,11 +685,6 @@ __device__ void clean_values(const Params &p, Shared &sh, unsigned char *ring) {
 }
 
 // ----------------------------------------------------------------- softmax
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // Two floats in one register pair, and the two-lane forms of fma and add.
 __device__ __forceinline__ uint64_t pair(float a, float b) {
   uint64_t r;
@@ -721,28 +709,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  uint32_t r;
-  if constexpr (std::is_same<T, __half>::value)
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  else
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-// The same for weights.  Those of fp16 stop at its largest number: scores past
-// 2^24, which 32 bits hold to a step of 2 and more, may be that much above m + 8.
-template <typename T>
-__device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
-  if constexpr (std::is_same<T, __half>::value) {
-    uint32_t r;
-    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-  } else {
-    return pack2<T>(lo, hi);
-  }
-}
-
 // The values that the cleaner zeroed in the positions that this row sees, for
 // the columns [d0, d0 + 32): weight > 0 times a NaN or infinity is itself.
 template <typename T, int D, bool PAGED>
@@ -1149,24 +1115,6 @@ __device__ __forceinline__ void ldmatrix4_t(uint32_t (&r)[4], uint32_t addr) {
                : "r"(addr)
                : "memory");
 }
-// D[16 x 8] += A[16 x 16] B[16 x 8], 16-bit operands, fp32 accumulators.
-template <typename T>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                         uint32_t b1) {
-  if constexpr (std::is_same<T, __half>::value)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
 struct FewParams {
   RaggedBatch batch;
   KeySource src;
@@ -1191,12 +1139,6 @@ struct Few {
   static constexpr uint32_t kRing = kFewStages * 2 * kSide;      // of a warp
   static constexpr uint32_t kSmem = kFewWarps * kRing + 1024;    // + alignment
 };
-
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
-  uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
-  return r;
-}
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(32 * kFewWarps, NT <= 2 ? 3 : 2)
@@ -1226,35 +1168,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, NT <= 2 ? 3 : 2)
   const int live = live_sequences(p.batch);
   int seq = (int)(unit / p.hkv), tok0 = 0;  // this CTA's tokens from tok0 on
   if (p.few > p.tokens) {
-    // pieces of the sequences, counted in their order, 32 sequences at a time
-    int rest = seq, found = -1;
-    for (int b = 0; b < live && found < 0; b += 32) {
-      int mine = 0;
-      if (b + lane < live) {
-        int row, end;
-        const bool good = sequence_bounds(p.batch, b + lane, &row, &end);
-        // (one that has no piece here, and with that no CTA to flag it)
-        if (!good) raise_error(p.batch.err, TIDE_DEVERR_POSITION);
-        const int n = good ? end - row : 0;
-        mine = n <= p.few ? (n + p.tokens - 1) / p.tokens : 0;
-      }
-      int upto = mine;
-#pragma unroll
-      for (int w = 1; w < 32; w *= 2) {
-        const int x = __shfl_up_sync(kFull, upto, w);
-        if (lane >= w) upto += x;
-      }
-      const unsigned past = __ballot_sync(kFull, upto > rest);
-      if (past) {
-        const int at = __ffs(past) - 1;
-        found = b + at;
-        tok0 = (rest - __shfl_sync(kFull, upto - mine, at)) * p.tokens;
-      } else {
-        rest -= __shfl_sync(kFull, upto, 31);
-      }
-    }
-    if (found < 0) return;
-    seq = found;
+    if (!find_piece(p.batch, live, p.few, p.tokens, &seq, &tok0)) return;
   }
   if (seq >= live) return;
   Sequence s = sequence(p.batch, seq);
@@ -1708,8 +1622,9 @@ struct Plan {
   size_t few_bytes, bytes;  // workspace
 };
 
+// tiles_only: no few-rows kernel, whatever the sequences.
 Plan plan_paged(bool one_token, int64_t n_tokens, int64_t n_seqs, int64_t hq, int64_t hkv, int64_t d,
-                int64_t max_kv) {
+                int64_t max_kv, bool tiles_only = false) {
   using namespace tide::ragged;
   Plan p{};
   const int64_t group = hq / hkv;
@@ -1724,6 +1639,7 @@ Plan plan_paged(bool one_token, int64_t n_tokens, int64_t n_seqs, int64_t hq, in
   // known.
   p.few = one_token ? 1 : 2 * p.tokens;
   if (!one_token && (n_tokens * group > n_seqs * 16 || (n_seqs == 1 && n_tokens > p.few))) p.nt = 0;
+  if (tiles_only) p.nt = 0;
   if (!p.nt) p.few = 0;
   if (n_tokens < p.few) p.few = (int)n_tokens;
   p.tiles = !p.nt || (!one_token && n_tokens > p.few);
@@ -1904,6 +1820,44 @@ void set_heads(tide::ragged::Params &p, int64_t hq, int64_t hkv, int64_t d, floa
 }
 
 }  // namespace
+
+namespace tide {
+
+int join_few_rows(int dtype, int64_t head_dim, const RaggedBatch &b, int hq, int few, int splits,
+                  const float *part_o, const float2 *part_ml, void *out, cudaStream_t s) {
+  if (dtype == TIDE_DTYPE_BF16)
+    return head_dim == 128
+               ? launch_join<__nv_bfloat16, 128, true>(b, hq, few, splits, part_o, part_ml, out, s)
+               : launch_join<__nv_bfloat16, 64, true>(b, hq, few, splits, part_o, part_ml, out, s);
+  return head_dim == 128 ? launch_join<__half, 128, true>(b, hq, few, splits, part_o, part_ml, out, s)
+                         : launch_join<__half, 64, true>(b, hq, few, splits, part_o, part_ml, out, s);
+}
+
+size_t paged_tiles_workspace_size(int64_t n_tokens, int64_t n_seqs, int64_t hq, int64_t hkv, int64_t d,
+                                  int64_t max_kv) {
+  if (n_tokens < 1 || n_seqs < 1 || max_kv < 1) return 0;
+  return plan_paged(false, n_tokens, n_seqs, hq, hkv, d, max_kv, true).bytes;
+}
+
+int paged_tiles(int dtype, int64_t head_dim, const RaggedBatch &b, const KeySource &src, int few,
+                const void *q, int64_t q_stride, void *out, int64_t hq, int64_t hkv, float scale,
+                void *workspace, cudaStream_t s) {
+  const int64_t d = head_dim, kv_rows = (int64_t)src.n_pages * hkv << src.page_shift;
+  Plan plan = plan_paged(false, b.n_tokens, b.n_seqs, hq, hkv, d, b.max_kv, true);
+  plan.few = few;
+  unsigned char *ws = static_cast<unsigned char *>(workspace);
+  ragged::Params p{};
+  p.batch = b;
+  p.src = src;
+  set_heads(p, hq, hkv, d, scale, out);
+  if (dtype == TIDE_DTYPE_BF16)
+    return d == 128 ? run_paged<__nv_bfloat16, 128>(plan, p, dtype, q, q_stride, kv_rows, ws, s)
+                    : run_paged<__nv_bfloat16, 64>(plan, p, dtype, q, q_stride, kv_rows, ws, s);
+  return d == 128 ? run_paged<__half, 128>(plan, p, dtype, q, q_stride, kv_rows, ws, s)
+                  : run_paged<__half, 64>(plan, p, dtype, q, q_stride, kv_rows, ws, s);
+}
+
+}  // namespace tide
 
 extern "C" int tide_packed_attention(int dtype, const void *q, const void *k, const void *v,
                                      int64_t q_row_stride, int64_t kv_row_stride,
