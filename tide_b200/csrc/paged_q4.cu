@@ -407,20 +407,29 @@ __global__ void __launch_bounds__(256) open_kernel(const __grid_constant__ OpenP
 // --------------------------------------------------- attention of few rows
 // Sequences with few rows (tokens times the query heads of a KV head).  A CTA
 // takes 8 NT rows of a sequence, or of a split of its keys; its four warps walk
-// over every fourth block of 16 tokens each on their own, with their own ring of
-// bulk copies (a block is one copy), running maxima, sums and outputs, and meet
-// once at the end.  The rows are the narrow side of the products:
+// over every fourth block of 16 tokens each on their own, with their own running
+// maxima, sums and outputs, and meet once at the end.  The rows are the narrow
+// side of the products:
 //   S^T[16 x 8 NT] = K Q^T,   O^T[D x 8 NT] += V^T P^T    (mma.sync m16n8k16).
-// A lane makes its operands in registers from the codes, each exactly the value
-// that they stand for, so nothing is staged as 16 bits.  The order of the
-// tokens of a block, and of the channels, is free in both products, and chosen
-// so that a lane reads what it needs in wide pieces without bank conflicts:
+// A lane makes its operands in registers from the codes, so nothing is staged as
+// 16 bits.  The order of the tokens of a block, and of the channels, is free in
+// both products, and chosen so that a lane reads what it needs in wide pieces:
 //   row g of S is token kappa(g) = g / 2 + 4 (g % 2), row g + 8 the one 8 further;
 //   k-elements of lane t (of four) of S are the D / 4 channels from D / 4 t on, in
 //   one scale group;
 //   rows g and g + 8 of O's tiles are the D / 8 channels from D / 8 g on, their
 //   k-elements of lane t the tokens t, t + 4, t + 8, t + 12, whose scales lie side
 //   by side and whose pairs of codes come from two words' halves.
+// Each warp has a ring of bulk copies, a block one copy, and takes the words of the
+// next keys from it where those before have been used.  The sum of the weights, as
+// they meet the values, is one more row of the values' product.
+//
+// What bounds it is the instructions that make operands, so bf16 ones are (c - 8) s
+// instead of (c - z) s: one fma of the number 128 + c, whose code is its last bits,
+// with s and -136 s, all three exact (17 times a scale's four bits are eight).  The
+// rest, (8 - z) s, is the same for a group, and joins as one more product on both
+// sides: against the sums of the queries' groups, three bf16 each (24 bits), and
+// for the values as a tile with a row per group.  (fp16 has no room for 136 s.)
 constexpr int kFewWarps = 4;
 
 template <int D, int NT>
@@ -428,6 +437,8 @@ struct Few {
   static constexpr int kStages = NT <= 2 ? 6 : 8;
   static constexpr int kRing = kStages * Layout<D>::kBytes;  // of a warp
   static constexpr int kSmem = kFewWarps * kRing;
+  static constexpr int kPitch = D + 4;  // of a row of a warp's outputs, in its ring at the end
+  static_assert(8 * NT * kPitch * 4 <= kRing, "a warp's outputs fit its ring");
   static constexpr int kCtas = NT == 1 ? 4 : NT == 2 ? 3 : 2;  // of an SM
 };
 
@@ -455,14 +466,30 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
   return __byte_perm(a, b, sel);
 }
 
-// The weights as they meet the values, for the sum that divides them.
+// Two operands at a time from codes in the lowest four bits of a word's halves, by
+// the scales in the halves of another: (c - z) s, or for bf16 (c - 8) s, of which
+// rest() is the remainder.
 template <typename T>
-__device__ __forceinline__ float2 unpack_weights(uint32_t x) {
-  if constexpr (std::is_same<T, __half>::value)
-    return __half22float2(as_pair<T>(x));
-  else
-    return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
-}
+struct Maker {
+  Pars<T> p;
+  __device__ __forceinline__ explicit Maker(uint32_t scales) : p(pars<T>(scales)) {}
+  __device__ __forceinline__ uint32_t operator()(uint32_t x) const { return value2<T>(x, p); }
+  __device__ __forceinline__ uint32_t rest() const { return 0u; }
+};
+template <>
+struct Maker<__nv_bfloat16> {
+  Pars<__nv_bfloat16> p;
+  __nv_bfloat162 minus;  // -136 s
+  __device__ __forceinline__ explicit Maker(uint32_t scales)
+      : p(pars<__nv_bfloat16>(scales)), minus(__hmul2(p.scale, __float2bfloat162_rn(-136.f))) {}
+  __device__ __forceinline__ uint32_t operator()(uint32_t x) const {
+    return as_bits(__hfma2(as_pair<__nv_bfloat16>(numbers<__nv_bfloat16>(x)), p.scale, minus));
+  }
+  // 136 s - (128 + z) s
+  __device__ __forceinline__ uint32_t rest() const {
+    return as_bits(__hneg2(__hfma2(p.zero, p.scale, minus)));
+  }
+};
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
@@ -474,10 +501,13 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
   constexpr int kRowsMost = 8 * NT, kSteps = D / 16;
   constexpr int kKWords = D / 32;  // words of a lane's channels in a key
   constexpr int kVWords = D / 64;  // in a value
+  constexpr bool kCentred = !std::is_same<T, __half>::value;
   extern __shared__ __align__(128) unsigned char dyn[];
   __shared__ uint64_t full[kFewWarps][F::kStages];
-  __shared__ float s_m[kFewWarps][kRowsMost], s_l[kFewWarps][kRowsMost];
   __shared__ int s_abort;
+  constexpr int kSumRow = 4;  // of the values' last tile
+  static_assert(D / kGroup <= kSumRow, "");
+  __shared__ float s_m[kFewWarps][kRowsMost], s_l[kFewWarps][kRowsMost];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   if (threadIdx.x == 0) {
@@ -515,19 +545,19 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
       p.part_ml[part + (int64_t)(r / p.group) * p.hq + r % p.group] = make_float2(-INFINITY, 0.f);
     return;
   }
+
   unsigned char *ring = dyn + warp * F::kRing;
   __syncthreads();
 
   // this warp's blocks: warp, warp + 4, ... of the split's
   const int blocks = max(0, ((k1 - k0 + kBlock - 1) / kBlock - warp + kFewWarps - 1) / kFewWarps);
   const int page = 1 << p.page_shift;
-  auto key_of = [&](int i) { return k0 + (warp + i * kFewWarps) * kBlock; };
   // where 32 blocks at a time are in the cache, one per lane, the next ones read
   // ahead; -1: a page outside it
   auto places = [&](int i0) {
     const int i = i0 + lane;
     if (i >= blocks) return -1;
-    const int at = key_of(i);
+    const int at = k0 + (warp + i * kFewWarps) * kBlock;
     const int pg = __ldg(p.tables + s.req * p.max_pages + (at >> p.page_shift));
     if (pg < 0 || pg >= p.n_pages) {
       raise_error(p.batch.err, TIDE_DEVERR_POSITION);
@@ -537,14 +567,13 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
   };
   const uint64_t once = l2_evict_first_policy();
   int now = places(0), next = places(32);
-  auto request = [&](int i) {
+  auto request = [&](int i, int st) {
     if (i >= blocks) return;
     if ((i & 31) == 0 && i) {
       now = next;
       next = places(i + 32);
     }
     const int place = __shfl_sync(kFull, now, i & 31);
-    const int st = i % F::kStages;
     unsigned char *to = ring + st * L::kBytes;
     if (place >= 0) {
       if (lane == 0) {
@@ -556,61 +585,21 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(&full[warp][st]);
     }
-    __syncwarp();
   };
-  for (int i = 0; i < F::kStages; ++i) request(i);
-
-  // Q^T: columns are rows 8 nt + g; the statistics of a column are kept by the
-  // lanes whose accumulators belong to it, columns 8 nt + 2 t and one further
-  uint32_t qb[NT][kSteps][2];
-  int sees[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int r = nt * 8 + g;
-    const bool valid = r < rows;
-    const T *q = static_cast<const T *>(p.q) + (s.row0 + (valid ? r / p.group : 0)) * p.q_stride +
-                 (int64_t)(kvh * p.group + (valid ? r % p.group : 0)) * D + t * (D / 4);
-#pragma unroll
-    for (int w = 0; w < kKWords; ++w) {
-      const uint4 x = valid ? *reinterpret_cast<const uint4 *>(q + 8 * w) : make_uint4(0, 0, 0, 0);
-      qb[nt][2 * w][0] = x.x;
-      qb[nt][2 * w][1] = x.y;
-      qb[nt][2 * w + 1][0] = x.z;
-      qb[nt][2 * w + 1][1] = x.w;
-    }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int c = nt * 8 + t * 2 + e;
-      sees[nt][e] = pos0 + (c < rows ? c / p.group : s.n - 1) + 1;
-    }
-  }
-  float o[NT][kSteps][4], m[NT][2], l[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    m[nt][0] = m[nt][1] = -INFINITY;
-    l[nt][0] = l[nt][1] = 0.f;
-#pragma unroll
-    for (int d = 0; d < kSteps; ++d) o[nt][d][0] = o[nt][d][1] = o[nt][d][2] = o[nt][d][3] = 0.f;
-  }
-  const float slack = kSlack / p.qs;
+#pragma unroll 1
+  for (int i = 0; i < F::kStages; ++i) request(i, i);
   const int kappa = (g >> 1) + 4 * (g & 1);
-  int i = 0;
-  for (; i < blocks; ++i) {
-    const int st = i % F::kStages;
-    if (!__all_sync(kFull, ptx::mbar_wait(&full[warp][st], (i / F::kStages) & 1, &s_abort))) {
-      raise_error(p.batch.err, TIDE_DEVERR_TIMEOUT);
-      s_abort = 1;
-      break;
-    }
-    const unsigned char *b = ring + st * L::kBytes;
-    const int key = key_of(i);
-    const int seen = s.kv - key;                   // keys of the block that exist
-    const bool partial = key + kBlock > pos0 + 1;  // some row does not see all of them
-    // the block's words and scales of this lane
-    uint32_t kw[2][kKWords], vw[4][kVWords];
+  const int k_at = L::codes(0, kappa) + t * (D / 8), ks_at = L::scale(0, t * (D / 4) / kGroup, g >> 1);
+  const int v_at = L::codes(1, t) + g * (D / 16), vs_at = L::scale(1, g * (D / 8) / kGroup, t);
+  const int vc_at = L::scale(1, g % (D / kGroup), t);
+  // what a lane needs of a block: words of two keys and of four values, and the
+  // scales of four tokens; vc: of the group that is its row of the last tile
+  uint32_t kw[2][kKWords], vw[4][kVWords];
+  uint2 ks, vs, vc = make_uint2(0, 0);
+  auto take_keys = [&](const unsigned char *b) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const unsigned char *at = b + L::codes(0, kappa + 8 * h) + t * (D / 8);
+      const unsigned char *at = b + k_at + 8 * h * L::kRow;
       if constexpr (D == 128) {
         const uint4 x = *reinterpret_cast<const uint4 *>(at);
         kw[h][0] = x.x, kw[h][1] = x.y, kw[h][2] = x.z, kw[h][3] = x.w;
@@ -619,9 +608,12 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
         kw[h][0] = x.x, kw[h][1] = x.y;
       }
     }
+    ks = *reinterpret_cast<const uint2 *>(b + ks_at);
+  };
+  auto take_values = [&](const unsigned char *b) {
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
-      const unsigned char *at = b + L::codes(1, t + 4 * h) + g * (D / 16);
+      const unsigned char *at = b + v_at + 4 * h * L::kRow;
       if constexpr (D == 128) {
         const uint2 x = *reinterpret_cast<const uint2 *>(at);
         vw[h][0] = x.x, vw[h][1] = x.y;
@@ -629,64 +621,151 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
         vw[h][0] = *reinterpret_cast<const uint32_t *>(at);
       }
     }
-    const int v_group = g * (D / 8) / kGroup;
-    const uint2 ks = *reinterpret_cast<const uint2 *>(b + L::scale(0, t * (D / 4) / kGroup, g >> 1));
-    uint2 vs = *reinterpret_cast<const uint2 *>(b + L::scale(1, v_group, t));
+    vs = *reinterpret_cast<const uint2 *>(b + vs_at);
+    if constexpr (kCentred) {
+      if (g < D / kGroup) vc = *reinterpret_cast<const uint2 *>(b + vc_at);
+    }
+  };
+
+  // Q^T: columns are rows 8 nt + g; the statistics of a column are kept by the
+  // lanes whose accumulators belong to it, columns 8 nt + 2 t and one further
+  uint32_t qb[NT][kSteps][2], qc[NT][2];
+  int sees[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = nt * 8 + g;
+    const bool valid = r < rows;
+    const T *q = static_cast<const T *>(p.q) + (s.row0 + (valid ? r / p.group : 0)) * p.q_stride +
+                 (int64_t)(kvh * p.group + (valid ? r % p.group : 0)) * D + t * (D / 4);
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kKWords; ++w) {
+      const uint4 x = valid ? *reinterpret_cast<const uint4 *>(q + 8 * w) : make_uint4(0, 0, 0, 0);
+      qb[nt][2 * w][0] = x.x;
+      qb[nt][2 * w][1] = x.y;
+      qb[nt][2 * w + 1][0] = x.z;
+      qb[nt][2 * w + 1][1] = x.w;
+      if constexpr (kCentred) {
+        float f[8];
+        unpack16<T>(x, f);
+        sum += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+      }
+    }
+    if constexpr (kCentred) {  // the group's sum in three numbers; where two lanes share it, the even one's
+      if (D == 64) sum += __shfl_xor_sync(kFull, sum, 1);
+      if (D == 64 && (t & 1)) sum = 0.f;
+      const float high = Elem<T>::to_f(Elem<T>::from_f(sum));
+      const float mid = Elem<T>::to_f(Elem<T>::from_f(sum - high));
+      qc[nt][0] = pack2<T>(high, mid);
+      qc[nt][1] = pack2<T>(sum - high - mid, 0.f);
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int c = nt * 8 + t * 2 + e;
+      sees[nt][e] = pos0 + (c < rows ? c / p.group : s.n - 1) + 1;
+    }
+  }
+  // (a weight is 2^(score qs + up); raised where a score passes `most`)
+  float o[NT][kSteps][4], oc[NT][4], up[NT][2], most[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    up[nt][0] = up[nt][1] = kLift<T>;
+    most[nt][0] = most[nt][1] = -INFINITY;
+    oc[nt][0] = oc[nt][1] = oc[nt][2] = oc[nt][3] = 0.f;
+#pragma unroll
+    for (int d = 0; d < kSteps; ++d) o[nt][d][0] = o[nt][d][1] = o[nt][d][2] = o[nt][d][3] = 0.f;
+  }
+  const float slack = kSlack / p.qs;
+  int st = 0;
+  uint32_t phase = 0;  // of the stage st
+  bool lost = false;   // a wait has run out
+  auto arrived = [&](int st, uint32_t phase) {
+    if (__all_sync(kFull, ptx::mbar_wait(&full[warp][st], phase, &s_abort))) return true;
+    raise_error(p.batch.err, TIDE_DEVERR_TIMEOUT);
+    s_abort = 1;
+    return false;
+  };
+  if (blocks) {
+    lost = !arrived(0, 0);
+    if (!lost) take_keys(ring);
+  }
+  int i = 0;
+#pragma unroll 1
+  for (; i < blocks && !lost; ++i) {
+    const int key = k0 + (warp + i * kFewWarps) * kBlock;
+    const int seen = s.kv - key;                   // keys of the block that exist
+    const bool partial = key + kBlock > pos0 + 1;  // some row does not see all of them
+    float sc[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+    {
+      const uint32_t both = g & 1 ? 0x3232u : 0x1010u;
+      const Maker<T> p0(prmt(ks.x, 0u, both)), p1(prmt(ks.y, 0u, both));
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) {
+        const int sh = 8 * (k & 1);
+        const uint32_t w0 = kw[0][k / 2], w1 = kw[1][k / 2];
+        const uint32_t a[4] = {p0(w0 >> sh), p1(w1 >> sh), p0(w0 >> (sh + 4)), p1(w1 >> (sh + 4))};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma16816<T>(sc[nt], a, qb[nt][k][0], qb[nt][k][1]);
+      }
+      if constexpr (kCentred) {
+        const uint32_t a[4] = {p0.rest(), p1.rest(), p0.rest(), p1.rest()};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma16816<T>(sc[nt], a, qc[nt][0], qc[nt][1]);
+      }
+    }
+    const unsigned char *b = ring + st * L::kBytes;
+    take_values(b);
+    const int st1 = st + 1 == F::kStages ? 0 : st + 1;
+    const uint32_t phase1 = phase ^ (st1 == 0);
+    if (i + 1 < blocks) {
+      lost = !arrived(st1, phase1);
+      if (!lost) take_keys(ring + st1 * L::kBytes);
+    }
     // Masked values: a weight of 0 does not silence a NaN.  Past the last key a
     // token's scales are dropped; before it, where rows differ, those that are
     // NaN are, and added to the rows that do see them.
-    if (seen < kBlock) {
-      if (t >= seen) vs.x &= 0xffff0000u;
-      if (t + 4 >= seen) vs.x &= 0x0000ffffu;
-      if (t + 8 >= seen) vs.y &= 0xffff0000u;
-      if (t + 12 >= seen) vs.y &= 0x0000ffffu;
-    }
-    if (partial && s.n > 1) {
-      auto odd = [](uint32_t x) { return (x & 0x7f80u) == 0x7f80u; };
-      if (__any_sync(kFull, odd(vs.x) || odd(vs.x >> 16) || odd(vs.y) || odd(vs.y >> 16))) {
-        // rare: token by token
+    if (partial) {
+      auto drop = [](uint2 &x, int h) {
+        if (h == 0) x.x &= 0xffff0000u;
+        if (h == 1) x.x &= 0x0000ffffu;
+        if (h == 2) x.y &= 0xffff0000u;
+        if (h == 3) x.y &= 0x0000ffffu;
+      };
+      auto odd = [](const uint2 &x, int h) {
+        return (((h < 2 ? x.x : x.y) >> (h & 1) * 16) & 0x7f80u) == 0x7f80u;
+      };
+#pragma unroll
+      for (int h = 0; h < 4; ++h)
+        if (t + 4 * h >= seen) drop(vs, h), drop(vc, h);
+      if (s.n > 1 && __any_sync(kFull, odd(vs, 0) || odd(vs, 1) || odd(vs, 2) || odd(vs, 3))) {
+        // rare: token by token, its scale being with lane 4 g + its number % 4
 #pragma unroll 1
-        for (int k = 0; k < min(seen, kBlock); ++k) {
-          if (!odd(*reinterpret_cast<const uint16_t *>(b + L::scale(1, v_group, k)))) continue;
+        for (int k = 0; k < kBlock; ++k) {
+          const uint32_t pair = __shfl_sync(kFull, k < 8 ? vs.x : vs.y, (lane & 28) + k % 4);
+          if (((pair >> (k / 4 & 1) * 16) & 0x7f80u) != 0x7f80u) continue;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int d = 0; d < kSteps; ++d)
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                if (key + k < sees[nt][e & 1]) o[nt][d][e] += NAN;
+                if (key + k < sees[nt][e & 1]) o[nt][d][e] = NAN;
         }
-        if (odd(vs.x)) vs.x &= 0xffff0000u;
-        if (odd(vs.x >> 16)) vs.x &= 0x0000ffffu;
-        if (odd(vs.y)) vs.y &= 0xffff0000u;
-        if (odd(vs.y >> 16)) vs.y &= 0x0000ffffu;
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          if (odd(vs, h)) drop(vs, h);
+          if (odd(vc, h)) drop(vc, h);
+        }
       }
     }
-    __syncwarp();  // the stage has been read
-    ptx::fence_proxy_async();
-    request(i + F::kStages);
 
-    float sc[NT][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
-    {
-      const uint32_t both = g & 1 ? 0x3232u : 0x1010u;
-      const Pars<T> p0 = pars<T>(prmt(ks.x, 0u, both)), p1 = pars<T>(prmt(ks.y, 0u, both));
-#pragma unroll
-      for (int k = 0; k < kSteps; ++k) {
-        const int sh = 8 * (k & 1);
-        const uint32_t w0 = kw[0][k / 2] >> sh, w1 = kw[1][k / 2] >> sh;
-        const uint32_t a[4] = {value2<T>(w0, p0), value2<T>(w1, p1), value2<T>(w0 >> 4, p0),
-                               value2<T>(w1 >> 4, p1)};
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          if (nt < tiles) mma16816<T>(sc[nt], a, qb[nt][k][0], qb[nt][k][1]);
-      }
-    }
     uint32_t pt[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      if (nt >= tiles) continue;
+      pt[nt][0] = pt[nt][1] = 0u;
+      if (NT > 1 && nt >= tiles) continue;
       bool raise = false;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -696,7 +775,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
           if (lim <= 0) sc[nt][e] = -INFINITY;
           if (lim <= 8) sc[nt][2 + e] = -INFINITY;
         }
-        raise |= fmaxf(sc[nt][e], sc[nt][2 + e]) > m[nt][e] + slack;  // (the first keys: m is -infinity)
+        raise |= fmaxf(sc[nt][e], sc[nt][2 + e]) > most[nt][e];  // (the first keys: of -infinity)
       }
       if (__any_sync(kFull, raise)) {
         float a[2];
@@ -705,10 +784,13 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
           float top = fmaxf(sc[nt][e], sc[nt][2 + e]);
 #pragma unroll
           for (int w = 4; w < 32; w *= 2) top = fmaxf(top, __shfl_xor_sync(kFull, top, w));
-          const bool up = top > m[nt][e] + slack;
-          a[e] = up ? ex2((m[nt][e] - top) * p.qs) : 1.f;
-          if (up) m[nt][e] = top;
-          l[nt][e] *= a[e];
+          const bool raised = top > most[nt][e];
+          const float to = raised ? fmaf(-top, p.qs, kLift<T>) : up[nt][e];
+          // (nothing there yet: whatever the factor)
+          a[e] = most[nt][e] == -INFINITY ? 0.f : ex2(to - up[nt][e]);
+          up[nt][e] = to;
+          if (raised) most[nt][e] = top + slack;
+          oc[nt][e] *= a[e];
         }
 #pragma unroll
         for (int d = 0; d < kSteps; ++d) {
@@ -720,65 +802,62 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
       }
       float x[4];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float mq = (m[nt][e] == -INFINITY ? 0.f : m[nt][e] * p.qs) - kLift<T>;
-        x[e] = ex2(fmaf(sc[nt][e], p.qs, -mq));
-        x[2 + e] = ex2(fmaf(sc[nt][2 + e], p.qs, -mq));
-      }
-      const uint32_t w0 = pack_weights<T>(x[0], x[1]), w1 = pack_weights<T>(x[2], x[3]);
-      const float2 f0 = unpack_weights<T>(w0), f1 = unpack_weights<T>(w1);
-      l[nt][0] += f0.x + f1.x;
-      l[nt][1] += f0.y + f1.y;
-      pt[nt][0] = transpose8x8(w0);
-      pt[nt][1] = transpose8x8(w1);
+      for (int e = 0; e < 4; ++e) x[e] = ex2(fmaf(sc[nt][e], p.qs, up[nt][e & 1]));
+      pt[nt][0] = transpose8x8(pack_weights<T>(x[0], x[1]));
+      pt[nt][1] = transpose8x8(pack_weights<T>(x[2], x[3]));
     }
     {
-      const Pars<T> p0 = pars<T>(vs.x), p1 = pars<T>(vs.y);
+      const Maker<T> p0(vs.x), p1(vs.y);
 #pragma unroll
-      for (int w = 0; w < kVWords; ++w) {
-        const uint32_t lo0 = prmt(vw[0][w], vw[1][w], 0x5410u), hi0 = prmt(vw[0][w], vw[1][w], 0x7632u);
-        const uint32_t lo1 = prmt(vw[2][w], vw[3][w], 0x5410u), hi1 = prmt(vw[2][w], vw[3][w], 0x7632u);
+      for (int x = 0; x < kVWords; ++x) {
+        const uint32_t lo0 = prmt(vw[0][x], vw[1][x], 0x5410u), hi0 = prmt(vw[0][x], vw[1][x], 0x7632u);
+        const uint32_t lo1 = prmt(vw[2][x], vw[3][x], 0x5410u), hi1 = prmt(vw[2][x], vw[3][x], 0x7632u);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const uint32_t a[4] = {value2<T>(lo0 >> 4 * k, p0), value2<T>(hi0 >> 4 * k, p0),
-                                 value2<T>(lo1 >> 4 * k, p1), value2<T>(hi1 >> 4 * k, p1)};
+          const uint32_t a[4] = {p0(lo0 >> 4 * k), p0(hi0 >> 4 * k), p1(lo1 >> 4 * k), p1(hi1 >> 4 * k)};
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            if (nt < tiles) mma16816<T>(o[nt][4 * w + k], a, pt[nt][0], pt[nt][1]);
+          for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[nt][4 * x + k], a, pt[nt][0], pt[nt][1]);
         }
       }
+      constexpr uint32_t kOnes = kCentred ? 0x3f803f80u : 0x3c003c00u;
+      const uint32_t a[4] = {g == kSumRow ? kOnes : Maker<T>(vc.x).rest(), 0u,
+                             g == kSumRow ? kOnes : Maker<T>(vc.y).rest(), 0u};
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) mma16816<T>(oc[nt], a, pt[nt][0], pt[nt][1]);
     }
+    __syncwarp();  // the stage has been read
+    ptx::fence_proxy_async();
+    if (!lost) request(i + F::kStages, st);
+    st = st1;
+    phase = phase1;
   }
-  if (i < blocks && lane == 0) {  // given up: wait for the copies in flight (bounded)
+  if (lost && lane == 0) {  // wait for the copies in flight (bounded)
     volatile int none = 0;
     for (int e = i; e < min(blocks, i + F::kStages); ++e)
       ptx::mbar_wait(&full[warp][e % F::kStages], (e / F::kStages) & 1, &none);
   }
   __syncwarp();
 
-  // the four warps' outputs meet: this warp's in its own ring, [row][D + 4]
-  constexpr int kPitch = D + 4;
+  // the four warps' outputs meet, [warp][row][D + 4]
   float *mine = reinterpret_cast<float *>(ring);
-  static_assert(kRowsMost * kPitch * 4 <= F::kRing, "a warp's output fits its ring");
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int r = nt * 8 + t * 2 + e;
-      float sum = l[nt][e];
-#pragma unroll
-      for (int w = 4; w < 32; w *= 2) sum += __shfl_xor_sync(kFull, sum, w);
-      if (g == 0) {
-        s_m[warp][r] = m[nt][e] * p.qs;
-        s_l[warp][r] = sum;
+      if (g == kSumRow) {
+        s_m[warp][r] = kLift<T> - up[nt][e];
+        s_l[warp][r] = oc[nt][e];
       }
+      // (the lane's channels are in group g * (D / 8) / 32, whose sum is row of that number)
+      const float rest =
+          kCentred ? __shfl_sync(kFull, oc[nt][e], g * (D / 8) / kGroup * 4 + t) : 0.f;
 #pragma unroll
       for (int d = 0; d < kSteps; ++d)
-        *reinterpret_cast<float2 *>(mine + r * kPitch + g * (D / 8) + 2 * d) =
-            make_float2(o[nt][d][e], o[nt][d][2 + e]);
+        *reinterpret_cast<float2 *>(mine + r * F::kPitch + g * (D / 8) + 2 * d) =
+            make_float2(o[nt][d][e] + rest, o[nt][d][2 + e] + rest);
     }
   __syncthreads();
-  const float *all = reinterpret_cast<const float *>(dyn);
   constexpr int kLanes = D / 4;  // lanes of a row, four columns each
   for (int r = threadIdx.x / kLanes; r < rows; r += 32 * kFewWarps / kLanes) {
     const int d = threadIdx.x % kLanes * 4;
@@ -791,7 +870,8 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
     for (int w = 0; w < kFewWarps; ++w) {
       if (s_l[w][r] == 0.f) continue;
       const float a = exp2f(s_m[w][r] - top);
-      const float4 y = *reinterpret_cast<const float4 *>(all + w * (F::kRing / 4) + r * kPitch + d);
+      const float4 y = *reinterpret_cast<const float4 *>(
+          reinterpret_cast<const float *>(dyn + w * F::kRing) + r * F::kPitch + d);
       sum = fmaf(a, s_l[w][r], sum);
       x.x = fmaf(a, y.x, x.x);
       x.y = fmaf(a, y.y, x.y);
@@ -924,13 +1004,12 @@ Plan plan_of(bool one_token, int64_t n_tokens, int64_t n_seqs, int64_t n_request
 template <typename T, int D, int NT>
 int launch_few(const tide::q4::FewParams &p, cudaStream_t s) {
   using namespace tide::q4;
-  using F = Few<D, NT>;
   auto kern = few_rows_kernel<T, D, NT>;
+  constexpr int smem = Few<D, NT>::kSmem;
   static std::atomic<uint64_t> set{0};  // per device
-  const cudaError_t e = tide::allow_smem(kern, F::kSmem, set);
+  const cudaError_t e = smem > 48 << 10 ? tide::allow_smem(kern, smem, set) : cudaSuccess;
   if (e != cudaSuccess) return report(e, "paged_attention_q4");
-  return start("paged_attention_q4", kern, (int64_t)p.pieces * p.hkv * p.splits, 32 * kFewWarps, F::kSmem,
-               s, p);
+  return start("paged_attention_q4", kern, (int64_t)p.pieces * p.hkv * p.splits, 32 * kFewWarps, smem, s, p);
 }
 
 template <typename T, int D>
