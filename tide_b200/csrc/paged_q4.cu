@@ -405,11 +405,18 @@ __global__ void __launch_bounds__(256) open_kernel(const __grid_constant__ OpenP
 }
 
 // --------------------------------------------------- attention of few rows
-// Sequences with few rows (tokens times the query heads of a KV head).  A CTA
-// takes 8 NT rows of a sequence, or of a split of its keys; its four warps walk
-// over every fourth block of 16 tokens each on their own, with their own running
-// maxima, sums and outputs, and meet once at the end.  The rows are the narrow
-// side of the products:
+// Sequences with few rows (tokens times the query heads of a KV head).  A unit is
+// up to 8 NT rows of a sequence, over the blocks of its keys in one head.  All
+// blocks of all units in a row are dealt out evenly to as many CTAs as run at once,
+// found from the lengths by a prefix sum that each makes, so a CTA has the end of
+// one unit, some whole ones, and the beginning of another; units that two or more
+// CTAs share are joined by a kernel of their own, in the order of the keys.  (With a
+// CTA a unit, and splits of equal length, a decode step of 192 requests left the
+// SMs idle for a sixth of its time, and one of three very different requests for
+// half.)  Short contexts are dealt out by whole units, and need no join.
+// A CTA's four warps walk over every fourth block of its part of a unit each on
+// their own, with their own running maxima, sums and outputs, and meet at its end.
+// The rows are the narrow side of the products:
 //   S^T[16 x 8 NT] = K Q^T,   O^T[D x 8 NT] += V^T P^T    (mma.sync m16n8k16).
 // A lane makes its operands in registers from the codes, so nothing is staged as
 // 16 bits.  The order of the tokens of a block, and of the channels, is free in
@@ -420,9 +427,9 @@ __global__ void __launch_bounds__(256) open_kernel(const __grid_constant__ OpenP
 //   rows g and g + 8 of O's tiles are the D / 8 channels from D / 8 g on, their
 //   k-elements of lane t the tokens t, t + 4, t + 8, t + 12, whose scales lie side
 //   by side and whose pairs of codes come from two words' halves.
-// Each warp has a ring of bulk copies, a block one copy, and takes the words of the
-// next keys from it where those before have been used.  The sum of the weights, as
-// they meet the values, is one more row of the values' product.
+// Each warp has two places for three blocks each, a bulk copy a block: one that it
+// works on and one under way.  The sum of the weights, as they meet the values, is
+// one more row of the values' product.
 //
 // What bounds it is the instructions that make operands, so bf16 ones are (c - 8) s
 // instead of (c - z) s: one fma of the number 128 + c, whose code is its last bits,
@@ -431,15 +438,25 @@ __global__ void __launch_bounds__(256) open_kernel(const __grid_constant__ OpenP
 // sides: against the sums of the queries' groups, three bf16 each (24 bits), and
 // for the values as a tile with a row per group.  (fp16 has no room for 136 s.)
 constexpr int kFewWarps = 4;
+constexpr int kBatch = 3;        // blocks of a place
+constexpr int kLeastBlocks = 8;  // of a CTA, where there are so few
 
 template <int D, int NT>
 struct Few {
-  static constexpr int kStages = NT <= 2 ? 6 : 8;
-  static constexpr int kRing = kStages * Layout<D>::kBytes;  // of a warp
+  static constexpr int kPlace = kBatch * Layout<D>::kBytes;
+  static constexpr int kPitch = D + 4;                     // of a row of a warp's outputs, in its ring at the end
+  static constexpr int kOutputs = 8 * NT * kPitch * 4;
+  static constexpr int kRing = 2 * kPlace > kOutputs ? 2 * kPlace : (kOutputs + 127) / 128 * 128;  // of a warp
   static constexpr int kSmem = kFewWarps * kRing;
-  static constexpr int kPitch = D + 4;  // of a row of a warp's outputs, in its ring at the end
-  static_assert(8 * NT * kPitch * 4 <= kRing, "a warp's outputs fit its ring");
-  static constexpr int kCtas = NT == 1 ? 4 : NT == 2 ? 3 : 2;  // of an SM
+  static constexpr int kCtas = NT == 1 ? 4 : 3;  // of an SM
+};
+
+// A unit that several CTAs share, as the second of them has it.
+struct Shared {
+  int first, last;  // CTAs; first < 0: none
+  int seq_row;      // its sequence's first packed row
+  int row, rows;    // its rows among the sequence's [token, head of the group]
+  int kvh;
 };
 
 struct FewParams {
@@ -451,16 +468,27 @@ struct FewParams {
   const void *q;
   int64_t q_stride;
   void *out;
-  float *part_o;    // [splits, n_seqs, few, hq, D] (splits > 1)
-  float2 *part_ml;  // [splits, n_seqs, few, hq]: maximum (scaled, base 2), sum
+  float *part_o;    // [CTAs, 2, 8 NT, D]: of a unit that the CTA ends, of one that it begins
+  float2 *part_ml;  // [CTAs, 2, 8 NT]: maximum (scaled, base 2), sum
+  Shared *shared;   // [CTAs]: the unit that it ends
   int hq, hkv, group;
-  int few;         // tokens a sequence may have
-  int tokens;      // of a CTA: 8 NT / group
-  int pieces;      // pieces of up to `tokens` tokens that the sequences may have
-  int splits;
-  int split_keys;  // keys of a split, a multiple of 16
+  int few;             // tokens a sequence may have
+  int whole;           // units are not split
   float qs;
+  uint32_t magic;      // kMagic of the rows' type
+  uint32_t per_group;  // 2^31 / group, rounded up
 };
+
+// Row r / group of a sequence (exact for r < 2^17).
+__device__ __forceinline__ int token_of(int r, uint32_t per_group) {
+  return (int)((uint64_t)(uint32_t)r * per_group >> 31);
+}
+
+// a / b, both positive: by 32-bit numbers, where they are (the other is a hundred
+// instructions).
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  return ((a | b) >> 31) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
   return __byte_perm(a, b, sel);
@@ -468,27 +496,37 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
 
 // Two operands at a time from codes in the lowest four bits of a word's halves, by
 // the scales in the halves of another: (c - z) s, or for bf16 (c - 8) s, of which
-// rest() is the remainder.
+// minus_rest() is the negative remainder.
 template <typename T>
 struct Maker {
   Pars<T> p;
-  __device__ __forceinline__ explicit Maker(uint32_t scales) : p(pars<T>(scales)) {}
-  __device__ __forceinline__ uint32_t operator()(uint32_t x) const { return value2<T>(x, p); }
-  __device__ __forceinline__ uint32_t rest() const { return 0u; }
+  uint32_t magic;
+  __device__ __forceinline__ Maker(uint32_t scales, uint32_t magic) : p(pars<T>(scales, magic)), magic(magic) {}
+  __device__ __forceinline__ uint32_t operator()(uint32_t x) const { return value2<T>(x, p, magic); }
+  __device__ __forceinline__ uint32_t minus_rest() const { return 0u; }
 };
 template <>
 struct Maker<__nv_bfloat16> {
   Pars<__nv_bfloat16> p;
   __nv_bfloat162 minus;  // -136 s
-  __device__ __forceinline__ explicit Maker(uint32_t scales)
-      : p(pars<__nv_bfloat16>(scales)), minus(__hmul2(p.scale, __float2bfloat162_rn(-136.f))) {}
+  uint32_t magic;
+  __device__ __forceinline__ Maker(uint32_t scales, uint32_t magic)
+      : p(pars<__nv_bfloat16>(scales, magic)),
+        minus(__hmul2(p.scale, __float2bfloat162_rn(-136.f))),
+        magic(magic) {}
   __device__ __forceinline__ uint32_t operator()(uint32_t x) const {
-    return as_bits(__hfma2(as_pair<__nv_bfloat16>(numbers<__nv_bfloat16>(x)), p.scale, minus));
+    return as_bits(__hfma2(as_pair<__nv_bfloat16>(numbers(x, magic)), p.scale, minus));
   }
-  // 136 s - (128 + z) s
-  __device__ __forceinline__ uint32_t rest() const {
-    return as_bits(__hneg2(__hfma2(p.zero, p.scale, minus)));
-  }
+  // (128 + z) s - 136 s
+  __device__ __forceinline__ uint32_t minus_rest() const { return as_bits(__hfma2(p.zero, p.scale, minus)); }
+};
+
+// A unit, or a CTA's part of it.
+struct Part {
+  Sequence s;
+  int seq, row;  // sequence, first of its rows
+  int kvh;
+  int b0, nb;    // first block of the part, blocks of the unit
 };
 
 template <typename T, int D, int NT>
@@ -502,312 +540,337 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
   constexpr int kKWords = D / 32;  // words of a lane's channels in a key
   constexpr int kVWords = D / 64;  // in a value
   constexpr bool kCentred = !std::is_same<T, __half>::value;
-  extern __shared__ __align__(128) unsigned char dyn[];
-  __shared__ uint64_t full[kFewWarps][F::kStages];
-  __shared__ int s_abort;
   constexpr int kSumRow = 4;  // of the values' last tile
   static_assert(D / kGroup <= kSumRow, "");
+  extern __shared__ __align__(128) unsigned char dyn[];
+  __shared__ uint64_t full[kFewWarps][2];
   __shared__ float s_m[kFewWarps][kRowsMost], s_l[kFewWarps][kRowsMost];
+  __shared__ long long s_sum[kFewWarps];
+  __shared__ Part s_part;
+  __shared__ int s_abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   if (threadIdx.x == 0) {
     for (int w = 0; w < kFewWarps; ++w)
-      for (int i = 0; i < F::kStages; ++i) ptx::mbar_init(&full[w][i], 1);
+      for (int i = 0; i < 2; ++i) ptx::mbar_init(&full[w][i], 1);
     ptx::fence_mbar_init();
     s_abort = 0;
   }
   ptx::grid_dependency_wait();  // up to here this overlaps the kernel before
   ptx::grid_dependents_launch();
-  const int split = (int)(blockIdx.x % p.splits);
-  const int64_t unit = blockIdx.x / p.splits;
-  const int kvh = (int)(unit % p.hkv);
   const int live = live_sequences(p.batch);
-  int seq = (int)(unit / p.hkv), tok0 = 0;  // this CTA's tokens from tok0 on
-  if (p.few > p.tokens && !find_piece(p.batch, live, p.few, p.tokens, &seq, &tok0)) return;
-  if (seq >= live) return;
-  Sequence s = sequence(p.batch, seq);
-  if (s.n > p.few || tok0 >= s.n) return;
-  {  // as a sequence of its own, which ends with its last token
-    const int rest = s.n - tok0 - p.tokens;
-    s.row0 += tok0;
-    s.n = rest > 0 ? p.tokens : s.n - tok0;
-    s.kv -= max(rest, 0);
+  // Keys that the last of the rows of a unit, from `row` on, sees; its blocks, and
+  // what it counts as where the units are dealt out.
+  auto keys_of = [&](const Sequence &s, int row) {
+    return s.kv - s.n + 1 + token_of(min(row + kRowsMost, s.n * p.group) - 1, p.per_group);
+  };
+  auto blocks_of = [&](const Sequence &s, int row) { return max((keys_of(s, row) + kBlock - 1) / kBlock, 1); };
+  auto cost_of = [&](const Sequence &s, int row) { return p.whole ? 1 : blocks_of(s, row); };
+  auto rows_of = [&](const Sequence &s) { return s.n <= p.few ? s.n * p.group : 0; };
+  auto weight = [&](const Sequence &s) {  // of all units of a sequence
+    long long w = 0;
+    for (int row = 0; row < rows_of(s); row += kRowsMost) w += cost_of(s, row);
+    return w * p.hkv;
+  };
+  long long pos, end;  // this CTA's are [pos, end) of all
+  int longer;          // the first `longer` CTAs have share + 1, the others share
+  long long share;
+  {
+    const int per = (live + 32 * kFewWarps - 1) / (32 * kFewWarps);
+    const int from = min((int)threadIdx.x * per, live), to = min(from + per, live);
+    long long sum = 0;
+    for (int i = from; i < to; ++i) sum += weight(sequence(p.batch, i));
+    long long upto = sum;
+#pragma unroll
+    for (int w = 1; w < 32; w *= 2) {
+      const long long x = __shfl_up_sync(kFull, upto, w);
+      if (lane >= w) upto += x;
+    }
+    if (lane == 31) s_sum[warp] = upto;
+    __syncthreads();
+    long long total = 0;
+    for (int w = 0; w < kFewWarps; ++w) {
+      if (w < warp) upto += s_sum[w];
+      total += s_sum[w];
+    }
+    const long long least = p.whole ? 1 : kLeastBlocks;
+    const int ctas = (int)min((long long)gridDim.x, (total + least - 1) / least);
+    if ((int)blockIdx.x >= ctas) {
+      if (threadIdx.x == 0 && !p.whole) p.shared[blockIdx.x].first = -1;
+      return;
+    }
+    share = quotient(total, ctas);
+    longer = (int)(total - share * ctas);
+    pos = share * blockIdx.x + min((int)blockIdx.x, longer);
+    end = pos + share + ((int)blockIdx.x < longer);
+    if (pos >= upto - sum && pos < upto) {
+      long long rest = pos - (upto - sum);
+      for (int i = from; i < to; ++i) {
+        const Sequence s = sequence(p.batch, i);
+        for (int row = 0; row < rows_of(s); row += kRowsMost) {
+          const long long c = cost_of(s, row);
+          if (rest >= 0 && rest < c * p.hkv) {
+            const int kvh = (int)quotient(rest, c);
+            s_part = {s, i, row, kvh, (int)(rest - kvh * c), blocks_of(s, row)};
+          }
+          rest -= c * p.hkv;
+        }
+      }
+    }
+    __syncthreads();
   }
-  const int rows = s.n * p.group;
-  const int tiles = (rows + 7) / 8;  // 8-row groups that there are
-  const int pos0 = s.kv - s.n;       // keys before the first token's own
-  const int k0 = split * p.split_keys, k1 = p.splits > 1 ? min(s.kv, k0 + p.split_keys) : s.kv;
-  const int64_t row0 = (int64_t)s.row0 * p.hq + kvh * p.group;  // of [token, head] rows
-  const int64_t part =
-      (((int64_t)split * p.batch.n_seqs + seq) * p.few + tok0) * p.hq + kvh * p.group;
-  if (p.splits > 1 && k0 >= k1) {  // no keys: a sum of 0
-    for (int r = threadIdx.x; r < rows; r += blockDim.x)
-      p.part_ml[part + (int64_t)(r / p.group) * p.hq + r % p.group] = make_float2(-INFINITY, 0.f);
-    return;
-  }
+  auto cta_of = [&](long long block) {
+    const long long at = longer * (share + 1);
+    return (int)(block < at ? quotient(block, share + 1) : longer + quotient(block - at, share));
+  };
 
   unsigned char *ring = dyn + warp * F::kRing;
-  __syncthreads();
-
-  // this warp's blocks: warp, warp + 4, ... of the split's
-  const int blocks = max(0, ((k1 - k0 + kBlock - 1) / kBlock - warp + kFewWarps - 1) / kFewWarps);
   const int page = 1 << p.page_shift;
-  // where 32 blocks at a time are in the cache, one per lane, the next ones read
-  // ahead; -1: a page outside it
-  auto places = [&](int i0) {
-    const int i = i0 + lane;
-    if (i >= blocks) return -1;
-    const int at = k0 + (warp + i * kFewWarps) * kBlock;
-    const int pg = __ldg(p.tables + s.req * p.max_pages + (at >> p.page_shift));
-    if (pg < 0 || pg >= p.n_pages) {
-      raise_error(p.batch.err, TIDE_DEVERR_POSITION);
-      return -1;
-    }
-    return (pg * p.hkv + kvh) * (page / kBlock) + (at & (page - 1)) / kBlock;
-  };
   const uint64_t once = l2_evict_first_policy();
-  int now = places(0), next = places(32);
-  auto request = [&](int i, int st) {
-    if (i >= blocks) return;
-    if ((i & 31) == 0 && i) {
-      now = next;
-      next = places(i + 32);
-    }
-    const int place = __shfl_sync(kFull, now, i & 31);
-    unsigned char *to = ring + st * L::kBytes;
-    if (place >= 0) {
-      if (lane == 0) {
-        ptx::mbar_expect_tx(&full[warp][st], L::kBytes);
-        ptx::bulk_load(to, p.cache + (int64_t)place * L::kBytes, L::kBytes, &full[warp][st], once);
-      }
-    } else {  // reads as zeros
-      for (int e = lane; e < L::kBytes / 16; e += 32) reinterpret_cast<uint4 *>(to)[e] = make_uint4(0, 0, 0, 0);
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&full[warp][st]);
-    }
-  };
-#pragma unroll 1
-  for (int i = 0; i < F::kStages; ++i) request(i, i);
   const int kappa = (g >> 1) + 4 * (g & 1);
   const int k_at = L::codes(0, kappa) + t * (D / 8), ks_at = L::scale(0, t * (D / 4) / kGroup, g >> 1);
   const int v_at = L::codes(1, t) + g * (D / 16), vs_at = L::scale(1, g * (D / 8) / kGroup, t);
   const int vc_at = L::scale(1, g % (D / kGroup), t);
-  // what a lane needs of a block: words of two keys and of four values, and the
-  // scales of four tokens; vc: of the group that is its row of the last tile
-  uint32_t kw[2][kKWords], vw[4][kVWords];
-  uint2 ks, vs, vc = make_uint2(0, 0);
-  auto take_keys = [&](const unsigned char *b) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const unsigned char *at = b + k_at + 8 * h * L::kRow;
-      if constexpr (D == 128) {
-        const uint4 x = *reinterpret_cast<const uint4 *>(at);
-        kw[h][0] = x.x, kw[h][1] = x.y, kw[h][2] = x.z, kw[h][3] = x.w;
-      } else {
-        const uint2 x = *reinterpret_cast<const uint2 *>(at);
-        kw[h][0] = x.x, kw[h][1] = x.y;
-      }
-    }
-    ks = *reinterpret_cast<const uint2 *>(b + ks_at);
-  };
-  auto take_values = [&](const unsigned char *b) {
-#pragma unroll
-    for (int h = 0; h < 4; ++h) {
-      const unsigned char *at = b + v_at + 4 * h * L::kRow;
-      if constexpr (D == 128) {
-        const uint2 x = *reinterpret_cast<const uint2 *>(at);
-        vw[h][0] = x.x, vw[h][1] = x.y;
-      } else {
-        vw[h][0] = *reinterpret_cast<const uint32_t *>(at);
-      }
-    }
-    vs = *reinterpret_cast<const uint2 *>(b + vs_at);
-    if constexpr (kCentred) {
-      if (g < D / kGroup) vc = *reinterpret_cast<const uint2 *>(b + vc_at);
-    }
-  };
-
-  // Q^T: columns are rows 8 nt + g; the statistics of a column are kept by the
-  // lanes whose accumulators belong to it, columns 8 nt + 2 t and one further
-  uint32_t qb[NT][kSteps][2], qc[NT][2];
-  int sees[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int r = nt * 8 + g;
-    const bool valid = r < rows;
-    const T *q = static_cast<const T *>(p.q) + (s.row0 + (valid ? r / p.group : 0)) * p.q_stride +
-                 (int64_t)(kvh * p.group + (valid ? r % p.group : 0)) * D + t * (D / 4);
-    float sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kKWords; ++w) {
-      const uint4 x = valid ? *reinterpret_cast<const uint4 *>(q + 8 * w) : make_uint4(0, 0, 0, 0);
-      qb[nt][2 * w][0] = x.x;
-      qb[nt][2 * w][1] = x.y;
-      qb[nt][2 * w + 1][0] = x.z;
-      qb[nt][2 * w + 1][1] = x.w;
-      if constexpr (kCentred) {
-        float f[8];
-        unpack16<T>(x, f);
-        sum += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
-      }
-    }
-    if constexpr (kCentred) {  // the group's sum in three numbers; where two lanes share it, the even one's
-      if (D == 64) sum += __shfl_xor_sync(kFull, sum, 1);
-      if (D == 64 && (t & 1)) sum = 0.f;
-      const float high = Elem<T>::to_f(Elem<T>::from_f(sum));
-      const float mid = Elem<T>::to_f(Elem<T>::from_f(sum - high));
-      qc[nt][0] = pack2<T>(high, mid);
-      qc[nt][1] = pack2<T>(sum - high - mid, 0.f);
-    }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int c = nt * 8 + t * 2 + e;
-      sees[nt][e] = pos0 + (c < rows ? c / p.group : s.n - 1) + 1;
-    }
-  }
-  // (a weight is 2^(score qs + up); raised where a score passes `most`)
-  float o[NT][kSteps][4], oc[NT][4], up[NT][2], most[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    up[nt][0] = up[nt][1] = kLift<T>;
-    most[nt][0] = most[nt][1] = -INFINITY;
-    oc[nt][0] = oc[nt][1] = oc[nt][2] = oc[nt][3] = 0.f;
-#pragma unroll
-    for (int d = 0; d < kSteps; ++d) o[nt][d][0] = o[nt][d][1] = o[nt][d][2] = o[nt][d][3] = 0.f;
-  }
   const float slack = kSlack / p.qs;
-  int st = 0;
-  uint32_t phase = 0;  // of the stage st
-  bool lost = false;   // a wait has run out
-  auto arrived = [&](int st, uint32_t phase) {
-    if (__all_sync(kFull, ptx::mbar_wait(&full[warp][st], phase, &s_abort))) return true;
-    raise_error(p.batch.err, TIDE_DEVERR_TIMEOUT);
-    s_abort = 1;
-    return false;
-  };
-  if (blocks) {
-    lost = !arrived(0, 0);
-    if (!lost) take_keys(ring);
-  }
-  int i = 0;
-#pragma unroll 1
-  for (; i < blocks && !lost; ++i) {
-    const int key = k0 + (warp + i * kFewWarps) * kBlock;
-    const int seen = s.kv - key;                   // keys of the block that exist
-    const bool partial = key + kBlock > pos0 + 1;  // some row does not see all of them
-    float sc[NT][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
-    {
-      const uint32_t both = g & 1 ? 0x3232u : 0x1010u;
-      const Maker<T> p0(prmt(ks.x, 0u, both)), p1(prmt(ks.y, 0u, both));
-#pragma unroll
-      for (int k = 0; k < kSteps; ++k) {
-        const int sh = 8 * (k & 1);
-        const uint32_t w0 = kw[0][k / 2], w1 = kw[1][k / 2];
-        const uint32_t a[4] = {p0(w0 >> sh), p1(w1 >> sh), p0(w0 >> (sh + 4)), p1(w1 >> (sh + 4))};
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma16816<T>(sc[nt], a, qb[nt][k][0], qb[nt][k][1]);
-      }
-      if constexpr (kCentred) {
-        const uint32_t a[4] = {p0.rest(), p1.rest(), p0.rest(), p1.rest()};
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma16816<T>(sc[nt], a, qc[nt][0], qc[nt][1]);
-      }
+  const uint32_t magic = p.magic;
+  uint32_t turn = 0;  // places used so far: the next is the last bit, its phase the one before
+  bool starts = true;
+  for (;;) {
+    const Part u = s_part;
+    const int pos0 = u.s.kv - u.s.n;  // keys before the first token's own
+    const int kv = keys_of(u.s, u.row);
+    const int rows = min(kRowsMost, u.s.n * p.group - u.row);
+    const int tiles = (rows + 7) / 8;  // 8-row groups that there are
+    const int b1 = p.whole ? u.nb : (int)min((long long)u.nb, u.b0 + (end - pos));
+    if (starts && !p.whole && threadIdx.x == 0) {
+      Shared x{-1, -1, u.s.row0, u.row, rows, u.kvh};
+      if (u.b0 > 0) x.first = cta_of(pos - u.b0), x.last = cta_of(pos - u.b0 + u.nb - 1);
+      p.shared[blockIdx.x] = x;
     }
-    const unsigned char *b = ring + st * L::kBytes;
-    take_values(b);
-    const int st1 = st + 1 == F::kStages ? 0 : st + 1;
-    const uint32_t phase1 = phase ^ (st1 == 0);
-    if (i + 1 < blocks) {
-      lost = !arrived(st1, phase1);
-      if (!lost) take_keys(ring + st1 * L::kBytes);
-    }
-    // Masked values: a weight of 0 does not silence a NaN.  Past the last key a
-    // token's scales are dropped; before it, where rows differ, those that are
-    // NaN are, and added to the rows that do see them.
-    if (partial) {
-      auto drop = [](uint2 &x, int h) {
-        if (h == 0) x.x &= 0xffff0000u;
-        if (h == 1) x.x &= 0x0000ffffu;
-        if (h == 2) x.y &= 0xffff0000u;
-        if (h == 3) x.y &= 0x0000ffffu;
-      };
-      auto odd = [](const uint2 &x, int h) {
-        return (((h < 2 ? x.x : x.y) >> (h & 1) * 16) & 0x7f80u) == 0x7f80u;
-      };
-#pragma unroll
-      for (int h = 0; h < 4; ++h)
-        if (t + 4 * h >= seen) drop(vs, h), drop(vc, h);
-      if (s.n > 1 && __any_sync(kFull, odd(vs, 0) || odd(vs, 1) || odd(vs, 2) || odd(vs, 3))) {
-        // rare: token by token, its scale being with lane 4 g + its number % 4
-#pragma unroll 1
-        for (int k = 0; k < kBlock; ++k) {
-          const uint32_t pair = __shfl_sync(kFull, k < 8 ? vs.x : vs.y, (lane & 28) + k % 4);
-          if (((pair >> (k / 4 & 1) * 16) & 0x7f80u) != 0x7f80u) continue;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int d = 0; d < kSteps; ++d)
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (key + k < sees[nt][e & 1]) o[nt][d][e] = NAN;
-        }
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          if (odd(vs, h)) drop(vs, h);
-          if (odd(vc, h)) drop(vc, h);
-        }
+    starts = false;
+    // this warp's blocks: b0 + warp, 4 further, ...
+    const int blocks = max(0, (b1 - u.b0 - warp + kFewWarps - 1) / kFewWarps);
+    const int block0 = u.b0 + warp;
+    // where 32 blocks at a time are in the cache, one per lane, the next ones read
+    // ahead; -1: a page outside it
+    auto places = [&](int i0) {
+      const int i = i0 + lane, at = (block0 + i * kFewWarps) * kBlock;
+      if (i >= blocks || at >= kv) return -1;  // (or a unit without keys)
+      const int pg = __ldg(p.tables + u.s.req * p.max_pages + (at >> p.page_shift));
+      if (pg < 0 || pg >= p.n_pages) {
+        raise_error(p.batch.err, TIDE_DEVERR_POSITION);
+        return -1;
       }
-    }
+      return (pg * p.hkv + u.kvh) * (page / kBlock) + (at & (page - 1)) / kBlock;
+    };
+    int base = 0, now = places(0), next = places(32);
+    // blocks [i, i + kBatch) to a place, a lane each
+    auto request = [&](int i, uint32_t to) {
+      const int n = min(kBatch, blocks - i);
+      if (n <= 0) return;
+      if (i - base >= 32) {
+        base += 32;
+        now = next;
+        next = places(base + 32);
+      }
+      const int k = i - base + lane;
+      const int place0 = __shfl_sync(kFull, now, k & 31), place1 = __shfl_sync(kFull, next, k & 31);
+      const int place = k < 32 ? place0 : place1;
+      uint64_t *bar = &full[warp][to];
+      unsigned char *at = ring + to * F::kPlace + lane * L::kBytes;
+      const bool copy = lane < n && place >= 0;
+      const int copies = __popc(__ballot_sync(kFull, copy));
+      if (lane < n && place < 0)  // reads as zeros
+        for (int e = 0; e < L::kBytes / 16; ++e) reinterpret_cast<uint4 *>(at)[e] = make_uint4(0, 0, 0, 0);
+      __syncwarp();
+      if (lane == 0) ptx::mbar_expect_tx(bar, copies * L::kBytes);
+      __syncwarp();
+      if (copy) ptx::bulk_load(at, p.cache + (int64_t)place * L::kBytes, L::kBytes, bar, once);
+    };
+    request(0, turn & 1);
+    request(kBatch, (turn & 1) ^ 1);
 
-    uint32_t pt[NT][2];
+    // Q^T: columns are rows 8 nt + g; the statistics of a column are kept by the
+    // lanes whose accumulators belong to it, columns 8 nt + 2 t and one further
+    uint32_t qb[NT][kSteps][2], qc[NT][2];
+    int sees[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      pt[nt][0] = pt[nt][1] = 0u;
-      if (NT > 1 && nt >= tiles) continue;
-      bool raise = false;
+      const int r = nt * 8 + g;
+      const bool valid = r < rows;
+      const int tok = token_of(u.row + (valid ? r : 0), p.per_group);
+      const T *q = static_cast<const T *>(p.q) + (u.s.row0 + tok) * p.q_stride +
+                   (int64_t)(u.kvh * p.group + u.row + (valid ? r : 0) - tok * p.group) * D + t * (D / 4);
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kKWords; ++w) {
+        const uint4 x = valid ? *reinterpret_cast<const uint4 *>(q + 8 * w) : make_uint4(0, 0, 0, 0);
+        qb[nt][2 * w][0] = x.x;
+        qb[nt][2 * w][1] = x.y;
+        qb[nt][2 * w + 1][0] = x.z;
+        qb[nt][2 * w + 1][1] = x.w;
+        if constexpr (kCentred) {
+          float f[8];
+          unpack16<T>(x, f);
+          sum += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+        }
+      }
+      if constexpr (kCentred) {  // the group's sum in three numbers; where two lanes share it, the even one's
+        if (D == 64) sum += __shfl_xor_sync(kFull, sum, 1);
+        if (D == 64 && (t & 1)) sum = 0.f;
+        sum = -sum;  // (of the negative remainders)
+        const float high = Elem<T>::to_f(Elem<T>::from_f(sum));
+        const float mid = Elem<T>::to_f(Elem<T>::from_f(sum - high));
+        qc[nt][0] = pack2<T>(high, mid);
+        qc[nt][1] = pack2<T>(sum - high - mid, 0.f);
+      }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        // tokens kappa and 8 further
-        if (partial) {
-          const int lim = sees[nt][e] - key - kappa;
-          if (lim <= 0) sc[nt][e] = -INFINITY;
-          if (lim <= 8) sc[nt][2 + e] = -INFINITY;
-        }
-        raise |= fmaxf(sc[nt][e], sc[nt][2 + e]) > most[nt][e];  // (the first keys: of -infinity)
+        const int c = min(nt * 8 + t * 2 + e, rows - 1);
+        sees[nt][e] = pos0 + token_of(u.row + c, p.per_group) + 1;
       }
-      if (__any_sync(kFull, raise)) {
-        float a[2];
+    }
+    // (a weight is 2^(score qs + up); up is lowered where a score passes `most`)
+    float o[NT][kSteps][4], oc[NT][4], up[NT][2], most[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      up[nt][0] = up[nt][1] = kLift<T>;
+      most[nt][0] = most[nt][1] = -INFINITY;
+      oc[nt][0] = oc[nt][1] = oc[nt][2] = oc[nt][3] = 0.f;
+#pragma unroll
+      for (int d = 0; d < kSteps; ++d) o[nt][d][0] = o[nt][d][1] = o[nt][d][2] = o[nt][d][3] = 0.f;
+    }
+    const int all_see = pos0 + token_of(u.row, p.per_group) + 1;  // keys that every row sees
+
+    // One block at b, keys from `key` on.  masked: not all rows see all of them.
+    auto work = [&](const unsigned char *b, int key, auto masked) {
+      constexpr bool kMasked = decltype(masked)::value;
+      uint32_t kw[2][kKWords], vw[4][kVWords];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const unsigned char *at = b + k_at + 8 * h * L::kRow;
+        if constexpr (D == 128) {
+          const uint4 x = *reinterpret_cast<const uint4 *>(at);
+          kw[h][0] = x.x, kw[h][1] = x.y, kw[h][2] = x.z, kw[h][3] = x.w;
+        } else {
+          const uint2 x = *reinterpret_cast<const uint2 *>(at);
+          kw[h][0] = x.x, kw[h][1] = x.y;
+        }
+      }
+      const uint2 ks = *reinterpret_cast<const uint2 *>(b + ks_at);
+      float sc[NT][4];
+      {
+        const uint32_t both = g & 1 ? 0x3232u : 0x1010u;
+        const Maker<T> p0(prmt(ks.x, 0u, both), magic), p1(prmt(ks.y, 0u, both), magic);
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          const int sh = 8 * (k & 1);
+          const uint32_t w0 = kw[0][k / 2], w1 = kw[1][k / 2];
+          const uint32_t a[4] = {p0(w0 >> sh), p1(w1 >> sh), p0(w0 >> (sh + 4)), p1(w1 >> (sh + 4))};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            if (k == 0) mma16816_first<T>(sc[nt], a, qb[nt][k][0], qb[nt][k][1]);
+            else mma16816<T>(sc[nt], a, qb[nt][k][0], qb[nt][k][1]);
+          }
+        }
+        if constexpr (kCentred) {
+          const uint32_t r0 = p0.minus_rest(), r1 = p1.minus_rest();
+          const uint32_t a[4] = {r0, r1, r0, r1};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma16816<T>(sc[nt], a, qc[nt][0], qc[nt][1]);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const unsigned char *at = b + v_at + 4 * h * L::kRow;
+        if constexpr (D == 128) {
+          const uint2 x = *reinterpret_cast<const uint2 *>(at);
+          vw[h][0] = x.x, vw[h][1] = x.y;
+        } else {
+          vw[h][0] = *reinterpret_cast<const uint32_t *>(at);
+        }
+      }
+      uint2 vs = *reinterpret_cast<const uint2 *>(b + vs_at), vc = make_uint2(0, 0);
+      if constexpr (kCentred) {
+        if (g < D / kGroup) vc = *reinterpret_cast<const uint2 *>(b + vc_at);
+      }
+      if constexpr (kMasked) {
+        // A weight of 0 does not silence a NaN.  Past the last key a token's scales
+        // are dropped; before it, where rows differ, those that are NaN are, and
+        // added to the rows that do see them.
+        auto drop = [](uint2 &x, int h) { (h < 2 ? x.x : x.y) &= h & 1 ? 0x0000ffffu : 0xffff0000u; };
+        auto odd = [](const uint2 &x, int h) {
+          return (((h < 2 ? x.x : x.y) >> (h & 1) * 16) & 0x7f80u) == 0x7f80u;
+        };
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+          if (key + t + 4 * h >= kv) drop(vs, h), drop(vc, h);
+        if (__any_sync(kFull, odd(vs, 0) || odd(vs, 1) || odd(vs, 2) || odd(vs, 3))) {
+          // rare: token by token, its scale being with lane 4 g + its number % 4
+#pragma unroll 1
+          for (int k = 0; k < kBlock; ++k) {
+            const uint32_t two = __shfl_sync(kFull, k < 8 ? vs.x : vs.y, (lane & 28) + k % 4);
+            const bool is = ((two >> (k / 4 & 1) * 16) & 0x7f80u) == 0x7f80u;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int d = 0; d < kSteps; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (is && key + k < sees[nt][e & 1]) o[nt][d][e] = NAN;
+          }
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            if (odd(vs, h)) drop(vs, h);
+            if (odd(vc, h)) drop(vc, h);
+          }
+        }
+      }
+      uint32_t pt[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        pt[nt][0] = pt[nt][1] = 0u;
+        if (NT > 1 && nt >= tiles) continue;
+        bool raise = false;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float top = fmaxf(sc[nt][e], sc[nt][2 + e]);
-#pragma unroll
-          for (int w = 4; w < 32; w *= 2) top = fmaxf(top, __shfl_xor_sync(kFull, top, w));
-          const bool raised = top > most[nt][e];
-          const float to = raised ? fmaf(-top, p.qs, kLift<T>) : up[nt][e];
-          // (nothing there yet: whatever the factor)
-          a[e] = most[nt][e] == -INFINITY ? 0.f : ex2(to - up[nt][e]);
-          up[nt][e] = to;
-          if (raised) most[nt][e] = top + slack;
-          oc[nt][e] *= a[e];
+          if constexpr (kMasked) {  // tokens kappa and 8 further
+            const int lim = sees[nt][e] - key - kappa;
+            if (lim <= 0) sc[nt][e] = -INFINITY;
+            if (lim <= 8) sc[nt][2 + e] = -INFINITY;
+          }
+          raise |= fmaxf(sc[nt][e], sc[nt][2 + e]) > most[nt][e];  // (the first keys: of -infinity)
         }
+        if (__any_sync(kFull, raise)) {
+          float a[2];
 #pragma unroll
-        for (int d = 0; d < kSteps; ++d) {
-          o[nt][d][0] *= a[0];
-          o[nt][d][1] *= a[1];
-          o[nt][d][2] *= a[0];
-          o[nt][d][3] *= a[1];
+          for (int e = 0; e < 2; ++e) {
+            float top = fmaxf(sc[nt][e], sc[nt][2 + e]);
+#pragma unroll
+            for (int w = 4; w < 32; w *= 2) top = fmaxf(top, __shfl_xor_sync(kFull, top, w));
+            const bool raised = top > most[nt][e];
+            const float to = raised ? fmaf(-top, p.qs, kLift<T>) : up[nt][e];
+            // (nothing there yet: whatever the factor)
+            a[e] = most[nt][e] == -INFINITY ? 0.f : ex2(to - up[nt][e]);
+            up[nt][e] = to;
+            if (raised) most[nt][e] = top + slack;
+            oc[nt][e] *= a[e];
+          }
+#pragma unroll
+          for (int d = 0; d < kSteps; ++d) {
+            o[nt][d][0] *= a[0];
+            o[nt][d][1] *= a[1];
+            o[nt][d][2] *= a[0];
+            o[nt][d][3] *= a[1];
+          }
         }
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = ex2(fmaf(sc[nt][e], p.qs, up[nt][e & 1]));
+        pt[nt][0] = transpose8x8(pack_weights<T>(x[0], x[1]));
+        pt[nt][1] = transpose8x8(pack_weights<T>(x[2], x[3]));
       }
-      float x[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = ex2(fmaf(sc[nt][e], p.qs, up[nt][e & 1]));
-      pt[nt][0] = transpose8x8(pack_weights<T>(x[0], x[1]));
-      pt[nt][1] = transpose8x8(pack_weights<T>(x[2], x[3]));
-    }
-    {
-      const Maker<T> p0(vs.x), p1(vs.y);
+      const Maker<T> p0(vs.x, magic), p1(vs.y, magic);
 #pragma unroll
       for (int x = 0; x < kVWords; ++x) {
         const uint32_t lo0 = prmt(vw[0][x], vw[1][x], 0x5410u), hi0 = prmt(vw[0][x], vw[1][x], 0x7632u);
@@ -820,73 +883,197 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
         }
       }
       constexpr uint32_t kOnes = kCentred ? 0x3f803f80u : 0x3c003c00u;
-      const uint32_t a[4] = {g == kSumRow ? kOnes : Maker<T>(vc.x).rest(), 0u,
-                             g == kSumRow ? kOnes : Maker<T>(vc.y).rest(), 0u};
+      const uint32_t a[4] = {g == kSumRow ? kOnes : Maker<T>(vc.x, magic).minus_rest(), 0u,
+                             g == kSumRow ? kOnes : Maker<T>(vc.y, magic).minus_rest(), 0u};
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) mma16816<T>(oc[nt], a, pt[nt][0], pt[nt][1]);
-    }
-    __syncwarp();  // the stage has been read
-    ptx::fence_proxy_async();
-    if (!lost) request(i + F::kStages, st);
-    st = st1;
-    phase = phase1;
-  }
-  if (lost && lane == 0) {  // wait for the copies in flight (bounded)
-    volatile int none = 0;
-    for (int e = i; e < min(blocks, i + F::kStages); ++e)
-      ptx::mbar_wait(&full[warp][e % F::kStages], (e / F::kStages) & 1, &none);
-  }
-  __syncwarp();
+    };
 
-  // the four warps' outputs meet, [warp][row][D + 4]
-  float *mine = reinterpret_cast<float *>(ring);
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = nt * 8 + t * 2 + e;
-      if (g == kSumRow) {
-        s_m[warp][r] = kLift<T> - up[nt][e];
-        s_l[warp][r] = oc[nt][e];
+    int i = 0;
+    bool lost = false;  // a wait has run out
+#pragma unroll 1
+    while (i < blocks) {
+      const uint32_t at = turn & 1;
+      if (!__all_sync(kFull, ptx::mbar_wait(&full[warp][at], turn >> 1 & 1, &s_abort))) {
+        raise_error(p.batch.err, TIDE_DEVERR_TIMEOUT);
+        s_abort = 1;
+        lost = true;
+        break;
       }
-      // (the lane's channels are in group g * (D / 8) / 32, whose sum is row of that number)
-      const float rest =
-          kCentred ? __shfl_sync(kFull, oc[nt][e], g * (D / 8) / kGroup * 4 + t) : 0.f;
-#pragma unroll
-      for (int d = 0; d < kSteps; ++d)
-        *reinterpret_cast<float2 *>(mine + r * F::kPitch + g * (D / 8) + 2 * d) =
-            make_float2(o[nt][d][e] + rest, o[nt][d][2 + e] + rest);
+      const unsigned char *b = ring + at * F::kPlace;
+      int key = (block0 + i * kFewWarps) * kBlock;
+      const int upto = min(i + kBatch, blocks);
+#pragma unroll 1
+      for (; i < upto; ++i, b += L::kBytes, key += kFewWarps * kBlock) {
+        if (key + kBlock <= all_see) work(b, key, std::false_type{});
+        else work(b, key, std::true_type{});
+      }
+      __syncwarp();  // the place has been read
+      ptx::fence_proxy_async();
+      request(i + kBatch, at);
+      ++turn;
     }
-  __syncthreads();
-  constexpr int kLanes = D / 4;  // lanes of a row, four columns each
-  for (int r = threadIdx.x / kLanes; r < rows; r += 32 * kFewWarps / kLanes) {
-    const int d = threadIdx.x % kLanes * 4;
-    float top = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kFewWarps; ++w)
-      if (s_l[w][r] != 0.f) top = fmaxf(top, s_m[w][r]);
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < kFewWarps; ++w) {
-      if (s_l[w][r] == 0.f) continue;
-      const float a = exp2f(s_m[w][r] - top);
-      const float4 y = *reinterpret_cast<const float4 *>(
-          reinterpret_cast<const float *>(dyn + w * F::kRing) + r * F::kPitch + d);
-      sum = fmaf(a, s_l[w][r], sum);
-      x.x = fmaf(a, y.x, x.x);
-      x.y = fmaf(a, y.y, x.y);
-      x.z = fmaf(a, y.z, x.z);
-      x.w = fmaf(a, y.w, x.w);
+    if (lost && lane == 0) {  // wait for the copies in flight (bounded)
+      volatile int none = 0;
+      for (int e = i; e < min(blocks, i + 2 * kBatch); e += kBatch, ++turn)
+        ptx::mbar_wait(&full[warp][turn & 1], turn >> 1 & 1, &none);
     }
-    const int64_t at = (int64_t)(r / p.group) * p.hq + r % p.group;
-    if (p.splits > 1) {
-      if (d == 0) p.part_ml[part + at] = make_float2(top, sum);
-      *reinterpret_cast<float4 *>(p.part_o + (part + at) * D + d) = x;
-    } else {
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + (row0 + at) * D + d) =
-          make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
+    __syncwarp();
+
+    // the four warps' outputs meet, [warp][row][D + 4]
+    float *mine = reinterpret_cast<float *>(ring);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = nt * 8 + t * 2 + e;
+        if (g == kSumRow) {
+          s_m[warp][r] = kLift<T> - up[nt][e];
+          s_l[warp][r] = oc[nt][e];
+        }
+        // (the lane's channels are in group g * (D / 8) / 32, whose rest is the row of that number)
+        const float rest = kCentred ? __shfl_sync(kFull, oc[nt][e], g * (D / 8) / kGroup * 4 + t) : 0.f;
+#pragma unroll
+        for (int d = 0; d < kSteps; ++d)
+          *reinterpret_cast<float2 *>(mine + r * F::kPitch + g * (D / 8) + 2 * d) =
+              make_float2(o[nt][d][e] - rest, o[nt][d][2 + e] - rest);
+      }
+    __syncthreads();
+    constexpr int kLanes = D / 4;  // lanes of a row, four columns each
+    for (int r = threadIdx.x / kLanes; r < rows; r += 32 * kFewWarps / kLanes) {
+      const int d = threadIdx.x % kLanes * 4;
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kFewWarps; ++w)
+        if (s_l[w][r] != 0.f) top = fmaxf(top, s_m[w][r]);
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kFewWarps; ++w) {
+        if (s_l[w][r] == 0.f) continue;
+        const float a = ex2(s_m[w][r] - top);
+        const float4 y = *reinterpret_cast<const float4 *>(
+            reinterpret_cast<const float *>(dyn + w * F::kRing) + r * F::kPitch + d);
+        sum = fmaf(a, s_l[w][r], sum);
+        x.x = fmaf(a, y.x, x.x);
+        x.y = fmaf(a, y.y, x.y);
+        x.z = fmaf(a, y.z, x.z);
+        x.w = fmaf(a, y.w, x.w);
+      }
+      if (u.b0 > 0 || b1 < u.nb) {
+        const int64_t part = (2 * (int64_t)blockIdx.x + (u.b0 == 0)) * kRowsMost + r;
+        if (d == 0) p.part_ml[part] = make_float2(top, sum);
+        *reinterpret_cast<float4 *>(p.part_o + part * D + d) = x;
+      } else {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const int tok = token_of(u.row + r, p.per_group);
+        const int64_t at = ((int64_t)u.s.row0 + tok) * p.hq + u.kvh * p.group + (u.row + r - tok * p.group);
+        *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + at * D + d) =
+            make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
+      }
     }
+    pos += p.whole ? 1 : b1 - u.b0;
+    if (pos >= end || *(volatile int *)&s_abort) return;
+    ptx::fence_proxy_async();  // (copies go where the outputs were)
+    __syncthreads();
+    if (warp == 0) {  // the next unit
+      const int row = u.row + kRowsMost;
+      if (u.kvh + 1 < p.hkv) {
+        if (lane == 0) s_part.kvh = u.kvh + 1, s_part.b0 = 0;
+      } else if (row < u.s.n * p.group) {
+        if (lane == 0) s_part = {u.s, u.seq, row, 0, 0, blocks_of(u.s, row)};
+      } else {  // the next sequence that has one, 32 at a time
+        for (int seq = u.seq + 1; seq < live; seq += 32) {
+          Sequence s{};
+          if (seq + lane < live) s = sequence(p.batch, seq + lane);
+          const unsigned have = __ballot_sync(kFull, rows_of(s) > 0);
+          if (have) {
+            if (lane == __ffs(have) - 1) s_part = {s, seq + lane, 0, 0, 0, blocks_of(s, 0)};
+            break;
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Joins the parts of the units that CTAs share, a CTA of this kernel for the second
+// of them: with M = max m_i, o = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i.  Warps
+// share the parts of a row where there are more warps than rows; eight parts each
+// at a time, whose loads are all in flight before the first is used.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(256)
+    join_units_kernel(const Shared *__restrict__ shared, const float *__restrict__ part_o,
+                      const float2 *__restrict__ part_ml, T *out, int hq, int group, uint32_t per_group) {
+  constexpr int kE = D / 32, kFlight = 8, kRows = 8 * NT;
+  __shared__ float s_m[8], s_l[8], s_o[8][D];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  ptx::grid_dependency_wait();
+  ptx::grid_dependents_launch();
+  const Shared u = shared[blockIdx.x];
+  if (u.first < 0 || u.first + 1 != (int)blockIdx.x) return;
+  const int parts = u.last - u.first + 1;
+  const int per = u.rows > 4 ? 1 : u.rows > 2 ? 2 : u.rows > 1 ? 4 : 8;  // warps of a row
+  for (int r0 = 0; r0 < u.rows; r0 += 8 / per) {
+    const int r = r0 + warp / per;
+    float m = -INFINITY, l = 0.f, o[kE];
+#pragma unroll
+    for (int e = 0; e < kE; ++e) o[e] = 0.f;
+    for (int i0 = warp % per; r < u.rows && i0 < parts; i0 += per * kFlight) {
+      float2 ml[kFlight];
+      float x[kFlight][kE];
+#pragma unroll
+      for (int b = 0; b < kFlight; ++b) {
+        const int i = min(i0 + b * per, parts - 1);
+        const int64_t at = (2 * (int64_t)(u.first + i) + (i == 0)) * kRows + r;
+        ml[b] = i0 + b * per < parts ? part_ml[at] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int e = 0; e < kE; ++e) x[b][e] = part_o[at * D + lane * kE + e];
+      }
+      float top = m;
+#pragma unroll
+      for (int b = 0; b < kFlight; ++b) top = ml[b].y != 0.f ? fmaxf(top, ml[b].x) : top;
+      const float a = l != 0.f ? exp2f(m - top) : 0.f;
+      l *= a;
+#pragma unroll
+      for (int e = 0; e < kE; ++e) o[e] = l != 0.f ? o[e] * a : 0.f;
+#pragma unroll
+      for (int b = 0; b < kFlight; ++b) {
+        if (ml[b].y == 0.f) continue;
+        const float f = exp2f(ml[b].x - top);
+        l = fmaf(f, ml[b].y, l);
+#pragma unroll
+        for (int e = 0; e < kE; ++e) o[e] = fmaf(f, x[b][e], o[e]);
+      }
+      m = top;
+    }
+    if (per > 1) {
+      if (lane == 0) s_m[warp] = m, s_l[warp] = l;
+#pragma unroll
+      for (int e = 0; e < kE; ++e) s_o[warp][lane * kE + e] = o[e];
+      __syncthreads();
+      float top = -INFINITY;
+      const int w0 = warp / per * per;
+      for (int w = w0; w < w0 + per; ++w)
+        if (s_l[w] != 0.f) top = fmaxf(top, s_m[w]);
+      l = 0.f;
+#pragma unroll
+      for (int e = 0; e < kE; ++e) o[e] = 0.f;
+      for (int w = w0; w < w0 + per; ++w) {
+        if (s_l[w] == 0.f) continue;
+        const float f = exp2f(s_m[w] - top);
+        l = fmaf(f, s_l[w], l);
+#pragma unroll
+        for (int e = 0; e < kE; ++e) o[e] = fmaf(f, s_o[w][lane * kE + e], o[e]);
+      }
+      __syncthreads();
+    }
+    if (r >= u.rows || warp % per) continue;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int tok = token_of(u.row + r, per_group);
+    T *to = out + (((int64_t)u.seq_row + tok) * hq + u.kvh * group + (u.row + r - tok * group)) * D + lane * kE;
+#pragma unroll
+    for (int e = 0; e < kE; ++e) to[e] = Elem<T>::from_f(o[e] * inv);
   }
 }
 
@@ -944,10 +1131,10 @@ int append(const tide::q4::AppendParams &p, cudaStream_t s) {
 // few-rows kernel, longer ones as 16-bit pages to the tiles; a call that cannot
 // have the one or the other does not launch it.
 struct Plan {
-  int nt;           // 8-row groups of a CTA of the few-rows kernel; 0: none
-  int few, tokens;
-  int64_t pieces;   // of up to `tokens` tokens, at most
-  int splits, split_keys;
+  int nt;           // 8-row groups of a unit of the few-rows kernel; 0: none
+  int few;
+  bool whole;       // its units are not split
+  int64_t ctas;
   bool tiles;       // whether the tiles run: in rounds of sequences, so that the
   int64_t wide;     // 16-bit pages of a round stay within 256 MB (or are one
   int64_t seqs;     // sequence's): pages of a sequence, sequences of a round
@@ -956,32 +1143,29 @@ struct Plan {
 
 Plan plan_of(bool one_token, int64_t n_tokens, int64_t n_seqs, int64_t n_requests, int64_t hq,
              int64_t hkv, int64_t d, int64_t max_kv) {
+  using namespace tide::q4;
   Plan p{};
-  const int64_t group = hq / hkv;
-  p.nt = group <= 8 ? 1 : group <= 16 ? 2 : group <= 32 ? 4 : 0;
-  if (!one_token) {
-    const int64_t rows = (n_tokens * group + n_seqs - 1) / n_seqs;  // of a sequence, on average
-    if (p.nt && p.nt < 2 && rows > 8) p.nt = 2;
-    if (p.nt && p.nt < 4 && rows > 16) p.nt = 4;
-    if (rows > 32 || (n_seqs == 1 && rows > 64)) p.nt = 0;
+  // The lengths are on the device; the average is known.  More rows a sequence than
+  // kMostRows on average go to the tiles; else a sequence of up to as many, or any
+  // where the call has few rows, goes to the few-rows kernel.
+  constexpr int64_t kMostRows = 64;
+  const int64_t group = hq / hkv, rows = (n_tokens * group + n_seqs - 1) / n_seqs;
+  p.nt = one_token || rows <= kMostRows ? (rows <= 8 ? 1 : 2) : 0;
+  if (n_seqs == 1 && n_tokens * group > 2 * kMostRows) p.nt = 0;
+  if (p.nt) {
+    p.few = (int)(one_token ? 1 : n_tokens * group <= 1024 ? n_tokens : 2 * kMostRows / group);
+    if (p.few < 1) p.few = 1;
+    p.whole = max_kv <= 512;
+    // as many CTAs as run at once, or fewer where there is not work for so many
+    const int64_t slots = 148 * (p.nt == 1 ? 4 : 3);
+    const int64_t units = (n_seqs + n_tokens * group / (8 * p.nt)) * hkv;
+    const int64_t blocks = (max_kv + kBlock - 1) / kBlock;
+    p.ctas = p.whole ? units : (units * (blocks < 1 ? 1 : blocks) + kLeastBlocks - 1) / kLeastBlocks;
+    if (p.ctas > slots) p.ctas = slots;
+    if (!p.whole)
+      p.few_bytes = (size_t)(p.ctas * (2 * 8 * p.nt * (d + 2) * 4 + (int64_t)sizeof(Shared)) + 15) / 16 * 16;
   }
-  p.tokens = (int)(p.nt * 8 / group);
-  p.few = !p.nt ? 0 : one_token ? 1 : 2 * p.tokens;
-  if (n_tokens < p.few) p.few = (int)n_tokens;
   p.tiles = !p.nt || (!one_token && n_tokens > p.few);
-  p.pieces = n_seqs + (p.few > p.tokens ? n_tokens / p.tokens : 0);
-  // Splits of the few-rows kernel, as paged_attention's: one round of CTAs where
-  // there are few units, else up to eight, for an even end.
-  const int64_t slots = 148 * (p.nt == 1 ? 4 : p.nt == 2 ? 3 : 2);
-  const int64_t units = p.pieces * hkv;
-  const bool one_round = units * 4 <= slots;
-  const int64_t least = one_round ? 128 : 512;
-  int64_t s = !p.nt ? 1 : one_round ? slots / units : (8 * slots + units - 1) / units;
-  if (s > (max_kv + least - 1) / least) s = (max_kv + least - 1) / least;
-  if (s < 1 || units >= 2 * slots) s = 1;
-  p.splits = (int)s;
-  p.split_keys = (int)(((max_kv + s - 1) / s + 63) / 64 * 64);
-  p.few_bytes = s > 1 ? (size_t)(s * n_seqs * p.few * hq * (d + 2) * 4 + 15) / 16 * 16 : 0;
   p.bytes = p.few_bytes;
   if (!p.tiles) return p;
   p.wide = (max_kv + tide::q4::kOpenPage - 1) / tide::q4::kOpenPage;
@@ -1002,19 +1186,23 @@ Plan plan_of(bool one_token, int64_t n_tokens, int64_t n_seqs, int64_t n_request
 }
 
 template <typename T, int D, int NT>
-int launch_few(const tide::q4::FewParams &p, cudaStream_t s) {
+int launch_few(int64_t ctas, const tide::q4::FewParams &p, cudaStream_t s) {
   using namespace tide::q4;
   auto kern = few_rows_kernel<T, D, NT>;
   constexpr int smem = Few<D, NT>::kSmem;
   static std::atomic<uint64_t> set{0};  // per device
-  const cudaError_t e = smem > 48 << 10 ? tide::allow_smem(kern, smem, set) : cudaSuccess;
+  const cudaError_t e = tide::allow_smem(kern, smem, set);
   if (e != cudaSuccess) return report(e, "paged_attention_q4");
-  return start("paged_attention_q4", kern, (int64_t)p.pieces * p.hkv * p.splits, 32 * kFewWarps, smem, s, p);
+  if (int rc = start("paged_attention_q4", kern, ctas, 32 * kFewWarps, smem, s, p)) return rc;
+  if (ctas == 1 || p.whole) return TIDE_OK;
+  return start("paged_attention_q4", join_units_kernel<T, D, NT>, ctas, 256, 0, s, (const Shared *)p.shared,
+               (const float *)p.part_o, (const float2 *)p.part_ml, static_cast<T *>(p.out), p.hq, p.group,
+               p.per_group);
 }
 
 template <typename T, int D>
-int few_rows(int nt, const tide::q4::FewParams &p, cudaStream_t s) {
-  return nt == 1 ? launch_few<T, D, 1>(p, s) : nt == 2 ? launch_few<T, D, 2>(p, s) : launch_few<T, D, 4>(p, s);
+int few_rows(int nt, int64_t ctas, const tide::q4::FewParams &p, cudaStream_t s) {
+  return nt == 1 ? launch_few<T, D, 1>(ctas, p, s) : launch_few<T, D, 2>(ctas, p, s);
 }
 
 template <typename T, int D>
@@ -1163,19 +1351,19 @@ extern "C" int tide_paged_attention_q4(int dtype, const void *q, int64_t q_row_s
                                 (int)n_tokens, (int)max_kv_len, error_word};
   int rc = TIDE_OK;
   if (plan.nt) {
+    const int64_t group = n_q_heads / n_kv_heads, rows = plan.ctas * 2 * 8 * plan.nt;
     float *part_o = reinterpret_cast<float *>(ws);
-    const int64_t part_rows = plan.splits * n_seqs * plan.few * n_q_heads;
-    float2 *part_ml = reinterpret_cast<float2 *>(part_o + part_rows * head_dim);
+    float2 *part_ml = reinterpret_cast<float2 *>(part_o + rows * head_dim);
     const tide::q4::FewParams f{batch, static_cast<const unsigned char *>(cache), block_tables, max_pages,
-                                (int)n_pages, shift, q, q_row_stride, out, part_o, part_ml, (int)n_q_heads,
-                                (int)n_kv_heads, (int)(n_q_heads / n_kv_heads), plan.few, plan.tokens,
-                                (int)plan.pieces, plan.splits, plan.split_keys,
-                                scale * tide::ragged::kLog2e};
-    rc = bf16 ? (wide ? few_rows<__nv_bfloat16, 128>(plan.nt, f, st) : few_rows<__nv_bfloat16, 64>(plan.nt, f, st))
-              : (wide ? few_rows<__half, 128>(plan.nt, f, st) : few_rows<__half, 64>(plan.nt, f, st));
-    if (!rc && plan.splits > 1)
-      rc = tide::join_few_rows(dtype, head_dim, batch, (int)n_q_heads, plan.few, plan.splits, part_o, part_ml,
-                               out, st);
+                                (int)n_pages, shift, q, q_row_stride, out, part_o, part_ml,
+                                reinterpret_cast<tide::q4::Shared *>(part_ml + rows), (int)n_q_heads,
+                                (int)n_kv_heads, (int)group, plan.few, plan.whole,
+                                scale * tide::ragged::kLog2e,
+                                bf16 ? tide::q4::kMagic<__nv_bfloat16> : tide::q4::kMagic<__half>,
+                                (uint32_t)(((1ll << 31) + group - 1) / group)};
+    const int64_t n = plan.ctas;
+    rc = bf16 ? (wide ? few_rows<__nv_bfloat16, 128>(plan.nt, n, f, st) : few_rows<__nv_bfloat16, 64>(plan.nt, n, f, st))
+              : (wide ? few_rows<__half, 128>(plan.nt, n, f, st) : few_rows<__half, 64>(plan.nt, n, f, st));
   }
   if (rc || !plan.tiles) return rc;
   ws += plan.few_bytes;

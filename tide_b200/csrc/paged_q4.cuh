@@ -64,12 +64,10 @@ __device__ __forceinline__ uint32_t as_bits(P2 v) {
 template <typename T>
 constexpr uint32_t kMagic = std::is_same<T, __half>::value ? 0x64006400u : 0x43004300u;
 
-// x's codes as such numbers.  One instruction with the mask and the number from
-// registers: written with & and | it is two, each with one of the constants.
-template <typename T>
-__device__ __forceinline__ uint32_t numbers(uint32_t x) {
-  uint32_t r, magic;
-  asm("mov.b32 %0, %1;" : "=r"(magic) : "n"(kMagic<T>));
+// x's codes as such numbers: one instruction, if the number is not a constant to
+// the compiler (which would load it anew each time, or use two).
+__device__ __forceinline__ uint32_t numbers(uint32_t x, uint32_t magic) {
+  uint32_t r;
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(0x000f000fu), "r"(magic));
   return r;
 }
@@ -81,9 +79,9 @@ struct Pars {
 };
 // Of two 16-bit scales in the halves of p.
 template <typename T>
-__device__ __forceinline__ Pars<T> pars(uint32_t p) {
+__device__ __forceinline__ Pars<T> pars(uint32_t p, uint32_t magic = kMagic<T>) {
   Pars<T> r;
-  r.zero = as_pair<T>(numbers<T>(p));
+  r.zero = as_pair<T>(numbers(p, magic));
   if constexpr (std::is_same<T, __half>::value)
     r.scale = __floats2half2_rn(__uint_as_float((p & 0xfff0u) << 16), __uint_as_float(p & 0xfff00000u));
   else
@@ -92,8 +90,8 @@ __device__ __forceinline__ Pars<T> pars(uint32_t p) {
 }
 // Two values whose codes are the lowest four bits of x's halves.
 template <typename T>
-__device__ __forceinline__ uint32_t value2(uint32_t x, const Pars<T> &p) {
-  const Pair<T> c = as_pair<T>(numbers<T>(x));
+__device__ __forceinline__ uint32_t value2(uint32_t x, const Pars<T> &p, uint32_t magic = kMagic<T>) {
+  const Pair<T> c = as_pair<T>(numbers(x, magic));
   return as_bits(__hmul2(__hsub2(c, p.zero), p.scale));
 }
 // The eight channels of a word.
