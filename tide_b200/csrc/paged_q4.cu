@@ -47,71 +47,86 @@ struct AppendParams {
   int32_t *err;
 };
 
-// x / s rounded to the nearest whole number, ties to the even one: the quotient
-// by multiplication may be off by a bit, and ties are common (values of eight
-// bits over scales of four), so the remainder, which is exact, decides.
-__device__ __forceinline__ float nearest(float x, float s, float inv) {
-  float n = rintf(x * inv);
-  const float r = fmaf(-n, s, x), a = fabsf(r), half = 0.5f * s;
-  const bool odd = ((int)n & 1) != 0;
-  if (a > half || (a == half && odd)) n += copysignf(1.f, r);
-  return n;
+// Added to a number below 2^22, its whole part (to nearest, ties to even) is in the
+// last bits.
+constexpr float kRounder = 12582912.f;  // 3 * 2^22
+
+// Least and largest value of the group of which this lane, of eight neighbours, has
+// four, 0 among them; whether one of them is not finite.
+__device__ __forceinline__ bool extent(const float (&x)[4], float *lo, float *hi) {
+  constexpr unsigned kFull = 0xffffffffu;
+  float a = fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), b = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+  const float all = (x[0] + x[1]) * 0.f + (x[2] + x[3]) * 0.f;  // NaN where one is not finite, or the sum is not
+  const unsigned who = __ballot_sync(kFull, !(all == 0.f));
+#pragma unroll
+  for (int w = 1; w < 8; w *= 2) {
+    a = fminf(a, __shfl_xor_sync(kFull, a, w));
+    b = fmaxf(b, __shfl_xor_sync(kFull, b, w));
+  }
+  *lo = fminf(a, 0.f);
+  *hi = fmaxf(b, 0.f);
+  if (!who) return false;
+  const bool odd = !(isfinite(x[0]) && isfinite(x[1]) && isfinite(x[2]) && isfinite(x[3]));
+  return __ballot_sync(kFull, odd) >> (threadIdx.x & 24) & 0xffu;
 }
 
-// The group of which this lane, of eight neighbours, has four values: its codes
-// as the nibbles 0, 4, 1, 5 of the result, and its scale and zero point.
+// The group's codes of this lane as the nibbles 0, 4, 1, 5 of the result, and its
+// scale and zero point.
 template <typename T>
 __device__ __forceinline__ uint32_t quantise(const float (&x)[4], uint32_t *par) {
-  constexpr unsigned kFull = 0xffffffffu;
   constexpr bool kHalf = std::is_same<T, __half>::value;
   constexpr float kMost = kHalf ? 65504.f : 3.3895313892515355e38f;
   constexpr float kLeast = kHalf ? 0x1p-21f : 0x1p-120f;
-  float lo = fminf(fminf(x[0], x[1]), fminf(x[2], x[3]));
-  float hi = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-  const bool odd = !(isfinite(x[0]) && isfinite(x[1]) && isfinite(x[2]) && isfinite(x[3]));
-  const unsigned who = __ballot_sync(kFull, odd);
-#pragma unroll
-  for (int w = 1; w < 8; w *= 2) {
-    lo = fminf(lo, __shfl_xor_sync(kFull, lo, w));
-    hi = fmaxf(hi, __shfl_xor_sync(kFull, hi, w));
-  }
-  if (who >> (threadIdx.x & 24) & 0xffu) {
-    *par = 0x7fc0u;
-    return 0u;
-  }
-  lo = fminf(lo, 0.f);
-  hi = fmaxf(hi, 0.f);
+  float lo, hi;
+  const bool odd = extent(x, &lo, &hi);
   // (half of each: their difference stays within 32 bits)
   const float t = __fdiv_rn(0.5f * hi - 0.5f * lo, 7.5f);
-  if (t == 0.f) {
-    *par = 0u;
+  if (odd || t == 0.f) {
+    *par = odd ? 0x7fc0u : 0u;
     return 0u;
   }
   const float s = fmaxf(__uint_as_float((__float_as_uint(t) + 0xfffffu) & 0xfff00000u), kLeast);
   const float inv = __frcp_rn(s);
-  const float z = nearest(-lo, s, inv);
+  // v / s, rounded once: the product may be a bit off, its remainder is exact and
+  // corrects it (Markstein).  Ties are common (values of eight bits over scales of
+  // four), so that bit counts.
+  auto over = [&](float v) {
+    const float q = v * inv;
+    return fmaf(fmaf(-q, s, v), inv, q);
+  };
+  const float z = (over(-lo) + kRounder) - kRounder;
   *par = __float_as_uint(s) >> 16 | (uint32_t)z;
-  uint32_t c[4];
+  // bits[e] = kRounder's + code - z; below 0 a code cannot be (the least value's is
+  // z - z), above 15 it can
+  uint32_t bits[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    float n = nearest(x[e], s, inv);
-    if (fabsf(n * s) > kMost) n -= copysignf(1.f, n);  // (next to the type's largest number)
-    c[e] = (uint32_t)fminf(fmaxf(n + z, 0.f), 15.f);
+  for (int e = 0; e < 4; ++e) bits[e] = __float_as_uint(fminf(over(x[e]) + kRounder, kRounder + (15.f - z)));
+  if (s > kMost / 16.f) {  // next to the type's largest number: none above it
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float n = __uint_as_float(bits[e]) - kRounder;
+      if (fabsf(n * s) > kMost) bits[e] = __float_as_uint(n - copysignf(1.f, n) + kRounder);
+    }
   }
-  return c[0] | c[1] << 16 | c[2] << 4 | c[3] << 20;
+  constexpr uint32_t kSpread = 1u + (1u << 4) + (1u << 16) + (1u << 20);
+  return bits[0] + (bits[2] << 4) + (bits[1] << 16) + (bits[3] << 20) +
+         ((uint32_t)z - 0x4b400000u) * kSpread;  // (modulo 2^32)
 }
 
 template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendParams p) {
+  using namespace ragged;
   using L = Layout<D>;
   constexpr unsigned kFull = 0xffffffffu;
   constexpr int kLanes = D / 8;         // of a head
   constexpr int kHeads = 32 / kLanes;   // of a warp
+  constexpr int kWarps = 8 / ROWS;      // of a row
   constexpr int kFlight = 4;            // heads of a lane, loaded before the first is used
-  __shared__ double2 turn[ROWS][D / 2];  // cosine and sine
-  __shared__ float2 turn32[ROWS][D / 2];
-  __shared__ int64_t s_slot[ROWS];       // -1: nothing to write
-  __shared__ bool s_row[ROWS];           // whether there is such a row
+  // cosine and sine of channel 4 j + e at [e][j]
+  __shared__ double2 turn[ROWS][4][kLanes];
+  __shared__ float2 turn32[ROWS][4][kLanes];
+  __shared__ int64_t s_block[ROWS];  // the slot's block in head 0; -1: nothing to write
+  __shared__ int s_token[ROWS];      // and its token there; -1: no such row
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int head = lane / kLanes, j = lane % kLanes;
   ptx::grid_dependency_wait();
@@ -121,23 +136,24 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
   const int64_t row0 = (int64_t)blockIdx.x * ROWS;
   if (row0 >= live) return;
   const int q_tasks = p.q ? (p.hq + kHeads - 1) / kHeads : 0, kv_tasks = (p.hkv + kHeads - 1) / kHeads;
-  const int per_row = q_tasks + 2 * kv_tasks;
-  const int tasks = (int)min((int64_t)ROWS, live - row0) * per_row;
-  // rows' slots; the angles' cosines and sines
+  const int r = warp / kWarps;
+  const int tasks = row0 + r < live ? q_tasks + 2 * kv_tasks : 0;  // warps of heads: q, k, v
+  const int head_blocks = p.page / kBlock;
+  // the rows' slots, and their angles' cosines and sines
   for (int i = threadIdx.x; i < ROWS * (D / 2); i += 256) {
-    const int r = i / (D / 2), f = i % (D / 2);
-    const int64_t row = row0 + r;
+    const int at = i / (D / 2), f = i % (D / 2);
+    const int64_t row = row0 + at;
     if (row >= live) continue;
     const int64_t m = p.row_ids ? (int64_t)__ldg(p.row_ids + row) : row;
     const bool known = m >= 0 && m < p.n_map;
     if (f == 0) {
-      int64_t slot = known ? __ldg(p.slot_map + m) : -1;
-      if (!known || slot < -1 || slot / p.page >= p.n_pages) {
-        raise_error(p.err, TIDE_DEVERR_POSITION);
-        slot = -1;
-      }
-      s_slot[r] = slot;
-      s_row[r] = known;
+      const int64_t slot = known ? __ldg(p.slot_map + m) : -1;
+      const int64_t pg = slot / p.page;
+      const bool real = slot >= 0 && pg < p.n_pages;
+      if (!known || (!real && slot != -1)) raise_error(p.err, TIDE_DEVERR_POSITION);
+      const int tok = (int)(slot - pg * p.page);
+      s_block[at] = real ? pg * p.hkv * head_blocks + tok / kBlock : -1;
+      s_token[at] = !known ? -1 : real ? tok % kBlock : 0;
     }
     if (p.inv_freq && known) {
       const double turns = (double)__ldg(p.positions + m) * (double)__ldg(p.inv_freq + f) *
@@ -146,32 +162,29 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
       sincospi(2.0 * (turns - rint(turns)), &s, &c);
       c *= (double)p.att_scale;
       s *= (double)p.att_scale;
-      turn[r][f] = make_double2(c, s);
-      turn32[r][f] = make_float2((float)c, (float)s);
+      turn[at][f % 4][f / 4] = make_double2(c, s);
+      turn32[at][f % 4][f / 4] = make_float2((float)c, (float)s);
     }
   }
+  // this lane's channels 4 j.. and D / 2 + 4 j.. of the heads of `kFlight` tasks
+  const T *const q = static_cast<const T *>(p.q) + (row0 + r) * p.q_stride + 4 * j;
+  const T *const k = static_cast<const T *>(p.k) + (row0 + r) * p.kv_stride + 4 * j;
+  const T *const v = static_cast<const T *>(p.v) + (row0 + r) * p.kv_stride + 4 * j;
+  auto kind_of = [&](int t) { return (t >= q_tasks) + (t >= q_tasks + kv_tasks); };
+  auto head_of = [&](int t, int kind) {
+    return (t - (kind > 0 ? q_tasks : 0) - (kind > 1 ? kv_tasks : 0)) * kHeads + head;
+  };
   bool ready = false;
-  for (int t0 = warp; t0 < tasks || !ready; t0 += 8 * kFlight) {
+  for (int t0 = warp % kWarps; t0 < tasks || !ready; t0 += kWarps * kFlight) {
     uint2 raw[kFlight][2];
 #pragma unroll
     for (int i = 0; i < kFlight; ++i) {
-      const int t = t0 + 8 * i, r = t / per_row;
-      int h = t % per_row;
-      const T *src = nullptr;
+      const int t = t0 + kWarps * i, kind = kind_of(t), h = head_of(t, kind);
       raw[i][0] = raw[i][1] = make_uint2(0u, 0u);
-      if (t >= tasks) continue;
-      if (h < q_tasks) {
-        h = h * kHeads + head;
-        if (h < p.hq) src = static_cast<const T *>(p.q) + (row0 + r) * p.q_stride + (int64_t)h * D;
-      } else {
-        const bool value = h >= q_tasks + kv_tasks;
-        h = (h - q_tasks - (value ? kv_tasks : 0)) * kHeads + head;
-        if (h < p.hkv)
-          src = static_cast<const T *>(value ? p.v : p.k) + (row0 + r) * p.kv_stride + (int64_t)h * D;
-      }
-      if (src) {
-        raw[i][0] = *reinterpret_cast<const uint2 *>(src + 4 * j);
-        raw[i][1] = *reinterpret_cast<const uint2 *>(src + D / 2 + 4 * j);
+      if (t < tasks && h < (kind ? p.hkv : p.hq)) {
+        const T *src = (kind == 0 ? q : kind == 1 ? k : v) + (int64_t)h * D;
+        raw[i][0] = __ldcs(reinterpret_cast<const uint2 *>(src));
+        raw[i][1] = __ldcs(reinterpret_cast<const uint2 *>(src + D / 2));
       }
     }
     if (!ready) {
@@ -180,11 +193,9 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
     }
 #pragma unroll
     for (int i = 0; i < kFlight; ++i) {
-      const int t = t0 + 8 * i, r = t / per_row;
+      const int t = t0 + kWarps * i;
       if (t >= tasks) break;
-      int h = t % per_row;
-      const int kind = h < q_tasks ? 0 : h < q_tasks + kv_tasks ? 1 : 2;
-      h = (kind == 0 ? h : kind == 1 ? h - q_tasks : h - q_tasks - kv_tasks) * kHeads + head;
+      const int kind = kind_of(t), h = head_of(t, kind);
       float x[2][4];
 #pragma unroll
       for (int a = 0; a < 2; ++a)
@@ -207,21 +218,18 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
         if (p.inv_freq) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float2 cs = turn32[r][4 * j + e];
+            const float2 cs = turn32[r][e][j];
             const float a = x[0][e], b = x[1][e];
             x[0][e] = fmaf(a, cs.x, -b * cs.y);
             x[1][e] = fmaf(b, cs.x, a * cs.y);
           }
         }
-        if (h < p.hq && s_row[r]) {
+        if (h < p.hq && s_token[r] >= 0) {
           T *to = static_cast<T *>(p.q_out) + ((row0 + r) * p.hq + h) * D + 4 * j;
 #pragma unroll
-          for (int a = 0; a < 2; ++a) {
-            uint2 o;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) reinterpret_cast<T *>(&o)[e] = Elem<T>::from_f(x[a][e]);
-            *reinterpret_cast<uint2 *>(to + a * (D / 2)) = o;
-          }
+          for (int a = 0; a < 2; ++a)
+            *reinterpret_cast<uint2 *>(to + a * (D / 2)) =
+                make_uint2(pack2<T>(x[a][0], x[a][1]), pack2<T>(x[a][2], x[a][3]));
         }
         continue;
       }
@@ -247,7 +255,7 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
         if (p.inv_freq) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const double2 cs = turn[r][4 * j + e];
+            const double2 cs = turn[r][e][j];
             const double a = y[0][e], b = y[1][e];
             y[0][e] = fma(a, cs.x, -(b * cs.y));
             y[1][e] = fma(b, cs.x, a * cs.y);
@@ -263,17 +271,14 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
       // eight channels are two lanes': the even one stores the lower half's word
       const uint32_t other = __shfl_xor_sync(kFull, j & 1 ? low : high, 1);
       const uint32_t word = j & 1 ? high << 8 | other : low | other << 8;
-      const int64_t slot = s_slot[r];
-      if (slot < 0 || h >= p.hkv) continue;
-      const int at = (int)(slot % p.page), side = kind - 1;
-      unsigned char *block =
-          p.cache + ((slot / p.page * p.hkv + h) * (p.page / kBlock) + at / kBlock) * L::kBytes;
-      *reinterpret_cast<uint32_t *>(block + L::codes(side, at % kBlock) + (j & 1) * (D / 4) + j / 2 * 4) = word;
+      if (s_block[r] < 0 || h >= p.hkv) continue;
+      const int tok = s_token[r], side = kind - 1;
+      unsigned char *block = p.cache + (s_block[r] + h * head_blocks) * L::kBytes;
+      *reinterpret_cast<uint32_t *>(block + L::codes(side, tok) + (j & 1) * (D / 4) + j / 2 * 4) = word;
       if (j % 8 == 0) {
 #pragma unroll
         for (int a = 0; a < 2; ++a)
-          *reinterpret_cast<uint16_t *>(block + L::scale(side, a * (D / 64) + j / 8, at % kBlock)) =
-              (uint16_t)par[a];
+          *reinterpret_cast<uint16_t *>(block + L::scale(side, a * (D / 64) + j / 8, tok)) = (uint16_t)par[a];
       }
     }
   }
@@ -309,35 +314,52 @@ __global__ void __launch_bounds__(256) zeros_kernel(const __grid_constant__ Appe
 }
 
 // -------------------------------------------------------------------- read
-// A thread per eight channels: four bytes of codes in, 16 bytes out.
+// A warp per row, eight channels a lane at a time, keys and values: four bytes of
+// codes in, 16 bytes out.  Four of each are loaded before the first is stored.
 template <typename T, int D>
 __global__ void __launch_bounds__(256)
     read_kernel(const unsigned char *__restrict__ cache, const int64_t *__restrict__ slots,
                 int64_t n_rows, int hkv, int64_t n_pages, int page, T *__restrict__ k_out,
                 T *__restrict__ v_out, int32_t *err) {
   using L = Layout<D>;
-  constexpr int kWords = D / 8;
+  constexpr int kWords = D / 8, kFlight = 4;
+  const int lane = threadIdx.x & 31;
   ptx::grid_dependency_wait();
   ptx::grid_dependents_launch();
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int word = (int)(i % kWords);
-  const int64_t head = i / kWords, row = head / hkv;
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (row >= n_rows) return;
   const int64_t slot = __ldg(slots + row);
   if (slot == -1) return;
-  if (slot < 0 || slot / page >= n_pages) {
-    raise_error(err, TIDE_DEVERR_POSITION);
+  const int64_t pg = slot / page;
+  if (slot < 0 || pg >= n_pages) {
+    if (lane == 0) raise_error(err, TIDE_DEVERR_POSITION);
     return;
   }
-  const int at = (int)(slot % page);
-  const unsigned char *block =
-      cache + ((slot / page * hkv + head % hkv) * (page / kBlock) + at / kBlock) * L::kBytes;
+  const int at = (int)(slot - pg * page), tok = at % kBlock, head_blocks = page / kBlock;
+  const unsigned char *first = cache + (pg * hkv * head_blocks + at / kBlock) * L::kBytes;
+  const int n = hkv * kWords;
+  uint4 *const out[2] = {reinterpret_cast<uint4 *>(k_out) + row * n, reinterpret_cast<uint4 *>(v_out) + row * n};
+  for (int e0 = lane; e0 < n; e0 += 32 * kFlight) {
+    uint32_t w[kFlight][2], s[kFlight][2];
 #pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    const uint32_t w = *reinterpret_cast<const uint32_t *>(block + L::codes(side, at % kBlock) + word * 4);
-    const uint32_t s = *reinterpret_cast<const uint16_t *>(block + L::scale(side, word / 4, at % kBlock));
-    T *out = side ? v_out : k_out;
-    reinterpret_cast<uint4 *>(out)[i] = value8<T>(w, pars<T>(s | s << 16));
+    for (int f = 0; f < kFlight; ++f) {
+      const int e = e0 + 32 * f, word = e % kWords;
+      if (e >= n) break;
+      const unsigned char *block = first + (int64_t)(e / kWords) * head_blocks * L::kBytes;
+#pragma unroll
+      for (int side = 0; side < 2; ++side) {
+        w[f][side] = __ldg(reinterpret_cast<const uint32_t *>(block + L::codes(side, tok) + word * 4));
+        s[f][side] = __ldg(reinterpret_cast<const uint16_t *>(block + L::scale(side, word / 4, tok)));
+      }
+    }
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) {
+      const int e = e0 + 32 * f;
+      if (e >= n) break;
+#pragma unroll
+      for (int side = 0; side < 2; ++side)
+        out[side][e] = value8<T>(w[f][side], pars<T>(s[f][side] | s[f][side] << 16));
+    }
   }
 }
 
@@ -358,20 +380,23 @@ struct OpenParams {
   int few;       // sequences of up to so many rows are not needed
 };
 constexpr int kOpenPage = 128;  // tokens of a 16-bit page
-constexpr int kOpenTokens = 64; // of a CTA
 
+// A warp per block of 16 tokens and head: 2 D / 32 words a lane, each 16 bytes out.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) open_kernel(const __grid_constant__ OpenParams p) {
   using L = Layout<D>;
-  constexpr int kWords = D / 8;
+  constexpr int kWords = D / 8, kPer = kBlock * kWords / 32;  // words of a row; of a lane and side
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   ptx::grid_dependency_wait();
   ptx::grid_dependents_launch();
-  const int64_t per = p.wide * (kOpenPage / kOpenTokens);
-  const int i = (int)(blockIdx.x / per);
-  const int tok0 = (int)(blockIdx.x % per) * kOpenTokens;
+  // eight blocks and heads a CTA, in order [sequence, block, head]
   const int live = live_sequences(p.batch) - p.first;
   if (blockIdx.x == 0 && threadIdx.x == 0) *p.out_live = min(max(live, 0), p.n);
-  if (i >= live) return;
+  const int per = (int)p.wide * (kOpenPage / kBlock) * p.hkv;
+  const int64_t item = (int64_t)blockIdx.x * 8 + warp;
+  const int i = (int)(item / per), left = (int)(item - (int64_t)i * per);
+  if (i >= min(live, p.n)) return;
+  const int block = left / p.hkv, h = left - block * p.hkv;
   const int seq = p.first + i;
   const int req = p.batch.seq_ids ? __ldg(p.batch.seq_ids + seq) : seq;
   // (bad bounds, a bad request or length are the attention's to flag)
@@ -380,27 +405,31 @@ __global__ void __launch_bounds__(256) open_kernel(const __grid_constant__ OpenP
     if (!p.batch.cu || !sequence_bounds(p.batch, seq, &row0, &end) || end - row0 <= p.few) return;
   }
   if (req < 0 || req >= p.batch.n_requests) return;
-  if (tok0 % kOpenPage == 0 && threadIdx.x == 0)
+  const int tok0 = block * kBlock;
+  if (tok0 % kOpenPage == 0 && h == 0 && lane == 0)
     p.out_tables[req * p.wide + tok0 / kOpenPage] = i * (int)p.wide + tok0 / kOpenPage;
   const int kv = __ldg(p.batch.kv_lens + req);
-  if (kv > p.batch.max_kv) return;
-  const int tokens = min(kv - tok0, kOpenTokens);
-  for (int e = threadIdx.x; e < tokens * p.hkv * kWords; e += 256) {
-    const int word = e % kWords, tok = tok0 + e / kWords % tokens, h = e / (kWords * tokens);
-    const int pg = __ldg(p.tables + req * p.max_pages + tok / p.page);
-    const bool real = pg >= 0 && pg < p.n_pages;
-    if (!real) raise_error(p.batch.err, TIDE_DEVERR_POSITION);
-    const int at = tok % p.page;
-    const unsigned char *block =
-        p.cache + (((int64_t)(real ? pg : 0) * p.hkv + h) * (p.page / kBlock) + at / kBlock) * L::kBytes;
-    const int64_t to = (((i * p.wide + tok / kOpenPage) * p.hkv + h) * kOpenPage + tok % kOpenPage) * kWords + word;
+  if (kv > p.batch.max_kv || tok0 >= kv) return;
+  const int pg = __ldg(p.tables + req * p.max_pages + tok0 / p.page);
+  const bool real = pg >= 0 && pg < p.n_pages;
+  if (!real && lane == 0) raise_error(p.batch.err, TIDE_DEVERR_POSITION);
+  const unsigned char *from =
+      p.cache + (((int64_t)(real ? pg : 0) * p.hkv + h) * (p.page / kBlock) + tok0 % p.page / kBlock) * L::kBytes;
+  const int64_t to = (((i * p.wide + tok0 / kOpenPage) * p.hkv + h) * kOpenPage + tok0 % kOpenPage) * kWords;
+  // (the tokens past the last key of its block are opened too: they are masked)
 #pragma unroll
-    for (int side = 0; side < 2; ++side) {
-      const uint32_t w = *reinterpret_cast<const uint32_t *>(block + L::codes(side, at % kBlock) + word * 4);
-      const uint32_t s = *reinterpret_cast<const uint16_t *>(block + L::scale(side, word / 4, at % kBlock));
-      reinterpret_cast<uint4 *>(side ? p.v : p.k)[to] =
-          real ? value8<T>(w, pars<T>(s | s << 16)) : make_uint4(0, 0, 0, 0);
+  for (int side = 0; side < 2; ++side) {
+    uint32_t w[kPer], s[kPer];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const int at = e * 32 + lane, tok = at / kWords, word = at % kWords;
+      w[e] = __ldg(reinterpret_cast<const uint32_t *>(from + L::codes(side, 0)) + at);
+      s[e] = __ldg(reinterpret_cast<const uint16_t *>(from + L::scale(side, word / 4, tok)));
     }
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+      reinterpret_cast<uint4 *>(side ? p.v : p.k)[to + e * 32 + lane] =
+          real ? value8<T>(w[e], pars<T>(s[e] | s[e] << 16)) : make_uint4(0, 0, 0, 0);
   }
 }
 
@@ -1208,7 +1237,8 @@ int few_rows(int nt, int64_t ctas, const tide::q4::FewParams &p, cudaStream_t s)
 template <typename T, int D>
 int open(const tide::q4::OpenParams &p, cudaStream_t s) {
   using namespace tide::q4;
-  return start("paged_attention_q4", open_kernel<T, D>, p.n * p.wide * (kOpenPage / kOpenTokens), 256, 0, s, p);
+  return start("paged_attention_q4", open_kernel<T, D>,
+               (p.n * p.wide * (kOpenPage / kBlock) * p.hkv + 7) / 8, 256, 0, s, p);
 }
 
 }  // namespace
@@ -1273,7 +1303,7 @@ extern "C" int tide_paged_read_q4(int dtype, const void *cache, int64_t n_pages,
   if (!cache || !slots || !k_out || !v_out) return fail(TIDE_ERR_INVALID, "paged_read_q4: NULL pointer");
   if (((uintptr_t)cache | (uintptr_t)k_out | (uintptr_t)v_out) & 15)
     return fail(TIDE_ERR_ALIGNMENT, "paged_read_q4: rows and cache must be 16-byte aligned");
-  const int64_t grid = (n_rows * n_kv_heads * (head_dim / 8) + 255) / 256;
+  const int64_t grid = (n_rows + 7) / 8;
   cudaStream_t s = (cudaStream_t)stream;
   const auto *c = static_cast<const unsigned char *>(cache);
   const int hkv = (int)n_kv_heads, page = (int)page_size;
@@ -1345,6 +1375,8 @@ extern "C" int tide_paged_attention_q4(int dtype, const void *q, int64_t q_row_s
   unsigned char *ws = static_cast<unsigned char *>(workspace);
   const Plan plan =
       plan_of(!cu_seqlens, n_tokens, n_seqs, n_requests, n_q_heads, n_kv_heads, head_dim, max_kv_len);
+  if (plan.tiles && plan.wide * (tide::q4::kOpenPage / 16) * n_kv_heads > INT32_MAX)
+    return fail(TIDE_ERR_INVALID, "paged_attention_q4: max_kv_len too large for so many heads");
   int shift = 0;
   while ((1 << shift) < page_size) ++shift;
   const tide::RaggedBatch batch{cu_seqlens, seq_ids, kv_lens, n_seqs_dev, (int)n_seqs, (int)n_requests,
