@@ -25,9 +25,9 @@ namespace q4 {
 // two cycles each, and a sine and cosine per row and frequency, which the CTA
 // makes once for all its heads; both run under the loads and stores.
 //
-// A lane has four neighbouring channels of a head's lower half and the four
-// that they are turned with, so D / 8 lanes share a head and the eight lanes of
-// a group find its least and largest value in three exchanges.
+// A lane has eight neighbouring channels of a head's lower half, which are a word
+// of codes, and the eight that they are turned with.  So D / 16 lanes share a head,
+// and the four lanes of a group find its least and largest value in two exchanges.
 struct AppendParams {
   const void *q, *k, *v;
   int64_t q_stride, kv_stride;
@@ -51,29 +51,31 @@ struct AppendParams {
 // last bits.
 constexpr float kRounder = 12582912.f;  // 3 * 2^22
 
-// Least and largest value of the group of which this lane, of eight neighbours, has
-// four, 0 among them; whether one of them is not finite.
-__device__ __forceinline__ bool extent(const float (&x)[4], float *lo, float *hi) {
+// Least and largest value of the group of which this lane, of four neighbours, has
+// eight, 0 among them; whether one of them is not finite.
+__device__ __forceinline__ bool extent(const float (&x)[8], float *lo, float *hi) {
   constexpr unsigned kFull = 0xffffffffu;
-  float a = fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), b = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-  const float all = (x[0] + x[1]) * 0.f + (x[2] + x[3]) * 0.f;  // NaN where one is not finite, or the sum is not
-  const unsigned who = __ballot_sync(kFull, !(all == 0.f));
+  float a = x[0], b = x[0], all = x[0] * 0.f;
 #pragma unroll
-  for (int w = 1; w < 8; w *= 2) {
+  for (int e = 1; e < 8; ++e) {
+    a = fminf(a, x[e]);
+    b = fmaxf(b, x[e]);
+    all = fmaf(x[e], 0.f, all);  // NaN where one is not finite
+  }
+  const unsigned who = __ballot_sync(kFull, all != 0.f);
+#pragma unroll
+  for (int w = 1; w < 4; w *= 2) {
     a = fminf(a, __shfl_xor_sync(kFull, a, w));
     b = fmaxf(b, __shfl_xor_sync(kFull, b, w));
   }
   *lo = fminf(a, 0.f);
   *hi = fmaxf(b, 0.f);
-  if (!who) return false;
-  const bool odd = !(isfinite(x[0]) && isfinite(x[1]) && isfinite(x[2]) && isfinite(x[3]));
-  return __ballot_sync(kFull, odd) >> (threadIdx.x & 24) & 0xffu;
+  return who >> (threadIdx.x & 28) & 0xfu;
 }
 
-// The group's codes of this lane as the nibbles 0, 4, 1, 5 of the result, and its
-// scale and zero point.
+// The group's word of codes of this lane, and its scale and zero point.
 template <typename T>
-__device__ __forceinline__ uint32_t quantise(const float (&x)[4], uint32_t *par) {
+__device__ __forceinline__ uint32_t quantise(const float (&x)[8], uint32_t *par) {
   constexpr bool kHalf = std::is_same<T, __half>::value;
   constexpr float kMost = kHalf ? 65504.f : 3.3895313892515355e38f;
   constexpr float kLeast = kHalf ? 0x1p-21f : 0x1p-120f;
@@ -98,49 +100,73 @@ __device__ __forceinline__ uint32_t quantise(const float (&x)[4], uint32_t *par)
   *par = __float_as_uint(s) >> 16 | (uint32_t)z;
   // bits[e] = kRounder's + code - z; below 0 a code cannot be (the least value's is
   // z - z), above 15 it can
-  uint32_t bits[4];
+  uint32_t bits[8];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) bits[e] = __float_as_uint(fminf(over(x[e]) + kRounder, kRounder + (15.f - z)));
+  for (int e = 0; e < 8; ++e) bits[e] = __float_as_uint(fminf(over(x[e]) + kRounder, kRounder + (15.f - z)));
   if (s > kMost / 16.f) {  // next to the type's largest number: none above it
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < 8; ++e) {
       const float n = __uint_as_float(bits[e]) - kRounder;
       if (fabsf(n * s) > kMost) bits[e] = __float_as_uint(n - copysignf(1.f, n) + kRounder);
     }
   }
-  constexpr uint32_t kSpread = 1u + (1u << 4) + (1u << 16) + (1u << 20);
-  return bits[0] + (bits[2] << 4) + (bits[1] << 16) + (bits[3] << 20) +
-         ((uint32_t)z - 0x4b400000u) * kSpread;  // (modulo 2^32)
+  uint32_t word = ((uint32_t)z - 0x4b400000u) * 0x11111111u;  // (modulo 2^32)
+#pragma unroll
+  for (int e = 0; e < 8; ++e) word += bits[e] * (1u << (4 * (e / 2) + 16 * (e % 2)));
+  return word;
 }
 
-template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendParams p) {
+// ROWS rows a CTA, WARPS warps a row; a warp has D / 16 lanes a head, so 4 or 8
+// heads at a time, of the values, of the keys, and of the queries in turn.
+template <typename T, int D, int ROWS, int WARPS>
+__global__ void __launch_bounds__(32 * ROWS * WARPS, 24 / (ROWS * WARPS))
+    append_kernel(const __grid_constant__ AppendParams p) {
   using namespace ragged;
   using L = Layout<D>;
   constexpr unsigned kFull = 0xffffffffu;
-  constexpr int kLanes = D / 8;         // of a head
-  constexpr int kHeads = 32 / kLanes;   // of a warp
-  constexpr int kWarps = 8 / ROWS;      // of a row
-  constexpr int kFlight = 4;            // heads of a lane, loaded before the first is used
-  // cosine and sine of channel 4 j + e at [e][j]
-  __shared__ double2 turn[ROWS][4][kLanes];
-  __shared__ float2 turn32[ROWS][4][kLanes];
+  constexpr int kThreads = 32 * ROWS * WARPS;
+  constexpr int kLanes = D / 16;              // of a head
+  constexpr int kHeads = 32 / kLanes;         // of a warp
+  constexpr int kStep = WARPS * kHeads;       // from a warp's heads to its next
+  // cosine and sine of channel 8 j + e at [e][j]
+  __shared__ double2 turn[ROWS][8][kLanes];
+  __shared__ float2 turn32[ROWS][8][kLanes];
   __shared__ int64_t s_block[ROWS];  // the slot's block in head 0; -1: nothing to write
   __shared__ int s_token[ROWS];      // and its token there; -1: no such row
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int head = lane / kLanes, j = lane % kLanes;
+  const int j = lane % kLanes, r = warp / WARPS;
+  // the first head of this lane: of the values, of the keys, which begin with the
+  // warps that have the fewest values, of the queries
+  const int kv_tasks = (p.hkv + kHeads - 1) / kHeads;
+  const int first_v = warp % WARPS * kHeads, first_k = (warp + kv_tasks * (WARPS - 1)) % WARPS * kHeads;
+  const int first_q = (warp + 2 * kv_tasks * (WARPS - 1)) % WARPS * kHeads, in = lane / kLanes;
   ptx::grid_dependency_wait();
   ptx::grid_dependents_launch();
   int64_t live = p.n_rows;
   if (p.n_dev) live = min((int64_t)max(__ldg(p.n_dev), 0), p.n_rows);
   const int64_t row0 = (int64_t)blockIdx.x * ROWS;
   if (row0 >= live) return;
-  const int q_tasks = p.q ? (p.hq + kHeads - 1) / kHeads : 0, kv_tasks = (p.hkv + kHeads - 1) / kHeads;
-  const int r = warp / kWarps;
-  const int tasks = row0 + r < live ? q_tasks + 2 * kv_tasks : 0;  // warps of heads: q, k, v
+  const bool mine = row0 + r < live;
   const int head_blocks = p.page / kBlock;
+  // this lane's channels 8 j.. and D / 2 + 8 j..
+  struct Raw {
+    uint4 a, b;
+  };
+  auto load = [&](const void *from, int64_t stride, int h, int heads) {
+    Raw x{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    if (mine && h < heads) {
+      const T *src = static_cast<const T *>(from) + (row0 + r) * stride + h * D + 8 * j;
+      x.a = __ldcs(reinterpret_cast<const uint4 *>(src));
+      x.b = __ldcs(reinterpret_cast<const uint4 *>(src + D / 2));
+    }
+    return x;
+  };
+  const int hq = p.q ? p.hq : 0;
+  Raw next_v = load(p.v, p.kv_stride, first_v + in, p.hkv);
+  Raw next_k = load(p.k, p.kv_stride, first_k + in, p.hkv);
+  Raw next_q = load(p.q, p.q_stride, first_q + in, hq);
   // the rows' slots, and their angles' cosines and sines
-  for (int i = threadIdx.x; i < ROWS * (D / 2); i += 256) {
+  for (int i = threadIdx.x; i < ROWS * (D / 2); i += kThreads) {
     const int at = i / (D / 2), f = i % (D / 2);
     const int64_t row = row0 + at;
     if (row >= live) continue;
@@ -162,124 +188,112 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
       sincospi(2.0 * (turns - rint(turns)), &s, &c);
       c *= (double)p.att_scale;
       s *= (double)p.att_scale;
-      turn[at][f % 4][f / 4] = make_double2(c, s);
-      turn32[at][f % 4][f / 4] = make_float2((float)c, (float)s);
+      turn[at][f % 8][f / 8] = make_double2(c, s);
+      turn32[at][f % 8][f / 8] = make_float2((float)c, (float)s);
     }
   }
-  // this lane's channels 4 j.. and D / 2 + 4 j.. of the heads of `kFlight` tasks
-  const T *const q = static_cast<const T *>(p.q) + (row0 + r) * p.q_stride + 4 * j;
-  const T *const k = static_cast<const T *>(p.k) + (row0 + r) * p.kv_stride + 4 * j;
-  const T *const v = static_cast<const T *>(p.v) + (row0 + r) * p.kv_stride + 4 * j;
-  auto kind_of = [&](int t) { return (t >= q_tasks) + (t >= q_tasks + kv_tasks); };
-  auto head_of = [&](int t, int kind) {
-    return (t - (kind > 0 ? q_tasks : 0) - (kind > 1 ? kv_tasks : 0)) * kHeads + head;
-  };
-  bool ready = false;
-  for (int t0 = warp % kWarps; t0 < tasks || !ready; t0 += kWarps * kFlight) {
-    uint2 raw[kFlight][2];
+  __syncthreads();
+  if (!mine || s_token[r] < 0) return;
+  const int tok = s_token[r];
+  // where the row's token has its codes and scales in head 0
+  unsigned char *const to = p.cache + s_block[r] * L::kBytes;
+  const bool place = s_block[r] >= 0;
+  auto store = [&](int side, int h, const float (&x)[2][8]) {
+    uint32_t par[2];
+    const uint32_t word[2] = {quantise<T>(x[0], &par[0]), quantise<T>(x[1], &par[1])};
+    if (!place || h >= p.hkv) return;
+    unsigned char *block = to + (int64_t)h * head_blocks * L::kBytes;
 #pragma unroll
-    for (int i = 0; i < kFlight; ++i) {
-      const int t = t0 + kWarps * i, kind = kind_of(t), h = head_of(t, kind);
-      raw[i][0] = raw[i][1] = make_uint2(0u, 0u);
-      if (t < tasks && h < (kind ? p.hkv : p.hq)) {
-        const T *src = (kind == 0 ? q : kind == 1 ? k : v) + (int64_t)h * D;
-        raw[i][0] = __ldcs(reinterpret_cast<const uint2 *>(src));
-        raw[i][1] = __ldcs(reinterpret_cast<const uint2 *>(src + D / 2));
+    for (int a = 0; a < 2; ++a) {
+      *reinterpret_cast<uint32_t *>(block + L::codes(side, tok) + a * (D / 4) + j * 4) = word[a];
+      if (j % 4 == 0)
+        *reinterpret_cast<uint16_t *>(block + L::scale(side, a * (D / 64) + j / 4, tok)) = (uint16_t)par[a];
+    }
+  };
+#pragma unroll 1
+  for (int h = first_v; h < p.hkv; h += kStep) {
+    float x[2][8];
+    unpack16<T>(next_v.a, x[0]);
+    unpack16<T>(next_v.b, x[1]);
+    next_v = load(p.v, p.kv_stride, h + in + kStep, p.hkv);
+    store(1, h + in, x);
+  }
+#pragma unroll 1
+  for (int h = first_k; h < p.hkv; h += kStep) {
+    float x[2][8];
+    unpack16<T>(next_k.a, x[0]);
+    unpack16<T>(next_k.b, x[1]);
+    next_k = load(p.k, p.kv_stride, h + in + kStep, p.hkv);
+    double rstd = 1.0;
+    const T *w = static_cast<const T *>(p.k_w) + 8 * j;
+    if (p.k_w) {
+      double ss = 0.0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        ss = fma((double)x[0][e], (double)x[0][e], fma((double)x[1][e], (double)x[1][e], ss));
+#pragma unroll
+      for (int i = 1; i < kLanes; i *= 2) ss += __shfl_xor_sync(kFull, ss, i);
+      rstd = rsqrt(ss / (double)D + (double)p.eps);
+    }
+    if (p.k_w || p.inv_freq) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        double a = (double)x[0][e], b = (double)x[1][e];
+        if (p.k_w) {
+          a *= rstd * (double)Elem<T>::to_f(w[e]);
+          b *= rstd * (double)Elem<T>::to_f(w[D / 2 + e]);
+        }
+        if (p.inv_freq) {
+          const double2 cs = turn[r][e][j];
+          const double y = fma(a, cs.x, -(b * cs.y));
+          b = fma(b, cs.x, a * cs.y);
+          a = y;
+        }
+        x[0][e] = (float)a;
+        x[1][e] = (float)b;
       }
     }
-    if (!ready) {
-      __syncthreads();
-      ready = true;
-    }
+    store(0, h + in, x);
+  }
+  if (first_q >= hq) return;
+  float2 cs[8];
 #pragma unroll
-    for (int i = 0; i < kFlight; ++i) {
-      const int t = t0 + kWarps * i;
-      if (t >= tasks) break;
-      const int kind = kind_of(t), h = head_of(t, kind);
-      float x[2][4];
+  for (int e = 0; e < 8; ++e) cs[e] = p.inv_freq ? turn32[r][e][j] : make_float2(1.f, 0.f);
+  T *const out = static_cast<T *>(p.q_out) + (row0 + r) * p.hq * D + 8 * j;
+#pragma unroll 1
+  for (int h = first_q; h < hq; h += kStep) {
+    float x[2][8];
+    unpack16<T>(next_q.a, x[0]);
+    unpack16<T>(next_q.b, x[1]);
+    next_q = load(p.q, p.q_stride, h + in + kStep, hq);
+    if (p.q_w) {
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss = fmaf(x[0][e], x[0][e], fmaf(x[1][e], x[1][e], ss));
+#pragma unroll
+      for (int i = 1; i < kLanes; i *= 2) ss += __shfl_xor_sync(kFull, ss, i);
+      const float rstd = rsqrtf(ss / (float)D + p.eps);
+      const T *w = static_cast<const T *>(p.q_w) + 8 * j;
 #pragma unroll
       for (int a = 0; a < 2; ++a)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[a][e] = Elem<T>::to_f(reinterpret_cast<const T *>(&raw[i][a])[e]);
-      if (kind == 0) {
-        if (p.q_w) {
-          float ss = 0.f;
+        for (int e = 0; e < 8; ++e) x[a][e] *= rstd * Elem<T>::to_f(w[a * (D / 2) + e]);
+    }
+    if (p.inv_freq) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) ss = fmaf(x[0][e], x[0][e], fmaf(x[1][e], x[1][e], ss));
-#pragma unroll
-          for (int w = 1; w < kLanes; w *= 2) ss += __shfl_xor_sync(kFull, ss, w);
-          const float rstd = rsqrtf(ss / (float)D + p.eps);
-          const T *w = static_cast<const T *>(p.q_w) + 4 * j;
-#pragma unroll
-          for (int a = 0; a < 2; ++a)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[a][e] *= rstd * Elem<T>::to_f(w[a * (D / 2) + e]);
-        }
-        if (p.inv_freq) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 cs = turn32[r][e][j];
-            const float a = x[0][e], b = x[1][e];
-            x[0][e] = fmaf(a, cs.x, -b * cs.y);
-            x[1][e] = fmaf(b, cs.x, a * cs.y);
-          }
-        }
-        if (h < p.hq && s_token[r] >= 0) {
-          T *to = static_cast<T *>(p.q_out) + ((row0 + r) * p.hq + h) * D + 4 * j;
-#pragma unroll
-          for (int a = 0; a < 2; ++a)
-            *reinterpret_cast<uint2 *>(to + a * (D / 2)) =
-                make_uint2(pack2<T>(x[a][0], x[a][1]), pack2<T>(x[a][2], x[a][3]));
-        }
-        continue;
+      for (int e = 0; e < 8; ++e) {
+        const float a = x[0][e], b = x[1][e];
+        x[0][e] = fmaf(a, cs[e].x, -b * cs[e].y);
+        x[1][e] = fmaf(b, cs[e].x, a * cs[e].y);
       }
-      if (kind == 1 && (p.k_w || p.inv_freq)) {
-        double y[2][4];
+    }
+    if (h + in < hq) {
+      T *at = out + (h + in) * D;
 #pragma unroll
-        for (int a = 0; a < 2; ++a)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) y[a][e] = (double)x[a][e];
-        if (p.k_w) {
-          double ss = 0.0;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) ss = fma(y[0][e], y[0][e], fma(y[1][e], y[1][e], ss));
-#pragma unroll
-          for (int w = 1; w < kLanes; w *= 2) ss += __shfl_xor_sync(kFull, ss, w);
-          const double rstd = rsqrt(ss / (double)D + (double)p.eps);
-          const T *w = static_cast<const T *>(p.k_w) + 4 * j;
-#pragma unroll
-          for (int a = 0; a < 2; ++a)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[a][e] *= rstd * (double)Elem<T>::to_f(w[a * (D / 2) + e]);
-        }
-        if (p.inv_freq) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const double2 cs = turn[r][e][j];
-            const double a = y[0][e], b = y[1][e];
-            y[0][e] = fma(a, cs.x, -(b * cs.y));
-            y[1][e] = fma(b, cs.x, a * cs.y);
-          }
-        }
-#pragma unroll
-        for (int a = 0; a < 2; ++a)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[a][e] = (float)y[a][e];
-      }
-      uint32_t par[2];
-      const uint32_t low = quantise<T>(x[0], &par[0]), high = quantise<T>(x[1], &par[1]);
-      // eight channels are two lanes': the even one stores the lower half's word
-      const uint32_t other = __shfl_xor_sync(kFull, j & 1 ? low : high, 1);
-      const uint32_t word = j & 1 ? high << 8 | other : low | other << 8;
-      if (s_block[r] < 0 || h >= p.hkv) continue;
-      const int tok = s_token[r], side = kind - 1;
-      unsigned char *block = p.cache + (s_block[r] + h * head_blocks) * L::kBytes;
-      *reinterpret_cast<uint32_t *>(block + L::codes(side, tok) + (j & 1) * (D / 4) + j / 2 * 4) = word;
-      if (j % 8 == 0) {
-#pragma unroll
-        for (int a = 0; a < 2; ++a)
-          *reinterpret_cast<uint16_t *>(block + L::scale(side, a * (D / 64) + j / 8, tok)) = (uint16_t)par[a];
-      }
+      for (int a = 0; a < 2; ++a)
+        *reinterpret_cast<uint4 *>(at + a * (D / 2)) =
+            make_uint4(pack2<T>(x[a][0], x[a][1]), pack2<T>(x[a][2], x[a][3]), pack2<T>(x[a][4], x[a][5]),
+                       pack2<T>(x[a][6], x[a][7]));
     }
   }
 }
@@ -1149,11 +1163,10 @@ bool bad_cache(int64_t n_pages, int64_t page_size, int64_t hkv) {
 template <typename T, int D>
 int append(const tide::q4::AppendParams &p, cudaStream_t s) {
   using namespace tide::q4;
-  // Four rows a CTA share its start and its angles' pass where there are CTAs
-  // enough for every SM without that; else a row, for more warps a row.
-  if (p.n_rows >= 148 * 16)
-    return start("paged_append_q4", append_kernel<T, D, 4>, (p.n_rows + 3) / 4, 256, 0, s, p);
-  return start("paged_append_q4", append_kernel<T, D, 1>, p.n_rows, 256, 0, s, p);
+  // Two warps a row where that fills the GPU; else eight, the more the sooner done.
+  if (p.n_rows * 2 >= 148 * 16)
+    return start("paged_append_q4", append_kernel<T, D, 2, 2>, (p.n_rows + 1) / 2, 128, 0, s, p);
+  return start("paged_append_q4", append_kernel<T, D, 1, 8>, p.n_rows, 256, 0, s, p);
 }
 
 // How an attention call is cut up.  Sequences of up to `few` tokens go to the
