@@ -452,8 +452,9 @@ __global__ void __launch_bounds__(256) open_kernel(const __grid_constant__ OpenP
 // up to 8 NT rows of a sequence, over the blocks of its keys in one head.  All
 // blocks of all units in a row are dealt out evenly to as many CTAs as run at once,
 // found from the lengths by a prefix sum that each makes, so a CTA has the end of
-// one unit, some whole ones, and the beginning of another; units that two or more
-// CTAs share are joined by a kernel of their own, in the order of the keys.  (With a
+// one unit, some whole ones, and the beginning of another (a unit counts as
+// kUnitCost blocks more, before its first); units that two or more CTAs share are
+// joined by a kernel of their own, in the order of the keys.  (With a
 // CTA a unit, and splits of equal length, a decode step of 192 requests left the
 // SMs idle for a sixth of its time, and one of three very different requests for
 // half.)  Short contexts are dealt out by whole units, and need no join.
@@ -482,7 +483,8 @@ __global__ void __launch_bounds__(256) open_kernel(const __grid_constant__ OpenP
 // for the values as a tile with a row per group.  (fp16 has no room for 136 s.)
 constexpr int kFewWarps = 4;
 constexpr int kBatch = 3;        // blocks of a place
-constexpr int kLeastBlocks = 8;  // of a CTA, where there are so few
+constexpr int kUnitCost = 8;     // what beginning and ending a unit costs, in blocks
+constexpr int kLeast = 16;       // cost of a CTA, where there is so little
 
 template <int D, int NT>
 struct Few {
@@ -569,7 +571,7 @@ struct Part {
   Sequence s;
   int seq, row;  // sequence, first of its rows
   int kvh;
-  int b0, nb;    // first block of the part, blocks of the unit
+  int at, nb;    // where the part begins in the unit's cost; blocks of the unit
 };
 
 template <typename T, int D, int NT>
@@ -608,7 +610,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
     return s.kv - s.n + 1 + token_of(min(row + kRowsMost, s.n * p.group) - 1, p.per_group);
   };
   auto blocks_of = [&](const Sequence &s, int row) { return max((keys_of(s, row) + kBlock - 1) / kBlock, 1); };
-  auto cost_of = [&](const Sequence &s, int row) { return p.whole ? 1 : blocks_of(s, row); };
+  auto cost_of = [&](const Sequence &s, int row) { return p.whole ? 1 : blocks_of(s, row) + kUnitCost; };
   auto rows_of = [&](const Sequence &s) { return s.n <= p.few ? s.n * p.group : 0; };
   auto weight = [&](const Sequence &s) {  // of all units of a sequence
     long long w = 0;
@@ -622,7 +624,11 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
     const int per = (live + 32 * kFewWarps - 1) / (32 * kFewWarps);
     const int from = min((int)threadIdx.x * per, live), to = min(from + per, live);
     long long sum = 0;
-    for (int i = from; i < to; ++i) sum += weight(sequence(p.batch, i));
+    Sequence s{};
+    for (int i = from; i < to; ++i) {
+      s = sequence(p.batch, i);
+      sum += weight(s);
+    }
     long long upto = sum;
 #pragma unroll
     for (int w = 1; w < 32; w *= 2) {
@@ -636,7 +642,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
       if (w < warp) upto += s_sum[w];
       total += s_sum[w];
     }
-    const long long least = p.whole ? 1 : kLeastBlocks;
+    const long long least = p.whole ? 1 : kLeast;
     const int ctas = (int)min((long long)gridDim.x, (total + least - 1) / least);
     if ((int)blockIdx.x >= ctas) {
       if (threadIdx.x == 0 && !p.whole) p.shared[blockIdx.x].first = -1;
@@ -649,7 +655,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
     if (pos >= upto - sum && pos < upto) {
       long long rest = pos - (upto - sum);
       for (int i = from; i < to; ++i) {
-        const Sequence s = sequence(p.batch, i);
+        if (per > 1) s = sequence(p.batch, i);
         for (int row = 0; row < rows_of(s); row += kRowsMost) {
           const long long c = cost_of(s, row);
           if (rest >= 0 && rest < c * p.hkv) {
@@ -662,9 +668,9 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
     }
     __syncthreads();
   }
-  auto cta_of = [&](long long block) {
+  auto cta_of = [&](long long cost) {
     const long long at = longer * (share + 1);
-    return (int)(block < at ? quotient(block, share + 1) : longer + quotient(block - at, share));
+    return (int)(cost < at ? quotient(cost, share + 1) : longer + quotient(cost - at, share));
   };
 
   unsigned char *ring = dyn + warp * F::kRing;
@@ -684,16 +690,26 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
     const int kv = keys_of(u.s, u.row);
     const int rows = min(kRowsMost, u.s.n * p.group - u.row);
     const int tiles = (rows + 7) / 8;  // 8-row groups that there are
-    const int b1 = p.whole ? u.nb : (int)min((long long)u.nb, u.b0 + (end - pos));
-    if (starts && !p.whole && threadIdx.x == 0) {
-      Shared x{-1, -1, u.s.row0, u.row, rows, u.kvh};
-      if (u.b0 > 0) x.first = cta_of(pos - u.b0), x.last = cta_of(pos - u.b0 + u.nb - 1);
-      p.shared[blockIdx.x] = x;
+    // its blocks [b0, b1) are this CTA's
+    const int left = p.whole ? 1 : u.nb + kUnitCost - u.at;  // of the unit's cost
+    const int b0 = p.whole ? 0 : max(u.at - kUnitCost, 0);
+    const int b1 = p.whole ? u.nb : u.nb - (int)min(max(left - (end - pos), 0ll), (long long)u.nb);
+    // and this warp's b0 + warp, 4 further, ...
+    const int blocks = max(0, (b1 - b0 - warp + kFewWarps - 1) / kFewWarps);
+    const int block0 = b0 + warp;
+    if (b1 > b0 || starts) {
+    uint4 raw[NT][kKWords];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = nt * 8 + g;
+      const bool valid = r < rows;
+      const int tok = token_of(u.row + (valid ? r : 0), p.per_group);
+      const T *q = static_cast<const T *>(p.q) + (u.s.row0 + tok) * p.q_stride +
+                   (int64_t)(u.kvh * p.group + u.row + (valid ? r : 0) - tok * p.group) * D + t * (D / 4);
+#pragma unroll
+      for (int w = 0; w < kKWords; ++w)
+        raw[nt][w] = valid ? *reinterpret_cast<const uint4 *>(q + 8 * w) : make_uint4(0, 0, 0, 0);
     }
-    starts = false;
-    // this warp's blocks: b0 + warp, 4 further, ...
-    const int blocks = max(0, (b1 - u.b0 - warp + kFewWarps - 1) / kFewWarps);
-    const int block0 = u.b0 + warp;
     // where 32 blocks at a time are in the cache, one per lane, the next ones read
     // ahead; -1: a page outside it
     auto places = [&](int i0) {
@@ -732,6 +748,13 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
     };
     request(0, turn & 1);
     request(kBatch, (turn & 1) ^ 1);
+    if (starts && !p.whole && threadIdx.x == 0) {
+      Shared x{-1, -1, u.s.row0, u.row, rows, u.kvh};
+      const long long block = pos - u.at + kUnitCost;  // the unit's first one's place in all
+      if (b0 > 0) x.first = cta_of(block), x.last = cta_of(block + u.nb - 1);
+      p.shared[blockIdx.x] = x;
+    }
+    starts = false;
 
     // Q^T: columns are rows 8 nt + g; the statistics of a column are kept by the
     // lanes whose accumulators belong to it, columns 8 nt + 2 t and one further
@@ -739,15 +762,10 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
     int sees[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int r = nt * 8 + g;
-      const bool valid = r < rows;
-      const int tok = token_of(u.row + (valid ? r : 0), p.per_group);
-      const T *q = static_cast<const T *>(p.q) + (u.s.row0 + tok) * p.q_stride +
-                   (int64_t)(u.kvh * p.group + u.row + (valid ? r : 0) - tok * p.group) * D + t * (D / 4);
       float sum = 0.f;
 #pragma unroll
       for (int w = 0; w < kKWords; ++w) {
-        const uint4 x = valid ? *reinterpret_cast<const uint4 *>(q + 8 * w) : make_uint4(0, 0, 0, 0);
+        const uint4 x = raw[nt][w];
         qb[nt][2 * w][0] = x.x;
         qb[nt][2 * w][1] = x.y;
         qb[nt][2 * w + 1][0] = x.z;
@@ -1002,8 +1020,8 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
         x.z = fmaf(a, y.z, x.z);
         x.w = fmaf(a, y.w, x.w);
       }
-      if (u.b0 > 0 || b1 < u.nb) {
-        const int64_t part = (2 * (int64_t)blockIdx.x + (u.b0 == 0)) * kRowsMost + r;
+      if (b0 > 0 || b1 < u.nb) {
+        const int64_t part = (2 * (int64_t)blockIdx.x + (b0 == 0)) * kRowsMost + r;
         if (d == 0) p.part_ml[part] = make_float2(top, sum);
         *reinterpret_cast<float4 *>(p.part_o + part * D + d) = x;
       } else {
@@ -1014,14 +1032,15 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
             make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
       }
     }
-    pos += p.whole ? 1 : b1 - u.b0;
+    }
+    pos += left;
     if (pos >= end || *(volatile int *)&s_abort) return;
     ptx::fence_proxy_async();  // (copies go where the outputs were)
     __syncthreads();
     if (warp == 0) {  // the next unit
       const int row = u.row + kRowsMost;
       if (u.kvh + 1 < p.hkv) {
-        if (lane == 0) s_part.kvh = u.kvh + 1, s_part.b0 = 0;
+        if (lane == 0) s_part.kvh = u.kvh + 1, s_part.at = 0;
       } else if (row < u.s.n * p.group) {
         if (lane == 0) s_part = {u.s, u.seq, row, 0, 0, blocks_of(u.s, row)};
       } else {  // the next sequence that has one, 32 at a time
@@ -1202,7 +1221,7 @@ Plan plan_of(bool one_token, int64_t n_tokens, int64_t n_seqs, int64_t n_request
     const int64_t slots = 148 * (p.nt == 1 ? 4 : 3);
     const int64_t units = (n_seqs + n_tokens * group / (8 * p.nt)) * hkv;
     const int64_t blocks = (max_kv + kBlock - 1) / kBlock;
-    p.ctas = p.whole ? units : (units * (blocks < 1 ? 1 : blocks) + kLeastBlocks - 1) / kLeastBlocks;
+    p.ctas = p.whole ? units : (units * ((blocks < 1 ? 1 : blocks) + kUnitCost) + kLeast - 1) / kLeast;
     if (p.ctas > slots) p.ctas = slots;
     if (!p.whole)
       p.few_bytes = (size_t)(p.ctas * (2 * 8 * p.nt * (d + 2) * 4 + (int64_t)sizeof(Shared)) + 15) / 16 * 16;

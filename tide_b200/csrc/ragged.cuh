@@ -48,6 +48,7 @@ __device__ __forceinline__ Sequence sequence(const RaggedBatch &b, int i) {
   Sequence s;
   s.row0 = i;
   s.n = 1;
+  const int named = b.kv_lens && b.seq_ids ? __ldg(b.seq_ids + i) : i;  // (with the bounds under way)
   if (b.cu) {
     int end;
     const bool good = sequence_bounds(b, i, &s.row0, &end);
@@ -60,7 +61,7 @@ __device__ __forceinline__ Sequence sequence(const RaggedBatch &b, int i) {
   s.req = i;
   s.kv = s.n;
   if (s.n && b.kv_lens) {
-    if (b.seq_ids) s.req = __ldg(b.seq_ids + i);
+    s.req = named;
     const bool known = s.req >= 0 && s.req < b.n_requests;
     s.kv = known ? __ldg(b.kv_lens + s.req) : -1;
     if (s.kv < 0 || s.kv > b.max_kv) {
