@@ -475,12 +475,8 @@ __global__ void __launch_bounds__(256) open_kernel(const __grid_constant__ OpenP
 // works on and one under way.  The sum of the weights, as they meet the values, is
 // one more row of the values' product.
 //
-// What bounds it is the instructions that make operands, so bf16 ones are (c - 8) s
-// instead of (c - z) s: one fma of the number 128 + c, whose code is its last bits,
-// with s and -136 s, all three exact (17 times a scale's four bits are eight).  The
-// rest, (8 - z) s, is the same for a group, and joins as one more product on both
-// sides: against the sums of the queries' groups, three bf16 each (24 bits), and
-// for the values as a tile with a row per group.  (fp16 has no room for 136 s.)
+// What bounds it is the instructions: of a block's 400 some 260 make operands from
+// codes, a shift, a mask, a difference and a product for two of them.
 constexpr int kFewWarps = 4;
 constexpr int kBatch = 3;        // blocks of a place
 constexpr int kUnitCost = 8;     // what beginning and ending a unit costs, in blocks
@@ -539,32 +535,8 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
   return __byte_perm(a, b, sel);
 }
 
-// Two operands at a time from codes in the lowest four bits of a word's halves, by
-// the scales in the halves of another: (c - z) s, or for bf16 (c - 8) s, of which
-// minus_rest() is the negative remainder.
 template <typename T>
-struct Maker {
-  Pars<T> p;
-  uint32_t magic;
-  __device__ __forceinline__ Maker(uint32_t scales, uint32_t magic) : p(pars<T>(scales, magic)), magic(magic) {}
-  __device__ __forceinline__ uint32_t operator()(uint32_t x) const { return value2<T>(x, p, magic); }
-  __device__ __forceinline__ uint32_t minus_rest() const { return 0u; }
-};
-template <>
-struct Maker<__nv_bfloat16> {
-  Pars<__nv_bfloat16> p;
-  __nv_bfloat162 minus;  // -136 s
-  uint32_t magic;
-  __device__ __forceinline__ Maker(uint32_t scales, uint32_t magic)
-      : p(pars<__nv_bfloat16>(scales, magic)),
-        minus(__hmul2(p.scale, __float2bfloat162_rn(-136.f))),
-        magic(magic) {}
-  __device__ __forceinline__ uint32_t operator()(uint32_t x) const {
-    return as_bits(__hfma2(as_pair<__nv_bfloat16>(numbers(x, magic)), p.scale, minus));
-  }
-  // (128 + z) s - 136 s
-  __device__ __forceinline__ uint32_t minus_rest() const { return as_bits(__hfma2(p.zero, p.scale, minus)); }
-};
+constexpr uint32_t kOnes = std::is_same<T, __half>::value ? 0x3c003c00u : 0x3f803f80u;  // two of them
 
 // A unit, or a CTA's part of it.
 struct Part {
@@ -584,9 +556,6 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
   constexpr int kRowsMost = 8 * NT, kSteps = D / 16;
   constexpr int kKWords = D / 32;  // words of a lane's channels in a key
   constexpr int kVWords = D / 64;  // in a value
-  constexpr bool kCentred = !std::is_same<T, __half>::value;
-  constexpr int kSumRow = 4;  // of the values' last tile
-  static_assert(D / kGroup <= kSumRow, "");
   extern __shared__ __align__(128) unsigned char dyn[];
   __shared__ uint64_t full[kFewWarps][2];
   __shared__ float s_m[kFewWarps][kRowsMost], s_l[kFewWarps][kRowsMost];
@@ -679,7 +648,6 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
   const int kappa = (g >> 1) + 4 * (g & 1);
   const int k_at = L::codes(0, kappa) + t * (D / 8), ks_at = L::scale(0, t * (D / 4) / kGroup, g >> 1);
   const int v_at = L::codes(1, t) + g * (D / 16), vs_at = L::scale(1, g * (D / 8) / kGroup, t);
-  const int vc_at = L::scale(1, g % (D / kGroup), t);
   const float slack = kSlack / p.qs;
   const uint32_t magic = p.magic;
   uint32_t turn = 0;  // places used so far: the next is the last bit, its phase the one before
@@ -758,11 +726,10 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
 
     // Q^T: columns are rows 8 nt + g; the statistics of a column are kept by the
     // lanes whose accumulators belong to it, columns 8 nt + 2 t and one further
-    uint32_t qb[NT][kSteps][2], qc[NT][2];
+    uint32_t qb[NT][kSteps][2];
     int sees[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float sum = 0.f;
 #pragma unroll
       for (int w = 0; w < kKWords; ++w) {
         const uint4 x = raw[nt][w];
@@ -770,20 +737,6 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
         qb[nt][2 * w][1] = x.y;
         qb[nt][2 * w + 1][0] = x.z;
         qb[nt][2 * w + 1][1] = x.w;
-        if constexpr (kCentred) {
-          float f[8];
-          unpack16<T>(x, f);
-          sum += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
-        }
-      }
-      if constexpr (kCentred) {  // the group's sum in three numbers; where two lanes share it, the even one's
-        if (D == 64) sum += __shfl_xor_sync(kFull, sum, 1);
-        if (D == 64 && (t & 1)) sum = 0.f;
-        sum = -sum;  // (of the negative remainders)
-        const float high = Elem<T>::to_f(Elem<T>::from_f(sum));
-        const float mid = Elem<T>::to_f(Elem<T>::from_f(sum - high));
-        qc[nt][0] = pack2<T>(high, mid);
-        qc[nt][1] = pack2<T>(sum - high - mid, 0.f);
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -822,23 +775,18 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
       float sc[NT][4];
       {
         const uint32_t both = g & 1 ? 0x3232u : 0x1010u;
-        const Maker<T> p0(prmt(ks.x, 0u, both), magic), p1(prmt(ks.y, 0u, both), magic);
+        const Pars<T> p0 = pars<T>(prmt(ks.x, 0u, both), magic), p1 = pars<T>(prmt(ks.y, 0u, both), magic);
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) {
           const int sh = 8 * (k & 1);
           const uint32_t w0 = kw[0][k / 2], w1 = kw[1][k / 2];
-          const uint32_t a[4] = {p0(w0 >> sh), p1(w1 >> sh), p0(w0 >> (sh + 4)), p1(w1 >> (sh + 4))};
+          const uint32_t a[4] = {value2<T>(w0 >> sh, p0, magic), value2<T>(w1 >> sh, p1, magic),
+                                 value2<T>(w0 >> (sh + 4), p0, magic), value2<T>(w1 >> (sh + 4), p1, magic)};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             if (k == 0) mma16816_first<T>(sc[nt], a, qb[nt][k][0], qb[nt][k][1]);
             else mma16816<T>(sc[nt], a, qb[nt][k][0], qb[nt][k][1]);
           }
-        }
-        if constexpr (kCentred) {
-          const uint32_t r0 = p0.minus_rest(), r1 = p1.minus_rest();
-          const uint32_t a[4] = {r0, r1, r0, r1};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816<T>(sc[nt], a, qc[nt][0], qc[nt][1]);
         }
       }
 #pragma unroll
@@ -851,10 +799,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
           vw[h][0] = *reinterpret_cast<const uint32_t *>(at);
         }
       }
-      uint2 vs = *reinterpret_cast<const uint2 *>(b + vs_at), vc = make_uint2(0, 0);
-      if constexpr (kCentred) {
-        if (g < D / kGroup) vc = *reinterpret_cast<const uint2 *>(b + vc_at);
-      }
+      uint2 vs = *reinterpret_cast<const uint2 *>(b + vs_at);
       if constexpr (kMasked) {
         // A weight of 0 does not silence a NaN.  Past the last key a token's scales
         // are dropped; before it, where rows differ, those that are NaN are, and
@@ -865,7 +810,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
         };
 #pragma unroll
         for (int h = 0; h < 4; ++h)
-          if (key + t + 4 * h >= kv) drop(vs, h), drop(vc, h);
+          if (key + t + 4 * h >= kv) drop(vs, h);
         if (__any_sync(kFull, odd(vs, 0) || odd(vs, 1) || odd(vs, 2) || odd(vs, 3))) {
           // rare: token by token, its scale being with lane 4 g + its number % 4
 #pragma unroll 1
@@ -881,10 +826,8 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
                   if (is && key + k < sees[nt][e & 1]) o[nt][d][e] = NAN;
           }
 #pragma unroll
-          for (int h = 0; h < 4; ++h) {
+          for (int h = 0; h < 4; ++h)
             if (odd(vs, h)) drop(vs, h);
-            if (odd(vc, h)) drop(vc, h);
-          }
         }
       }
       uint32_t pt[NT][2];
@@ -931,21 +874,22 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
         pt[nt][0] = transpose8x8(pack_weights<T>(x[0], x[1]));
         pt[nt][1] = transpose8x8(pack_weights<T>(x[2], x[3]));
       }
-      const Maker<T> p0(vs.x, magic), p1(vs.y, magic);
+      const Pars<T> p0 = pars<T>(vs.x, magic), p1 = pars<T>(vs.y, magic);
 #pragma unroll
       for (int x = 0; x < kVWords; ++x) {
         const uint32_t lo0 = prmt(vw[0][x], vw[1][x], 0x5410u), hi0 = prmt(vw[0][x], vw[1][x], 0x7632u);
         const uint32_t lo1 = prmt(vw[2][x], vw[3][x], 0x5410u), hi1 = prmt(vw[2][x], vw[3][x], 0x7632u);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const uint32_t a[4] = {p0(lo0 >> 4 * k), p0(hi0 >> 4 * k), p1(lo1 >> 4 * k), p1(hi1 >> 4 * k)};
+          const uint32_t a[4] = {value2<T>(lo0 >> 4 * k, p0, magic), value2<T>(hi0 >> 4 * k, p0, magic),
+                                 value2<T>(lo1 >> 4 * k, p1, magic), value2<T>(hi1 >> 4 * k, p1, magic)};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[nt][4 * x + k], a, pt[nt][0], pt[nt][1]);
         }
       }
-      constexpr uint32_t kOnes = kCentred ? 0x3f803f80u : 0x3c003c00u;
-      const uint32_t a[4] = {g == kSumRow ? kOnes : Maker<T>(vc.x, magic).minus_rest(), 0u,
-                             g == kSumRow ? kOnes : Maker<T>(vc.y, magic).minus_rest(), 0u};
+      // the weights' sum: values of 1 in the rows of channel 0
+      const uint32_t ones = g == 0 ? kOnes<T> : 0u;
+      const uint32_t a[4] = {ones, 0u, ones, 0u};
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) mma16816<T>(oc[nt], a, pt[nt][0], pt[nt][1]);
     };
@@ -988,16 +932,14 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = nt * 8 + t * 2 + e;
-        if (g == kSumRow) {
+        if (g == 0) {
           s_m[warp][r] = kLift<T> - up[nt][e];
           s_l[warp][r] = oc[nt][e];
         }
-        // (the lane's channels are in group g * (D / 8) / 32, whose rest is the row of that number)
-        const float rest = kCentred ? __shfl_sync(kFull, oc[nt][e], g * (D / 8) / kGroup * 4 + t) : 0.f;
 #pragma unroll
         for (int d = 0; d < kSteps; ++d)
           *reinterpret_cast<float2 *>(mine + r * F::kPitch + g * (D / 8) + 2 * d) =
-              make_float2(o[nt][d][e] - rest, o[nt][d][2 + e] - rest);
+              make_float2(o[nt][d][e], o[nt][d][2 + e]);
       }
     __syncthreads();
     constexpr int kLanes = D / 4;  // lanes of a row, four columns each
