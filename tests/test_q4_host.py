@@ -125,3 +125,20 @@ def test_numbers_next_to_the_types_largest_stay_finite():
     y = torch.full((1, 64), torch.finfo(torch.bfloat16).max, dtype=torch.bfloat16)
     y[0, 3] = -y[0, 3]
     assert bool(Q.values(y, torch.bfloat16).to(torch.bfloat16).isfinite().all())
+
+
+def test_the_paged_cache_and_generate_refuse_what_4_bits_cannot():
+    from tests.test_mask_refusals_host import Reached, generate
+    from tide_b200.paged import PagedKVCache
+
+    cpu = torch.device("cpu")
+    for bits, d, dtype in ((8, 128, torch.bfloat16), (4, 96, torch.bfloat16), (4, 128, torch.float32)):
+        with pytest.raises(ValueError):
+            PagedKVCache(1, 2, 4, 16, 2, d, 64, dtype, cpu, bits=bits)
+    c = PagedKVCache(2, 2, 4, 32, 2, 128, 64, torch.bfloat16, cpu, bits=4)
+    assert c.k == [] and [tuple(x.shape) for x in c.kv] == [(4, 2, 2, 2304)] * 2
+    for kw in (dict(kv_bits=8, live=True, paged=True), dict(kv_bits=4), dict(kv_bits=4, live=True)):
+        with pytest.raises(ValueError, match="kv_bits"):
+            generate(**kw)
+    with pytest.raises(Reached):
+        generate(kv_bits=4, live=True, paged=True)

@@ -19,18 +19,29 @@ from tide_b200.live import LiveDecoder, _StepBuffers
 
 class PagedKVCache:
     """Keys and values [n_pages, kv_heads, page_size, head_dim] per layer, and
-    the requests' block tables and lengths, on the device."""
+    the requests' block tables and lengths, on the device.  With bits=4 they
+    are `kv` [n_pages, kv_heads, page_size / 16, 18 head_dim] bytes per layer
+    instead, 4.5 bits a value (the format is in include/tide_b200.h), for rows
+    of `dtype`."""
 
     def __init__(self, n_layers: int, n_requests: int, n_pages: int, page_size: int, kv_heads: int,
                  head_dim: int, max_len: int, dtype: torch.dtype, device: torch.device,
-                 error_word: Optional[torch.Tensor] = None):
+                 error_word: Optional[torch.Tensor] = None, bits: int = 16):
         if page_size < 16 or page_size & (page_size - 1):
             raise ValueError("page_size must be a power of two of at least 16")
         if not 1 <= n_requests <= 8192:
             raise ValueError("1 to 8192 requests")
+        if bits not in (4, 16):
+            raise ValueError("bits must be 16 or 4")
+        if bits == 4 and (head_dim not in (64, 128) or dtype not in (torch.bfloat16, torch.float16)):
+            raise ValueError("a cache in 4 bits takes bf16 or fp16 rows with a head dimension of 64 or 128")
         shape = (n_pages, kv_heads, page_size, head_dim)
-        self.k = [torch.empty(shape, dtype=dtype, device=device) for _ in range(n_layers)]
-        self.v = [torch.empty(shape, dtype=dtype, device=device) for _ in range(n_layers)]
+        n16, n4 = (0, n_layers) if bits == 4 else (n_layers, 0)
+        self.k = [torch.empty(shape, dtype=dtype, device=device) for _ in range(n16)]
+        self.v = [torch.empty(shape, dtype=dtype, device=device) for _ in range(n16)]
+        self.kv = [torch.empty((n_pages, kv_heads, page_size // 16, 18 * head_dim), dtype=torch.uint8,
+                               device=device) for _ in range(n4)]
+        self.bits, self.dtype, self.kv_heads, self.head_dim = bits, dtype, kv_heads, head_dim
         self.page_size, self.max_len, self.n_requests = page_size, max_len, n_requests
 
         def i32(*size, value=0):
@@ -62,8 +73,45 @@ class PagedKVCache:
         (None: zeros to every slot)."""
         from tide_b200 import _native
 
-        _native.ops().paged_append(k, v, slot_map, row_ids, n_rows, self.k[layer], self.v[layer],
-                                   self.error_word)
+        if self.bits == 4:
+            _native.ops().paged_append_q4(None, k, v, slot_map, row_ids, n_rows, None, None, 1.0, None,
+                                          None, 0.0, None, self.kv[layer], self.error_word)
+        else:
+            _native.ops().paged_append(k, v, slot_map, row_ids, n_rows, self.k[layer], self.v[layer],
+                                       self.error_word)
+
+    def append_rotated(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                       slot_map: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
+                       scaling: float = 1.0, q_weight: Optional[torch.Tensor] = None,
+                       k_weight: Optional[torch.Tensor] = None, eps: float = 0.0,
+                       row_ids: Optional[torch.Tensor] = None,
+                       n_rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """append (bits=4) with the heads' RMSNorms (weights, or None) and the
+        rotary embedding at positions[row_ids[i]] on the way; returns q [n,
+        heads, head_dim] with the same done to it."""
+        from tide_b200 import _native
+
+        if self.bits != 4:
+            raise NotImplementedError("append_rotated is for a cache in 4 bits")
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        _native.ops().paged_append_q4(q, k, v, slot_map, row_ids, n_rows, positions, inv_freq, scaling,
+                                      q_weight, k_weight, eps, out, self.kv[layer], self.error_word)
+        return out
+
+    def read(self, layer: int, slots: torch.Tensor):
+        """The keys and values at `slots` (int64): two tensors [n, kv_heads,
+        head_dim]; zeros for a slot of -1."""
+        from tide_b200 import _native
+
+        n = slots.numel()
+        k = torch.zeros(n, self.kv_heads, self.head_dim, dtype=self.dtype, device=slots.device)
+        v = torch.zeros_like(k)
+        if self.bits == 4:
+            _native.ops().paged_read_q4(self.kv[layer], slots, k, v, self.error_word)
+            return k, v
+        real = (slots >= 0)[:, None, None]
+        page, at = slots.clamp(min=0) // self.page_size, slots.clamp(min=0) % self.page_size
+        return tuple(torch.where(real, c[layer][page, :, at], z) for c, z in ((self.k, k), (self.v, v)))
 
     def attend(self, layer: int, q: torch.Tensor, scale: float, *, chunk: bool,
                seq_ids: Optional[torch.Tensor] = None,
@@ -73,9 +121,13 @@ class PagedKVCache:
         from tide_b200 import _native
 
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        _native.ops().paged_attention(q, self.k[layer], self.v[layer], self.block_tables,
-                                      self.kv_lens, self.cu_seqlens if chunk else None, seq_ids, out,
-                                      self.max_len, scale, self.error_word, n_seqs)
+        cu = self.cu_seqlens if chunk else None
+        if self.bits == 4:
+            _native.ops().paged_attention_q4(q, self.kv[layer], self.block_tables, self.kv_lens, cu, seq_ids,
+                                             out, self.max_len, scale, self.error_word, n_seqs)
+        else:
+            _native.ops().paged_attention(q, self.k[layer], self.v[layer], self.block_tables, self.kv_lens,
+                                          cu, seq_ids, out, self.max_len, scale, self.error_word, n_seqs)
         return out
 
 
@@ -87,17 +139,23 @@ class PagedLiveDecoder(LiveDecoder):
     requests, whatever their lengths.  A row that exits leaves zeros at its
     position in the later layers (the reference's "zero_pad",
     python/TIDE/runtime.py:194-221).  The host keeps the lengths too and
-    refuses a step that the pool has no pages for."""
+    refuses a step that the pool has no pages for.  kv_bits=4 keeps keys and
+    values in 4.5 bits each (3.6 times the tokens in the same memory): they are
+    rounded to sixteen levels a group of 32 channels, so logits differ by that;
+    the norms and the rotary embedding before it are then rounded once, not
+    where the model's modules round."""
 
     def __init__(self, runtime, n_requests: int, max_len: int, n_pages: Optional[int] = None,
-                 page_size: int = 64, graph: bool = False, fused_layers: bool = True):
+                 page_size: int = 64, graph: bool = False, fused_layers: bool = True, kv_bits: int = 16):
         super().__init__(runtime, 1, 1, graph=graph, fused_layers=fused_layers)
         fam = self.fam
         if n_pages is None:
             n_pages = n_requests * -(-max_len // page_size)
         self.cache = PagedKVCache(len(fam.layers), n_requests, n_pages, page_size, fam.kv_heads(),
-                                  fam.head_dim(), max_len, self.dtype, self.dev, self.err)
-        self.k, self.v = self.cache.k, self.cache.v
+                                  fam.head_dim(), max_len, self.dtype, self.dev, self.err, kv_bits)
+        self.k, self.v = self.cache.k, self.cache.v  # (empty lists with kv_bits=4)
+        # norm and rotary embedding on the way into the cache
+        self._rotates = kv_bits == 4 and self.fused
         self.n_slots, self.max_len, self.n_pages = n_requests, max_len, n_pages
         self.lengths: List[int] = [0] * n_requests  # the device's kv_lens, as the host knows them
         self._requests: List[int] = []
@@ -118,6 +176,11 @@ class PagedLiveDecoder(LiveDecoder):
         self.lengths = lens
         for c in self.k + self.v:
             c.copy_(torch.randn(c.shape, generator=generator, device=c.device))
+        for i in range(len(self.cache.kv)):
+            for at in slot_map[:n].split(1 << 16):
+                shape = (2, at.numel(), self.cache.kv_heads, self.cache.head_dim)
+                k, v = torch.randn(shape, generator=generator, device=self.dev).to(self.dtype)
+                self.cache.append(i, k, v, at)
 
     def _i32(self, values) -> torch.Tensor:
         return torch.tensor(values, dtype=torch.int32, device=self.dev)
@@ -132,34 +195,57 @@ class PagedLiveDecoder(LiveDecoder):
         return lens
 
     # ---- one layer on rows whose slots and positions are known
+    def _projected(self, i: int, h: torch.Tensor, n_live: Optional[torch.Tensor]):
+        """q, k and v of rows h before norm and rotary embedding (column slices
+        of one GEMM's output), and the norms' weights and eps."""
+        fam, layer = self.fam, self.fam.layers[i]
+        attn = layer.self_attn
+        n = h.shape[0]
+        x, _ = fam.rms_norm(layer.input_layernorm, h, n_live)
+        w, b = fam._qkv_weight(i, attn)
+        qkv = torch.nn.functional.linear(x, w, b)
+        dq, dk = attn.q_proj.out_features, attn.k_proj.out_features
+        qn, kn = getattr(attn, "q_norm", None), getattr(attn, "k_norm", None)
+        return (qkv[:, :dq].view(n, -1, 128), qkv[:, dq:dq + dk].view(n, -1, 128),
+                qkv[:, dq + dk:].view(n, -1, 128), qn.weight if qn is not None else None,
+                kn.weight if kn is not None else None,
+                float(qn.variance_epsilon) if qn is not None else 0.0)
+
+    def _append(self, i: int, h: torch.Tensor, positions: torch.Tensor, places: torch.Tensor,
+                slot_map: torch.Tensor, slot_positions: torch.Tensor,
+                row_ids: Optional[torch.Tensor] = None,
+                n_live: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Keys and values of rows h to their slots; returns the rotated q.  The
+        rows' positions are `positions`, those of slot_map slot_positions."""
+        if self._rotates:
+            q, k, v, qw, kw, eps = self._projected(i, h, n_live)
+            fam = self.fam
+            return self.cache.append_rotated(i, q, k, v, slot_map, slot_positions, fam._inv_freq(),
+                                             float(getattr(fam.rotary, "attention_scaling", 1.0)), qw, kw,
+                                             eps, row_ids, n_live)
+        q, k, v = self._qkv(i, h, positions, places, n_live)
+        self.cache.append(i, k, v, slot_map, row_ids, n_live)
+        return q
+
     def _qkv(self, i: int, h: torch.Tensor, positions: torch.Tensor, places: torch.Tensor,
              n_live: Optional[torch.Tensor]):
         """Rotated q, rotated k, and v of rows h at the given positions
         (places: 0, 1, 2, ... in int32)."""
         from tide_b200 import _native
 
-        fam, layer = self.fam, self.fam.layers[i]
-        attn = layer.self_attn
+        fam = self.fam
         n = h.shape[0]
         if not self.fused:
-            q, k, v = fam._qkv(layer, h, positions)
+            q, k, v = fam._qkv(fam.layers[i], h, positions)
             return (q.to(self.dtype).contiguous(), k.to(self.dtype).contiguous(),
                     v.to(self.dtype).contiguous())
-        x, _ = fam.rms_norm(layer.input_layernorm, h, n_live)
-        w, b = fam._qkv_weight(i, attn)
-        qkv = torch.nn.functional.linear(x, w, b)
-        dq, dk = attn.q_proj.out_features, attn.k_proj.out_features
-        q = qkv[:, :dq].view(n, -1, 128)
-        k = qkv[:, dq:dq + dk].view(n, -1, 128)
-        v = qkv[:, dq + dk:].view(n, -1, 128)
-        qn, kn = getattr(attn, "q_norm", None), getattr(attn, "k_norm", None)
+        q, k, v, qw, kw, eps = self._projected(i, h, n_live)
         q_rot = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         # (each row its own place in a cache of one position a row)
         k_new = torch.empty(n, k.shape[1], 1, 128, dtype=k.dtype, device=k.device)
         v_new = torch.empty_like(k_new)
         _native.ops().qk_norm_rope(
-            q, k, v, qn.weight if qn is not None else None, kn.weight if kn is not None else None,
-            float(qn.variance_epsilon) if qn is not None else 0.0, fam._inv_freq(),
+            q, k, v, qw, kw, eps, fam._inv_freq(),
             float(getattr(fam.rotary, "attention_scaling", 1.0)), 0, None, positions, places, n_live,
             q_rot, k_new, v_new, None)
         return q_rot, k_new.view(n, -1, 128), v_new.view(n, -1, 128)
@@ -210,8 +296,7 @@ class PagedLiveDecoder(LiveDecoder):
         places = torch.arange(n, dtype=torch.int32, device=self.dev)
         h = self.fam.embed_tokens(tokens)
         for i in range(len(self.fam.layers)):
-            q, k, v = self._qkv(i, h, positions, places, None)
-            self.cache.append(i, k, v, slot_map)
+            q = self._append(i, h, positions, places, slot_map, positions)
             o = self.cache.attend(i, q, float(self.fam.layers[i].self_attn.scaling), chunk=True)
             h = self._rest(i, h, o, None)
         got = [r for r in range(self.n_slots) if new[r]]
@@ -282,11 +367,11 @@ class PagedLiveDecoder(LiveDecoder):
                slots: torch.Tensor, n_live: torch.Tensor) -> torch.Tensor:
         if rows is not b.live_rows:  # compacted since the last layer; past the live ones: anything
             b.live_rows, b.row_ids = rows, rows.to(torch.int32)
-            b.live_positions = b.positions.index_select(0, rows.clamp(0, b.B - 1))
-        q, k, v = self._qkv(i, h, b.live_positions, b.places, n_live)
+            if not self._rotates:
+                b.live_positions = b.positions.index_select(0, rows.clamp(0, b.B - 1))
         if rows is not b.rows0:  # some may have exited: zeros in their place
             self.cache.append(i, None, None, b.slot_map)
-        self.cache.append(i, k, v, b.slot_map, b.row_ids, n_live)
+        q = self._append(i, h, b.live_positions, b.places, b.slot_map, b.positions, b.row_ids, n_live)
         o = self.cache.attend(i, q, float(self.fam.layers[i].self_attn.scaling), chunk=False,
                               seq_ids=slots, n_seqs=n_live)
         return self._rest(i, h, o, n_live)

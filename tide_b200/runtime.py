@@ -323,10 +323,16 @@ class TIDERuntime(nn.Module):
         each row from the tokens that `attention_mask` (zeros: padding, left
         or right) leaves of it.  live=True without paged=True refuses a mask
         with zeros; the reference's loop, which takes no mask, warns that the
-        padding counts as tokens there."""
+        padding counts as tokens there.  kv_bits=4 (with live=True and
+        paged=True) keeps that cache in 4.5 bits a value."""
         paged, mask = kwargs.get("paged", False), kwargs.get("attention_mask")
+        kv_bits = kwargs.get("kv_bits", 16)
         if paged and not live:
             raise ValueError("generate(paged=True) is a form of live decoding: pass live=True")
+        if kv_bits not in (4, 16):
+            raise ValueError("generate: kv_bits must be 16 or 4")
+        if kv_bits == 4 and not paged:
+            raise ValueError("generate(kv_bits=4) is for the paged cache: pass live=True and paged=True")
         if mask is not None and not (live and paged) and not bool(mask.bool().all()):
             if live:
                 raise ValueError("generate(live=True) takes an attention_mask with zeros on the paged "
@@ -345,7 +351,7 @@ class TIDERuntime(nn.Module):
 
             room, graph = input_ids.shape[1] + max_new_tokens + 1, kwargs.get("live_graph", True)
             if paged:
-                dec = PagedLiveDecoder(self, B, room, graph=graph)
+                dec = PagedLiveDecoder(self, B, room, graph=graph, kv_bits=kv_bits)
                 next_logits = dec.prefill(input_ids, mask)
             else:
                 dec = LiveDecoder(self, B, room, graph=graph)
