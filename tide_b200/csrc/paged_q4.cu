@@ -12,6 +12,12 @@
 namespace tide {
 namespace q4 {
 
+// a / b, both positive: by 32-bit numbers, where they are (the other is a hundred
+// instructions).
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  return ((a | b) >> 31) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
 // ------------------------------------------------------------------ append
 // y = norm(x) turned by the angle position * inv_freq: of q, rounded to its
 // type once, and of k, which is rounded to 32 bits once and goes to the cache
@@ -51,68 +57,93 @@ struct AppendParams {
 // last bits.
 constexpr float kRounder = 12582912.f;  // 3 * 2^22
 
+// Two neighbouring channels in the halves of a register pair, whose sums and
+// products are one instruction.
+using Two = uint64_t;
+
+template <typename T>
+__device__ __forceinline__ void unpack_twos(const uint4 &v, Two (&x)[4]) {
+  float f[8];
+  unpack16<T>(v, f);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = ragged::pair(f[2 * e], f[2 * e + 1]);
+}
+
 // Least and largest value of the group of which this lane, of four neighbours, has
 // eight, 0 among them; whether one of them is not finite.
-__device__ __forceinline__ bool extent(const float (&x)[8], float *lo, float *hi) {
+__device__ __forceinline__ bool extent(const Two (&x)[4], float *lo, float *hi) {
+  using namespace ragged;
   constexpr unsigned kFull = 0xffffffffu;
-  float a = x[0], b = x[0], all = x[0] * 0.f;
+  float v[8];
+  Two odd = 0;  // NaN where one is not finite
 #pragma unroll
-  for (int e = 1; e < 8; ++e) {
-    a = fminf(a, x[e]);
-    b = fmaxf(b, x[e]);
-    all = fmaf(x[e], 0.f, all);  // NaN where one is not finite
+  for (int e = 0; e < 4; ++e) {
+    unpair(x[e], &v[2 * e], &v[2 * e + 1]);
+    odd = fma2(x[e], 0, odd);
   }
-  const unsigned who = __ballot_sync(kFull, all != 0.f);
+  float a = min3(min3(v[0], v[1], v[2]), min3(v[3], v[4], v[5]), min3(v[6], v[7], 0.f));
+  float b = max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), max3(v[6], v[7], 0.f));
+  float odd0, odd1;
+  unpair(odd, &odd0, &odd1);
+  const unsigned who = __ballot_sync(kFull, odd0 + odd1 != 0.f);
 #pragma unroll
   for (int w = 1; w < 4; w *= 2) {
     a = fminf(a, __shfl_xor_sync(kFull, a, w));
     b = fmaxf(b, __shfl_xor_sync(kFull, b, w));
   }
-  *lo = fminf(a, 0.f);
-  *hi = fmaxf(b, 0.f);
+  *lo = a;
+  *hi = b;
   return who >> (threadIdx.x & 28) & 0xfu;
 }
 
 // The group's word of codes of this lane, and its scale and zero point.
 template <typename T>
-__device__ __forceinline__ uint32_t quantise(const float (&x)[8], uint32_t *par) {
+__device__ __forceinline__ uint32_t quantise(const Two (&x)[4], uint32_t *par) {
+  using namespace ragged;
   constexpr bool kHalf = std::is_same<T, __half>::value;
   constexpr float kMost = kHalf ? 65504.f : 3.3895313892515355e38f;
   constexpr float kLeast = kHalf ? 0x1p-21f : 0x1p-120f;
   float lo, hi;
   const bool odd = extent(x, &lo, &hi);
+  // v / by, rounded once, with inv = 1 / by rounded once: the product may be a bit
+  // off, its remainder is exact and corrects it (Markstein).  Ties are common
+  // (values of eight bits over scales of four), so that bit counts.
+  auto over = [](float v, float by, float inv) {
+    const float q = v * inv;
+    return fmaf(fmaf(-q, by, v), inv, q);
+  };
   // (half of each: their difference stays within 32 bits)
-  const float t = __fdiv_rn(0.5f * hi - 0.5f * lo, 7.5f);
+  const float t = over(0.5f * hi - 0.5f * lo, 7.5f, 1.f / 7.5f);
   if (odd || t == 0.f) {
     *par = odd ? 0x7fc0u : 0u;
     return 0u;
   }
   const float s = fmaxf(__uint_as_float((__float_as_uint(t) + 0xfffffu) & 0xfff00000u), kLeast);
   const float inv = __frcp_rn(s);
-  // v / s, rounded once: the product may be a bit off, its remainder is exact and
-  // corrects it (Markstein).  Ties are common (values of eight bits over scales of
-  // four), so that bit counts.
-  auto over = [&](float v) {
-    const float q = v * inv;
-    return fmaf(fmaf(-q, s, v), inv, q);
-  };
-  const float z = (over(-lo) + kRounder) - kRounder;
+  const float z = (over(-lo, s, inv) + kRounder) - kRounder;
   *par = __float_as_uint(s) >> 16 | (uint32_t)z;
-  // bits[e] = kRounder's + code - z; below 0 a code cannot be (the least value's is
-  // z - z), above 15 it can
-  uint32_t bits[8];
+  // f[e] = kRounder + code - z; below 0 a code cannot be (the least value's is z -
+  // z), above 15 it can
+  const Two by2 = pair(-s, -s), inv2 = pair(inv, inv), rounder2 = pair(kRounder, kRounder);
+  const float most = kRounder + (15.f - z);
+  float f[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) bits[e] = __float_as_uint(fminf(over(x[e]) + kRounder, kRounder + (15.f - z)));
+  for (int e = 0; e < 4; ++e) {
+    const Two q = mul2(x[e], inv2);
+    unpair(add2(fma2(fma2(q, by2, x[e]), inv2, q), rounder2), &f[2 * e], &f[2 * e + 1]);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = fminf(f[e], most);
   if (s > kMost / 16.f) {  // next to the type's largest number: none above it
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float n = __uint_as_float(bits[e]) - kRounder;
-      if (fabsf(n * s) > kMost) bits[e] = __float_as_uint(n - copysignf(1.f, n) + kRounder);
+      const float n = f[e] - kRounder;
+      if (fabsf(n * s) > kMost) f[e] = n - copysignf(1.f, n) + kRounder;
     }
   }
   uint32_t word = ((uint32_t)z - 0x4b400000u) * 0x11111111u;  // (modulo 2^32)
 #pragma unroll
-  for (int e = 0; e < 8; ++e) word += bits[e] * (1u << (4 * (e / 2) + 16 * (e % 2)));
+  for (int e = 0; e < 8; ++e) word += __float_as_uint(f[e]) * (1u << (4 * (e / 2) + 16 * (e % 2)));
   return word;
 }
 
@@ -128,9 +159,10 @@ __global__ void __launch_bounds__(32 * ROWS * WARPS, 24 / (ROWS * WARPS))
   constexpr int kLanes = D / 16;              // of a head
   constexpr int kHeads = 32 / kLanes;         // of a warp
   constexpr int kStep = WARPS * kHeads;       // from a warp's heads to its next
-  // cosine and sine of channel 8 j + e at [e][j]
+  // cosine and sine of channel 8 j + e at [e][j]; of 8 j + 2 e and the next, the two
+  // cosines and the two sines, in 32 bits at [e][j]
   __shared__ double2 turn[ROWS][8][kLanes];
-  __shared__ float2 turn32[ROWS][8][kLanes];
+  __shared__ float2 cosines[ROWS][4][kLanes], sines[ROWS][4][kLanes];
   __shared__ int64_t s_block[ROWS];  // the slot's block in head 0; -1: nothing to write
   __shared__ int s_token[ROWS];      // and its token there; -1: no such row
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -174,7 +206,7 @@ __global__ void __launch_bounds__(32 * ROWS * WARPS, 24 / (ROWS * WARPS))
     const bool known = m >= 0 && m < p.n_map;
     if (f == 0) {
       const int64_t slot = known ? __ldg(p.slot_map + m) : -1;
-      const int64_t pg = slot / p.page;
+      const int64_t pg = slot < 0 ? 0 : quotient(slot, p.page);
       const bool real = slot >= 0 && pg < p.n_pages;
       if (!known || (!real && slot != -1)) raise_error(p.err, TIDE_DEVERR_POSITION);
       const int tok = (int)(slot - pg * p.page);
@@ -189,7 +221,8 @@ __global__ void __launch_bounds__(32 * ROWS * WARPS, 24 / (ROWS * WARPS))
       c *= (double)p.att_scale;
       s *= (double)p.att_scale;
       turn[at][f % 8][f / 8] = make_double2(c, s);
-      turn32[at][f % 8][f / 8] = make_float2((float)c, (float)s);
+      (f % 2 ? cosines[at][f % 8 / 2][f / 8].y : cosines[at][f % 8 / 2][f / 8].x) = (float)c;
+      (f % 2 ? sines[at][f % 8 / 2][f / 8].y : sines[at][f % 8 / 2][f / 8].x) = (float)s;
     }
   }
   __syncthreads();
@@ -198,7 +231,7 @@ __global__ void __launch_bounds__(32 * ROWS * WARPS, 24 / (ROWS * WARPS))
   // where the row's token has its codes and scales in head 0
   unsigned char *const to = p.cache + s_block[r] * L::kBytes;
   const bool place = s_block[r] >= 0;
-  auto store = [&](int side, int h, const float (&x)[2][8]) {
+  auto store = [&](int side, int h, const Two (&x)[2][4]) {
     uint32_t par[2];
     const uint32_t word[2] = {quantise<T>(x[0], &par[0]), quantise<T>(x[1], &par[1])};
     if (!place || h >= p.hkv) return;
@@ -212,17 +245,17 @@ __global__ void __launch_bounds__(32 * ROWS * WARPS, 24 / (ROWS * WARPS))
   };
 #pragma unroll 1
   for (int h = first_v; h < p.hkv; h += kStep) {
-    float x[2][8];
-    unpack16<T>(next_v.a, x[0]);
-    unpack16<T>(next_v.b, x[1]);
+    Two x[2][4];
+    unpack_twos<T>(next_v.a, x[0]);
+    unpack_twos<T>(next_v.b, x[1]);
     next_v = load(p.v, p.kv_stride, h + in + kStep, p.hkv);
     store(1, h + in, x);
   }
 #pragma unroll 1
   for (int h = first_k; h < p.hkv; h += kStep) {
-    float x[2][8];
-    unpack16<T>(next_k.a, x[0]);
-    unpack16<T>(next_k.b, x[1]);
+    float f[2][8];
+    unpack16<T>(next_k.a, f[0]);
+    unpack16<T>(next_k.b, f[1]);
     next_k = load(p.k, p.kv_stride, h + in + kStep, p.hkv);
     double rstd = 1.0;
     const T *w = static_cast<const T *>(p.k_w) + 8 * j;
@@ -230,7 +263,7 @@ __global__ void __launch_bounds__(32 * ROWS * WARPS, 24 / (ROWS * WARPS))
       double ss = 0.0;
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        ss = fma((double)x[0][e], (double)x[0][e], fma((double)x[1][e], (double)x[1][e], ss));
+        ss = fma((double)f[0][e], (double)f[0][e], fma((double)f[1][e], (double)f[1][e], ss));
 #pragma unroll
       for (int i = 1; i < kLanes; i *= 2) ss += __shfl_xor_sync(kFull, ss, i);
       rstd = rsqrt(ss / (double)D + (double)p.eps);
@@ -238,7 +271,7 @@ __global__ void __launch_bounds__(32 * ROWS * WARPS, 24 / (ROWS * WARPS))
     if (p.k_w || p.inv_freq) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        double a = (double)x[0][e], b = (double)x[1][e];
+        double a = (double)f[0][e], b = (double)f[1][e];
         if (p.k_w) {
           a *= rstd * (double)Elem<T>::to_f(w[e]);
           b *= rstd * (double)Elem<T>::to_f(w[D / 2 + e]);
@@ -249,27 +282,41 @@ __global__ void __launch_bounds__(32 * ROWS * WARPS, 24 / (ROWS * WARPS))
           b = fma(b, cs.x, a * cs.y);
           a = y;
         }
-        x[0][e] = (float)a;
-        x[1][e] = (float)b;
+        f[0][e] = (float)a;
+        f[1][e] = (float)b;
       }
     }
+    Two x[2][4];
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[a][e] = pair(f[a][2 * e], f[a][2 * e + 1]);
     store(0, h + in, x);
   }
   if (first_q >= hq) return;
-  float2 cs[8];
+  Two c[4], sn[4], minus[4];  // cosines, sines, and their negatives
 #pragma unroll
-  for (int e = 0; e < 8; ++e) cs[e] = p.inv_freq ? turn32[r][e][j] : make_float2(1.f, 0.f);
+  for (int e = 0; e < 4; ++e) {
+    const float2 cc = p.inv_freq ? cosines[r][e][j] : make_float2(1.f, 1.f);
+    const float2 ss = p.inv_freq ? sines[r][e][j] : make_float2(0.f, 0.f);
+    c[e] = pair(cc.x, cc.y);
+    sn[e] = pair(ss.x, ss.y);
+    minus[e] = pair(-ss.x, -ss.y);
+  }
   T *const out = static_cast<T *>(p.q_out) + (row0 + r) * p.hq * D + 8 * j;
 #pragma unroll 1
   for (int h = first_q; h < hq; h += kStep) {
-    float x[2][8];
-    unpack16<T>(next_q.a, x[0]);
-    unpack16<T>(next_q.b, x[1]);
+    Two x[2][4];
+    unpack_twos<T>(next_q.a, x[0]);
+    unpack_twos<T>(next_q.b, x[1]);
     next_q = load(p.q, p.q_stride, h + in + kStep, hq);
     if (p.q_w) {
-      float ss = 0.f;
+      Two sum = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(x[0][e], x[0][e], fmaf(x[1][e], x[1][e], ss));
+      for (int e = 0; e < 4; ++e) sum = fma2(x[0][e], x[0][e], fma2(x[1][e], x[1][e], sum));
+      float ss, more;
+      unpair(sum, &ss, &more);
+      ss += more;
 #pragma unroll
       for (int i = 1; i < kLanes; i *= 2) ss += __shfl_xor_sync(kFull, ss, i);
       const float rstd = rsqrtf(ss / (float)D + p.eps);
@@ -277,23 +324,31 @@ __global__ void __launch_bounds__(32 * ROWS * WARPS, 24 / (ROWS * WARPS))
 #pragma unroll
       for (int a = 0; a < 2; ++a)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[a][e] *= rstd * Elem<T>::to_f(w[a * (D / 2) + e]);
+        for (int e = 0; e < 4; ++e)
+          x[a][e] = mul2(x[a][e], pair(rstd * Elem<T>::to_f(w[a * (D / 2) + 2 * e]),
+                                       rstd * Elem<T>::to_f(w[a * (D / 2) + 2 * e + 1])));
     }
     if (p.inv_freq) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float a = x[0][e], b = x[1][e];
-        x[0][e] = fmaf(a, cs[e].x, -b * cs[e].y);
-        x[1][e] = fmaf(b, cs[e].x, a * cs[e].y);
+      for (int e = 0; e < 4; ++e) {
+        const Two a = x[0][e], b = x[1][e];
+        x[0][e] = fma2(a, c[e], mul2(b, minus[e]));
+        x[1][e] = fma2(b, c[e], mul2(a, sn[e]));
       }
     }
     if (h + in < hq) {
       T *at = out + (h + in) * D;
 #pragma unroll
-      for (int a = 0; a < 2; ++a)
-        *reinterpret_cast<uint4 *>(at + a * (D / 2)) =
-            make_uint4(pack2<T>(x[a][0], x[a][1]), pack2<T>(x[a][2], x[a][3]), pack2<T>(x[a][4], x[a][5]),
-                       pack2<T>(x[a][6], x[a][7]));
+      for (int a = 0; a < 2; ++a) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float lo, hi;
+          unpair(x[a][e], &lo, &hi);
+          w[e] = pack2<T>(lo, hi);
+        }
+        *reinterpret_cast<uint4 *>(at + a * (D / 2)) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
     }
   }
 }
@@ -523,12 +578,6 @@ struct FewParams {
 // Row r / group of a sequence (exact for r < 2^17).
 __device__ __forceinline__ int token_of(int r, uint32_t per_group) {
   return (int)((uint64_t)(uint32_t)r * per_group >> 31);
-}
-
-// a / b, both positive: by 32-bit numbers, where they are (the other is a hundred
-// instructions).
-__device__ __forceinline__ long long quotient(long long a, long long b) {
-  return ((a | b) >> 31) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
 }
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
@@ -1124,7 +1173,10 @@ bool bad_cache(int64_t n_pages, int64_t page_size, int64_t hkv) {
 template <typename T, int D>
 int append(const tide::q4::AppendParams &p, cudaStream_t s) {
   using namespace tide::q4;
-  // Two warps a row where that fills the GPU; else eight, the more the sooner done.
+  // A warp a row where that fills the GPU more than once, two where they fill it;
+  // else eight, the more the sooner done.
+  if (p.n_rows >= 148 * 24 * 2)
+    return start("paged_append_q4", append_kernel<T, D, 4, 1>, (p.n_rows + 3) / 4, 128, 0, s, p);
   if (p.n_rows * 2 >= 148 * 16)
     return start("paged_append_q4", append_kernel<T, D, 2, 2>, (p.n_rows + 1) / 2, 128, 0, s, p);
   return start("paged_append_q4", append_kernel<T, D, 1, 8>, p.n_rows, 256, 0, s, p);
