@@ -827,10 +827,10 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
         const Pars<T> p0 = pars<T>(prmt(ks.x, 0u, both), magic), p1 = pars<T>(prmt(ks.y, 0u, both), magic);
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) {
-          const int sh = 8 * (k & 1);
+          const int at = 2 * (k & 1);
           const uint32_t w0 = kw[0][k / 2], w1 = kw[1][k / 2];
-          const uint32_t a[4] = {value2<T>(w0 >> sh, p0, magic), value2<T>(w1 >> sh, p1, magic),
-                                 value2<T>(w0 >> (sh + 4), p0, magic), value2<T>(w1 >> (sh + 4), p1, magic)};
+          const uint32_t a[4] = {value2_at<T>(w0, at, p0, magic), value2_at<T>(w1, at, p1, magic),
+                                 value2_at<T>(w0, at + 1, p0, magic), value2_at<T>(w1, at + 1, p1, magic)};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             if (k == 0) mma16816_first<T>(sc[nt], a, qb[nt][k][0], qb[nt][k][1]);
@@ -930,8 +930,8 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
         const uint32_t lo1 = prmt(vw[2][x], vw[3][x], 0x5410u), hi1 = prmt(vw[2][x], vw[3][x], 0x7632u);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const uint32_t a[4] = {value2<T>(lo0 >> 4 * k, p0, magic), value2<T>(hi0 >> 4 * k, p0, magic),
-                                 value2<T>(lo1 >> 4 * k, p1, magic), value2<T>(hi1 >> 4 * k, p1, magic)};
+          const uint32_t a[4] = {value2_at<T>(lo0, k, p0, magic), value2_at<T>(hi0, k, p0, magic),
+                                 value2_at<T>(lo1, k, p1, magic), value2_at<T>(hi1, k, p1, magic)};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[nt][4 * x + k], a, pt[nt][0], pt[nt][1]);
         }

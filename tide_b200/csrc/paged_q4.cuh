@@ -66,9 +66,10 @@ constexpr uint32_t kMagic = std::is_same<T, __half>::value ? 0x64006400u : 0x430
 
 // x's codes as such numbers: one instruction, if the number is not a constant to
 // the compiler (which would load it anew each time, or use two).
+template <uint32_t MASK = 0x000f000fu>
 __device__ __forceinline__ uint32_t numbers(uint32_t x, uint32_t magic) {
   uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(0x000f000fu), "r"(magic));
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(MASK), "r"(magic));
   return r;
 }
 
@@ -94,10 +95,24 @@ __device__ __forceinline__ uint32_t value2(uint32_t x, const Pars<T> &p, uint32_
   const Pair<T> c = as_pair<T>(numbers(x, magic));
   return as_bits(__hmul2(__hsub2(c, p.zero), p.scale));
 }
+// The same of nibbles `at` and at + 4 of a word, at < 4.  fp16 has bits enough to
+// take those with an odd number where they lie: 2^10 + 16 c.
+template <typename T>
+__device__ __forceinline__ uint32_t value2_at(uint32_t w, int at, const Pars<T> &p, uint32_t magic = kMagic<T>) {
+  if constexpr (std::is_same<T, __half>::value) {
+    if (at & 1) {
+      const Pair<T> c = as_pair<T>(numbers<0x00f000f0u>(w >> 4 * (at - 1), magic));
+      // (64 + c) - (64 + z), the latter being (1024 + z) - 960
+      const Pair<T> d = __hfma2(c, __float2half2_rn(0.0625f), __hsub2(__float2half2_rn(960.f), p.zero));
+      return as_bits(__hmul2(d, p.scale));
+    }
+  }
+  return value2<T>(w >> 4 * at, p, magic);
+}
 // The eight channels of a word.
 template <typename T>
 __device__ __forceinline__ uint4 value8(uint32_t w, const Pars<T> &p) {
-  return make_uint4(value2<T>(w, p), value2<T>(w >> 4, p), value2<T>(w >> 8, p), value2<T>(w >> 12, p));
+  return make_uint4(value2_at<T>(w, 0, p), value2_at<T>(w, 1, p), value2_at<T>(w, 2, p), value2_at<T>(w, 3, p));
 }
 
 }  // namespace q4
