@@ -476,3 +476,54 @@ def test_a_step_after_another(graph):
             expect(buf, [1] * B, [c + i for c in ctx0], q_rot, out)
     torch.cuda.current_stream().wait_stream(side)
     assert int(err) == 0
+
+
+def test_attention_of_single_tokens_beside_a_prompt():
+    """A batch whose calls need both kernels: many single tokens and one long chunk."""
+    hq, hkv, d, dtype = 8, 2, 128, BF
+    new = [1] * 40 + [300] + [2] * 20 + [0, 33]
+    q, cache, held, tables, lens, ids = q4_case(new, [13 * i % 700 for i in range(len(new))], hq, hkv, d, dtype, 16, 4)
+    for most in (max(lens), 5000):
+        wide = torch.cat([tables, torch.full((len(new), 5000 // 16), -1, dtype=torch.int32, device=DEV)], 1).contiguous()
+        err = i32([0])
+        out = attend(q, cache, wide, lens, new, ids, most, err=err)
+        assert int(err) == 0
+        check(out, q, held, tables, lens, new, ids)
+
+
+def test_attention_of_very_many_sequences():
+    hq, hkv, d, dtype, B = 4, 1, 64, HF, 1500
+    new = [i % 3 for i in range(B)]
+    q, cache, held, tables, lens, ids = q4_case(new, [7 * i % 90 for i in range(B)], hq, hkv, d, dtype, 16, 2)
+    for most in (max(lens), 600):
+        wide = torch.cat([tables, torch.full((B, 600 // 16), -1, dtype=torch.int32, device=DEV)], 1).contiguous()
+        check(attend(q, cache, wide, lens, new, ids, most), q, held, tables, lens, new, ids)
+    single = [r for n, r in zip(new, ids) if n]
+    x = torch.randn(len(single), hq, d, device=DEV).to(dtype)
+    check(attend(x, cache, tables, lens, [1] * len(single), single, single=True), x, held, tables, lens,
+          [1] * len(single), single)
+
+
+def test_a_cache_past_4_gigabytes():
+    """Pages whose bytes lie past 2^32: what a small cache gives."""
+    hq, hkv, d, dtype, page = 8, 8, 128, BF, 64
+    pages = 60000  # of 73728 bytes
+    big = torch.empty(pages, hkv, page // 16, 18 * d, dtype=torch.uint8, device=DEV)
+    place = torch.tensor([pages - 1, 58254, pages - 7], device=DEV)
+    q, k, v = rows(150, hq, hkv, d, dtype, 3)
+    at = torch.arange(150, device=DEV)
+    slots = place[at // page] * page + at % page
+    q_rot = append(q, k, v, slots, big, positions=at, freq=inv_freq(d))
+    gk, gv = read(big, slots, dtype)
+    kf = Q.turned(k, at, inv_freq(d), None, 0.0)[0].float()
+    assert torch.equal(gk.double(), Q.values(kf, dtype)) and torch.equal(gv.double(), Q.values(v, dtype))
+    held = [torch.zeros(3 * page, hkv, d, dtype=dtype, device=DEV) for _ in range(2)]
+    held[0][:150], held[1][:150] = gk, gv
+    held = [x.view(3, page, hkv, d).transpose(1, 2).contiguous() for x in held]
+    tables = place.view(1, 3).int()
+    for new in ([1], [20], [150]):
+        x = q_rot[150 - new[0]:].contiguous()
+        out = attend(x, big, tables, [150], new, [0], single=new == [1])
+        check(out, x, held, torch.tensor([[0, 1, 2]], device=DEV), [150], new, [0])
+    _native.ops().paged_append_q4(None, None, None, slots, None, None, None, None, 1.0, None, None, 0.0, None, big, None)
+    assert not read(big, slots, dtype, fill=1.0)[0].any()
