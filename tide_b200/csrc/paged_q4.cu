@@ -447,6 +447,7 @@ struct OpenParams {
   int64_t wide;  // pages of a sequence in k and v
   int32_t *out_tables, *out_live;
   int few;       // sequences of up to so many rows are not needed
+  const int32_t *needed;  // 0: none is; NULL: not known
 };
 constexpr int kOpenPage = 128;  // tokens of a 16-bit page
 
@@ -458,6 +459,7 @@ __global__ void __launch_bounds__(256) open_kernel(const __grid_constant__ OpenP
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   ptx::grid_dependency_wait();
   ptx::grid_dependents_launch();
+  if (p.needed && __ldcg(p.needed) == 0) return;
   // eight blocks and heads a CTA, in order [sequence, block, head]
   const int live = live_sequences(p.batch) - p.first;
   if (blockIdx.x == 0 && threadIdx.x == 0) *p.out_live = min(max(live, 0), p.n);
@@ -534,7 +536,7 @@ __global__ void __launch_bounds__(256) open_kernel(const __grid_constant__ OpenP
 // codes, a shift, a mask, a difference and a product for two of them.
 constexpr int kFewWarps = 4;
 constexpr int kBatch = 3;        // blocks of a place
-constexpr int kUnitCost = 8;     // what beginning and ending a unit costs, in blocks
+constexpr int kUnitCost = 12;    // what beginning and ending a unit costs, in blocks
 constexpr int kLeast = 16;       // cost of a CTA, where there is so little
 
 template <int D, int NT>
@@ -567,6 +569,7 @@ struct FewParams {
   float *part_o;    // [CTAs, 2, 8 NT, D]: of a unit that the CTA ends, of one that it begins
   float2 *part_ml;  // [CTAs, 2, 8 NT]: maximum (scaled, base 2), sum
   Shared *shared;   // [CTAs]: the unit that it ends
+  int32_t *longer;  // whether a sequence has more than `few` tokens; or NULL
   int hq, hkv, group;
   int few;             // tokens a sequence may have
   int whole;           // units are not split
@@ -643,9 +646,11 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
     const int from = min((int)threadIdx.x * per, live), to = min(from + per, live);
     long long sum = 0;
     Sequence s{};
+    bool above = false;
     for (int i = from; i < to; ++i) {
       s = sequence(p.batch, i);
       sum += weight(s);
+      above |= s.n > p.few;
     }
     long long upto = sum;
 #pragma unroll
@@ -654,7 +659,8 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
       if (lane >= w) upto += x;
     }
     if (lane == 31) s_sum[warp] = upto;
-    __syncthreads();
+    above = __syncthreads_or(above);
+    if (p.longer && blockIdx.x == 0 && threadIdx.x == 0) *p.longer = above;
     long long total = 0;
     for (int w = 0; w < kFewWarps; ++w) {
       if (w < warp) upto += s_sum[w];
@@ -1173,11 +1179,13 @@ bool bad_cache(int64_t n_pages, int64_t page_size, int64_t hkv) {
 template <typename T, int D>
 int append(const tide::q4::AppendParams &p, cudaStream_t s) {
   using namespace tide::q4;
-  // A warp a row where that fills the GPU more than once, two where they fill it;
-  // else eight, the more the sooner done.
-  if (p.n_rows >= 148 * 24 * 2)
+  // Warps a row, us for 32 / 8 heads of 128 and for 12 of 64 (8, 2 and 1 warps):
+  // 192 rows 4.1, 4.9, 7.6 and 3.7, 4.5, 6.1; 512 rows 7.1, 6.1, 9.3 and 6.3, 5.0,
+  // 6.3; 4096 rows 34.6, 24.8, 28.2 and 28.3, 16.1, 16.5; 16384 rows 125, 77, 78 and
+  // 114, 54, 48; 32768 rows of the former - , 151, 145.
+  if (p.n_rows >= 148 * 96)
     return start("paged_append_q4", append_kernel<T, D, 4, 1>, (p.n_rows + 3) / 4, 128, 0, s, p);
-  if (p.n_rows * 2 >= 148 * 16)
+  if (p.n_rows >= 148 * 2)
     return start("paged_append_q4", append_kernel<T, D, 2, 2>, (p.n_rows + 1) / 2, 128, 0, s, p);
   return start("paged_append_q4", append_kernel<T, D, 1, 8>, p.n_rows, 256, 0, s, p);
 }
@@ -1201,8 +1209,16 @@ Plan plan_of(bool one_token, int64_t n_tokens, int64_t n_seqs, int64_t n_request
   using namespace tide::q4;
   Plan p{};
   // The lengths are on the device; the average is known.  More rows a sequence than
-  // kMostRows on average go to the tiles; else a sequence of up to as many, or any
-  // where the call has few rows, goes to the few-rows kernel.
+  // kMostRows on average go to the tiles (16 requests over 4000 to 8000 keys, us as
+  // few rows and as tiles: 32 rows 87 and 232, 64 rows 157 and 276, 128 rows 296 and
+  // 316; over 500 to 1000: 28 and 34, 40 and 35, 61 and 37).  Else sequences of up to
+  // twice as many rows go to the few-rows kernel, or all where the call has few rows,
+  // which saves the launches of the tiles that find nothing.
+  // Rows of a unit: 8 for up to as many on average, else 16 (64 requests over 1000 to
+  // 2000 keys, 8 and 16: 4 rows 42 and 48 us, 8 rows 43 and 49, 12 rows 70 and 54).
+  // Whole units for short contexts (us, whole and split: one request of 500 keys 8.8
+  // and 10.8, of 1000 13.4 and 11.2; 64 of 250 to 500 14.8 and 20.6; 256 of those 49
+  // and 47, of 500 to 1000 84 and 74).
   constexpr int64_t kMostRows = 64;
   const int64_t group = hq / hkv, rows = (n_tokens * group + n_seqs - 1) / n_seqs;
   p.nt = one_token || rows <= kMostRows ? (rows <= 8 ? 1 : 2) : 0;
@@ -1408,13 +1424,16 @@ extern "C" int tide_paged_attention_q4(int dtype, const void *q, int64_t q_row_s
   const tide::RaggedBatch batch{cu_seqlens, seq_ids, kv_lens, n_seqs_dev, (int)n_seqs, (int)n_requests,
                                 (int)n_tokens, (int)max_kv_len, error_word};
   int rc = TIDE_OK;
+  // behind the tiles' live count: whether there is a sequence for them
+  int32_t *live = plan.tiles ? reinterpret_cast<int32_t *>(ws + plan.few_bytes + 2 * plan.side) : nullptr;
+  int32_t *longer = plan.tiles && plan.nt ? live + 1 : nullptr;
   if (plan.nt) {
     const int64_t group = n_q_heads / n_kv_heads, rows = plan.ctas * 2 * 8 * plan.nt;
     float *part_o = reinterpret_cast<float *>(ws);
     float2 *part_ml = reinterpret_cast<float2 *>(part_o + rows * head_dim);
     const tide::q4::FewParams f{batch, static_cast<const unsigned char *>(cache), block_tables, max_pages,
                                 (int)n_pages, shift, q, q_row_stride, out, part_o, part_ml,
-                                reinterpret_cast<tide::q4::Shared *>(part_ml + rows), (int)n_q_heads,
+                                reinterpret_cast<tide::q4::Shared *>(part_ml + rows), longer, (int)n_q_heads,
                                 (int)n_kv_heads, (int)group, plan.few, plan.whole,
                                 scale * tide::ragged::kLog2e,
                                 bf16 ? tide::q4::kMagic<__nv_bfloat16> : tide::q4::kMagic<__half>,
@@ -1425,13 +1444,12 @@ extern "C" int tide_paged_attention_q4(int dtype, const void *q, int64_t q_row_s
   }
   if (rc || !plan.tiles) return rc;
   ws += plan.few_bytes;
-  int32_t *live = reinterpret_cast<int32_t *>(ws + 2 * plan.side);
   int32_t *tables = live + 4;
   for (int64_t i = 0; i < n_seqs; i += plan.seqs) {
     const int64_t n = n_seqs - i < plan.seqs ? n_seqs - i : plan.seqs;
     const tide::q4::OpenParams o{batch, (int)i, (int)n, static_cast<const unsigned char *>(cache),
                                  block_tables, max_pages, (int)n_pages, (int)page_size, (int)n_kv_heads, ws,
-                                 ws + plan.side, plan.wide, tables, live, plan.few};
+                                 ws + plan.side, plan.wide, tables, live, plan.few, longer};
     rc = bf16 ? (wide ? open<__nv_bfloat16, 128>(o, st) : open<__nv_bfloat16, 64>(o, st))
               : (wide ? open<__half, 128>(o, st) : open<__half, 64>(o, st));
     if (rc) return rc;
@@ -1445,7 +1463,7 @@ extern "C" int tide_paged_attention_q4(int dtype, const void *q, int64_t q_row_s
     const tide::KeySource src{ws, ws + plan.side, 0, tables + skip * plan.wide, plan.wide,
                               (int)(plan.seqs * plan.wide), 7};
     static_assert(tide::q4::kOpenPage == 1 << 7, "");
-    rc = tide::paged_tiles(dtype, head_dim, part, src, plan.few,
+    rc = tide::paged_tiles(dtype, head_dim, part, src, plan.few, longer,
                            static_cast<const unsigned char *>(q) + row * q_row_stride * 2, q_row_stride,
                            static_cast<unsigned char *>(out) + row * n_q_heads * head_dim * 2, n_q_heads,
                            n_kv_heads, scale, ws + 2 * plan.side + plan.tables, st);

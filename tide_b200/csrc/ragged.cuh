@@ -164,11 +164,12 @@ void set_last_error(const char *msg);
 // The join of the few-rows kernels' splits, [splits, n_seqs, few, hq] rows.
 int join_few_rows(int dtype, int64_t head_dim, const RaggedBatch &b, int hq, int few, int splits,
                   const float *part_o, const float2 *part_ml, void *out, cudaStream_t s);
-// Sequences with more than `few` rows over 16-bit pages, by tiles.
+// Sequences with more than `few` rows over 16-bit pages, by tiles; *needed 0: there
+// is none (NULL: not known).
 size_t paged_tiles_workspace_size(int64_t n_tokens, int64_t n_seqs, int64_t hq, int64_t hkv, int64_t d,
                                   int64_t max_kv);
 int paged_tiles(int dtype, int64_t head_dim, const RaggedBatch &b, const KeySource &src, int few,
-                const void *q, int64_t q_stride, void *out, int64_t hq, int64_t hkv, float scale,
-                void *workspace, cudaStream_t s);
+                const int32_t *needed, const void *q, int64_t q_stride, void *out, int64_t hq,
+                int64_t hkv, float scale, void *workspace, cudaStream_t s);
 
 }  // namespace tide

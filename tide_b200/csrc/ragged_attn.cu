@@ -127,6 +127,7 @@ struct Params {
   int take_over;   // whether there are more CTAs than run at once
   int boxes;       // whether a warp's 32 rows are a box of the output's map
   int behind_few;  // launched over the few-rows kernel of the same call
+  const int32_t *needed;  // 0: no sequence is this kernel's; NULL: not known
   float qs;        // scale * log2(e)
 };
 
@@ -975,6 +976,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   unsigned char *q_smem = base, *ring = base + 2 * S::kQ;
   unsigned char *staging = ring + S::kStages * S::kBlock;
   const int warp = threadIdx.x >> 5;
+  if (p.needed) {  // (its set-up costs a round of CTAs some 9 us)
+    ptx::grid_dependency_wait();
+    if (__ldcg(p.needed) == 0) return;
+  }
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
       ptx::mbar_init(&sh.q_full[t], 1);
@@ -1816,8 +1821,8 @@ size_t paged_tiles_workspace_size(int64_t n_tokens, int64_t n_seqs, int64_t hq, 
 }
 
 int paged_tiles(int dtype, int64_t head_dim, const RaggedBatch &b, const KeySource &src, int few,
-                const void *q, int64_t q_stride, void *out, int64_t hq, int64_t hkv, float scale,
-                void *workspace, cudaStream_t s) {
+                const int32_t *needed, const void *q, int64_t q_stride, void *out, int64_t hq,
+                int64_t hkv, float scale, void *workspace, cudaStream_t s) {
   const int64_t d = head_dim, kv_rows = (int64_t)src.n_pages * hkv << src.page_shift;
   Plan plan = plan_paged(false, b.n_tokens, b.n_seqs, hq, hkv, d, b.max_kv, true);
   plan.few = few;
@@ -1825,6 +1830,7 @@ int paged_tiles(int dtype, int64_t head_dim, const RaggedBatch &b, const KeySour
   ragged::Params p{};
   p.batch = b;
   p.src = src;
+  p.needed = needed;
   set_heads(p, hq, hkv, d, scale, out);
   if (dtype == TIDE_DTYPE_BF16)
     return d == 128 ? run_paged<__nv_bfloat16, 128>(plan, p, dtype, q, q_stride, kv_rows, ws, s)
