@@ -527,3 +527,71 @@ def test_a_cache_past_4_gigabytes():
         check(out, x, held, torch.tensor([[0, 1, 2]], device=DEV), [150], new, [0])
     _native.ops().paged_append_q4(None, None, None, slots, None, None, None, None, 1.0, None, None, 0.0, None, big, None)
     assert not read(big, slots, dtype, fill=1.0)[0].any()
+
+
+def test_a_captured_chunk_call_takes_other_lengths():
+    """One captured call over tokens dealt to the sequences in several ways: all
+    short, one long, one empty, which the two kernels share differently."""
+    hq, hkv, d, dtype, B = 8, 2, 128, BF, 61
+    n = 6 * B
+    splits = [[6] * B, [1] * 30 + [n - 60] + [1] * 30, [n] + [0] * (B - 1), [0, 12] * 30 + [6]]
+    _, cache, held, tables, lens, ids = q4_case([n] * B, [100 + 3 * i for i in range(B)], hq, hkv, d, dtype, 16, 5)
+    most = max(lens)
+    x = torch.randn(n, hq, d, device=DEV).to(dtype)
+    cu, kv, out, err = i32([0] * (B + 1)), i32([0] * len(lens)), torch.zeros_like(x), i32([0])
+
+    def call():
+        _native.ops().paged_attention_q4(x, cache, tables, kv, cu, i32_ids, out, most, d ** -0.5, err)
+
+    i32_ids = i32(ids)
+    graph = None
+    for new in splits + splits[:1]:
+        cu.copy_(i32(starts(new)))
+        mine = list(lens)
+        for k, r in zip(new, ids):
+            mine[r] = 90 + k
+        kv.copy_(i32(mine))
+        if graph is None:
+            call()
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                call()
+        out.fill_(7.0)
+        graph.replay()
+        assert int(err) == 0
+        check(out, x, held, tables, mine, new, ids)
+
+
+def test_calls_on_two_streams_do_not_meet():
+    """Attention and appends of two caches at once, each on a stream of its own,
+    against the same one after the other."""
+    hq, hkv, d, dtype = 8, 2, 128, BF
+    cases = [q4_case([1] * 40, [50 * i for i in range(40)], hq, hkv, d, dtype, 16, s) for s in (1, 2)]
+    chunk = [q4_case([30, 90, 2], [900, 20, 500], hq, hkv, d, dtype, 32, s) for s in (3, 4)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+
+    def work(c, k):
+        outs = []
+        for q, cache, _, tables, lens, ids in (c, k):
+            for _ in range(3):
+                new = [1] * 40 if q.shape[0] == 40 else [30, 90, 2]
+                outs.append(attend(q, cache, tables, lens, new, ids, max(lens),
+                                   single=q.shape[0] == 40))
+                kk = torch.full((5, hkv, d), 0.5, dtype=dtype, device=DEV)
+                mine = empty_cache(2, hkv, 16, d)
+                append(None, kk, kk, torch.arange(5, device=DEV), mine)
+                outs.append(mine)
+        return outs
+
+    want = [work(c, k) for c, k in zip(cases, chunk)]
+    torch.cuda.synchronize()
+    got = []
+    for s, c, k in zip(streams, cases, chunk):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append(work(c, k))
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
