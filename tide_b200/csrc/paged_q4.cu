@@ -27,13 +27,16 @@ __device__ __forceinline__ long long quotient(long long a, long long b) {
 // one step of its group off where the last bit of a 32-bit sum is, and the
 // angle of a far position has lost more than that.  A key is therefore made in
 // 64 bits (the angle in turns, its whole part dropped: exact to 1e-10 at
-// position 2^20).  That is 24 operations of the 64-bit pipe for a key of a lane,
-// two cycles each, and a sine and cosine per row and frequency, which the CTA
-// makes once for all its heads; both run under the loads and stores.
+// position 2^20).  The 64-bit pipe has time for that (7 % of it in a long prompt's
+// append); a row's sines and cosines are made once for all its heads.
 //
 // A lane has eight neighbouring channels of a head's lower half, which are a word
 // of codes, and the eight that they are turned with.  So D / 16 lanes share a head,
 // and the four lanes of a group find its least and largest value in two exchanges.
+//
+// 32768 rows of 32 + 8 + 8 heads of 128 take 145 us (4.5 TB/s), 60 % of the issue
+// slots; some 2800 warp instructions a row, half of them the codes'.  192 rows 4.1
+// us, all latency.
 struct AppendParams {
   const void *q, *k, *v;
   int64_t q_stride, kv_stride;
@@ -385,6 +388,7 @@ __global__ void __launch_bounds__(256) zeros_kernel(const __grid_constant__ Appe
 // -------------------------------------------------------------------- read
 // A warp per row, eight channels a lane at a time, keys and values: four bytes of
 // codes in, 16 bytes out.  Four of each are loaded before the first is stored.
+// Bound by HBM: 26003 tokens of 8 heads of 128 in 25.4 us, 5.4 TB/s.
 template <typename T, int D>
 __global__ void __launch_bounds__(256)
     read_kernel(const unsigned char *__restrict__ cache, const int64_t *__restrict__ slots,
@@ -434,8 +438,9 @@ __global__ void __launch_bounds__(256)
 
 // ------------------------------------------------- attention of many rows
 // The keys and values of each sequence as 16-bit pages in its order, for the
-// tiles of paged_attention: a pass of 4.5 bits in and 16 out per value, 1 / 30 of
-// the time that 2048 rows over them take.
+// tiles of paged_attention: a pass of 4.5 bits in and 16 out per value (28051 tokens
+// of 8 heads of 128 in 27 us, where 2048 rows over them take 800).  Made in the tile
+// kernel instead, each tile of rows would make them anew.
 struct OpenParams {
   RaggedBatch batch;  // of these sequences: seq_ids and n_dev of all
   int first, n;       // of the call's sequences
@@ -532,11 +537,19 @@ __global__ void __launch_bounds__(256) open_kernel(const __grid_constant__ OpenP
 // works on and one under way.  The sum of the weights, as they meet the values, is
 // one more row of the values' product.
 //
-// What bounds it is the instructions: of a block's 400 some 260 make operands from
-// codes, a shift, a mask, a difference and a product for two of them.
+// What bounds it is the instructions: of a block's 420 some 260 make operands from
+// codes, a shift, a mask, a difference and a product for two of them.  An ALU
+// instruction takes two cycles of its pipe, and a product some nine in which it does
+// little else, so 190 of the one and 17 of the other are 530 cycles of the 700 that a
+// block takes a scheduler.
+// 32 query heads on 8 KV heads of 128, with the join: 192 requests of 512 to 1535
+// keys 72 us (3.1 TB/s), three of 9000 to 40000 keys 32 us, 16 requests of 1 to 9
+// tokens over up to 2100 keys 30 us; two short ones 5.9 us.
 constexpr int kFewWarps = 4;
 constexpr int kBatch = 3;        // blocks of a place
-constexpr int kUnitCost = 12;    // what beginning and ending a unit costs, in blocks
+// What beginning and ending a unit costs, in blocks (with 4, 8 and 12, us: those 16
+// requests, some of them short, 41.8, 31.5, 30.3; the 192 73.7, 72.5, 72.2).
+constexpr int kUnitCost = 12;
 constexpr int kLeast = 16;       // cost of a CTA, where there is so little
 
 template <int D, int NT>
@@ -721,314 +734,314 @@ __global__ void __launch_bounds__(32 * kFewWarps, Few<D, NT>::kCtas)
     const int blocks = max(0, (b1 - b0 - warp + kFewWarps - 1) / kFewWarps);
     const int block0 = b0 + warp;
     if (b1 > b0 || starts) {
-    uint4 raw[NT][kKWords];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int r = nt * 8 + g;
-      const bool valid = r < rows;
-      const int tok = token_of(u.row + (valid ? r : 0), p.per_group);
-      const T *q = static_cast<const T *>(p.q) + (u.s.row0 + tok) * p.q_stride +
-                   (int64_t)(u.kvh * p.group + u.row + (valid ? r : 0) - tok * p.group) * D + t * (D / 4);
-#pragma unroll
-      for (int w = 0; w < kKWords; ++w)
-        raw[nt][w] = valid ? *reinterpret_cast<const uint4 *>(q + 8 * w) : make_uint4(0, 0, 0, 0);
-    }
-    // where 32 blocks at a time are in the cache, one per lane, the next ones read
-    // ahead; -1: a page outside it
-    auto places = [&](int i0) {
-      const int i = i0 + lane, at = (block0 + i * kFewWarps) * kBlock;
-      if (i >= blocks || at >= kv) return -1;  // (or a unit without keys)
-      const int pg = __ldg(p.tables + u.s.req * p.max_pages + (at >> p.page_shift));
-      if (pg < 0 || pg >= p.n_pages) {
-        raise_error(p.batch.err, TIDE_DEVERR_POSITION);
-        return -1;
-      }
-      return (pg * p.hkv + u.kvh) * (page / kBlock) + (at & (page - 1)) / kBlock;
-    };
-    int base = 0, now = places(0), next = places(32);
-    // blocks [i, i + kBatch) to a place, a lane each
-    auto request = [&](int i, uint32_t to) {
-      const int n = min(kBatch, blocks - i);
-      if (n <= 0) return;
-      if (i - base >= 32) {
-        base += 32;
-        now = next;
-        next = places(base + 32);
-      }
-      const int k = i - base + lane;
-      const int place0 = __shfl_sync(kFull, now, k & 31), place1 = __shfl_sync(kFull, next, k & 31);
-      const int place = k < 32 ? place0 : place1;
-      uint64_t *bar = &full[warp][to];
-      unsigned char *at = ring + to * F::kPlace + lane * L::kBytes;
-      const bool copy = lane < n && place >= 0;
-      const int copies = __popc(__ballot_sync(kFull, copy));
-      if (lane < n && place < 0)  // reads as zeros
-        for (int e = 0; e < L::kBytes / 16; ++e) reinterpret_cast<uint4 *>(at)[e] = make_uint4(0, 0, 0, 0);
-      __syncwarp();
-      if (lane == 0) ptx::mbar_expect_tx(bar, copies * L::kBytes);
-      __syncwarp();
-      if (copy) ptx::bulk_load(at, p.cache + (int64_t)place * L::kBytes, L::kBytes, bar, once);
-    };
-    request(0, turn & 1);
-    request(kBatch, (turn & 1) ^ 1);
-    if (starts && !p.whole && threadIdx.x == 0) {
-      Shared x{-1, -1, u.s.row0, u.row, rows, u.kvh};
-      const long long block = pos - u.at + kUnitCost;  // the unit's first one's place in all
-      if (b0 > 0) x.first = cta_of(block), x.last = cta_of(block + u.nb - 1);
-      p.shared[blockIdx.x] = x;
-    }
-    starts = false;
-
-    // Q^T: columns are rows 8 nt + g; the statistics of a column are kept by the
-    // lanes whose accumulators belong to it, columns 8 nt + 2 t and one further
-    uint32_t qb[NT][kSteps][2];
-    int sees[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int w = 0; w < kKWords; ++w) {
-        const uint4 x = raw[nt][w];
-        qb[nt][2 * w][0] = x.x;
-        qb[nt][2 * w][1] = x.y;
-        qb[nt][2 * w + 1][0] = x.z;
-        qb[nt][2 * w + 1][1] = x.w;
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int c = min(nt * 8 + t * 2 + e, rows - 1);
-        sees[nt][e] = pos0 + token_of(u.row + c, p.per_group) + 1;
-      }
-    }
-    // (a weight is 2^(score qs + up); up is lowered where a score passes `most`)
-    float o[NT][kSteps][4], oc[NT][4], up[NT][2], most[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      up[nt][0] = up[nt][1] = kLift<T>;
-      most[nt][0] = most[nt][1] = -INFINITY;
-      oc[nt][0] = oc[nt][1] = oc[nt][2] = oc[nt][3] = 0.f;
-#pragma unroll
-      for (int d = 0; d < kSteps; ++d) o[nt][d][0] = o[nt][d][1] = o[nt][d][2] = o[nt][d][3] = 0.f;
-    }
-    const int all_see = pos0 + token_of(u.row, p.per_group) + 1;  // keys that every row sees
-
-    // One block at b, keys from `key` on.  masked: not all rows see all of them.
-    auto work = [&](const unsigned char *b, int key, auto masked) {
-      constexpr bool kMasked = decltype(masked)::value;
-      uint32_t kw[2][kKWords], vw[4][kVWords];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const unsigned char *at = b + k_at + 8 * h * L::kRow;
-        if constexpr (D == 128) {
-          const uint4 x = *reinterpret_cast<const uint4 *>(at);
-          kw[h][0] = x.x, kw[h][1] = x.y, kw[h][2] = x.z, kw[h][3] = x.w;
-        } else {
-          const uint2 x = *reinterpret_cast<const uint2 *>(at);
-          kw[h][0] = x.x, kw[h][1] = x.y;
-        }
-      }
-      const uint2 ks = *reinterpret_cast<const uint2 *>(b + ks_at);
-      float sc[NT][4];
-      {
-        const uint32_t both = g & 1 ? 0x3232u : 0x1010u;
-        const Pars<T> p0 = pars<T>(prmt(ks.x, 0u, both), magic), p1 = pars<T>(prmt(ks.y, 0u, both), magic);
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-          const int at = 2 * (k & 1);
-          const uint32_t w0 = kw[0][k / 2], w1 = kw[1][k / 2];
-          const uint32_t a[4] = {value2_at<T>(w0, at, p0, magic), value2_at<T>(w1, at, p1, magic),
-                                 value2_at<T>(w0, at + 1, p0, magic), value2_at<T>(w1, at + 1, p1, magic)};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            if (k == 0) mma16816_first<T>(sc[nt], a, qb[nt][k][0], qb[nt][k][1]);
-            else mma16816<T>(sc[nt], a, qb[nt][k][0], qb[nt][k][1]);
-          }
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        const unsigned char *at = b + v_at + 4 * h * L::kRow;
-        if constexpr (D == 128) {
-          const uint2 x = *reinterpret_cast<const uint2 *>(at);
-          vw[h][0] = x.x, vw[h][1] = x.y;
-        } else {
-          vw[h][0] = *reinterpret_cast<const uint32_t *>(at);
-        }
-      }
-      uint2 vs = *reinterpret_cast<const uint2 *>(b + vs_at);
-      if constexpr (kMasked) {
-        // A weight of 0 does not silence a NaN.  Past the last key a token's scales
-        // are dropped; before it, where rows differ, those that are NaN are, and
-        // added to the rows that do see them.
-        auto drop = [](uint2 &x, int h) { (h < 2 ? x.x : x.y) &= h & 1 ? 0x0000ffffu : 0xffff0000u; };
-        auto odd = [](const uint2 &x, int h) {
-          return (((h < 2 ? x.x : x.y) >> (h & 1) * 16) & 0x7f80u) == 0x7f80u;
-        };
-#pragma unroll
-        for (int h = 0; h < 4; ++h)
-          if (key + t + 4 * h >= kv) drop(vs, h);
-        if (__any_sync(kFull, odd(vs, 0) || odd(vs, 1) || odd(vs, 2) || odd(vs, 3))) {
-          // rare: token by token, its scale being with lane 4 g + its number % 4
-#pragma unroll 1
-          for (int k = 0; k < kBlock; ++k) {
-            const uint32_t two = __shfl_sync(kFull, k < 8 ? vs.x : vs.y, (lane & 28) + k % 4);
-            const bool is = ((two >> (k / 4 & 1) * 16) & 0x7f80u) == 0x7f80u;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int d = 0; d < kSteps; ++d)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (is && key + k < sees[nt][e & 1]) o[nt][d][e] = NAN;
-          }
-#pragma unroll
-          for (int h = 0; h < 4; ++h)
-            if (odd(vs, h)) drop(vs, h);
-        }
-      }
-      uint32_t pt[NT][2];
+      uint4 raw[NT][kKWords];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        pt[nt][0] = pt[nt][1] = 0u;
-        if (NT > 1 && nt >= tiles) continue;
-        bool raise = false;
+        const int r = nt * 8 + g;
+        const bool valid = r < rows;
+        const int tok = token_of(u.row + (valid ? r : 0), p.per_group);
+        const T *q = static_cast<const T *>(p.q) + (u.s.row0 + tok) * p.q_stride +
+                     (int64_t)(u.kvh * p.group + u.row + (valid ? r : 0) - tok * p.group) * D + t * (D / 4);
+#pragma unroll
+        for (int w = 0; w < kKWords; ++w)
+          raw[nt][w] = valid ? *reinterpret_cast<const uint4 *>(q + 8 * w) : make_uint4(0, 0, 0, 0);
+      }
+      // where 32 blocks at a time are in the cache, one per lane, the next ones read
+      // ahead; -1: a page outside it
+      auto places = [&](int i0) {
+        const int i = i0 + lane, at = (block0 + i * kFewWarps) * kBlock;
+        if (i >= blocks || at >= kv) return -1;  // (or a unit without keys)
+        const int pg = __ldg(p.tables + u.s.req * p.max_pages + (at >> p.page_shift));
+        if (pg < 0 || pg >= p.n_pages) {
+          raise_error(p.batch.err, TIDE_DEVERR_POSITION);
+          return -1;
+        }
+        return (pg * p.hkv + u.kvh) * (page / kBlock) + (at & (page - 1)) / kBlock;
+      };
+      int base = 0, now = places(0), next = places(32);
+      // blocks [i, i + kBatch) to a place, a lane each
+      auto request = [&](int i, uint32_t to) {
+        const int n = min(kBatch, blocks - i);
+        if (n <= 0) return;
+        if (i - base >= 32) {
+          base += 32;
+          now = next;
+          next = places(base + 32);
+        }
+        const int k = i - base + lane;
+        const int place0 = __shfl_sync(kFull, now, k & 31), place1 = __shfl_sync(kFull, next, k & 31);
+        const int place = k < 32 ? place0 : place1;
+        uint64_t *bar = &full[warp][to];
+        unsigned char *at = ring + to * F::kPlace + lane * L::kBytes;
+        const bool copy = lane < n && place >= 0;
+        const int copies = __popc(__ballot_sync(kFull, copy));
+        if (lane < n && place < 0)  // reads as zeros
+          for (int e = 0; e < L::kBytes / 16; ++e) reinterpret_cast<uint4 *>(at)[e] = make_uint4(0, 0, 0, 0);
+        __syncwarp();
+        if (lane == 0) ptx::mbar_expect_tx(bar, copies * L::kBytes);
+        __syncwarp();
+        if (copy) ptx::bulk_load(at, p.cache + (int64_t)place * L::kBytes, L::kBytes, bar, once);
+      };
+      request(0, turn & 1);
+      request(kBatch, (turn & 1) ^ 1);
+      if (starts && !p.whole && threadIdx.x == 0) {
+        Shared x{-1, -1, u.s.row0, u.row, rows, u.kvh};
+        const long long block = pos - u.at + kUnitCost;  // the unit's first one's place in all
+        if (b0 > 0) x.first = cta_of(block), x.last = cta_of(block + u.nb - 1);
+        p.shared[blockIdx.x] = x;
+      }
+      starts = false;
+
+      // Q^T: columns are rows 8 nt + g; the statistics of a column are kept by the
+      // lanes whose accumulators belong to it, columns 8 nt + 2 t and one further
+      uint32_t qb[NT][kSteps][2];
+      int sees[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int w = 0; w < kKWords; ++w) {
+          const uint4 x = raw[nt][w];
+          qb[nt][2 * w][0] = x.x;
+          qb[nt][2 * w][1] = x.y;
+          qb[nt][2 * w + 1][0] = x.z;
+          qb[nt][2 * w + 1][1] = x.w;
+        }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          if constexpr (kMasked) {  // tokens kappa and 8 further
-            const int lim = sees[nt][e] - key - kappa;
-            if (lim <= 0) sc[nt][e] = -INFINITY;
-            if (lim <= 8) sc[nt][2 + e] = -INFINITY;
-          }
-          raise |= fmaxf(sc[nt][e], sc[nt][2 + e]) > most[nt][e];  // (the first keys: of -infinity)
+          const int c = min(nt * 8 + t * 2 + e, rows - 1);
+          sees[nt][e] = pos0 + token_of(u.row + c, p.per_group) + 1;
         }
-        if (__any_sync(kFull, raise)) {
-          float a[2];
+      }
+      // (a weight is 2^(score qs + up); up is lowered where a score passes `most`)
+      float o[NT][kSteps][4], oc[NT][4], up[NT][2], most[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        up[nt][0] = up[nt][1] = kLift<T>;
+        most[nt][0] = most[nt][1] = -INFINITY;
+        oc[nt][0] = oc[nt][1] = oc[nt][2] = oc[nt][3] = 0.f;
+#pragma unroll
+        for (int d = 0; d < kSteps; ++d) o[nt][d][0] = o[nt][d][1] = o[nt][d][2] = o[nt][d][3] = 0.f;
+      }
+      const int all_see = pos0 + token_of(u.row, p.per_group) + 1;  // keys that every row sees
+
+      // One block at b, keys from `key` on.  masked: not all rows see all of them.
+      auto work = [&](const unsigned char *b, int key, auto masked) {
+        constexpr bool kMasked = decltype(masked)::value;
+        uint32_t kw[2][kKWords], vw[4][kVWords];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const unsigned char *at = b + k_at + 8 * h * L::kRow;
+          if constexpr (D == 128) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(at);
+            kw[h][0] = x.x, kw[h][1] = x.y, kw[h][2] = x.z, kw[h][3] = x.w;
+          } else {
+            const uint2 x = *reinterpret_cast<const uint2 *>(at);
+            kw[h][0] = x.x, kw[h][1] = x.y;
+          }
+        }
+        const uint2 ks = *reinterpret_cast<const uint2 *>(b + ks_at);
+        float sc[NT][4];
+        {
+          const uint32_t both = g & 1 ? 0x3232u : 0x1010u;
+          const Pars<T> p0 = pars<T>(prmt(ks.x, 0u, both), magic), p1 = pars<T>(prmt(ks.y, 0u, both), magic);
+#pragma unroll
+          for (int k = 0; k < kSteps; ++k) {
+            const int at = 2 * (k & 1);
+            const uint32_t w0 = kw[0][k / 2], w1 = kw[1][k / 2];
+            const uint32_t a[4] = {value2_at<T>(w0, at, p0, magic), value2_at<T>(w1, at, p1, magic),
+                                   value2_at<T>(w0, at + 1, p0, magic), value2_at<T>(w1, at + 1, p1, magic)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              if (k == 0) mma16816_first<T>(sc[nt], a, qb[nt][k][0], qb[nt][k][1]);
+              else mma16816<T>(sc[nt], a, qb[nt][k][0], qb[nt][k][1]);
+            }
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const unsigned char *at = b + v_at + 4 * h * L::kRow;
+          if constexpr (D == 128) {
+            const uint2 x = *reinterpret_cast<const uint2 *>(at);
+            vw[h][0] = x.x, vw[h][1] = x.y;
+          } else {
+            vw[h][0] = *reinterpret_cast<const uint32_t *>(at);
+          }
+        }
+        uint2 vs = *reinterpret_cast<const uint2 *>(b + vs_at);
+        if constexpr (kMasked) {
+          // A weight of 0 does not silence a NaN.  Past the last key a token's scales
+          // are dropped; before it, where rows differ, those that are NaN are, and
+          // added to the rows that do see them.
+          auto drop = [](uint2 &x, int h) { (h < 2 ? x.x : x.y) &= h & 1 ? 0x0000ffffu : 0xffff0000u; };
+          auto odd = [](const uint2 &x, int h) {
+            return (((h < 2 ? x.x : x.y) >> (h & 1) * 16) & 0x7f80u) == 0x7f80u;
+          };
+#pragma unroll
+          for (int h = 0; h < 4; ++h)
+            if (key + t + 4 * h >= kv) drop(vs, h);
+          if (__any_sync(kFull, odd(vs, 0) || odd(vs, 1) || odd(vs, 2) || odd(vs, 3))) {
+            // rare: token by token, its scale being with lane 4 g + its number % 4
+#pragma unroll 1
+            for (int k = 0; k < kBlock; ++k) {
+              const uint32_t two = __shfl_sync(kFull, k < 8 ? vs.x : vs.y, (lane & 28) + k % 4);
+              const bool is = ((two >> (k / 4 & 1) * 16) & 0x7f80u) == 0x7f80u;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int d = 0; d < kSteps; ++d)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e)
+                    if (is && key + k < sees[nt][e & 1]) o[nt][d][e] = NAN;
+            }
+#pragma unroll
+            for (int h = 0; h < 4; ++h)
+              if (odd(vs, h)) drop(vs, h);
+          }
+        }
+        uint32_t pt[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          pt[nt][0] = pt[nt][1] = 0u;
+          if (NT > 1 && nt >= tiles) continue;
+          bool raise = false;
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float top = fmaxf(sc[nt][e], sc[nt][2 + e]);
+            if constexpr (kMasked) {  // tokens kappa and 8 further
+              const int lim = sees[nt][e] - key - kappa;
+              if (lim <= 0) sc[nt][e] = -INFINITY;
+              if (lim <= 8) sc[nt][2 + e] = -INFINITY;
+            }
+            raise |= fmaxf(sc[nt][e], sc[nt][2 + e]) > most[nt][e];  // (the first keys: of -infinity)
+          }
+          if (__any_sync(kFull, raise)) {
+            float a[2];
 #pragma unroll
-            for (int w = 4; w < 32; w *= 2) top = fmaxf(top, __shfl_xor_sync(kFull, top, w));
-            const bool raised = top > most[nt][e];
-            const float to = raised ? fmaf(-top, p.qs, kLift<T>) : up[nt][e];
-            // (nothing there yet: whatever the factor)
-            a[e] = most[nt][e] == -INFINITY ? 0.f : ex2(to - up[nt][e]);
-            up[nt][e] = to;
-            if (raised) most[nt][e] = top + slack;
-            oc[nt][e] *= a[e];
+            for (int e = 0; e < 2; ++e) {
+              float top = fmaxf(sc[nt][e], sc[nt][2 + e]);
+#pragma unroll
+              for (int w = 4; w < 32; w *= 2) top = fmaxf(top, __shfl_xor_sync(kFull, top, w));
+              const bool raised = top > most[nt][e];
+              const float to = raised ? fmaf(-top, p.qs, kLift<T>) : up[nt][e];
+              // (nothing there yet: whatever the factor)
+              a[e] = most[nt][e] == -INFINITY ? 0.f : ex2(to - up[nt][e]);
+              up[nt][e] = to;
+              if (raised) most[nt][e] = top + slack;
+              oc[nt][e] *= a[e];
+            }
+#pragma unroll
+            for (int d = 0; d < kSteps; ++d) {
+              o[nt][d][0] *= a[0];
+              o[nt][d][1] *= a[1];
+              o[nt][d][2] *= a[0];
+              o[nt][d][3] *= a[1];
+            }
+          }
+          float x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = ex2(fmaf(sc[nt][e], p.qs, up[nt][e & 1]));
+          pt[nt][0] = transpose8x8(pack_weights<T>(x[0], x[1]));
+          pt[nt][1] = transpose8x8(pack_weights<T>(x[2], x[3]));
+        }
+        const Pars<T> p0 = pars<T>(vs.x, magic), p1 = pars<T>(vs.y, magic);
+#pragma unroll
+        for (int x = 0; x < kVWords; ++x) {
+          const uint32_t lo0 = prmt(vw[0][x], vw[1][x], 0x5410u), hi0 = prmt(vw[0][x], vw[1][x], 0x7632u);
+          const uint32_t lo1 = prmt(vw[2][x], vw[3][x], 0x5410u), hi1 = prmt(vw[2][x], vw[3][x], 0x7632u);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t a[4] = {value2_at<T>(lo0, k, p0, magic), value2_at<T>(hi0, k, p0, magic),
+                                   value2_at<T>(lo1, k, p1, magic), value2_at<T>(hi1, k, p1, magic)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[nt][4 * x + k], a, pt[nt][0], pt[nt][1]);
+          }
+        }
+        // the weights' sum: values of 1 in the rows of channel 0
+        const uint32_t ones = g == 0 ? kOnes<T> : 0u;
+        const uint32_t a[4] = {ones, 0u, ones, 0u};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma16816<T>(oc[nt], a, pt[nt][0], pt[nt][1]);
+      };
+
+      int i = 0;
+      bool lost = false;  // a wait has run out
+#pragma unroll 1
+      while (i < blocks) {
+        const uint32_t at = turn & 1;
+        if (!__all_sync(kFull, ptx::mbar_wait(&full[warp][at], turn >> 1 & 1, &s_abort))) {
+          raise_error(p.batch.err, TIDE_DEVERR_TIMEOUT);
+          s_abort = 1;
+          lost = true;
+          break;
+        }
+        const unsigned char *b = ring + at * F::kPlace;
+        int key = (block0 + i * kFewWarps) * kBlock;
+        const int upto = min(i + kBatch, blocks);
+#pragma unroll 1
+        for (; i < upto; ++i, b += L::kBytes, key += kFewWarps * kBlock) {
+          if (key + kBlock <= all_see) work(b, key, std::false_type{});
+          else work(b, key, std::true_type{});
+        }
+        __syncwarp();  // the place has been read
+        ptx::fence_proxy_async();
+        request(i + kBatch, at);
+        ++turn;
+      }
+      if (lost && lane == 0) {  // wait for the copies in flight (bounded)
+        volatile int none = 0;
+        for (int e = i; e < min(blocks, i + 2 * kBatch); e += kBatch, ++turn)
+          ptx::mbar_wait(&full[warp][turn & 1], turn >> 1 & 1, &none);
+      }
+      __syncwarp();
+
+      // the four warps' outputs meet, [warp][row][D + 4]
+      float *mine = reinterpret_cast<float *>(ring);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = nt * 8 + t * 2 + e;
+          if (g == 0) {
+            s_m[warp][r] = kLift<T> - up[nt][e];
+            s_l[warp][r] = oc[nt][e];
           }
 #pragma unroll
-          for (int d = 0; d < kSteps; ++d) {
-            o[nt][d][0] *= a[0];
-            o[nt][d][1] *= a[1];
-            o[nt][d][2] *= a[0];
-            o[nt][d][3] *= a[1];
-          }
+          for (int d = 0; d < kSteps; ++d)
+            *reinterpret_cast<float2 *>(mine + r * F::kPitch + g * (D / 8) + 2 * d) =
+                make_float2(o[nt][d][e], o[nt][d][2 + e]);
         }
-        float x[4];
+      __syncthreads();
+      constexpr int kLanes = D / 4;  // lanes of a row, four columns each
+      for (int r = threadIdx.x / kLanes; r < rows; r += 32 * kFewWarps / kLanes) {
+        const int d = threadIdx.x % kLanes * 4;
+        float top = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = ex2(fmaf(sc[nt][e], p.qs, up[nt][e & 1]));
-        pt[nt][0] = transpose8x8(pack_weights<T>(x[0], x[1]));
-        pt[nt][1] = transpose8x8(pack_weights<T>(x[2], x[3]));
-      }
-      const Pars<T> p0 = pars<T>(vs.x, magic), p1 = pars<T>(vs.y, magic);
+        for (int w = 0; w < kFewWarps; ++w)
+          if (s_l[w][r] != 0.f) top = fmaxf(top, s_m[w][r]);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int x = 0; x < kVWords; ++x) {
-        const uint32_t lo0 = prmt(vw[0][x], vw[1][x], 0x5410u), hi0 = prmt(vw[0][x], vw[1][x], 0x7632u);
-        const uint32_t lo1 = prmt(vw[2][x], vw[3][x], 0x5410u), hi1 = prmt(vw[2][x], vw[3][x], 0x7632u);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t a[4] = {value2_at<T>(lo0, k, p0, magic), value2_at<T>(hi0, k, p0, magic),
-                                 value2_at<T>(lo1, k, p1, magic), value2_at<T>(hi1, k, p1, magic)};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[nt][4 * x + k], a, pt[nt][0], pt[nt][1]);
+        for (int w = 0; w < kFewWarps; ++w) {
+          if (s_l[w][r] == 0.f) continue;
+          const float a = ex2(s_m[w][r] - top);
+          const float4 y = *reinterpret_cast<const float4 *>(
+              reinterpret_cast<const float *>(dyn + w * F::kRing) + r * F::kPitch + d);
+          sum = fmaf(a, s_l[w][r], sum);
+          x.x = fmaf(a, y.x, x.x);
+          x.y = fmaf(a, y.y, x.y);
+          x.z = fmaf(a, y.z, x.z);
+          x.w = fmaf(a, y.w, x.w);
+        }
+        if (b0 > 0 || b1 < u.nb) {
+          const int64_t part = (2 * (int64_t)blockIdx.x + (b0 == 0)) * kRowsMost + r;
+          if (d == 0) p.part_ml[part] = make_float2(top, sum);
+          *reinterpret_cast<float4 *>(p.part_o + part * D + d) = x;
+        } else {
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          const int tok = token_of(u.row + r, p.per_group);
+          const int64_t at = ((int64_t)u.s.row0 + tok) * p.hq + u.kvh * p.group + (u.row + r - tok * p.group);
+          *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + at * D + d) =
+              make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
         }
       }
-      // the weights' sum: values of 1 in the rows of channel 0
-      const uint32_t ones = g == 0 ? kOnes<T> : 0u;
-      const uint32_t a[4] = {ones, 0u, ones, 0u};
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) mma16816<T>(oc[nt], a, pt[nt][0], pt[nt][1]);
-    };
-
-    int i = 0;
-    bool lost = false;  // a wait has run out
-#pragma unroll 1
-    while (i < blocks) {
-      const uint32_t at = turn & 1;
-      if (!__all_sync(kFull, ptx::mbar_wait(&full[warp][at], turn >> 1 & 1, &s_abort))) {
-        raise_error(p.batch.err, TIDE_DEVERR_TIMEOUT);
-        s_abort = 1;
-        lost = true;
-        break;
-      }
-      const unsigned char *b = ring + at * F::kPlace;
-      int key = (block0 + i * kFewWarps) * kBlock;
-      const int upto = min(i + kBatch, blocks);
-#pragma unroll 1
-      for (; i < upto; ++i, b += L::kBytes, key += kFewWarps * kBlock) {
-        if (key + kBlock <= all_see) work(b, key, std::false_type{});
-        else work(b, key, std::true_type{});
-      }
-      __syncwarp();  // the place has been read
-      ptx::fence_proxy_async();
-      request(i + kBatch, at);
-      ++turn;
-    }
-    if (lost && lane == 0) {  // wait for the copies in flight (bounded)
-      volatile int none = 0;
-      for (int e = i; e < min(blocks, i + 2 * kBatch); e += kBatch, ++turn)
-        ptx::mbar_wait(&full[warp][turn & 1], turn >> 1 & 1, &none);
-    }
-    __syncwarp();
-
-    // the four warps' outputs meet, [warp][row][D + 4]
-    float *mine = reinterpret_cast<float *>(ring);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = nt * 8 + t * 2 + e;
-        if (g == 0) {
-          s_m[warp][r] = kLift<T> - up[nt][e];
-          s_l[warp][r] = oc[nt][e];
-        }
-#pragma unroll
-        for (int d = 0; d < kSteps; ++d)
-          *reinterpret_cast<float2 *>(mine + r * F::kPitch + g * (D / 8) + 2 * d) =
-              make_float2(o[nt][d][e], o[nt][d][2 + e]);
-      }
-    __syncthreads();
-    constexpr int kLanes = D / 4;  // lanes of a row, four columns each
-    for (int r = threadIdx.x / kLanes; r < rows; r += 32 * kFewWarps / kLanes) {
-      const int d = threadIdx.x % kLanes * 4;
-      float top = -INFINITY, sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < kFewWarps; ++w)
-        if (s_l[w][r] != 0.f) top = fmaxf(top, s_m[w][r]);
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < kFewWarps; ++w) {
-        if (s_l[w][r] == 0.f) continue;
-        const float a = ex2(s_m[w][r] - top);
-        const float4 y = *reinterpret_cast<const float4 *>(
-            reinterpret_cast<const float *>(dyn + w * F::kRing) + r * F::kPitch + d);
-        sum = fmaf(a, s_l[w][r], sum);
-        x.x = fmaf(a, y.x, x.x);
-        x.y = fmaf(a, y.y, x.y);
-        x.z = fmaf(a, y.z, x.z);
-        x.w = fmaf(a, y.w, x.w);
-      }
-      if (b0 > 0 || b1 < u.nb) {
-        const int64_t part = (2 * (int64_t)blockIdx.x + (b0 == 0)) * kRowsMost + r;
-        if (d == 0) p.part_ml[part] = make_float2(top, sum);
-        *reinterpret_cast<float4 *>(p.part_o + part * D + d) = x;
-      } else {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        const int tok = token_of(u.row + r, p.per_group);
-        const int64_t at = ((int64_t)u.s.row0 + tok) * p.hq + u.kvh * p.group + (u.row + r - tok * p.group);
-        *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + at * D + d) =
-            make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
-      }
-    }
     }
     pos += left;
     if (pos >= end || *(volatile int *)&s_abort) return;
@@ -1085,9 +1098,9 @@ __global__ void __launch_bounds__(256)
       for (int b = 0; b < kFlight; ++b) {
         const int i = min(i0 + b * per, parts - 1);
         const int64_t at = (2 * (int64_t)(u.first + i) + (i == 0)) * kRows + r;
-        ml[b] = i0 + b * per < parts ? part_ml[at] : make_float2(-INFINITY, 0.f);
+        ml[b] = i0 + b * per < parts ? __ldcg(part_ml + at) : make_float2(-INFINITY, 0.f);
 #pragma unroll
-        for (int e = 0; e < kE; ++e) x[b][e] = part_o[at * D + lane * kE + e];
+        for (int e = 0; e < kE; ++e) x[b][e] = __ldcg(part_o + at * D + lane * kE + e);
       }
       float top = m;
 #pragma unroll

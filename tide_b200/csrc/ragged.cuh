@@ -97,43 +97,6 @@ __device__ __forceinline__ int sequence_of_row(const RaggedBatch &b, int live, i
   return -1;
 }
 
-// Piece *seq of the sequences' pieces of up to `tokens` tokens, counted in the
-// sequences' order, 32 of them at a time; those with more than `few` tokens have
-// none.  Sets its sequence and first token; false if there are not so many.  The
-// same for a whole warp.
-__device__ __forceinline__ bool find_piece(const RaggedBatch &b, int live, int few, int tokens, int *seq,
-                                           int *tok0) {
-  constexpr unsigned kFull = 0xffffffffu;
-  const int lane = threadIdx.x & 31;
-  int rest = *seq;
-  for (int base = 0; base < live; base += 32) {
-    int mine = 0;
-    if (base + lane < live) {
-      int row, end;
-      const bool good = sequence_bounds(b, base + lane, &row, &end);
-      // (one that has no piece here, and with that no CTA to flag it)
-      if (!good) raise_error(b.err, TIDE_DEVERR_POSITION);
-      const int n = good ? end - row : 0;
-      mine = n <= few ? (n + tokens - 1) / tokens : 0;
-    }
-    int upto = mine;
-#pragma unroll
-    for (int w = 1; w < 32; w *= 2) {
-      const int x = __shfl_up_sync(kFull, upto, w);
-      if (lane >= w) upto += x;
-    }
-    const unsigned past = __ballot_sync(kFull, upto > rest);
-    if (past) {
-      const int at = __ffs(past) - 1;
-      *seq = base + at;
-      *tok0 = (rest - __shfl_sync(kFull, upto - mine, at)) * tokens;
-      return true;
-    }
-    rest -= __shfl_sync(kFull, upto, 31);
-  }
-  return false;
-}
-
 // Where the keys are: rows of a packed tensor, or pages.
 struct KeySource {
   const void *k, *v;
@@ -160,12 +123,8 @@ inline cudaError_t allow_smem(K kern, int bytes, std::atomic<uint64_t> &set) {
 
 void set_last_error(const char *msg);
 
-// Parts of paged_attention for its kin (ragged_attn.cu).
-// The join of the few-rows kernels' splits, [splits, n_seqs, few, hq] rows.
-int join_few_rows(int dtype, int64_t head_dim, const RaggedBatch &b, int hq, int few, int splits,
-                  const float *part_o, const float2 *part_ml, void *out, cudaStream_t s);
-// Sequences with more than `few` rows over 16-bit pages, by tiles; *needed 0: there
-// is none (NULL: not known).
+// A part of paged_attention for its kin (ragged_attn.cu): sequences with more than
+// `few` rows over 16-bit pages, by tiles; *needed 0: there is none (NULL: not known).
 size_t paged_tiles_workspace_size(int64_t n_tokens, int64_t n_seqs, int64_t hq, int64_t hkv, int64_t d,
                                   int64_t max_kv);
 int paged_tiles(int dtype, int64_t head_dim, const RaggedBatch &b, const KeySource &src, int few,

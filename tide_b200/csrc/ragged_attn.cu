@@ -1149,7 +1149,35 @@ __global__ void __launch_bounds__(32 * kFewWarps, NT <= 2 ? 3 : 2)
   const int live = live_sequences(p.batch);
   int seq = (int)(unit / p.hkv), tok0 = 0;  // this CTA's tokens from tok0 on
   if (p.few > p.tokens) {
-    if (!find_piece(p.batch, live, p.few, p.tokens, &seq, &tok0)) return;
+    // pieces of the sequences, counted in their order, 32 sequences at a time
+    int rest = seq, found = -1;
+    for (int b = 0; b < live && found < 0; b += 32) {
+      int mine = 0;
+      if (b + lane < live) {
+        int row, end;
+        const bool good = sequence_bounds(p.batch, b + lane, &row, &end);
+        // (one that has no piece here, and with that no CTA to flag it)
+        if (!good) raise_error(p.batch.err, TIDE_DEVERR_POSITION);
+        const int n = good ? end - row : 0;
+        mine = n <= p.few ? (n + p.tokens - 1) / p.tokens : 0;
+      }
+      int upto = mine;
+#pragma unroll
+      for (int w = 1; w < 32; w *= 2) {
+        const int x = __shfl_up_sync(kFull, upto, w);
+        if (lane >= w) upto += x;
+      }
+      const unsigned past = __ballot_sync(kFull, upto > rest);
+      if (past) {
+        const int at = __ffs(past) - 1;
+        found = b + at;
+        tok0 = (rest - __shfl_sync(kFull, upto - mine, at)) * p.tokens;
+      } else {
+        rest -= __shfl_sync(kFull, upto, 31);
+      }
+    }
+    if (found < 0) return;
+    seq = found;
   }
   if (seq >= live) return;
   Sequence s = sequence(p.batch, seq);
@@ -1803,16 +1831,6 @@ void set_heads(tide::ragged::Params &p, int64_t hq, int64_t hkv, int64_t d, floa
 }  // namespace
 
 namespace tide {
-
-int join_few_rows(int dtype, int64_t head_dim, const RaggedBatch &b, int hq, int few, int splits,
-                  const float *part_o, const float2 *part_ml, void *out, cudaStream_t s) {
-  if (dtype == TIDE_DTYPE_BF16)
-    return head_dim == 128
-               ? launch_join<__nv_bfloat16, 128, true>(b, hq, few, splits, part_o, part_ml, out, s)
-               : launch_join<__nv_bfloat16, 64, true>(b, hq, few, splits, part_o, part_ml, out, s);
-  return head_dim == 128 ? launch_join<__half, 128, true>(b, hq, few, splits, part_o, part_ml, out, s)
-                         : launch_join<__half, 64, true>(b, hq, few, splits, part_o, part_ml, out, s);
-}
 
 size_t paged_tiles_workspace_size(int64_t n_tokens, int64_t n_seqs, int64_t hq, int64_t hkv, int64_t d,
                                   int64_t max_kv) {
