@@ -352,7 +352,8 @@ int tide_paged_append(int dtype, const void *k_new, const void *v_new, int64_t k
  *   c = min(max(round(x / s) + z, 0), 15)    (ties to even).
  * So a value is off by s / 2 at most (by s where s / 2 more would pass the rows'
  * largest number), and zero is held as zero.  A group with a value that is not
- * finite reads as NaN.  A cache is read as the type that it was written from.
+ * finite in the rows' type reads as NaN (a key after its norm and rotation).  A
+ * cache is read as the type that it was written from.
  *
  * The cache is [n_pages, n_kv_heads, page_size / 16, 18 head_dim] bytes.  The 18
  * head_dim bytes of 16 tokens of a head: the codes of the keys

@@ -595,3 +595,27 @@ def test_calls_on_two_streams_do_not_meet():
     for a, b in zip(want, got):
         for x, y in zip(a, b):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype,x,scaling,finite", [
+    (HF, 43648.0, 1.5, True), (HF, 43680.0, 1.5, False), (HF, -43680.0, 1.5, False), (HF, 65504.0, 2.0, False),
+    (BF, 2.0 ** 127, 510 / 256, True), (BF, 2.0 ** 127, 511 / 256, False), (BF, 2.0 ** 127, 2.0, False)], ids=str)
+def test_keys_that_the_rotation_takes_past_their_type(dtype, x, scaling, finite):
+    """At position 0 the rotation is the scaling alone, exact here: keys that round
+    to infinity in their type make their group NaN, the others are held."""
+    n, hkv, d = 3, 2, 128
+    _, k, v = rows(n, 2, hkv, d, dtype, 9)
+    k[1, 1, 40] = x
+    slots = torch.arange(n, device=DEV)
+    cache = empty_cache(1, hkv, 16, d)
+    append(None, k, v, slots, cache, positions=torch.zeros_like(slots), freq=torch.ones(d // 2, device=DEV),
+           scaling=scaling)
+    turned = k.double() * scaling
+    if not finite:
+        turned[1, 1, 40] = float("inf")
+    got, values = read(cache, slots, dtype)
+    odd = torch.zeros_like(got, dtype=torch.bool)
+    odd[1, 1, 32:64] = not finite
+    assert torch.equal(got.isnan(), odd) and bool(got.isfinite()[~odd].all())
+    for y, want in ((got, turned), (values, v)):
+        assert torch.equal(y.double().nan_to_num(0.5), Q.values(want, dtype).nan_to_num(0.5))

@@ -106,8 +106,10 @@ __device__ __forceinline__ uint32_t quantise(const Two (&x)[4], uint32_t *par) {
   constexpr bool kHalf = std::is_same<T, __half>::value;
   constexpr float kMost = kHalf ? 65504.f : 3.3895313892515355e38f;
   constexpr float kLeast = kHalf ? 0x1p-21f : 0x1p-120f;
+  constexpr float kPast = kHalf ? 65520.f : 0x1.ffp127f;  // what the type rounds to infinity
   float lo, hi;
-  const bool odd = extent(x, &lo, &hi);
+  bool odd = extent(x, &lo, &hi);
+  odd |= fmaxf(hi, -lo) >= kPast;  // (a key that norm and rotation took there)
   // v / by, rounded once, with inv = 1 / by rounded once: the product may be a bit
   // off, its remainder is exact and corrects it (Markstein).  Ties are common
   // (values of eight bits over scales of four), so that bit counts.
@@ -1367,7 +1369,8 @@ extern "C" int tide_paged_read_q4(int dtype, const void *cache, int64_t n_pages,
   };
   if (dtype == TIDE_DTYPE_BF16) {
     auto *k = static_cast<__nv_bfloat16 *>(k_out), *v = static_cast<__nv_bfloat16 *>(v_out);
-    return head_dim == 128 ? run(read_kernel<__nv_bfloat16, 128>, k, v) : run(read_kernel<__nv_bfloat16, 64>, k, v);
+    return head_dim == 128 ? run(read_kernel<__nv_bfloat16, 128>, k, v)
+                           : run(read_kernel<__nv_bfloat16, 64>, k, v);
   }
   auto *k = static_cast<__half *>(k_out), *v = static_cast<__half *>(v_out);
   return head_dim == 128 ? run(read_kernel<__half, 128>, k, v) : run(read_kernel<__half, 64>, k, v);
@@ -1452,8 +1455,9 @@ extern "C" int tide_paged_attention_q4(int dtype, const void *q, int64_t q_row_s
                                 bf16 ? tide::q4::kMagic<__nv_bfloat16> : tide::q4::kMagic<__half>,
                                 (uint32_t)(((1ll << 31) + group - 1) / group)};
     const int64_t n = plan.ctas;
-    rc = bf16 ? (wide ? few_rows<__nv_bfloat16, 128>(plan.nt, n, f, st) : few_rows<__nv_bfloat16, 64>(plan.nt, n, f, st))
-              : (wide ? few_rows<__half, 128>(plan.nt, n, f, st) : few_rows<__half, 64>(plan.nt, n, f, st));
+    const int nt = plan.nt;
+    rc = bf16 ? (wide ? few_rows<__nv_bfloat16, 128>(nt, n, f, st) : few_rows<__nv_bfloat16, 64>(nt, n, f, st))
+              : (wide ? few_rows<__half, 128>(nt, n, f, st) : few_rows<__half, 64>(nt, n, f, st));
   }
   if (rc || !plan.tiles) return rc;
   ws += plan.few_bytes;
