@@ -142,3 +142,18 @@ def test_the_paged_cache_and_generate_refuse_what_4_bits_cannot():
             generate(**kw)
     with pytest.raises(Reached):
         generate(kv_bits=4, live=True, paged=True)
+
+
+def test_reading_a_16_bit_cache_flags_slots_outside_it():
+    from tide_b200.paged import PagedKVCache
+
+    c = PagedKVCache(2, 2, 3, 16, 2, 64, 64, torch.float32, torch.device("cpu"))
+    for side in (c.k, c.v):
+        for x in side:
+            x.normal_()
+    k, v = c.read(1, torch.tensor([17, -1, 47], dtype=torch.int64))
+    assert torch.equal(k[0], c.k[1][1, :, 1]) and torch.equal(v[2], c.v[1][2, :, 15]) and not k[1].any()
+    assert int(c.error_word) == 0
+    k, v = c.read(0, torch.tensor([48, 3, -2, 1 << 60], dtype=torch.int64))
+    assert torch.equal(v[1], c.v[0][0, :, 3]) and not k[[0, 2, 3]].any() and not v[[0, 2, 3]].any()
+    assert int(c.error_word) == capi.DEVERR_POSITION

@@ -100,8 +100,9 @@ class PagedKVCache:
 
     def read(self, layer: int, slots: torch.Tensor):
         """The keys and values at `slots` (int64): two tensors [n, kv_heads,
-        head_dim]; zeros for a slot of -1."""
-        from tide_b200 import _native
+        head_dim]; zeros for a slot of -1, and for one outside the cache, which
+        the error word notes."""
+        from tide_b200 import _native, capi
 
         n = slots.numel()
         k = torch.zeros(n, self.kv_heads, self.head_dim, dtype=self.dtype, device=slots.device)
@@ -109,8 +110,10 @@ class PagedKVCache:
         if self.bits == 4:
             _native.ops().paged_read_q4(self.kv[layer], slots, k, v, self.error_word)
             return k, v
-        real = (slots >= 0)[:, None, None]
-        page, at = slots.clamp(min=0) // self.page_size, slots.clamp(min=0) % self.page_size
+        real = (slots >= 0) & (slots < self.k[layer].shape[0] * self.page_size)
+        self.error_word |= (~real & (slots != -1)).any().int() * capi.DEVERR_POSITION
+        slots = slots.where(real, 0)
+        page, at, real = slots // self.page_size, slots % self.page_size, real[:, None, None]
         return tuple(torch.where(real, c[layer][page, :, at], z) for c, z in ((self.k, k), (self.v, v)))
 
     def attend(self, layer: int, q: torch.Tensor, scale: float, *, chunk: bool,
