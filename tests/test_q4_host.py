@@ -157,3 +157,21 @@ def test_reading_a_16_bit_cache_flags_slots_outside_it():
     k, v = c.read(0, torch.tensor([48, 3, -2, 1 << 60], dtype=torch.int64))
     assert torch.equal(v[1], c.v[0][0, :, 3]) and not k[[0, 2, 3]].any() and not v[[0, 2, 3]].any()
     assert int(c.error_word) == capi.DEVERR_POSITION
+
+
+@pytest.mark.parametrize("kw", [
+    dict(d=0), dict(d=-64), dict(d=96), dict(n=0), dict(n=1 << 62), dict(n_seqs=0), dict(n_seqs=1 << 62),
+    dict(n_req=-1), dict(n_req=1 << 62), dict(hq=0), dict(hkv=0), dict(hq=1 << 62), dict(hq=1024), dict(max_kv=-1),
+    dict(max_kv=1 << 62)], ids=str)
+def test_no_workspace_for_what_the_call_refuses(kw):
+    a = dict(n=800, n_seqs=2, n_req=4, hq=8, hkv=2, d=128, max_kv=100)
+    assert _native.lib().tide_paged_attention_q4_workspace_size(*a.values()) > 0
+    a.update(kw)
+    assert _native.lib().tide_paged_attention_q4_workspace_size(*a.values()) == 0
+
+
+def test_the_workspace_of_the_largest_sizes():
+    most = (1 << 30) - 1
+    for n, n_seqs in ((most, most), (most, 1), (most, 1 << 20)):
+        got = _native.lib().tide_paged_attention_q4_workspace_size(n, n_seqs, 8, 65536, 65536 // 2, 128, most)
+        assert got < 1 << 62 and (n == n_seqs or got > 1 << 40)  # (few rows, or one sequence's pages)

@@ -1244,7 +1244,8 @@ Plan plan_of(bool one_token, int64_t n_tokens, int64_t n_seqs, int64_t n_request
     p.whole = max_kv <= 512;
     // as many CTAs as run at once, or fewer where there is not work for so many
     const int64_t slots = 148 * (p.nt == 1 ? 4 : 3);
-    const int64_t units = (n_seqs + n_tokens * group / (8 * p.nt)) * hkv;
+    int64_t units = (n_seqs + n_tokens * group / (8 * p.nt)) * hkv;
+    if (units > slots * kLeast) units = slots * kLeast;  // (enough for all; the product below fits)
     const int64_t blocks = (max_kv + kBlock - 1) / kBlock;
     p.ctas = p.whole ? units : (units * ((blocks < 1 ? 1 : blocks) + kUnitCost) + kLeast - 1) / kLeast;
     if (p.ctas > slots) p.ctas = slots;
@@ -1379,8 +1380,11 @@ extern "C" int tide_paged_read_q4(int dtype, const void *cache, int64_t n_pages,
 extern "C" size_t tide_paged_attention_q4_workspace_size(int64_t n_tokens, int64_t n_seqs, int64_t n_requests,
                                                          int64_t n_q_heads, int64_t n_kv_heads,
                                                          int64_t head_dim, int64_t max_kv_len) {
-  if (n_tokens < 1 || n_seqs < 1 || n_requests < 0 || n_kv_heads < 1 || n_q_heads < n_kv_heads ||
-      max_kv_len < 0 || n_q_heads / n_kv_heads > 128)
+  // (the limits of the call, within which nothing below overflows)
+  constexpr int64_t kMost = INT32_MAX / 2;
+  if (n_tokens < 1 || n_tokens > kMost || n_seqs < 1 || n_seqs > kMost || n_requests < 0 ||
+      n_requests > INT32_MAX || n_kv_heads < 1 || n_q_heads < n_kv_heads || n_q_heads > 65536 ||
+      n_q_heads / n_kv_heads > 128 || (head_dim != 64 && head_dim != 128) || max_kv_len < 0 || max_kv_len > kMost)
     return 0;
   // (cu_seqlens or not: the larger need of the two)
   const size_t one = plan_of(true, n_tokens, n_seqs, n_requests, n_q_heads, n_kv_heads, head_dim, max_kv_len).bytes;
