@@ -1080,6 +1080,7 @@ __global__ void __launch_bounds__(256)
     join_units_kernel(const Shared *__restrict__ shared, const float *__restrict__ part_o,
                       const float2 *__restrict__ part_ml, T *out, int hq, int group, uint32_t per_group) {
   constexpr int kE = D / 32, kFlight = 8, kRows = 8 * NT;
+  using Vec = typename std::conditional<kE == 4, float4, float2>::type;  // a lane's columns
   __shared__ float s_m[8], s_l[8], s_o[8][D];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   ptx::grid_dependency_wait();
@@ -1095,14 +1096,13 @@ __global__ void __launch_bounds__(256)
     for (int e = 0; e < kE; ++e) o[e] = 0.f;
     for (int i0 = warp % per; r < u.rows && i0 < parts; i0 += per * kFlight) {
       float2 ml[kFlight];
-      float x[kFlight][kE];
+      __align__(16) float x[kFlight][kE];
 #pragma unroll
       for (int b = 0; b < kFlight; ++b) {
         const int i = min(i0 + b * per, parts - 1);
         const int64_t at = (2 * (int64_t)(u.first + i) + (i == 0)) * kRows + r;
         ml[b] = i0 + b * per < parts ? __ldcg(part_ml + at) : make_float2(-INFINITY, 0.f);
-#pragma unroll
-        for (int e = 0; e < kE; ++e) x[b][e] = __ldcg(part_o + at * D + lane * kE + e);
+        *reinterpret_cast<Vec *>(x[b]) = __ldcg(reinterpret_cast<const Vec *>(part_o + at * D) + lane);
       }
       float top = m;
 #pragma unroll
@@ -1147,7 +1147,7 @@ __global__ void __launch_bounds__(256)
     const int tok = token_of(u.row + r, per_group);
     T *to = out + (((int64_t)u.seq_row + tok) * hq + u.kvh * group + (u.row + r - tok * group)) * D + lane * kE;
 #pragma unroll
-    for (int e = 0; e < kE; ++e) to[e] = Elem<T>::from_f(o[e] * inv);
+    for (int e = 0; e < kE; e += 2) reinterpret_cast<uint32_t *>(to)[e / 2] = ragged::pack2<T>(o[e] * inv, o[e + 1] * inv);
   }
 }
 
