@@ -545,14 +545,17 @@ __global__ void __launch_bounds__(256) open_kernel(const __grid_constant__ OpenP
 // little else, so 190 of the one and 17 of the other are 530 cycles of the 700 that a
 // block takes a scheduler.
 // 32 query heads on 8 KV heads of 128, with the join: 192 requests of 512 to 1535
-// keys 72 us (3.1 TB/s), three of 9000 to 40000 keys 32 us, 16 requests of 1 to 9
-// tokens over up to 2100 keys 30 us; two short ones 5.9 us.
+// keys 71 us (3.1 TB/s), three of 9000 to 40000 keys 31 us, 16 requests of 1 to 9
+// tokens over up to 2100 keys 28.5 us; two short ones 5.9 us.
 constexpr int kFewWarps = 4;
 constexpr int kBatch = 3;        // blocks of a place
-// What beginning and ending a unit costs, in blocks (with 4, 8 and 12, us: those 16
-// requests, some of them short, 41.8, 31.5, 30.3; the 192 73.7, 72.5, 72.2).
+// What beginning and ending a unit costs, in blocks (with 6, 9, 12 and 16, us: those
+// 16 requests, some of them short, 30.5, 29.2, 28.5, 28.3; the 192 72.0, 71.4, 71.4,
+// 71.5; one of 1000 keys 11.7, 10.3, 10.5, 10.6).
 constexpr int kUnitCost = 12;
-constexpr int kLeast = 16;       // cost of a CTA, where there is so little
+// The cost of a CTA, where there is so little (8, 16 and 32: one request of 1000 keys
+// 9.6, 10.5, 12.9 us, 16 of them 15.4, 15.4, 19.3).
+constexpr int kLeast = 8;
 
 template <int D, int NT>
 struct Few {
@@ -1147,7 +1150,8 @@ __global__ void __launch_bounds__(256)
     const int tok = token_of(u.row + r, per_group);
     T *to = out + (((int64_t)u.seq_row + tok) * hq + u.kvh * group + (u.row + r - tok * group)) * D + lane * kE;
 #pragma unroll
-    for (int e = 0; e < kE; e += 2) reinterpret_cast<uint32_t *>(to)[e / 2] = ragged::pack2<T>(o[e] * inv, o[e + 1] * inv);
+    for (int e = 0; e < kE; e += 2)
+      reinterpret_cast<uint32_t *>(to)[e / 2] = ragged::pack2<T>(o[e] * inv, o[e + 1] * inv);
   }
 }
 
@@ -1231,9 +1235,9 @@ Plan plan_of(bool one_token, int64_t n_tokens, int64_t n_seqs, int64_t n_request
   // which saves the launches of the tiles that find nothing.
   // Rows of a unit: 8 for up to as many on average, else 16 (64 requests over 1000 to
   // 2000 keys, 8 and 16: 4 rows 42 and 48 us, 8 rows 43 and 49, 12 rows 70 and 54).
-  // Whole units for short contexts (us, whole and split: one request of 500 keys 8.8
-  // and 10.8, of 1000 13.4 and 11.2; 64 of 250 to 500 14.8 and 20.6; 256 of those 49
-  // and 47, of 500 to 1000 84 and 74).
+  // Whole units for short contexts (us, whole and split: one request of 500 keys 8.7
+  // and 10.2, of 1000 13.3 and 9.6; 64 of 250 to 500 14.7 and 19.6; 256 of those 49
+  // and 48, of 500 to 1000 84 and 73).
   constexpr int64_t kMostRows = 64;
   const int64_t group = hq / hkv, rows = (n_tokens * group + n_seqs - 1) / n_seqs;
   p.nt = one_token || rows <= kMostRows ? (rows <= 8 ? 1 : 2) : 0;
