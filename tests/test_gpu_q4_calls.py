@@ -1,0 +1,40 @@
+"""Calls of the 4-bit cache's attention in which some of the sequences, or some of
+its kernels, have nothing to do: against 64-bit references, with what must not be
+touched or flagged."""
+import pytest
+import torch
+
+from tests.gpu_helpers import ptr, stream
+from tests.test_gpu_q4 import attend, check, q4_case
+from tests.test_gpu_ragged import i32, starts
+from tide_b200 import _native, capi
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF, HF = torch.bfloat16, torch.float16
+
+
+def test_no_long_sequence_among_the_live_ones():
+    """Twelve live sequences of 8 tokens before longer ones that are not live: both
+    kernels are launched, the tiles' keys split, and no sequence is theirs.  The
+    workspace holds what an earlier call left, large numbers here."""
+    hq, hkv, d, dtype, most = 8, 2, 128, BF, 8000
+    new = [8] * 12 + [100, 40, 33, 51, 0, 0, 0, 0]
+    q, cache, held, tables, lens, ids = q4_case(new, [29 * i for i in range(20)], hq, hkv, d, dtype, 16, 7)
+    wide = torch.cat([tables, torch.full((20, most // 16), -1, dtype=torch.int32, device=DEV)], 1).contiguous()
+    n, lib = q.shape[0], _native.lib()
+    size = lib.tide_paged_attention_q4_workspace_size(n, 20, 20, hq, hkv, d, most)
+    cu, kv, who = i32(starts(new)), i32(lens), i32(ids)
+    for live, byte in ((12, 0x7F), (12, 0), (0, 0x7F), (12, 0xFF), (13, 0x7F)):
+        ws = torch.full((size,), byte, dtype=torch.uint8, device=DEV)
+        out, err, n_dev = torch.full_like(q, 7.0), i32([0]), i32([live])
+        rc = lib.tide_paged_attention_q4(
+            capi.DTYPE_BF16, ptr(q), 0, ptr(cache), cache.shape[0], 16, ptr(wide), wide.shape[1], 20, ptr(kv),
+            ptr(cu), ptr(who), 20, ptr(n_dev), ptr(out), n, hq, hkv, d, most, d ** -0.5, ptr(ws), size,
+            ptr(err), stream())
+        capi.check(lib, rc, "tide_paged_attention_q4")
+        at = starts(new)[live]
+        assert int(err) == 0, (live, byte)
+        assert bool((out[at:] == 7).all()), (live, byte)
+        if live:
+            check(out[:at], q[:at], held, wide, lens, new[:live], ids[:live])

@@ -466,10 +466,12 @@ __global__ void __launch_bounds__(256) open_kernel(const __grid_constant__ OpenP
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   ptx::grid_dependency_wait();
   ptx::grid_dependents_launch();
-  if (p.needed && __ldcg(p.needed) == 0) return;
-  // eight blocks and heads a CTA, in order [sequence, block, head]
-  const int live = live_sequences(p.batch) - p.first;
+  const bool none = p.needed && __ldcg(p.needed) == 0;
+  const int live = none ? 0 : live_sequences(p.batch) - p.first;
+  // (the join of the tiles' splits reads it where none is needed, too)
   if (blockIdx.x == 0 && threadIdx.x == 0) *p.out_live = min(max(live, 0), p.n);
+  if (none) return;
+  // eight blocks and heads a CTA, in order [sequence, block, head]
   const int per = (int)p.wide * (kOpenPage / kBlock) * p.hkv;
   const int64_t item = (int64_t)blockIdx.x * 8 + warp;
   const int i = (int)(item / per), left = (int)(item - (int64_t)i * per);
