@@ -38,3 +38,22 @@ def test_no_long_sequence_among_the_live_ones():
         assert bool((out[at:] == 7).all()), (live, byte)
         if live:
             check(out[:at], q[:at], held, wide, lens, new[:live], ids[:live])
+
+
+@pytest.mark.parametrize("new", [[150, 0, 40], [0, 200, 0], [4, 0, 2]], ids=str)
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (HF, 64)], ids=str)
+def test_sequences_without_new_tokens_are_not_looked_at(new, dtype, d):
+    """Their requests' pages may be anything (paged_attention's rule): no error, and
+    the others' results as before."""
+    hq, hkv = 4, 2
+    q, cache, held, tables, lens, ids = q4_case(new, [100, 70, 300], hq, hkv, d, dtype, 16, 11)
+    err = i32([0])
+    want = attend(q, cache, tables, lens, new, ids, err=err)
+    check(want, q, held, tables, lens, new, ids)
+    broken = tables.clone()
+    for n, r in zip(new, ids):
+        if n == 0:
+            broken[r] = torch.tensor([-1, 1 << 30, cache.shape[0]] * tables.shape[1])[:tables.shape[1]]
+    out = attend(q, cache, broken, lens, new, ids, err=err)
+    assert int(err) == 0
+    assert torch.equal(out, want)

@@ -453,7 +453,7 @@ struct OpenParams {
   void *k, *v;
   int64_t wide;  // pages of a sequence in k and v
   int32_t *out_tables, *out_live;
-  int few;       // sequences of up to so many rows are not needed
+  int few;       // sequences of up to so many tokens are not needed
   const int32_t *needed;  // 0: none is; NULL: not known
 };
 constexpr int kOpenPage = 128;  // tokens of a 16-bit page
@@ -479,11 +479,10 @@ __global__ void __launch_bounds__(256) open_kernel(const __grid_constant__ OpenP
   const int block = left / p.hkv, h = left - block * p.hkv;
   const int seq = p.first + i;
   const int req = p.batch.seq_ids ? __ldg(p.batch.seq_ids + seq) : seq;
-  // (bad bounds, a bad request or length are the attention's to flag)
-  if (p.few) {
-    int row0, end;
-    if (!p.batch.cu || !sequence_bounds(p.batch, seq, &row0, &end) || end - row0 <= p.few) return;
-  }
+  // (bad bounds, a bad request or length are the attention's to flag; a sequence
+  // without new tokens, which few = 0 means too, has pages that may be anything)
+  int row0, end;
+  if (!sequence_bounds(p.batch, seq, &row0, &end) || end - row0 <= p.few) return;
   if (req < 0 || req >= p.batch.n_requests) return;
   const int tok0 = block * kBlock;
   if (tok0 % kOpenPage == 0 && h == 0 && lane == 0)
