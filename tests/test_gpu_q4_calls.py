@@ -57,3 +57,25 @@ def test_sequences_without_new_tokens_are_not_looked_at(new, dtype, d):
     out = attend(q, cache, broken, lens, new, ids, err=err)
     assert int(err) == 0
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("named", [True, False])
+def test_both_kernels_in_rounds(named):
+    """Short and long sequences in one call whose 16-bit pages take a round each,
+    with and without named requests and a live count from the device."""
+    hq, hkv, d, dtype, B, most = 8, 2, 128, HF, 37, 200000
+    new = [1 + i % 5 for i in range(B)]
+    new[3], new[20], new[21], new[36] = 90, 0, 70, 110
+    q, cache, held, tables, lens, ids = q4_case(new, [11 * i for i in range(B)], hq, hkv, d, dtype, 16, 13)
+    wide = torch.cat([tables, torch.full((B, most // 16), -1, dtype=torch.int32, device=DEV)], 1).contiguous()
+    if not named:
+        wide, lens, ids = wide[ids].contiguous(), [lens[r] for r in ids], list(range(B))
+    for live in (None, 36, 21, 3, 0):
+        out, err = torch.full_like(q, 7.0), i32([0])
+        _native.ops().paged_attention_q4(q, cache, wide, i32(lens), i32(starts(new)), i32(ids) if named else None,
+                                         out, most, d ** -0.5, err, None if live is None else i32([live]))
+        n = B if live is None else live
+        at = starts(new)[n]
+        assert int(err) == 0 and bool((out[at:] == 7).all())
+        if n:
+            check(out[:at], q[:at], held, wide, lens, new[:n], ids[:n])

@@ -175,3 +175,10 @@ def test_the_workspace_of_the_largest_sizes():
     for n, n_seqs in ((most, most), (most, 1), (most, 1 << 20)):
         got = _native.lib().tide_paged_attention_q4_workspace_size(n, n_seqs, 8, 65536, 65536 // 2, 128, most)
         assert got < 1 << 62 and (n == n_seqs or got > 1 << 40)  # (few rows, or one sequence's pages)
+
+
+def test_no_workspace_for_single_tokens_where_there_are_offsets():
+    """More tokens than sequences come with offsets: 4000 tokens a sequence go to the
+    tiles alone, whose 16-bit pages for 2 x 1000 keys of a head of 64 are 512 KB."""
+    got = _native.lib().tide_paged_attention_q4_workspace_size(8000, 2, 2, 8, 1, 64, 1000)
+    assert 1 << 19 <= got < 1 << 20

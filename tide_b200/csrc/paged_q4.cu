@@ -1218,9 +1218,9 @@ struct Plan {
   int few;
   bool whole;       // its units are not split
   int64_t ctas;
-  bool tiles;       // whether the tiles run: in rounds of sequences, so that the
-  int64_t wide;     // 16-bit pages of a round stay within 256 MB (or are one
-  int64_t seqs;     // sequence's): pages of a sequence, sequences of a round
+  bool tiles;       // whether the tiles run (single tokens never need them): in rounds
+  int64_t wide;     // of sequences, so that the 16-bit pages of a round stay within 256 MB
+  int64_t seqs;     // (or are one sequence's): pages of a sequence, sequences of a round
   size_t few_bytes, side, tables, inner, bytes;  // workspace
 };
 
@@ -1242,7 +1242,7 @@ Plan plan_of(bool one_token, int64_t n_tokens, int64_t n_seqs, int64_t n_request
   constexpr int64_t kMostRows = 64;
   const int64_t group = hq / hkv, rows = (n_tokens * group + n_seqs - 1) / n_seqs;
   p.nt = one_token || rows <= kMostRows ? (rows <= 8 ? 1 : 2) : 0;
-  if (n_seqs == 1 && n_tokens * group > 2 * kMostRows) p.nt = 0;
+  if (!one_token && n_seqs == 1 && n_tokens * group > 2 * kMostRows) p.nt = 0;
   if (p.nt) {
     p.few = (int)(one_token ? 1 : n_tokens * group <= 1024 ? n_tokens : 2 * kMostRows / group);
     if (p.few < 1) p.few = 1;
@@ -1257,7 +1257,7 @@ Plan plan_of(bool one_token, int64_t n_tokens, int64_t n_seqs, int64_t n_request
     if (!p.whole)
       p.few_bytes = (size_t)(p.ctas * (2 * 8 * p.nt * (d + 2) * 4 + (int64_t)sizeof(Shared)) + 15) / 16 * 16;
   }
-  p.tiles = !p.nt || (!one_token && n_tokens > p.few);
+  p.tiles = !one_token && (!p.nt || n_tokens > p.few);
   p.bytes = p.few_bytes;
   if (!p.tiles) return p;
   p.wide = (max_kv + tide::q4::kOpenPage - 1) / tide::q4::kOpenPage;
@@ -1269,8 +1269,7 @@ Plan plan_of(bool one_token, int64_t n_tokens, int64_t n_seqs, int64_t n_request
   p.side = (size_t)(p.seqs * p.wide * page);
   p.tables = (size_t)((n_requests * p.wide * 4 + 16 + 15) / 16 * 16);  // and the live count
   for (const int64_t n : {p.seqs, n_seqs % p.seqs}) {  // (the last round may be a smaller one)
-    const size_t inner =
-        tide::paged_tiles_workspace_size(one_token ? n : n_tokens, n, hq, hkv, d, max_kv);
+    const size_t inner = tide::paged_tiles_workspace_size(n_tokens, n, hq, hkv, d, max_kv);
     if (inner > p.inner) p.inner = inner;
   }
   p.bytes += 2 * p.side + p.tables + p.inner;
@@ -1391,9 +1390,10 @@ extern "C" size_t tide_paged_attention_q4_workspace_size(int64_t n_tokens, int64
       n_requests > INT32_MAX || n_kv_heads < 1 || n_q_heads < n_kv_heads || n_q_heads > 65536 ||
       n_q_heads / n_kv_heads > 128 || (head_dim != 64 && head_dim != 128) || max_kv_len < 0 || max_kv_len > kMost)
     return 0;
+  const size_t many = plan_of(false, n_tokens, n_seqs, n_requests, n_q_heads, n_kv_heads, head_dim, max_kv_len).bytes;
+  if (n_tokens != n_seqs) return many;
   // (cu_seqlens or not: the larger need of the two)
   const size_t one = plan_of(true, n_tokens, n_seqs, n_requests, n_q_heads, n_kv_heads, head_dim, max_kv_len).bytes;
-  const size_t many = plan_of(false, n_tokens, n_seqs, n_requests, n_q_heads, n_kv_heads, head_dim, max_kv_len).bytes;
   return one > many ? one : many;
 }
 
@@ -1481,17 +1481,13 @@ extern "C" int tide_paged_attention_q4(int dtype, const void *q, int64_t q_row_s
     if (rc) return rc;
     // sequence i of this round is request i of the call where none are named
     const int64_t skip = seq_ids ? 0 : i;
-    const int64_t row = cu_seqlens ? 0 : i;
-    const tide::RaggedBatch part{cu_seqlens ? cu_seqlens + i : nullptr, seq_ids ? seq_ids + i : nullptr,
-                                 kv_lens + skip, n_seqs_dev ? live : nullptr, (int)n,
-                                 (int)(n_requests - skip), (int)(cu_seqlens ? n_tokens : n),
-                                 (int)max_kv_len, error_word};
+    const tide::RaggedBatch part{cu_seqlens + i, seq_ids ? seq_ids + i : nullptr, kv_lens + skip,
+                                 n_seqs_dev ? live : nullptr, (int)n, (int)(n_requests - skip),
+                                 (int)n_tokens, (int)max_kv_len, error_word};
     const tide::KeySource src{ws, ws + plan.side, 0, tables + skip * plan.wide, plan.wide,
                               (int)(plan.seqs * plan.wide), 7};
     static_assert(tide::q4::kOpenPage == 1 << 7, "");
-    rc = tide::paged_tiles(dtype, head_dim, part, src, plan.few, longer,
-                           static_cast<const unsigned char *>(q) + row * q_row_stride * 2, q_row_stride,
-                           static_cast<unsigned char *>(out) + row * n_q_heads * head_dim * 2, n_q_heads,
+    rc = tide::paged_tiles(dtype, head_dim, part, src, plan.few, longer, q, q_row_stride, out, n_q_heads,
                            n_kv_heads, scale, ws + 2 * plan.side + plan.tables, st);
     if (rc) return rc;
   }
