@@ -182,3 +182,21 @@ def test_no_workspace_for_single_tokens_where_there_are_offsets():
     tiles alone, whose 16-bit pages for 2 x 1000 keys of a head of 64 are 512 KB."""
     got = _native.lib().tide_paged_attention_q4_workspace_size(8000, 2, 2, 8, 1, 64, 1000)
     assert 1 << 19 <= got < 1 << 20
+
+
+@pytest.mark.parametrize("held,other", [(torch.bfloat16, torch.float16), (torch.float16, torch.bfloat16)])
+def test_the_paged_cache_refuses_rows_of_another_type(held, other):
+    from tide_b200.paged import PagedKVCache
+
+    c = PagedKVCache(1, 2, 4, 16, 2, 64, 64, held, torch.device("cpu"), bits=4)
+    slots, freq = torch.arange(3), torch.ones(32)
+    a, b = torch.zeros(3, 2, 64, dtype=held), torch.zeros(3, 2, 64, dtype=other)
+    for k, v in ((b, b), (a, b), (b, a)):
+        with pytest.raises(ValueError, match="cache in 4 bits"):
+            c.append(0, k, v, slots)
+    for q, k, v in ((b, b, b), (b, a, a), (a, b, a), (a, a, b)):
+        with pytest.raises(ValueError, match="cache in 4 bits"):
+            c.append_rotated(0, q, k, v, slots, slots, freq)
+    for chunk in (False, True):
+        with pytest.raises(ValueError, match="cache in 4 bits"):
+            c.attend(0, b, 0.1, chunk=chunk)

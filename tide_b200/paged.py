@@ -22,7 +22,7 @@ class PagedKVCache:
     the requests' block tables and lengths, on the device.  With bits=4 they
     are `kv` [n_pages, kv_heads, page_size / 16, 18 head_dim] bytes per layer
     instead, 4.5 bits a value (the format is in include/tide_b200.h), for rows
-    of `dtype`."""
+    of `dtype` and no other."""
 
     def __init__(self, n_layers: int, n_requests: int, n_pages: int, page_size: int, kv_heads: int,
                  head_dim: int, max_len: int, dtype: torch.dtype, device: torch.device,
@@ -66,6 +66,13 @@ class PagedKVCache:
                                   self.block_tables, self.page_size, self.n_free, self.kv_lens,
                                   self.cu_seqlens, slot_map, positions, self.error_word)
 
+    def _check_rows(self, *rows: Optional[torch.Tensor]) -> None:
+        """The bytes of a cache in 4 bits have no type of their own: rows of the other
+        16-bit type would be held, or met, as what they are not."""
+        for x in rows:
+            if self.bits == 4 and x is not None and x.dtype != self.dtype:
+                raise ValueError(f"rows of {x.dtype} for a cache in 4 bits of {self.dtype}")
+
     def append(self, layer: int, k: Optional[torch.Tensor], v: Optional[torch.Tensor],
                slot_map: torch.Tensor, row_ids: Optional[torch.Tensor] = None,
                n_rows: Optional[torch.Tensor] = None) -> None:
@@ -73,6 +80,7 @@ class PagedKVCache:
         (None: zeros to every slot)."""
         from tide_b200 import _native
 
+        self._check_rows(k, v)
         if self.bits == 4:
             _native.ops().paged_append_q4(None, k, v, slot_map, row_ids, n_rows, None, None, 1.0, None,
                                           None, 0.0, None, self.kv[layer], self.error_word)
@@ -93,6 +101,7 @@ class PagedKVCache:
 
         if self.bits != 4:
             raise NotImplementedError("append_rotated is for a cache in 4 bits")
+        self._check_rows(q, k, v)
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         _native.ops().paged_append_q4(q, k, v, slot_map, row_ids, n_rows, positions, inv_freq, scaling,
                                       q_weight, k_weight, eps, out, self.kv[layer], self.error_word)
@@ -123,6 +132,7 @@ class PagedKVCache:
         requests (chunk), or one row per request, of request seq_ids[i]."""
         from tide_b200 import _native
 
+        self._check_rows(q)
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         cu = self.cu_seqlens if chunk else None
         if self.bits == 4:
