@@ -387,7 +387,9 @@ int tide_paged_append(int dtype, const void *k_new, const void *v_new, int64_t k
  *
  * tide_paged_attention_q4: tide_paged_attention over it, with the same
  * arguments and rules.  A key or value group that reads as NaN reaches the tokens
- * that see it, and no others. */
+ * that see it, and no others.  Where sequences may have many rows the workspace
+ * holds contexts in 16 bits: up to 256 MB, or those of one sequence of max_kv_len
+ * keys if they are more. */
 int tide_paged_append_q4(int dtype, const void *q, int64_t q_row_stride, const void *k_new,
                          const void *v_new, int64_t kv_row_stride, const void *q_norm_weight,
                          const void *k_norm_weight, float eps, const float *inv_freq,
