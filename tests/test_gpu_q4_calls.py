@@ -79,3 +79,31 @@ def test_both_kernels_in_rounds(named):
         assert int(err) == 0 and bool((out[at:] == 7).all())
         if n:
             check(out[:at], q[:at], held, wide, lens, new[:n], ids[:n])
+
+
+def test_a_captured_call_takes_other_live_counts():
+    """The call of the first test, captured once: replays with and without a long
+    sequence among the live ones, which all of its kernels have to notice."""
+    hq, hkv, d, dtype, most = 8, 2, 128, BF, 8000
+    new = [8] * 12 + [100, 40, 33, 51, 0, 0, 0, 0]
+    q, cache, held, tables, lens, ids = q4_case(new, [29 * i for i in range(20)], hq, hkv, d, dtype, 16, 17)
+    wide = torch.cat([tables, torch.full((20, most // 16), -1, dtype=torch.int32, device=DEV)], 1).contiguous()
+    kv, cu, who, err, n_dev = i32(lens), i32(starts(new)), i32(ids), i32([0]), i32([20])
+    out = torch.zeros_like(q)
+
+    def call():
+        _native.ops().paged_attention_q4(q, cache, wide, kv, cu, who, out, most, d ** -0.5, err, n_dev)
+
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for live in (12, 16, 3, 14, 0, 20, 12):
+        n_dev.fill_(live)
+        out.fill_(7.0)
+        graph.replay()
+        at = starts(new)[live]
+        assert int(err) == 0 and bool((out[at:] == 7).all()), live
+        if live:
+            check(out[:at], q[:at], held, wide, lens, new[:live], ids[:live])
